@@ -1,8 +1,8 @@
 """The C ABI of ``libsophia_kda.so`` as a ctypes table, with no torch import.
 
 Status codes, element types and flag bits of include/sophia_kda.h and every
-entry point of include/sophia_kda.h and include/sophia_decoder.h with its
-ctypes signature.  ``sophia_amd._native`` binds the library through this
+entry point of include/sophia_kda.h, include/sophia_decoder.h and
+include/sophia_draft.h with its ctypes signature.  ``sophia_amd._native`` binds the library through this
 table; the CPU tests also bind a host-sanitized build of the library with it
 (torch is not loaded into that process).
 """
@@ -26,8 +26,23 @@ SCAN_NO_SEGMENTS = 8
 BWD_RECURRENT = 16
 BWD_GRAD_BF16 = 32
 
-# Every symbol of include/sophia_kda.h and include/sophia_decoder.h, with its
-# ctypes signature.
+TREE_NODES = 64          # SOPHIA_TREE_NODES of include/sophia_draft.h
+
+
+class CommitKda(ctypes.Structure):
+    """sophia_commit_kda of include/sophia_draft.h."""
+    _fields_ = [("tape", ctypes.c_void_p), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("conv_state", ctypes.c_void_p), ("state", ctypes.c_void_p)]
+
+
+class CommitMla(ctypes.Structure):
+    """sophia_commit_mla of include/sophia_draft.h."""
+    _fields_ = [("latent", ctypes.c_void_p), ("latent_stride", ctypes.c_int64), ("cache", ctypes.c_void_p),
+                ("slot_stride", ctypes.c_int64)]
+
+
+# Every symbol of include/sophia_kda.h, include/sophia_decoder.h and
+# include/sophia_draft.h, with its ctypes signature.
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
@@ -89,6 +104,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                        _i64, _i64, _i32, _i32, _i32, _f32, _i32, _vp]),
     "sophia_mla_decode_attn": (_i32, [_vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _f32, _vp,
                                       _i64, _i32, _i64, _i32, _i32, _i32, _vp, _sz, _vp]),
+    "sophia_kda_tree_step": (_i32, [_vp, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i64, _i32, _vp, _i64, _i32,
+                                    _vp, _vp, _f32, _f32, _u32, _vp, _i32, _vp, _vp, _vp, _i32, _i64, _i32, _i32,
+                                    _i32, _vp, _i64, _vp, _vp]),
+    "sophia_tree_commit": (_i32, [_vp, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i32, _vp, _i32, _i32, _i32, _i32,
+                                  _i32, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),
+    "sophia_mla_tree_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "sophia_mla_tree_attn": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32,
+                                    _i64, _i32, _f32, _vp, _i64, _i32, _i32, _i32, _vp, _sz, _vp]),
+    "sophia_adjust_logits": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _i64, _vp, _vp, _i32, _vp, _vp,
+                                    _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp]),
+    "sophia_tree_accept_workspace_size": (_sz, [_i64, _i32]),
+    "sophia_tree_accept": (_i32, [_vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _vp, _vp, _vp,
+                                  _vp, _sz, _vp]),
 }
 
 

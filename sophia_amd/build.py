@@ -2,7 +2,7 @@
 
 hipcc for gfx950 only; each translation unit is compiled to an object in
 sophia_amd/_build/ and linked into one shared library exporting the C ABI of
-include/sophia_kda.h and include/sophia_decoder.h.  Run ``python -m sophia_amd.build``.
+include/sophia_kda.h, include/sophia_decoder.h and include/sophia_draft.h.  Run ``python -m sophia_amd.build``.
 """
 
 from __future__ import annotations
@@ -21,7 +21,7 @@ LIB_NAME = "libsophia_kda.so"
 LIB_PATH = os.path.join(LIB_DIR, LIB_NAME)
 ARCH = "gfx950"
 SOURCES = ("errors.cpp", "short_conv.hip", "kda_decode.hip", "kda_chunk.hip", "decoder_ops.hip", "kda_bwd.hip",
-           "row_linear.hip")
+           "row_linear.hip", "kda_tree.hip", "mla_tree.hip", "logits.hip")
 
 # Packed-fp32 VALU ops are switched off for all device code.
 COMMON_FLAGS = [

@@ -16,6 +16,7 @@ FlashKDA seam (sm120_concurrent_ffn.py:375-423), so they drop into
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import torch
 
@@ -1612,6 +1613,428 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         float(hd ** -0.5 if scale is None else scale), nat.DTYPE_BF16, nat.stream_handle(q.device))
     nat.check(rc, "sophia_causal_attention")
     return y
+
+
+# ------------------------------------------------------------------ drafted tokens
+TREE_NODES = nat.TREE_NODES   # nodes of a tree of drafted tokens, at most
+
+
+def _same_device(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None:
+            _gpu(t, name)
+            if t.device != device:
+                raise RuntimeError(f"{name} must be on {device}, got {t.device}")
+
+
+def _on(device):
+    """The device as the current one for a launch (a stream handle alone does
+    not name it)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _trees(cu_nodes: torch.Tensor, parents: torch.Tensor, max_nodes: int, rows: int, device) -> int:
+    """Checks the trees over ``rows`` packed nodes; returns their number."""
+    cu = _int32(cu_nodes, "cu_nodes", device)
+    par = _int32(parents, "parents", device)
+    if cu is None or cu.dim() != 1 or cu.numel() < 1:
+        raise RuntimeError("cu_nodes must hold one offset per tree and the end of the last")
+    if par is None or int(par.numel()) != rows:
+        raise RuntimeError(f"parents must hold one entry per node, {rows}")
+    if not 1 <= int(max_nodes) <= TREE_NODES:
+        raise RuntimeError(f"max_nodes must be in [1, {TREE_NODES}], got {max_nodes}")
+    return int(cu.numel()) - 1
+
+
+def _int64(t: torch.Tensor, name: str, n: int, device) -> torch.Tensor:
+    if t.dtype != torch.int64 or t.device != device or not t.is_contiguous() or int(t.numel()) != n:
+        raise RuntimeError(f"{name} must be a contiguous int64 tensor of {n} entries on {device}")
+    return t
+
+
+def _tree_slots(slots: torch.Tensor | None, n: int, n_slots: int, device) -> torch.Tensor | None:
+    sl = _int32(slots, "slots", device)
+    _slot_count(sl, n)
+    if sl is None and n_slots < n:
+        raise RuntimeError("the caches have fewer slots than there are trees")
+    return sl
+
+
+def _latents(cache: torch.Tensor, rank: int, name: str) -> int:
+    """Slot stride of a latent cache [slots, max_seq, rank] with dense rows."""
+    if (cache.dim() != 3 or cache.dtype != torch.float32 or int(cache.size(2)) != rank or cache.stride(2) != 1
+            or cache.stride(1) != rank):
+        raise RuntimeError(f"{name} must be fp32 [slots, max_seq, {rank}] with dense rows")
+    return int(cache.stride(0)) if int(cache.size(0)) > 1 else int(cache.size(1)) * rank
+
+
+def mla_tree_attn(qa: torch.Tensor, latent: torch.Tensor, latent_cache: torch.Tensor, cu_nodes: torch.Tensor,
+                  parents: torch.Tensor, slots: torch.Tensor | None, cached: torch.Tensor, scale: float, *,
+                  max_nodes: int, max_len: int | None = None, splits: int | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """``mla_decode_attn`` for a tree of drafted tokens of each sequence: node i
+    of tree s attends to the cached latents 0 .. cached[s] - 1 of slot slots[s]
+    and to the drafted latents of its ancestors and itself, which are not in the
+    cache (sophia_mla_tree_attn).
+
+    qa: [rows, heads, rank] (bf16 or fp32, heads <= 16, rank in 32/64/128/256),
+    the nodes of all trees; latent: [rows, rank] of qa's dtype; latent_cache:
+    [n_slots, max_seq, rank] fp32 with dense rows; cu_nodes int32 [N + 1], the
+    rows of each tree; parents int32 [rows], a node's parent as an index into
+    its own tree, before the node (else, -1 say, the node is a root, which
+    follows the cached tokens); slots int32 [N] (None: s); cached int64 [N].
+    ``max_nodes`` (host int, at most 64) bounds the nodes of a tree, ``max_len``
+    (host int) bounds ``cached`` and sizes the key splits; ``splits`` overrides
+    them.  Rows of no tree are left as they are.  Returns [rows, heads, rank] in
+    qa's dtype."""
+    _gpu(qa, "qa")
+    if qa.dim() != 3:
+        raise RuntimeError(f"qa must be [rows, heads, rank], got {tuple(qa.shape)}")
+    device = qa.device
+    rows, heads, rank = (int(v) for v in qa.shape)
+    _same_device(device, latent=latent, latent_cache=latent_cache, cached=cached, out=out)
+    qs = _heads_rows(qa, "qa", heads, rank)
+    ls = _rows(latent, "latent", rank)
+    _nrows(latent, "latent", rows)
+    if latent.dtype != qa.dtype:
+        raise RuntimeError("latent must have qa's dtype")
+    n = _trees(cu_nodes, parents, max_nodes, rows, device)
+    slot_stride = _latents(latent_cache, rank, "latent_cache")
+    n_slots, max_seq = int(latent_cache.size(0)), int(latent_cache.size(1))
+    sl = _tree_slots(slots, n, n_slots, device)
+    _int64(cached, "cached", n, device)
+    y = out if out is not None else torch.empty((rows, heads, rank), dtype=qa.dtype, device=device)
+    os_ = _heads_rows(y, "out", heads, rank)
+    _nrows(y, "out", rows)
+    if y.dtype != qa.dtype:
+        raise RuntimeError("out must have qa's dtype")
+    if splits is None:
+        bound = max_seq if max_len is None else min(int(max_len), max_seq)
+        splits = mla_tree_splits(n, int(max_nodes), bound)
+    lib = nat.lib()
+    with _on(device):
+        ws_bytes = int(lib.sophia_mla_tree_workspace_size(rows, rank, int(splits)))
+        ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
+        rc = lib.sophia_mla_tree_attn(
+            nat.ptr(qa), qs, nat.ptr(latent), ls, nat.dtype_code(qa.dtype), nat.ptr(latent_cache), slot_stride, n_slots,
+            max_seq, nat.ptr(sl), nat.ptr(cached), nat.ptr(cu_nodes), nat.ptr(parents), n, rows, int(max_nodes),
+            float(scale), nat.ptr(y), os_, heads, rank, int(splits), nat.ptr(ws), ws_bytes, nat.stream_handle(device))
+    nat.check(rc, "sophia_mla_tree_attn")
+    return y
+
+
+def mla_tree_splits(trees: int, max_nodes: int, max_len: int) -> int:
+    """Key splits of ``mla_tree_attn``: about two work-groups per CU, at least
+    four 64-key tiles each."""
+    groups = max(trees, 1) * -(-max_nodes // 8)
+    return max(1, min(2 * _CUS // groups, -(-max_len // 256), 32))
+
+
+def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: torch.Tensor | None, g: torch.Tensor,
+                  beta: torch.Tensor, state: torch.Tensor, cu_nodes: torch.Tensor, parents: torch.Tensor, *,
+                  max_nodes: int, A_log=None, dt_bias=None, scale: float | None = None, lower_bound: float = -5.0,
+                  use_qk_l2norm: bool = True, use_gate: bool = True, use_beta_sigmoid: bool = True,
+                  state_slots: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  tape: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``kda_decode_conv_step`` along every path of a tree of drafted tokens of
+    each sequence, from its cached state and conv history, which are left as they
+    are (sophia_kda_tree_step): a node's conv samples and its state are those of
+    its ancestors, then the cached ones.
+
+    x_qkv: [rows, 3 * H * 128] pre-conv projection rows of the nodes (row stride
+    a multiple of 8, 16-byte aligned); conv_weight: [3 * H * 128, K] fp32 taps
+    rounded to x_qkv.dtype, K in 1..4; conv_state: fp32 [slots, 3 * H * 128,
+    K - 1] (None for K = 1); g: [rows, H, 128] decay logits, or with
+    ``use_gate=False`` finite log-decays; beta: [rows, H]; state: fp32 [slots, H,
+    128, 128]; cu_nodes, parents, max_nodes: as in ``mla_tree_attn``.  q, k and v
+    stay in fp32 from the conv on.  Returns (o [rows, H, 128] in x_qkv.dtype,
+    tape [rows, H, 3, 128] fp32: what ``tree_commit`` takes to advance the state
+    along an accepted path)."""
+    _gpu(x_qkv, "x_qkv")
+    _gpu(g, "g")
+    device = x_qkv.device
+    rows = int(x_qkv.size(0))
+    heads = int(g.size(1)) if g.dim() == 3 else 0
+    inner = heads * HEAD_DIM
+    xs = _rows(x_qkv, "x_qkv", 3 * inner)
+    gs = _heads_rows(g, "g", heads, HEAD_DIM)
+    bs = _rows(beta, "beta", heads)
+    _same_device(device, conv_weight=conv_weight, conv_state=conv_state, g=g, beta=beta, state=state, out=out, tape=tape)
+    for t, name in ((g, "g"), (beta, "beta")):
+        _nrows(t, name, rows)
+    n = _trees(cu_nodes, parents, max_nodes, rows, device)
+    taps = _tree_taps(conv_weight, conv_state, inner)
+    _state(state, "state", heads, device)
+    n_slots = int(state.size(0))
+    if conv_state is not None and int(conv_state.size(0)) != n_slots:
+        raise RuntimeError("conv_state and state must have the same number of slots")
+    slots = _tree_slots(state_slots, n, n_slots, device)
+    a_log, dtb = _gate_params(use_gate, A_log, dt_bias, heads, device)
+    o = out if out is not None else torch.empty((rows, heads, HEAD_DIM), dtype=x_qkv.dtype, device=device)
+    os_ = _heads_rows(o, "out", heads, HEAD_DIM)
+    _nrows(o, "out", rows)
+    if o.dtype != x_qkv.dtype:
+        raise RuntimeError("out must have x_qkv's dtype")
+    if tape is None:
+        tape = torch.empty((rows, heads, 3, HEAD_DIM), dtype=torch.float32, device=device)
+    _tape(tape, rows, heads)
+    base, esz = x_qkv.data_ptr(), x_qkv.element_size()
+    with _on(device):
+        rc = nat.lib().sophia_kda_tree_step(
+            base, base + inner * esz, base + 2 * inner * esz, xs, nat.dtype_code(x_qkv.dtype), nat.ptr(conv_weight),
+            nat.ptr(conv_state), taps, nat.ptr(g), gs, nat.dtype_code(g.dtype), nat.ptr(beta), bs,
+            nat.dtype_code(beta.dtype), nat.ptr(a_log), nat.ptr(dtb), float(HEAD_DIM ** -0.5 if scale is None else scale),
+            float(lower_bound), _flags(use_qk_l2norm, use_gate, use_beta_sigmoid), nat.ptr(state), n_slots,
+            nat.ptr(slots), nat.ptr(cu_nodes), nat.ptr(parents), n, rows, int(max_nodes), heads, HEAD_DIM, nat.ptr(o),
+            os_, nat.ptr(tape), nat.stream_handle(device))
+    nat.check(rc, "sophia_kda_tree_step")
+    return o, tape
+
+
+def _tree_taps(conv_weight: torch.Tensor, conv_state: torch.Tensor | None, inner: int) -> int:
+    taps = int(conv_weight.size(1)) if conv_weight.dim() == 2 else 0
+    if (conv_weight.dtype != torch.float32 or not conv_weight.is_contiguous() or not 1 <= taps <= 4
+            or int(conv_weight.size(0)) != 3 * inner):
+        raise RuntimeError(f"conv_weight must be contiguous fp32 [{3 * inner}, K], K in 1..4")
+    _conv_history(conv_state, inner, taps)
+    return taps
+
+
+def _conv_history(conv_state: torch.Tensor | None, inner: int, taps: int) -> None:
+    if conv_state is None:
+        if taps > 1:
+            raise RuntimeError("conv_state is needed for a conv of more than one tap")
+    elif (conv_state.dtype != torch.float32 or not conv_state.is_contiguous() or conv_state.dim() != 3
+          or tuple(conv_state.shape[1:]) != (3 * inner, taps - 1)):
+        raise RuntimeError(f"conv_state must be contiguous fp32 [slots, {3 * inner}, {taps - 1}]")
+
+
+def _tape(tape: torch.Tensor, rows: int, heads: int) -> None:
+    if tape.dtype != torch.float32 or not tape.is_contiguous() or tuple(tape.shape) != (rows, heads, 3, HEAD_DIM):
+        raise RuntimeError(f"tape must be contiguous fp32 [{rows}, {heads}, 3, {HEAD_DIM}]")
+
+
+def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor, slots: torch.Tensor | None, *,
+                kda=(), mla=(), cached: torch.Tensor | None = None) -> None:
+    """Writes an accepted path of every tree into the caches of all layers, in
+    place and in one launch (sophia_tree_commit): what the path's tokens, decoded
+    one by one, would have left there.
+
+    path: int32 [N, max_path], node indices within the tree from a root
+    downwards; n_path: int32 [N], how many of them count (0: the tree's caches
+    stay as they are; an index that is no node of the tree ends the path);
+    cu_nodes, slots: as in ``mla_tree_attn``; the trees of one call have different
+    slots.  kda: for each KDA layer (tape, x_qkv, conv_state, state), the tape
+    and the arguments of its ``kda_tree_step``; mla: for each MLA layer (latent,
+    latent_cache) of its ``mla_tree_attn``, and ``cached`` int64 [N]: node t of
+    the path goes to position cached[s] + t (past the cache's end: left out)."""
+    _gpu(path, "path")
+    device = path.device
+    if path.dim() != 2 or path.dtype != torch.int32 or path.stride(1) != 1:
+        raise RuntimeError("path must be int32 [trees, max_path] with dense rows")
+    n, max_path = int(path.size(0)), int(path.size(1))
+    if not 1 <= max_path <= TREE_NODES:
+        raise RuntimeError(f"path rows must hold 1..{TREE_NODES} entries, got {max_path}")
+    _same_device(device, n_path=n_path, cu_nodes=cu_nodes, slots=slots, cached=cached)
+    count = _int32(n_path, "n_path", device)
+    cu = _int32(cu_nodes, "cu_nodes", device)
+    if int(count.numel()) != n or int(cu.numel()) != n + 1:
+        raise RuntimeError(f"n_path must hold {n} and cu_nodes {n + 1} entries")
+    kda, mla = list(kda), list(mla)
+    rows = n_slots = None
+    heads, taps, x_dtype = 1, 1, torch.float32
+
+    def agree(what, got, want):
+        if want is not None and got != want:
+            raise RuntimeError(f"every layer must have the same {what}, got {got} and {want}")
+        return got
+
+    kda_args = (nat.CommitKda * max(len(kda), 1))()
+    for i, (tape, x, conv_state, state) in enumerate(kda):
+        _same_device(device, tape=tape, x_qkv=x, conv_state=conv_state, state=state)
+        h = int(tape.size(1)) if tape.dim() == 4 else 0
+        t = int(conv_state.size(-1)) + 1 if conv_state is not None else 1
+        if i:
+            agree("heads, conv taps and x_qkv type", (h, t, x.dtype), (heads, taps, x_dtype))
+        heads, taps, x_dtype = h, t, x.dtype
+        if not 1 <= taps <= 4:
+            raise RuntimeError("conv_state must hold at most 3 samples")
+        xs = _rows(x, "x_qkv", 3 * heads * HEAD_DIM)
+        rows = agree("rows", int(x.size(0)), rows)
+        _tape(tape, rows, heads)
+        _state(state, "state", heads, device)
+        _conv_history(conv_state, heads * HEAD_DIM, taps)
+        n_slots = agree("slots", int(state.size(0)), n_slots)
+        if conv_state is not None:
+            agree("slots", int(conv_state.size(0)), n_slots)
+        kda_args[i] = nat.CommitKda(tape.data_ptr(), x.data_ptr(), xs, nat.ptr(conv_state), state.data_ptr())
+    rank = max_seq = lat_dtype = None
+    mla_args = (nat.CommitMla * max(len(mla), 1))()
+    for i, (latent, cache) in enumerate(mla):
+        _same_device(device, latent=latent, latent_cache=cache)
+        rank = agree("rank", int(latent.size(-1)), rank)
+        lat_dtype = agree("latent type", latent.dtype, lat_dtype)
+        ls = _rows(latent, "latent", rank)
+        ss = _latents(cache, rank, "latent_cache")
+        rows = agree("rows", int(latent.size(0)), rows)
+        n_slots = agree("slots", int(cache.size(0)), n_slots)
+        max_seq = agree("cache length", int(cache.size(1)), max_seq)
+        mla_args[i] = nat.CommitMla(latent.data_ptr(), ls, cache.data_ptr(), ss)
+    if rows is None:
+        return
+    sl = _tree_slots(slots, n, n_slots, device)
+    if mla:
+        if cached is None:
+            raise RuntimeError("MLA layers need cached")
+        _int64(cached, "cached", n, device)
+    with _on(device):
+        rc = nat.lib().sophia_tree_commit(
+            nat.ptr(path), int(path.stride(0)) if n > 1 else max_path, nat.ptr(count), max_path, nat.ptr(cu), n, rows,
+            nat.ptr(sl), n_slots, kda_args, len(kda), heads, HEAD_DIM, taps, nat.dtype_code(x_dtype), mla_args, len(mla),
+            nat.ptr(cached) if mla else None, max_seq or 0, rank or 0, nat.dtype_code(lat_dtype or torch.float32),
+            nat.stream_handle(device))
+    nat.check(rc, "sophia_tree_commit")
+
+
+def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, history_len: torch.Tensor | None = None,
+                  prompt_len: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
+                  presence: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                  bias_ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                  allowed: torch.Tensor | None = None, allowed_rows: torch.Tensor | None = None,
+                  cu_nodes: torch.Tensor | None = None, parents: torch.Tensor | None = None,
+                  tokens: torch.Tensor | None = None, max_nodes: int = 0,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties for repeated tokens, biases and grammar masks on logits [rows,
+    vocab] (bf16 or fp32, any row stride), in one pass (sophia_adjust_logits).
+
+    Row r is sequence r, or with ``cu_nodes`` int32 [N + 1], ``parents`` int32
+    [rows], ``tokens`` int64 [rows] and ``max_nodes`` (as in ``mla_tree_attn``)
+    a node of a tree: its ancestors' tokens and its own count as generated ones.
+    Of each sequence (all optional): ``history`` int64 [N, L] with
+    ``history_len`` int32 [N], the tokens so far, of which the first
+    ``prompt_len`` int32 [N] (None: none) count for the repetition penalty only;
+    ``repetition`` (> 0), ``presence``, ``frequency`` fp32 [N]; ``bias_ids``
+    int64 [N, M] with ``bias`` fp32 [N, M], ids outside the vocabulary ignored,
+    an id given twice adds twice.  ``allowed`` int32 [masks, ceil(vocab / 32)],
+    bit v % 32 of word v // 32 allows token v; row r has mask
+    ``allowed_rows``[r] (int32 [rows]; out of range: no mask; None: mask r).
+
+    A token seen before has x / repetition (x > 0) or x * repetition, less
+    frequency * count and presence; then the biases are added; tokens that are
+    not allowed get -inf (a row whose mask allows nothing is all -inf).  Returns
+    ``out`` (may be ``logits``; default a new tensor of logits' dtype)."""
+    _gpu(logits, "logits")
+    device = logits.device
+    if logits.dim() != 2:
+        raise RuntimeError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = (int(v) for v in logits.shape)
+    xs = _rows(logits, "logits", vocab)
+    _same_device(device, history=history, history_len=history_len, prompt_len=prompt_len, repetition=repetition,
+                 presence=presence, frequency=frequency, bias_ids=bias_ids, bias=bias, allowed=allowed,
+                 allowed_rows=allowed_rows, tokens=tokens, out=out)
+    if cu_nodes is not None:
+        if parents is None or tokens is None:
+            raise RuntimeError("trees need parents and tokens")
+        n = _trees(cu_nodes, parents, max_nodes, rows, device)
+        _int64(tokens, "tokens", rows, device)
+    else:
+        if parents is not None or tokens is not None:
+            raise RuntimeError("parents and tokens belong to trees: cu_nodes is missing")
+        n = rows
+    hist_stride = hist_max = 0
+    if history is not None:
+        if history.dtype != torch.int64 or history.dim() != 2 or int(history.size(0)) != n or (
+                history.size(1) > 1 and history.stride(1) != 1):
+            raise RuntimeError(f"history must be int64 [{n}, L] with dense rows")
+        if history_len is None:
+            raise RuntimeError("history needs history_len")
+        hist_max = int(history.size(1))
+        hist_stride = int(history.stride(0)) if n > 1 else hist_max
+    elif history_len is not None or prompt_len is not None:
+        raise RuntimeError("history_len and prompt_len belong to history")
+    for t, name in ((history_len, "history_len"), (prompt_len, "prompt_len")):
+        if _int32(t, name, device) is not None and int(t.numel()) != n:
+            raise RuntimeError(f"{name} must hold {n} entries")
+    for t, name in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or int(t.numel()) != n):
+            raise RuntimeError(f"{name} must be contiguous fp32 of {n} entries")
+    if (bias_ids is None) != (bias is None):
+        raise RuntimeError("bias_ids and bias go together")
+    n_bias = 0
+    if bias is not None:
+        n_bias = int(bias.size(1)) if bias.dim() == 2 else -1
+        if (bias.dtype != torch.float32 or bias_ids.dtype != torch.int64 or tuple(bias.shape) != (n, n_bias)
+                or tuple(bias_ids.shape) != (n, n_bias) or not bias.is_contiguous() or not bias_ids.is_contiguous()):
+            raise RuntimeError(f"bias_ids and bias must be contiguous int64 and fp32 [{n}, M]")
+    n_masks = 0
+    if allowed is not None:
+        n_masks = int(allowed.size(0)) if allowed.dim() == 2 else -1
+        if allowed.dtype != torch.int32 or tuple(allowed.shape) != (n_masks, -(-vocab // 32)) or not allowed.is_contiguous():
+            raise RuntimeError(f"allowed must be contiguous int32 [masks, {-(-vocab // 32)}]")
+        if allowed_rows is None and n_masks != rows:
+            raise RuntimeError(f"allowed must hold a mask for each of {rows} rows, or allowed_rows be given")
+        if _int32(allowed_rows, "allowed_rows", device) is not None and int(allowed_rows.numel()) != rows:
+            raise RuntimeError(f"allowed_rows must hold {rows} entries")
+    elif allowed_rows is not None:
+        raise RuntimeError("allowed_rows belongs to allowed")
+    y = out if out is not None else torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+    ys = _rows(y, "out", vocab)
+    _nrows(y, "out", rows)
+    if y.dtype != logits.dtype:
+        raise RuntimeError("out must have logits' dtype")
+    if out is not None and rows and vocab and (y.data_ptr() != logits.data_ptr() or ys != xs):
+        x0, y0, e = logits.data_ptr(), y.data_ptr(), logits.element_size()
+        if x0 < y0 + ((rows - 1) * ys + vocab) * e and y0 < x0 + ((rows - 1) * xs + vocab) * e:
+            raise RuntimeError("out must be logits itself or not overlap it")
+    with _on(device):
+        rc = nat.lib().sophia_adjust_logits(
+            nat.ptr(logits), xs, nat.ptr(y), ys, nat.dtype_code(logits.dtype), rows, vocab, nat.ptr(history), hist_stride,
+            nat.ptr(history_len), nat.ptr(prompt_len), hist_max, nat.ptr(repetition), nat.ptr(presence),
+            nat.ptr(frequency), nat.ptr(bias_ids), nat.ptr(bias), n_bias, nat.ptr(allowed), n_masks,
+            nat.ptr(allowed_rows), nat.ptr(cu_nodes), nat.ptr(parents), nat.ptr(tokens), n, int(max_nodes),
+            nat.stream_handle(device))
+    nat.check(rc, "sophia_adjust_logits")
+    return y
+
+
+def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tensor, parents: torch.Tensor, *,
+                max_nodes: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The greedy choice at every node of the trees, and the walk along the
+    drafted tokens that agree with it (sophia_tree_accept).
+
+    logits: [rows, vocab] (bf16 or fp32, any row stride) at each node; tokens:
+    int64 [rows]; cu_nodes, parents, max_nodes: as in ``mla_tree_attn``.  A path
+    starts at node 0 of its tree (the token that was known already) and goes on to
+    the first child whose token is its parent's choice.  Returns (path int32 [N,
+    max_nodes], -1 behind its end; n_path int32 [N]; next_token int64 [N], the
+    choice at the path's end; chosen int64 [rows], the lowest index of each row's
+    greatest logit, NaN never, and of rows without a value above -inf 0).  A tree
+    without nodes has an empty path and next_token -1.  To sample instead of choosing, add Gumbel noise to the logits."""
+    _gpu(logits, "logits")
+    device = logits.device
+    if logits.dim() != 2 or int(logits.size(1)) < 1:
+        raise RuntimeError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = (int(v) for v in logits.shape)
+    xs = _rows(logits, "logits", vocab)
+    _same_device(device, tokens=tokens)
+    n = _trees(cu_nodes, parents, max_nodes, rows, device)
+    _int64(tokens, "tokens", rows, device)
+    lib = nat.lib()
+    with _on(device):
+        path = torch.empty((n, int(max_nodes)), dtype=torch.int32, device=device)
+        n_path = torch.empty(n, dtype=torch.int32, device=device)
+        next_token = torch.empty(n, dtype=torch.int64, device=device)
+        chosen = torch.empty(rows, dtype=torch.int64, device=device)
+        buf, addr, nbytes = _workspace(int(lib.sophia_tree_accept_workspace_size(rows, vocab)), device)
+        rc = lib.sophia_tree_accept(
+            nat.ptr(logits), xs, nat.dtype_code(logits.dtype), rows, vocab, nat.ptr(tokens), nat.ptr(cu_nodes),
+            nat.ptr(parents), n, int(max_nodes), nat.ptr(path), int(max_nodes), nat.ptr(n_path), nat.ptr(next_token),
+            nat.ptr(chosen), addr, nbytes, nat.stream_handle(device))
+    nat.check(rc, "sophia_tree_accept")
+    del buf
+    return path, n_path, next_token, chosen
 
 
 from . import torch_ops  # noqa: E402  (registers the sophia:: custom ops; imports this module)
