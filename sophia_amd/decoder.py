@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import itertools
 import math
+from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
@@ -264,6 +265,46 @@ class SophiaMLA(nn.Module):
         missing = int(k_len) - int(known.size(1))
         return F.pad(known, (0, missing), value=True) if missing > 0 else known
 
+    def _project(self, x: torch.Tensor):
+        """q_down, kv_down and output_gate of x [n, dim] in one GEMM: views
+        (q latents, kv latents, gate logits), before the norms."""
+        y = ops.linear(x, self._input_weight(x.dtype))
+        a, b = self.q_rank, self.q_rank + self.kv_rank
+        return y[:, :a], y[:, a:b], y[:, b:]
+
+    def _norms_kernel(self, q_lat: torch.Tensor) -> bool:
+        """Whether ``ops.mla_latent_norms`` takes the projected rows."""
+        r = self.kv_rank
+        return (self.q_rank % 8 == 0 and r % 8 == 0 and self.q_rank + r <= 512 and int(q_lat.stride(0)) % 8 == 0
+                and q_lat.dtype in (torch.float32, torch.bfloat16))
+
+    def _heads_kernel(self, q: torch.Tensor) -> bool:
+        return ops.head_linear_takes(q, self.k_up.weight, self.v_up.weight)
+
+    # The per-head products on the head kernel where it takes them, else batched
+    # GEMMs.  It reads both weights as they lie: an edit of them in place, by
+    # whatever means, is seen by the next step and by replays.
+    def _latent_queries(self, q: torch.Tensor, heads_kernel: bool) -> torch.Tensor:
+        """W_k,h^T q of rows q [n, heads, head_dim]: [n, heads, kv_rank]."""
+        w = self.k_up.weight.view(self.num_heads, self.head_dim, self.kv_rank)
+        if heads_kernel:
+            return ops.head_linear(q, w, weight_kn=True).contiguous()
+        return torch.bmm(q.transpose(0, 1).contiguous(), w.to(q.dtype)).transpose(0, 1).contiguous()
+
+    def _latent_values(self, ctx: torch.Tensor, heads_kernel: bool, out: torch.Tensor,
+                       gate: torch.Tensor | None = None) -> bool:
+        """W_v,h ctx of rows ctx [n, heads, kv_rank] into out [n, heads,
+        head_dim]; with ``gate``, the output gate on the products as they are
+        formed where that can be.  Returns whether it was."""
+        h, d, r = self.num_heads, self.head_dim, self.kv_rank
+        if heads_kernel:
+            own = (gate is not None and gate.dtype == out.dtype and gate.stride(0) % 4 == 0
+                   and gate.data_ptr() % 8 == 0 and ops._values_only(gate))
+            ops.head_linear(ctx, self.v_up.weight.view(h, d, r), out=out, gate=gate.unflatten(1, (h, d)) if own else None)
+            return own
+        out.copy_(torch.bmm(ctx.transpose(0, 1).contiguous(), self._v_up_t(out.dtype)).transpose(0, 1))
+        return False
+
     def forward_mixed(self, x: torch.Tensor, step: dict) -> torch.Tensor:
         """Packed continuous-batching step (``step`` from Transformer.forward_step).
 
@@ -292,11 +333,9 @@ class SophiaMLA(nn.Module):
         cache = self.latent_cache
         # q_down, kv_down and output_gate in one GEMM; q_norm, kv_norm and the
         # latent-cache writes of every row in one kernel
-        y = ops.linear(x, self._input_weight(x.dtype))
-        q_lat, latent, gate = y[:, :self.q_rank], y[:, self.q_rank:self.q_rank + r], y[:, self.q_rank + r:]
+        q_lat, latent, gate = self._project(x)
         rect = npre > 0 and bool(step["rectangular"])
-        if (self.q_rank % 8 == 0 and r % 8 == 0 and self.q_rank + r <= 512 and int(y.stride(0)) % 8 == 0
-                and x.dtype in (torch.float32, torch.bfloat16)):
+        if self._norms_kernel(q_lat):
             ops.mla_latent_norms(
                 q_lat, latent, self.q_norm.weight, self.q_norm.eps, self.kv_norm.weight, self.kv_norm.eps,
                 latent_cache=cache, n_prefill=npre,
@@ -334,30 +373,36 @@ class SophiaMLA(nn.Module):
             self._causal(q[:npre], k, v, step["cu_prefill"], int(step["max_prefill_len"]), out[:npre],
                          cu_k=cu_k, cu_host=step["cu_prefill_host"], cu_k_host=cu_k_host)
         if nd > 0:
-            # the per-head products on the head kernel where it takes them, else
-            # batched GEMMs.  It reads both weights as they lie: an edit of them
-            # in place, by whatever means, is seen by the next step and by replays.
-            w_k, w_v = self.k_up.weight, self.v_up.weight
-            heads_kernel = ops.head_linear_takes(q, w_k, w_v)
-            if heads_kernel:
-                qa = ops.head_linear(q[npre:], w_k.view(h, d, r), weight_kn=True)           # [D, h, r]
-            else:
-                qa = torch.bmm(q[npre:].transpose(0, 1).contiguous(),
-                               w_k.view(h, d, r).to(x.dtype)).transpose(0, 1)               # [D, h, r]
+            heads_kernel = self._heads_kernel(q)
+            qa = self._latent_queries(q[npre:], heads_kernel)
             # softmax over cached latents 0..pos and their weighted sum, one kernel
-            ctx = ops.mla_decode_attn(qa.contiguous(), cache, step["decode_slots"], step["decode_pos"],
+            ctx = ops.mla_decode_attn(qa, cache, step["decode_slots"], step["decode_pos"],
                                       d ** -0.5, max_len=int(step["max_decode_len"]))   # [D, h, r]
-            if heads_kernel:
-                # decode rows alone: the output gate on the products as they are formed
-                own = npre == 0 and gate.dtype == x.dtype and gate.stride(0) % 4 == 0 and gate.data_ptr() % 8 == 0 and ops._values_only(gate)
-                ops.head_linear(ctx, w_v.view(h, d, r), out=out[npre:],
-                                gate=gate.unflatten(1, (h, d)) if own else None)
-                if own:
-                    return self.o_proj(out.view(n, self.inner_dim))
-            else:
-                o = torch.bmm(ctx.transpose(0, 1).contiguous(), self._v_up_t(x.dtype))
-                out[npre:] = o.transpose(0, 1)
+            if self._latent_values(ctx, heads_kernel, out[npre:], gate if npre == 0 else None):
+                return self.o_proj(out.view(n, self.inner_dim))
         return self._gate_out(x, out, gate)
+
+    def forward_tree(self, x: torch.Tensor, trees: "DraftTrees"):
+        """Nodes x [n, dim] of trees of drafted tokens: each attends to its
+        sequence's cached latents and to those of its ancestors and itself, in
+        latent space (``ops.mla_tree_attn``).  The cache is only read.  Returns
+        (output [n, dim], the nodes' latents [n, kv_rank] for a commit)."""
+        n, h, d = int(x.size(0)), self.num_heads, self.head_dim
+        q_lat, latent, gate = self._project(x)
+        if self._norms_kernel(q_lat):
+            ops.mla_latent_norms(q_lat, latent, self.q_norm.weight, self.q_norm.eps, self.kv_norm.weight,
+                                 self.kv_norm.eps)
+        else:
+            q_lat, latent, gate = self.q_norm(q_lat), self.kv_norm(latent), gate.contiguous()
+        q = self.q_up(q_lat).view(n, h, d)
+        heads_kernel = self._heads_kernel(q)
+        ctx = ops.mla_tree_attn(self._latent_queries(q, heads_kernel), latent, self.latent_cache, trees.cu_nodes,
+                                trees.parents, trees.slots, trees.cached, d ** -0.5, max_nodes=trees.max_nodes,
+                                max_len=trees.max_len)
+        out = torch.empty((n, h, d), dtype=x.dtype, device=x.device)
+        if self._latent_values(ctx, heads_kernel, out, gate):
+            return self.o_proj(out.view(n, self.inner_dim)), latent
+        return self._gate_out(x, out, gate), latent
 
 
 class FeedForward(nn.Module):
@@ -521,6 +566,49 @@ class SophiaBlock(nn.Module):
                 step["decode_slots"], prefill_reads_cache=step["reads_cache"],
                 cu_prefill_host=step["cu_prefill_host"])
         return self._mix(partial_block, completed_blocks, attn, pending, defer)
+
+    def forward_tree(self, partial_block, completed_blocks, trees: "DraftTrees", kept: list, *, pending=None,
+                     defer: bool = False):
+        """The nodes of trees of drafted tokens; what a commit needs of this
+        layer is appended to ``kept``."""
+        def attn(y):
+            out, keep = self.attn.forward_tree(y, trees)
+            kept.append(keep)
+            return out
+        return self._mix(partial_block, completed_blocks, attn, pending, defer)
+
+
+@dataclass
+class DraftTrees:
+    """Trees of drafted tokens, one for each of N running sequences, as packed
+    rows on the device (``runtime.pack_trees`` lays them out).
+
+    The nodes of tree s are rows cu_nodes[s] .. cu_nodes[s + 1): token
+    ``token_ids`` [rows] int64, parent ``parents`` [rows] int32 as an index into
+    the tree (before the node; -1: a root).  Node 0 is the sequence's last known
+    token, which is in no cache yet, the others are drafted continuations.
+    ``slots`` [N] int32 are the (different) cache slots, ``cached`` [N] int64
+    the tokens in them.  ``max_nodes`` (at most 64) bounds the nodes of a tree,
+    ``max_len`` bounds ``cached``: host ints."""
+
+    token_ids: torch.Tensor
+    cu_nodes: torch.Tensor
+    parents: torch.Tensor
+    slots: torch.Tensor
+    cached: torch.Tensor
+    max_nodes: int
+    max_len: int
+
+
+@dataclass
+class DraftStep:
+    """What ``Transformer.forward_tree`` computed: logits of every node, and of
+    every layer what ``commit_tree`` writes into its caches."""
+
+    trees: DraftTrees
+    logits: torch.Tensor
+    kept: list
+    committed: bool = False
 
 
 def init_weights(model: nn.Module, args: ModelArgs) -> None:
@@ -832,6 +920,50 @@ class Transformer(nn.Module):
         return self.output(self._final_mix(hidden[last], completed[last],
                                            None if pending is None else pending[last]))
 
+    @torch.no_grad()
+    def forward_tree(self, trees: DraftTrees) -> DraftStep:
+        """One step over the nodes of trees of drafted tokens, which the
+        reference cannot express (one token per sequence after the prompt,
+        transformer.py:146-160): every node sees its sequence's caches and its
+        own path through the tree, and the caches are left as they are.
+        ``DraftStep.logits`` [rows, vocab] are those of a decode step that had
+        taken each node's path token by token; ``commit_tree`` then advances
+        the caches along one path of each tree.  Nothing is read back on the
+        host, so the step is capturable.  Values only (no gradient)."""
+        _require_gpu(trees.token_ids)
+        rows, n = int(trees.token_ids.numel()), int(trees.slots.numel())
+        if rows == 0 or n == 0:
+            raise ValueError("empty step")
+        if int(trees.max_len) < 0 or int(trees.max_len) + int(trees.max_nodes) > int(self.args.max_seq_len):
+            raise ValueError("sequence exceeds max_seq_len")
+        if not self.args.use_cache:
+            raise RuntimeError("forward_tree needs use_cache=True (it reads cache slots)")
+        hidden = self.tok_embeddings(trees.token_ids.reshape(-1))
+        completed = depth_store(hidden, self.args.n_layers, self.args.attn_res_block_size)
+        pending, kept = None, []
+        for layer in self.layers:
+            hidden, completed, pending = layer.forward_tree(hidden, completed, trees, kept, pending=pending, defer=True)
+        return DraftStep(trees, self.output(self._final_mix(hidden, completed, pending)), kept)
+
+    @torch.no_grad()
+    def commit_tree(self, draft: DraftStep, path: torch.Tensor, n_path: torch.Tensor) -> None:
+        """Advances the caches of every layer along one path of each tree of
+        ``draft`` (``ops.tree_commit``: one launch for all layers): ``path``
+        int32 [N, max_path] node indices from a root downwards, ``n_path`` int32
+        [N] how many of them, as ``ops.tree_accept`` returns them.  The caches
+        must be those that ``forward_tree`` read; a step is committed once."""
+        if draft.committed:
+            raise RuntimeError("this drafted step has been committed already")
+        trees, kda, mla = draft.trees, [], []
+        for layer, kept in zip(self.layers, draft.kept):
+            attn = layer.attn
+            if layer.layer_type == "mla":
+                mla.append((kept, attn.latent_cache))
+            else:
+                kda.append((*kept, attn.conv_history(), attn.recurrent_state))
+        ops.tree_commit(path, n_path, trees.cu_nodes, trees.slots, kda=kda, mla=mla, cached=trees.cached)
+        draft.committed = True
+
     def forward_mixed(self, prefill_ids: torch.Tensor, decode_ids: torch.Tensor, *,
                       prefill_slots: torch.Tensor, decode_slots: torch.Tensor,
                       decode_pos: torch.Tensor, max_decode_len: int,
@@ -903,5 +1035,5 @@ class MixedStepGraph:
         return self.logits
 
 
-__all__ = ["AttentionResidualMixer", "FeedForward", "MixedStepGraph", "SophiaBlock",
+__all__ = ["AttentionResidualMixer", "DraftStep", "DraftTrees", "FeedForward", "MixedStepGraph", "SophiaBlock",
            "SophiaMLA", "Transformer", "init_weights"]

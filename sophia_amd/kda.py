@@ -597,6 +597,28 @@ class SophiaKDA(nn.Module):
         return self._output(o, gate_logits, x2.dtype)
 
 
+    def conv_history(self) -> torch.Tensor | None:
+        """``conv_state`` as the kernels take it, [slots, 3 * inner, K - 1] (None
+        when the conv has one tap)."""
+        hist = self.conv_kernel - 1
+        return self.conv_state.view(self.conv_state.size(0), 3 * self.inner_dim, hist) if hist > 0 else None
+
+    def forward_tree(self, x: torch.Tensor, trees):
+        """Nodes x [n, dim] of trees of drafted tokens (``decoder.DraftTrees``):
+        the ShortConv and the recurrence run along every path from the cached
+        history and state of the tree's slot, which are only read
+        (``ops.kda_tree_step``).  Returns (output [n, dim], (tape, pre-conv
+        rows): what a commit needs of the nodes)."""
+        n = int(x.size(0))
+        qkv, dd, beta_logits, gate_logits = self._project(x)
+        decay = self.decay_up(dd).view(n, self.num_heads, self.head_dim)
+        o, tape = ops.kda_tree_step(
+            qkv, self._conv_weight(qkv.dtype), self.conv_history(), decay, beta_logits, self.recurrent_state,
+            trees.cu_nodes, trees.parents, max_nodes=trees.max_nodes, A_log=self.A_log, dt_bias=self.dt_bias,
+            lower_bound=self.lower_bound, state_slots=trees.slots)
+        return self._output(o, gate_logits, x.dtype), (tape, qkv)
+
+
 def set_pad_mask(model: nn.Module, mask: torch.Tensor | None) -> None:
     """attention.py:660-670: hang a [B, T] bool mask (True = real token) on
     every token mixer (KDA and, in the hybrid decoder, MLA), or clear it.

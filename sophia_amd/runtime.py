@@ -12,6 +12,10 @@ advances it and returns the logits with the new state.  The reference runs
 tokens after the first step one position at a time (its model takes T > 1
 only at start_pos 0, runtime_host.py:146-170); here every step is one
 ``forward_step``, whatever its number of tokens.
+
+``pack_trees`` and ``verify_trees`` are greedy decoding with drafted tokens: a
+server proposes a tree of continuations for each running sequence, one step runs
+all of them, and the longest part that the model itself would have said is kept.
 """
 
 from __future__ import annotations
@@ -20,7 +24,8 @@ from dataclasses import dataclass
 
 import torch
 
-from .decoder import Transformer
+from . import ops
+from .decoder import DraftTrees, Transformer
 from .state import RuntimeCacheSnapshot
 
 
@@ -148,4 +153,72 @@ def forward_cached_decode(*, model: Transformer, input_ids: torch.Tensor,
                                      batch_size=bsz, cache_pos=next_pos)
 
 
-__all__ = ["RuntimeCacheState", "SlotAllocator", "forward_cached_decode"]
+def pack_trees(model: Transformer, trees, slots, cached) -> DraftTrees:
+    """``DraftTrees`` on the model's device from host lists: ``trees[s]`` =
+    (tokens, parents) of sequence s, node 0 its last known token (parent -1),
+    each other node after its parent (an index into the tree); ``slots[s]`` its
+    cache slot and ``cached[s]`` the tokens in it."""
+    dev = model.tok_embeddings.weight.device
+    slots, cached = ([int(v) for v in (t.tolist() if isinstance(t, torch.Tensor) else t)] for t in (slots, cached))
+    if not len(trees) == len(slots) == len(cached):
+        raise ValueError("slots and cached need one entry per tree")
+    if len(set(slots)) != len(slots):
+        raise ValueError(f"two trees share a cache slot: {sorted(slots)}")
+    capacity = model.runtime_batch_capacity()
+    if any(not 0 <= s < capacity for s in slots):
+        raise ValueError(f"cache slots must be in [0, {capacity})")
+    tokens, parents, offsets = [], [], [0]
+    for toks, pars in trees:
+        if len(toks) != len(pars) or not 1 <= len(toks) <= ops.TREE_NODES:
+            raise ValueError(f"a tree has 1..{ops.TREE_NODES} nodes, each with a token and a parent")
+        if int(pars[0]) != -1 or any(not 0 <= int(p) < i for i, p in enumerate(pars) if i):
+            raise ValueError("node 0 is the root (parent -1), and every other node comes after its parent")
+        if any(not 0 <= int(t) < int(model.args.vocab_size) for t in toks):
+            raise ValueError("a token is outside the vocabulary")
+        tokens += [int(t) for t in toks]
+        parents += [int(p) for p in pars]
+        offsets.append(len(tokens))
+    if any(c < 0 for c in cached):
+        raise ValueError("cached token counts must be >= 0")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    i64 = lambda v: torch.tensor(v, dtype=torch.int64, device=dev)  # noqa: E731
+    return DraftTrees(i64(tokens), i32(offsets), i32(parents), i32(slots), i64(cached),
+                      max((len(t) for t, _ in trees), default=0), max(cached, default=0))
+
+
+@dataclass
+class Verified:
+    """The outcome of ``verify_trees``, on the device: ``path`` int32 [N,
+    max_nodes] (the kept nodes, -1 behind them), ``n_path`` int32 [N],
+    ``next_token`` int64 [N] (the token after the path: the next tree's node 0),
+    ``cached`` int64 [N] (tokens in the caches now), ``logits`` [rows, vocab] of
+    every node, adjusted."""
+
+    path: torch.Tensor
+    n_path: torch.Tensor
+    next_token: torch.Tensor
+    cached: torch.Tensor
+    logits: torch.Tensor
+
+
+def verify_trees(model: Transformer, trees: DraftTrees, **controls) -> Verified:
+    """One step of greedy decoding with drafted tokens: the nodes of all trees
+    through the model, their logits adjusted (``controls``: the penalties, biases
+    and masks of ``ops.adjust_logits``, per sequence; allowed_rows per node), the
+    drafted tokens walked as far as they are the model's own choices, and the
+    caches advanced along that path.  A sequence gains n_path tokens in its
+    caches and knows the next one: what decoding them one at a time gives, at
+    least one token per step.  Nothing is read back on the host, so the step is
+    capturable."""
+    draft = model.forward_tree(trees)
+    logits = draft.logits
+    if controls:
+        logits = ops.adjust_logits(logits, cu_nodes=trees.cu_nodes, parents=trees.parents, tokens=trees.token_ids,
+                                   max_nodes=trees.max_nodes, out=logits, **controls)
+    path, n_path, next_token, _ = ops.tree_accept(logits, trees.token_ids, trees.cu_nodes, trees.parents,
+                                                  max_nodes=trees.max_nodes)
+    model.commit_tree(draft, path, n_path)
+    return Verified(path, n_path, next_token, trees.cached + n_path, logits)
+
+
+__all__ = ["RuntimeCacheState", "SlotAllocator", "Verified", "forward_cached_decode", "pack_trees", "verify_trees"]
