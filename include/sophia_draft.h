@@ -36,8 +36,8 @@ extern "C" {
  * attention.py:226-258, 330-348 of the reference for each node).  With anc(i) =
  * node i and its ancestors:
  *   q, k, v = silu(conv) of the q | k | v channels, whose earlier samples are the
- *             node's ancestors and then the cached history; q, k normalised (flag),
- *             q times scale
+ *             node's ancestors and then the cached history (rounded to x's type, as the
+ *             decode step rounds it); q, k normalised (flag), q times scale
  *   G_i = sum over anc(i) of the log-decay
  *   u_i = beta_i (v_i - S^T (k_i e^G_i) - sum_{j in anc(i), j != i} (k_i . k_j e^(G_i - G_j)) u_j)
  *   o_i = S^T (q_i e^G_i) + sum_{j in anc(i)} (q_i . k_j e^(G_i - G_j)) u_j

@@ -8,24 +8,29 @@
 //   (I + A) U = beta (V - (K e^G) S),   O = (Q e^G) S + B U.
 // The state is read once and not written; a node's own state is never formed.
 //
-// One 256-thread work-group per (tree, head).  Each wavefront owns 32 value
-// columns, of which its lanes hold S as B operands of v_mfma_f32_16x16x4_f32
-// from the start (issued before anything else); q, k, G, A and B are formed
-// together in LDS, and from the products with S on no wavefront waits for
-// another: an accumulator holds rows 4 (lane / 16) + i of a 16-row tile, which
-// is a B operand whose k index runs 4 (lane / 16) + step, so U goes from one
-// product to the next in registers.
+// One work-group per (tree, head).  A wavefront owns 16 or 32 value columns, of
+// which its lanes hold S as B operands of v_mfma_f32_16x16x4_f32 from the start;
+// every load is issued before the first is waited for, the state last.  q, k, v and
+// the log-decay of a node are then 8 channels in each of 16 threads, in registers;
+// the conv's samples, G along the paths, and the operands of the matrix products go
+// through LDS.  From the products with S on no wavefront waits for another but
+// once: an accumulator holds rows 4 (lane / 16) + i of a 16-row tile, which is a B
+// operand whose k index runs 4 (lane / 16) + step, so U goes from one product to
+// the next in registers.
 //
 // Everything is fp32 (the matrix products too): u enters the cached state with
 // the accepted path, and the decode step that the state otherwise comes from
-// is fp32 as well.  The exponents e^(G_i - G_j) are formed per pair, on the
-// vector unit, for ancestors alone: their arguments are never positive, however
-// long the path and strong the decay, where a factored form e^(G_i) e^(-G_j)
-// overflows past 17 steps of the lower bound -5.
+// is fp32 as well.  A and B are (K e^G) (K e^-G)^T and (Q e^G) (K e^-G)^T on MFMAs
+// where |G| stays below kFactored; beyond it e^-G would leave the range of fp32, and
+// they are formed per pair of a node and an ancestor on the vector unit, from
+// e^(G_i - G_j), whose argument is never positive.
 //
 // A node with an input that is not finite would reach its siblings through the
 // products (0 times infinity): its rows enter them as zeros, and what lies on a
 // path with it ends as NaN.
+#include <cstdlib>
+#include <type_traits>
+
 #include "common.hpp"
 #include "tree.hpp"
 
@@ -63,85 +68,82 @@ struct TreeStepArgs {
   float *tape;
 };
 
-template <int N>
-struct alignas(4 * N) Floats {
-  float v[N];
+// |G| up to which A and B are formed from e^G and e^-G: e^-60 times a component of
+// k stays a normal fp32 number down to 1.3e-12.
+constexpr float kFactored = 60.f;
+
+// Eight consecutive elements as they lie, and as floats.
+template <int DT>
+struct Raw8 {
+  u4 w[DT == SOPHIA_DTYPE_BF16 ? 1 : 2];
+};
+template <int DT>
+__device__ __forceinline__ Raw8<DT> raw8(const void *p) {
+  Raw8<DT> r;
+  r.w[0] = static_cast<const u4 *>(p)[0];
+  if constexpr (DT == SOPHIA_DTYPE_F32) r.w[1] = static_cast<const u4 *>(p)[1];
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void to_float(const Raw8<DT> &r, float (&f)[8]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    if constexpr (DT == SOPHIA_DTYPE_BF16)
+      f[c] = __uint_as_float(c & 1 ? r.w[0][c >> 1] & 0xffff0000u : r.w[0][c >> 1] << 16);
+    else
+      f[c] = __uint_as_float(r.w[c >> 2][c & 3]);
+  }
+}
+__device__ __forceinline__ void read8(const float *p, float (&f)[8]) { to_float(raw8<SOPHIA_DTYPE_F32>(p), f); }
+__device__ __forceinline__ void write8(float *p, const float (&f)[8]) {
+  reinterpret_cast<f4 *>(p)[0] = f4{f[0], f[1], f[2], f[3]};
+  reinterpret_cast<f4 *>(p)[1] = f4{f[4], f[5], f[6], f[7]};
+}
+
+// LDS of the step: first the rows before the conv, then the matrices.
+template <int MT, int DT>
+struct StepLds {
+  static constexpr int T = 16 * MT, LA = T + 4;
+  static constexpr int kRow = 3 * kD + 8;   // elements of a raw row: q | k | v
+  using Elem = typename std::conditional<DT == SOPHIA_DTYPE_BF16, uint16_t, float>::type;
+  struct Conv {
+    float w[4][3 * kD];                     // by the distance of the sample
+    Elem x[3 + T][kRow];                    // the history, oldest first, then the nodes
+  };
+  struct Mat {
+    float q[T][kLd], k[T][kLd], g[T][kLd];
+    float a[T][LA];                         // -A, its diagonal blocks later (I + A)^-1
+    float b[T][LA];
+  };
+  union {
+    Conv conv;
+    Mat mat;
+  };
 };
 
-// N consecutive elements (N * size bytes aligned) as floats.
-template <int DT, int N>
-__device__ __forceinline__ void load_n(const void *base, int64_t idx, float (&r)[N]) {
-  if constexpr (N == 2 && DT == SOPHIA_DTYPE_BF16) {
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(base) + idx);
-    r[0] = __uint_as_float(w << 16);
-    r[1] = __uint_as_float(w & 0xffff0000u);
-  } else if constexpr (N == 2) {
-    const f2 w = *reinterpret_cast<const f2 *>(static_cast<const float *>(base) + idx);
-    r[0] = w.x;
-    r[1] = w.y;
-  } else {
-#pragma unroll
-    for (int c = 0; c < N; c += 4) {
-      const f4 w = load4(base, idx + c, DT);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[c + i] = w[i];
-    }
-  }
-}
-
-// silu(conv) of N consecutive channels (the first is `ch` of the fused q | k | v
-// channels, `col` of its own part `x`) at a node.  Predecessors are counted from
-// the oldest history sample: 0, 1, 2, then node i as 3 + i.
-template <int DT, int N>
-__device__ __forceinline__ void conv_node(const TreeStepArgs &a, const void *x, int64_t base, int64_t col, int64_t ch,
-                                          const float *hist, const int *par, int node, float (&y)[N]) {
-  float acc[N];
-#pragma unroll
-  for (int c = 0; c < N; ++c) acc[c] = 0.f;
-  int e = node + 3;
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    if (d >= a.taps) break;
-    float s[N];
-    if (e >= 3) {
-      load_n<DT>(x, (base + e - 3) * a.x_stride + col, s);
-      const int p = par[e - 3];
-      e = p < 0 ? 2 : p + 3;
-    } else {
-      const int hist_len = a.taps - 1;   // (e + hist_len - 3 >= 0: the taps reach that far)
-#pragma unroll
-      for (int c = 0; c < N; ++c) s[c] = hist[(ch + c) * hist_len + e + hist_len - 3];
-      --e;
-    }
-#pragma unroll
-    for (int c = 0; c < N; ++c) acc[c] = fmaf(a.conv_w[(ch + c) * a.taps + a.taps - 1 - d], s[c], acc[c]);
-  }
-#pragma unroll
-  for (int c = 0; c < N; ++c) y[c] = acc[c] * sigmoid_f(acc[c]);
-}
-
-// MT: tiles of 16 nodes.
-template <int MT, int DT>
-__global__ __launch_bounds__(256, MT == 1 ? 2 : 1) void kda_tree_step_kernel(TreeStepArgs a) {
-  constexpr int T = 16 * MT, LA = T + 4;
-  __shared__ __align__(16) float s_q[T][kLd], s_k[T][kLd], s_g[T][kLd];
-  __shared__ __align__(16) float s_a[T][LA];   // -A, its diagonal blocks later (I + A)^-1
-  __shared__ __align__(16) float s_b[T][LA];
+// MT: tiles of 16 nodes; NT: threads.
+template <int MT, int NT, int DT>
+__global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2))) void kda_tree_step_kernel(TreeStepArgs a) {
+  using Lds = StepLds<MT, DT>;
+  constexpr int T = Lds::T, NW = NT / 64;
+  constexpr int CW = kD / NW, CE = CW / 16;             // columns of a wavefront, and per lane
+  constexpr int RP = NT / 16, P = (T + RP - 1) / RP;    // nodes at a time, and how often
+  __shared__ __align__(16) Lds lds;
   __shared__ float s_beta[T];
-  __shared__ int s_bad[kTreeNodes];
   __shared__ uint64_t s_path[kTreeNodes];
-  __shared__ int s_up[6][kTreeNodes];          // s_up[0]: parents
+  __shared__ int s_up[6][kTreeNodes];                   // s_up[0]: parents
+  __shared__ int s_bad[kTreeNodes], s_far;
+  auto &mat = lds.mat;
 
   const int h = blockIdx.x, tree = blockIdx.y;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int c16 = lane & 15, grp = lane >> 4;
   int64_t base;
   const int n = tree_nodes(a.trees, tree, base);
-  if (n == 0) return;
   const int slot = a.slots ? a.slots[tree] : tree;
-  const int col2 = 32 * wave + 2 * c16;   // this lane's two value columns
+  if (n == 0) return;
   if (slot < 0 || slot >= a.n_slots) {
-    for (int i = t; i < n * kD; i += 256) {
+    for (int i = t; i < n * kD; i += NT) {
       const int64_t row = base + i / kD;
       store_elem(a.o, row * a.o_stride + static_cast<int64_t>(h) * kD + i % kD, DT, 0.f);
       float *tp = a.tape + (row * a.heads + h) * kTape + i % kD;
@@ -149,63 +151,155 @@ __global__ __launch_bounds__(256, MT == 1 ? 2 : 1) void kda_tree_step_kernel(Tre
     }
     return;
   }
-  // S rows 16 blk + 4 grp + s of the lane's columns: 4 rows of 128 bytes per load.
-  f2 st[kD / 4];
-  const float *S = a.state + (static_cast<int64_t>(slot) * a.heads + h) * kD * kD;
-#pragma unroll
-  for (int i = 0; i < kD / 4; ++i)
-    st[i] = __builtin_nontemporal_load(
-        reinterpret_cast<const f2 *>(S + (16 * (i >> 2) + 4 * grp + (i & 3)) * kD + col2));
 
+  // ---- loads
+  const int64_t inner = static_cast<int64_t>(a.heads) * kD;
+  const int r0 = t >> 4, seg = 8 * (t & 15);            // this thread's nodes r0 + RP p, channels seg .. + 7
+  const int64_t hc = static_cast<int64_t>(h) * kD + seg;
+  constexpr int kEsz = DT == SOPHIA_DTYPE_BF16 ? 2 : 4;
   const int parent = tree_parent(a.trees, base, n, lane);
+  Raw8<DT> raw[P][3];
+  Raw8<SOPHIA_DTYPE_F32> raw_g[P];
+  const bool g16 = a.g_dtype == SOPHIA_DTYPE_BF16;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int64_t row = base + min(r0 + RP * p, n - 1);
+#pragma unroll
+    for (int part = 0; part < 3; ++part)
+      raw[p][part] = raw8<DT>(static_cast<const uint8_t *>(a.x[part]) + (row * a.x_stride + hc) * kEsz);
+    const u4 *gp = reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(a.g) + (row * a.g_stride + hc) * (g16 ? 2 : 4));
+    raw_g[p].w[0] = gp[0];
+    raw_g[p].w[1] = gp[g16 ? 0 : 1];   // (bf16: the same again, no branch around a load)
+  }
+  // Taps by distance and history samples of channels t, t + NT of the head's 384;
+  // those that a shorter conv lacks are zeros.
+  constexpr int kCh = (3 * kD + NT - 1) / NT;
+  float taps[kCh][4], past[kCh][3];
+  const int hist = a.taps - 1;
+#pragma unroll
+  for (int j = 0; j < kCh; ++j) {
+    const int i = min(t + NT * j, 3 * kD - 1);
+    const int64_t ch = (i / kD) * inner + static_cast<int64_t>(h) * kD + i % kD;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) taps[j][d] = d <= hist ? a.conv_w[ch * a.taps + hist - d] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      past[j][e] = e + hist >= 3 ? a.conv_state[(static_cast<int64_t>(slot) * 3 * inner + ch) * hist + e + hist - 3] : 0.f;
+  }
+  const uint32_t raw_beta = load_raw(a.beta, (base + min(t, n - 1)) * a.beta_stride + h, a.beta_dtype);
+  const bool gate = (a.flags & SOPHIA_KDA_GATE_IN_KERNEL) != 0;
+  Raw8<SOPHIA_DTYPE_F32> raw_bias = {};
+  if (gate) raw_bias = raw8<SOPHIA_DTYPE_F32>(a.dt_bias + hc);
+  const float a_log = gate ? a.A_log[h] : 0.f;
+  // S rows 16 blk + 4 grp + s of the lane's columns, the state last: the waits for
+  // the others do not include it.
+  asm volatile("" ::: "memory");
+  using St = typename std::conditional<CE == 2, f2, float>::type;
+  St st[kD / 4];
+  const int col = CW * wave + CE * c16;
+  {
+    const float *S = a.state + (static_cast<int64_t>(slot) * a.heads + h) * kD * kD + col;
+#pragma unroll
+    for (int i = 0; i < kD / 4; ++i)
+      st[i] = __builtin_nontemporal_load(reinterpret_cast<const St *>(S + (16 * (i >> 2) + 4 * grp + (i & 3)) * kD));
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  const auto sval = [&](int i, int e) {
+    if constexpr (CE == 2)
+      return st[i][e];
+    else
+      return st[i];
+  };
+
+  // ---- paths, and the raw rows into LDS
   const uint64_t path = tree_paths(parent, n, lane, [&](int r, int up) {
     if (wave == 0) s_up[r][lane] = up;
   });
-  if (wave == 0) s_path[lane] = path;
   int depth = __popcll(path);
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) depth = max(depth, __shfl_xor(depth, m, 64));
-  for (int i = t; i < T * LA; i += 256) (&s_a[0][0])[i] = (&s_b[0][0])[i] = 0.f;
-  if (t < T) {
-    float b = t < n ? load_elem(a.beta, (base + t) * a.beta_stride + h, a.beta_dtype) : 0.f;
-    if (a.flags & SOPHIA_KDA_BETA_SIGMOID) b = sigmoid_f(b);
-    s_beta[t] = t < n && is_finite(b) ? b : 0.f;
-    s_bad[t] = !is_finite(b);
-  }
-  __syncthreads();
-
-  // q, k and the log-decay: 16 nodes at a time, 8 channels per thread.
-  const int64_t inner = static_cast<int64_t>(a.heads) * kD;
-  const float *hist = a.conv_state + static_cast<int64_t>(slot) * 3 * inner * (a.taps - 1);
-  const int seg = 8 * (t & 15);
-  const int64_t hc = static_cast<int64_t>(h) * kD + seg;
+  depth = __builtin_amdgcn_readfirstlane(depth);
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int node = 16 * m + (t >> 4);
-    float q[8], k[8], g[8];
-    if (node < n) {
-      conv_node<DT>(a, a.x[0], base, hc, hc, hist, s_up[0], node, q);
-      conv_node<DT>(a, a.x[1], base, hc, inner + hc, hist, s_up[0], node, k);
-      if (a.g_dtype == SOPHIA_DTYPE_BF16)
-        load_n<SOPHIA_DTYPE_BF16>(a.g, (base + node) * a.g_stride + hc, g);
-      else
-        load_n<SOPHIA_DTYPE_F32>(a.g, (base + node) * a.g_stride + hc, g);
-      if (a.flags & SOPHIA_KDA_GATE_IN_KERNEL) {
-        const float head_scale = __expf(a.A_log[h]);
+  for (int p = 0; p < P; ++p)
+    if (r0 + RP * p < T)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) g[c] = kda_log_decay(g[c], head_scale, a.dt_bias[hc + c], a.lower_bound);
+      for (int part = 0; part < 3; ++part) {
+        u4 *d = reinterpret_cast<u4 *>(&lds.conv.x[3 + r0 + RP * p][part * kD + seg]);
+        d[0] = raw[p][part].w[0];
+        if constexpr (DT == SOPHIA_DTYPE_F32) d[1] = raw[p][part].w[1];
       }
-    } else {
 #pragma unroll
-      for (int c = 0; c < 8; ++c) q[c] = k[c] = g[c] = 0.f;
+  for (int j = 0; j < kCh; ++j) {
+    const int i = t + NT * j;
+    if (i >= 3 * kD) continue;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) lds.conv.w[d][i] = taps[j][d];
+#pragma unroll
+    for (int e = 0; e < 3; ++e) store_elem(lds.conv.x[e], i, DT, past[j][e]);
+  }
+  if (wave == 0) s_path[lane] = path;
+  if (t < kTreeNodes) {
+    float b = t < n ? raw_to_f32(raw_beta, a.beta_dtype) : 0.f;
+    if (a.flags & SOPHIA_KDA_BETA_SIGMOID) b = sigmoid_f(b);
+    const bool ok = is_finite(b);
+    if (t < T) s_beta[t] = t < n && ok ? b : 0.f;
+    s_bad[t] = !ok;
+  }
+  if (t == 0) s_far = 0;
+  lds_barrier();
+
+  // ---- conv, norms, log-decay: in registers
+  // Predecessors, counted from the oldest history sample: 0, 1, 2, then node i as 3 + i.
+  float qkv[3][P][8], g[P][8], bias[8];
+  to_float(raw_bias, bias);
+  const float head_scale = __expf(a_log);
+  auto &q = qkv[0], &k = qkv[1], &v = qkv[2];
+  int e[P][4];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int node = r0 + RP * p;
+    e[p][0] = 3 + (node < n ? node : 0);
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+      const int at = e[p][d - 1], up = s_up[0][max(at - 3, 0)];
+      e[p][d] = at < 3 ? at - 1 : (up < 0 ? 2 : up + 3);
     }
+  }
+#pragma unroll
+  for (int part = 0; part < 3; ++part) {
+    float w[4][8];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) read8(&lds.conv.w[d][part * kD + seg], w[d]);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      float (&y)[8] = qkv[part][p];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) y[c] = 0.f;
+      if (r0 + RP * p >= n) continue;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        float s[8];
+        to_float(raw8<DT>(&lds.conv.x[e[p][d]][part * kD + seg]), s);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) y[c] = fmaf(w[d][c], s[c], y[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) y[c] *= sigmoid_f(y[c]);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int node = r0 + RP * p;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) g[p][c] = 0.f;
+    if (node >= n) continue;
     float qs = a.scale, ks = 1.f;
     if (a.flags & SOPHIA_KDA_QK_L2NORM) {
       float sq = 0.f, sk = 0.f;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        sq = fmaf(q[c], q[c], sq);
-        sk = fmaf(k[c], k[c], sk);
+        sq = fmaf(q[p][c], q[p][c], sq);
+        sk = fmaf(k[p][c], k[p][c], sk);
       }
       qs = a.scale / fmaxf(sqrtf(row_sum16(sq)), 1e-12f);
       ks = 1.f / fmaxf(sqrtf(row_sum16(sk)), 1e-12f);
@@ -213,180 +307,248 @@ __global__ __launch_bounds__(256, MT == 1 ? 2 : 1) void kda_tree_step_kernel(Tre
     bool ok = true;
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
-      q[c] *= qs;
-      k[c] *= ks;
-      ok &= is_finite(q[c]) && is_finite(k[c]) && is_finite(g[c]);
+      q[p][c] *= qs;
+      k[p][c] *= ks;
+      const uint32_t w = raw_g[p].w[0][c >> 1];
+      const float z = g16 ? __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16) : __uint_as_float(raw_g[p].w[c >> 2][c & 3]);
+      g[p][c] = gate ? kda_log_decay(z, head_scale, bias[c], a.lower_bound) : z;
+      ok &= is_finite(q[p][c]) && is_finite(k[p][c]) && is_finite(v[p][c]) && is_finite(g[p][c]);
     }
     if (((__ballot(!ok) >> (lane & 48)) & 0xffff) != 0) {   // (of the node's 16 threads alike)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) q[c] = k[c] = g[c] = 0.f;
+      for (int c = 0; c < 8; ++c) q[p][c] = k[p][c] = v[p][c] = g[p][c] = 0.f;
       s_bad[node] = 1;
     }
-#pragma unroll
-    for (int c = 0; c < 8; c += 4) {
-      *reinterpret_cast<f4 *>(&s_q[node][seg + c]) = f4{q[c], q[c + 1], q[c + 2], q[c + 3]};
-      *reinterpret_cast<f4 *>(&s_k[node][seg + c]) = f4{k[c], k[c + 1], k[c + 2], k[c + 3]};
-      *reinterpret_cast<f4 *>(&s_g[node][seg + c]) = f4{g[c], g[c + 1], g[c + 2], g[c + 3]};
-    }
   }
-  __syncthreads();
+  lds_barrier();
 
-  uint64_t bad = __ballot(lane < T && s_bad[lane < T ? lane : 0] != 0);
-
-  // G: sums of the log-decay along the paths, by doubling (as many rounds as the
-  // deepest path needs).
-  for (int r = 0; (1 << r) < depth; ++r) {
-    f4 add[MT][2];
+  // ---- G: sums of the log-decay along the paths, by doubling (as many rounds as the
+  // deepest path needs), between two buffers
+  const auto put_g = [&](float (*buf)[kLd]) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int up = s_up[r][16 * m + (t >> 4)];
-      add[m][0] = up < 0 ? f4{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<const f4 *>(&s_g[up][seg]);
-      add[m][1] = up < 0 ? f4{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<const f4 *>(&s_g[up][seg + 4]);
-    }
-    __syncthreads();
+    for (int p = 0; p < P; ++p)
+      if (r0 + RP * p < T) {
+        write8(&buf[r0 + RP * p][seg], g[p]);
+        float top = 0.f;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      *reinterpret_cast<f4 *>(&s_g[16 * m + (t >> 4)][seg]) += add[m][0];
-      *reinterpret_cast<f4 *>(&s_g[16 * m + (t >> 4)][seg + 4]) += add[m][1];
-    }
-    __syncthreads();
-  }
-
-  // A and B: a wavefront takes every fourth node, 16 lanes one of its ancestors.
-  for (int i = wave; i < n; i += 4) {
-    uint64_t left = s_path[i];
-    float qi[8], ki[8], gi[8];
-    load_n<SOPHIA_DTYPE_F32>(&s_q[i][0], 8 * c16, qi);
-    load_n<SOPHIA_DTYPE_F32>(&s_k[i][0], 8 * c16, ki);
-    load_n<SOPHIA_DTYPE_F32>(&s_g[i][0], 8 * c16, gi);
-    while (left) {
-      int j = -1;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int low = left ? __ffsll(static_cast<unsigned long long>(left)) - 1 : -1;
-        if (grp == e) j = low;
-        left &= left - 1;   // (0 stays 0)
+        for (int c = 0; c < 8; ++c) top = fmaxf(top, fabsf(g[p][c]));
+        if (top > kFactored) s_far = 1;
       }
-      float kk = 0.f, qk = 0.f;
-      if (j >= 0) {
-        float kj[8], gj[8];
-        load_n<SOPHIA_DTYPE_F32>(&s_k[j][0], 8 * c16, kj);
-        load_n<SOPHIA_DTYPE_F32>(&s_g[j][0], 8 * c16, gj);
+  };
+  put_g(mat.g);
+  lds_barrier();
+  for (int r = 0; (1 << r) < depth; ++r) {
+    float (*from)[kLd] = r & 1 ? mat.q : mat.g, (*to)[kLd] = r & 1 ? mat.g : mat.q;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const float w = kj[c] * __expf(gi[c] - gj[c]);
-          kk = fmaf(ki[c], w, kk);
-          qk = fmaf(qi[c], w, qk);
+    for (int p = 0; p < P; ++p) {
+      const int up = r0 + RP * p < T ? s_up[r][r0 + RP * p] : -1;
+      if (up >= 0) {
+        float add[8];
+        read8(&from[up][seg], add);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) g[p][c] += add[c];
+      }
+    }
+    put_g(to);
+    lds_barrier();
+  }
+  const uint64_t bad = __ballot(s_bad[lane] != 0);
+  const bool far = s_far != 0;
+  const int mt = MT == 1 ? 1 : (n + 15) >> 4;   // tiles that hold nodes
+
+  // ---- the tape's k and G; the operands
+  const auto operands = [&]() {   // Q e^G, K e^G
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int node = r0 + RP * p;
+      if (node >= T) continue;
+      float qe[8], ke[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float e = __expf(g[p][c]);
+        qe[c] = q[p][c] * e;
+        ke[c] = k[p][c] * e;
+      }
+      write8(&mat.q[node][seg], qe);
+      write8(&mat.k[node][seg], ke);
+    }
+  };
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int node = r0 + RP * p;
+    if (node >= n) continue;
+    const float nan = s_path[node] & bad ? NAN : 0.f;
+    float *tp = a.tape + ((base + node) * a.heads + h) * kTape + seg;
+    float kt[8], gt[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      kt[c] = k[p][c] + nan;
+      gt[c] = g[p][c] + nan;
+    }
+    write8(tp + kD, kt);
+    write8(tp + 2 * kD, gt);
+  }
+  if (!far) {
+    operands();
+#pragma unroll
+    for (int p = 0; p < P; ++p) {   // K e^-G
+      if (r0 + RP * p >= T) continue;
+      float ki[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) ki[c] = k[p][c] * __expf(-g[p][c]);
+      write8(&mat.g[r0 + RP * p][seg], ki);
+    }
+    lds_barrier();
+    // Units (row tile, column tile, A or B), one wavefront each.
+    for (int u = wave; u < mt * (mt + 1); u += NW) {
+      int ti = 0, tj = u >> 1;
+      while (tj > ti) tj -= ++ti;
+      const float (*left)[kLd] = u & 1 ? mat.q : mat.k;
+      f4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int blk = 0; blk < kD / 16; ++blk) {
+        const f4 l = *reinterpret_cast<const f4 *>(&left[16 * ti + c16][16 * blk + 4 * grp]);
+        const f4 r = *reinterpret_cast<const f4 *>(&mat.g[16 * tj + c16][16 * blk + 4 * grp]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) acc[s & 1] = mfma_f32(l[s], r[s], acc[s & 1]);
+      }
+      const int j = 16 * tj + c16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * ti + 4 * grp + i;
+        const bool on = (s_path[row] >> j) & 1;
+        const float x = acc[0][i] + acc[1][i];
+        if (u & 1)
+          mat.b[row][j] = on ? x : 0.f;
+        else
+          mat.a[row][j] = on && row != j ? -s_beta[row] * x : 0.f;
+      }
+    }
+    lds_barrier();
+  } else {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (r0 + RP * p < T) {
+        write8(&mat.q[r0 + RP * p][seg], q[p]);
+        write8(&mat.k[r0 + RP * p][seg], k[p]);
+        write8(&mat.g[r0 + RP * p][seg], g[p]);
+      }
+    for (int i = t; i < T * Lds::LA; i += NT) (&mat.a[0][0])[i] = (&mat.b[0][0])[i] = 0.f;
+    lds_barrier();
+    // A wavefront takes a node, 16 lanes one of its ancestors.
+    for (int i = wave; i < n; i += NW) {
+      uint64_t left = s_path[i];
+      float qi[8], ki[8], gi[8];
+      read8(&mat.q[i][8 * c16], qi);
+      read8(&mat.k[i][8 * c16], ki);
+      read8(&mat.g[i][8 * c16], gi);
+      while (left) {
+        int j = -1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int low = left ? __ffsll(static_cast<unsigned long long>(left)) - 1 : -1;
+          if (grp == e) j = low;
+          left &= left - 1;   // (0 stays 0)
+        }
+        float kk = 0.f, qk = 0.f;
+        if (j >= 0) {
+          float kj[8], gj[8];
+          read8(&mat.k[j][8 * c16], kj);
+          read8(&mat.g[j][8 * c16], gj);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float w = kj[c] * __expf(gi[c] - gj[c]);
+            kk = fmaf(ki[c], w, kk);
+            qk = fmaf(qi[c], w, qk);
+          }
+        }
+        kk = row_sum16(kk);
+        qk = row_sum16(qk);
+        if (j >= 0 && c16 == 0) {
+          mat.b[i][j] = qk;
+          if (j != i) mat.a[i][j] = -s_beta[i] * kk;
         }
       }
-      kk = row_sum16(kk);
-      qk = row_sum16(qk);
-      if (j >= 0 && c16 == 0) {
-        s_b[i][j] = qk;
-        if (j != i) s_a[i][j] = -s_beta[i] * kk;
-      }
     }
+    lds_barrier();
+    operands();
+    lds_barrier();
   }
-  __syncthreads();
 
-  // The tape's k and G, and in their place K e^G and Q e^G.  One wavefront also
-  // inverts the unit lower triangular diagonal blocks of I + A, a column per lane.
+  // ---- v to where K e^-G was; one wavefront inverts the unit lower triangular
+  // diagonal blocks of I + A, a column per lane; (K e^G) S and (Q e^G) S
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int node = 16 * m + (t >> 4);
-    float *tp = a.tape + ((base + node) * a.heads + h) * kTape + seg;
-#pragma unroll
-    for (int c = 0; c < 8; c += 4) {
-      f4 *pq = reinterpret_cast<f4 *>(&s_q[node][seg + c]), *pk = reinterpret_cast<f4 *>(&s_k[node][seg + c]);
-      const f4 gv = *reinterpret_cast<const f4 *>(&s_g[node][seg + c]), kv = *pk;
-      if (node < n) {
-        const float nan = s_path[node] & bad ? NAN : 0.f;
-        *reinterpret_cast<f4 *>(tp + kD + c) = kv + nan;
-        *reinterpret_cast<f4 *>(tp + 2 * kD + c) = gv + nan;
-      }
-      f4 e;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = __expf(gv[i]);
-      *pq *= e;
-      *pk = kv * e;
-    }
-  }
-  if (wave == 3 && grp < MT) {
+  for (int p = 0; p < P; ++p)
+    if (r0 + RP * p < T) write8(&mat.g[r0 + RP * p][seg], v[p]);
+  if (wave == NW - 1 && grp < MT) {
     float inv[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float x = i == c16 ? 1.f : 0.f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) x = fmaf(s_a[16 * grp + i][16 * grp + j], inv[j], x);
+      for (int j = 0; j < i; ++j) x = fmaf(mat.a[16 * grp + i][16 * grp + j], inv[j], x);
       inv[i] = x;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s_a[16 * grp + i][16 * grp + c16] = inv[i];
+    for (int i = 0; i < 16; ++i) mat.a[16 * grp + i][16 * grp + c16] = inv[i];
   }
-  __syncthreads();
-
-  // (K e^G) S and (Q e^G) S for this wavefront's columns.
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  f4 u[MT][2], o[MT][2];
+  f4 u[MT][CE], o[MT][CE];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) u[m][0] = u[m][1] = o[m][0] = o[m][1] = zero;
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int e = 0; e < CE; ++e) u[m][e] = o[m][e] = zero;
 #pragma unroll
   for (int blk = 0; blk < kD / 16; ++blk)
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const f4 ak = *reinterpret_cast<const f4 *>(&s_k[16 * m + c16][16 * blk + 4 * grp]);
-      const f4 aq = *reinterpret_cast<const f4 *>(&s_q[16 * m + c16][16 * blk + 4 * grp]);
+      if (m >= mt) break;
+      const f4 ak = *reinterpret_cast<const f4 *>(&mat.k[16 * m + c16][16 * blk + 4 * grp]);
+      const f4 aq = *reinterpret_cast<const f4 *>(&mat.q[16 * m + c16][16 * blk + 4 * grp]);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          u[m][e] = mfma_f32(ak[s], st[4 * blk + s][e], u[m][e]);
-          o[m][e] = mfma_f32(aq[s], st[4 * blk + s][e], o[m][e]);
+        for (int e = 0; e < CE; ++e) {
+          u[m][e] = mfma_f32(ak[s], sval(4 * blk + s, e), u[m][e]);
+          o[m][e] = mfma_f32(aq[s], sval(4 * blk + s, e), o[m][e]);
         }
     }
+  lds_barrier();
 
-  // Block forward substitution, and the outputs.
-  const int64_t vc = static_cast<int64_t>(h) * kD + col2;
+  // ---- block forward substitution, and the outputs
+  const int64_t vc = static_cast<int64_t>(h) * kD + col;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    f4 rhs[2];
+    if (m >= mt) break;
+    f4 rhs[CE];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int node = 16 * m + 4 * grp + i;
-      float v[2] = {0.f, 0.f};
-      if (node < n) conv_node<DT>(a, a.x[2], base, vc, 2 * inner + vc, hist, s_up[0], node, v);
-      const bool ok = is_finite(v[0]) && is_finite(v[1]);
-      const uint64_t rows = __ballot(!ok);
-      if (rows) {   // (of this wavefront's columns)
-        if (!ok) v[0] = v[1] = 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if ((rows >> (16 * r)) & 0xffff) bad |= 1ull << (16 * m + 4 * r + i);
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) rhs[e][i] = s_beta[node] * (v[e] - u[m][e][i]);
+      for (int e = 0; e < CE; ++e) rhs[e][i] = s_beta[node] * (mat.g[node][col + e] - u[m][e][i]);
     }
 #pragma unroll
     for (int p = 0; p < m; ++p) {
-      const f4 l = *reinterpret_cast<const f4 *>(&s_a[16 * m + c16][16 * p + 4 * grp]);
+      const f4 l = *reinterpret_cast<const f4 *>(&mat.a[16 * m + c16][16 * p + 4 * grp]);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) rhs[e] = mfma_f32(l[s], u[p][e][s], rhs[e]);
+        for (int e = 0; e < CE; ++e) rhs[e] = mfma_f32(l[s], u[p][e][s], rhs[e]);
     }
-    const f4 inv = *reinterpret_cast<const f4 *>(&s_a[16 * m + c16][16 * m + 4 * grp]);
-    u[m][0] = u[m][1] = zero;
+    const f4 inv = *reinterpret_cast<const f4 *>(&mat.a[16 * m + c16][16 * m + 4 * grp]);
+#pragma unroll
+    for (int e = 0; e < CE; ++e) u[m][e] = zero;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) u[m][e] = mfma_f32(inv[s], rhs[e][s], u[m][e]);
+      for (int e = 0; e < CE; ++e) u[m][e] = mfma_f32(inv[s], rhs[e][s], u[m][e]);
 #pragma unroll
     for (int p = 0; p <= m; ++p) {
-      const f4 b = *reinterpret_cast<const f4 *>(&s_b[16 * m + c16][16 * p + 4 * grp]);
+      const f4 b = *reinterpret_cast<const f4 *>(&mat.b[16 * m + c16][16 * p + 4 * grp]);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) o[m][e] = mfma_f32(b[s], u[p][e][s], o[m][e]);
+        for (int e = 0; e < CE; ++e) o[m][e] = mfma_f32(b[s], u[p][e][s], o[m][e]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -394,12 +556,18 @@ __global__ __launch_bounds__(256, MT == 1 ? 2 : 1) void kda_tree_step_kernel(Tre
       if (node >= n) continue;
       const int64_t row = base + node;
       const float nan = s_path[node] & bad ? NAN : 0.f;
-      const float o0 = o[m][0][i] + nan, o1 = o[m][1][i] + nan;
-      if constexpr (DT == SOPHIA_DTYPE_BF16)
-        *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.o) + row * a.o_stride + vc) = pack_bf16x2(o0, o1);
-      else
-        *reinterpret_cast<f2 *>(static_cast<float *>(a.o) + row * a.o_stride + vc) = f2{o0, o1};
-      *reinterpret_cast<f2 *>(a.tape + (row * a.heads + h) * kTape + col2) = f2{u[m][0][i] + nan, u[m][1][i] + nan};
+      const int64_t at = row * a.o_stride + vc;
+      float *tp = a.tape + (row * a.heads + h) * kTape + col;
+      if constexpr (CE == 2) {
+        if constexpr (DT == SOPHIA_DTYPE_BF16)
+          *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.o) + at) = pack_bf16x2(o[m][0][i] + nan, o[m][1][i] + nan);
+        else
+          *reinterpret_cast<f2 *>(static_cast<float *>(a.o) + at) = f2{o[m][0][i] + nan, o[m][1][i] + nan};
+        *reinterpret_cast<f2 *>(tp) = f2{u[m][0][i] + nan, u[m][1][i] + nan};
+      } else {
+        store_elem(a.o, at, DT, o[m][0][i] + nan);
+        *tp = u[m][0][i] + nan;
+      }
     }
   }
 }
@@ -549,17 +717,27 @@ extern "C" int sophia_kda_tree_step(const void *x_q, const void *x_k, const void
                        lower_bound, flags, state, n_slots, slots, num_heads, o, o_row_stride, tape};
   const dim3 grid(num_heads, n_trees);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-#define SOPHIA_TREE_STEP(MT)                                                                              \
-  if (x_dtype == SOPHIA_DTYPE_BF16)                                                                       \
-    hipLaunchKernelGGL((kda_tree_step_kernel<MT, SOPHIA_DTYPE_BF16>), grid, dim3(256), 0, st, a);         \
-  else                                                                                                    \
-    hipLaunchKernelGGL((kda_tree_step_kernel<MT, SOPHIA_DTYPE_F32>), grid, dim3(256), 0, st, a);
+#define SOPHIA_TREE_STEP(MT, NT)                                                                            \
+  if (x_dtype == SOPHIA_DTYPE_BF16)                                                                         \
+    hipLaunchKernelGGL((kda_tree_step_kernel<MT, NT, SOPHIA_DTYPE_BF16>), grid, dim3(NT), 0, st, a);        \
+  else                                                                                                      \
+    hipLaunchKernelGGL((kda_tree_step_kernel<MT, NT, SOPHIA_DTYPE_F32>), grid, dim3(NT), 0, st, a);
+  const bool wide = static_cast<int64_t>(num_heads) * n_trees <= 256;
+  static const bool narrow = getenv("TREE_NARROW") != nullptr;
   if (max_nodes <= 16) {
-    SOPHIA_TREE_STEP(1)
+    if (wide || !narrow) {
+      SOPHIA_TREE_STEP(1, 512)
+    } else {
+      SOPHIA_TREE_STEP(1, 256)
+    }
   } else if (max_nodes <= 32) {
-    SOPHIA_TREE_STEP(2)
+    if (wide || !narrow) {
+      SOPHIA_TREE_STEP(2, 512)
+    } else {
+      SOPHIA_TREE_STEP(2, 256)
+    }
   } else {
-    SOPHIA_TREE_STEP(4)
+    SOPHIA_TREE_STEP(4, 512)
   }
 #undef SOPHIA_TREE_STEP
   return check_launch("kda_tree_step");
