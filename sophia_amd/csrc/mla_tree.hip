@@ -4,13 +4,22 @@
 // sum.  Keys and values are the same rows, so a tile of 64 of them is staged in
 // LDS once and read twice, as K rows and, transposed, as V.
 //
-// A work-group (4 wavefronts) takes 8 nodes of one tree and a range of its keys:
+// A work-group (4 wavefronts) takes some nodes of one tree and a range of its keys:
 // the 16 heads of a node are 16 columns of the matrix products, so a wavefront
-// holds 2 nodes.  The drafted latents are the last tile of the last range, the
-// only one with a mask per column.  A drafted latent that is not finite would
-// reach every node through the products (0 times infinity): it enters them as
-// zeros, and the nodes that do see it end as NaN.  Work-groups of one (tree, range) run on one
-// XCD, whose L2 serves all but the first of them.
+// holds 2 nodes in bf16, 1 in fp32.  Contexts and trees of a batch differ by far, and
+// the host does not know them: every work-group finds its share in the list of all
+// (tree, range, nodes), which it counts itself, a tree per lane.  A tree's ranges are
+// equally long, and all have about the same length.  Neighbours in the list, which
+// read the same keys, run on one XCD, whose L2 serves all but the first of them.  A
+// tree of one range writes its result at once, the others partials that a second
+// kernel joins, both in the order in which the lanes hold them.
+//
+// The drafted latents are one more tile of the last range, taken first, the only one
+// with a mask per column.  A drafted latent that is not finite would reach every
+// node through the products (0 times infinity): it enters them as zeros, and the
+// nodes that do see it end as NaN.
+#include <type_traits>
+
 #include "common.hpp"
 #include "tree.hpp"
 
@@ -19,7 +28,8 @@
 namespace sophia {
 namespace {
 
-constexpr int kGroup = 8;        // nodes per work-group
+template <bool F32>
+constexpr int kGroup = F32 ? 4 : 8;   // nodes per work-group
 constexpr int kTile = 64;        // keys per tile (a whole tree)
 static_assert(kTile == kTreeNodes, "the drafted latents are one tile");
 
@@ -37,8 +47,8 @@ struct MlaTreeArgs {
   float scale_log2;
   void *out;
   int64_t out_stride;
-  float *part;             // [rows, splits, 16, R + 4] when splits > 1
-  int heads, splits, groups, n_trees;
+  float *part;             // when splits > 1: kPart<R, F32> floats per (group, range)
+  int heads, splits, split_tiles, n_trees;
 };
 
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -55,35 +65,91 @@ __device__ __forceinline__ int cached_keys(const MlaTreeArgs &a, int tree, int64
   return static_cast<int>(iclamp64(a.cached[tree], 0, a.max_seq));
 }
 
-// Tiles of a range: an even division.
-__device__ __forceinline__ int tiles_per_split(int tiles, int splits) { return (tiles + splits - 1) / splits; }
+// Ranges of a tree with `tiles` tiles.
+__device__ __forceinline__ int ranges(const MlaTreeArgs &a, int tiles) {
+  return min(a.splits, (tiles + a.split_tiles - 1) / a.split_tiles);
+}
 
-// What a work-group does: tree, first node, range; false when there is nothing.
+// What a work-group does.
 struct Work {
-  int tree, node0, split, n, keys, t0, t1;   // tiles [t0, t1); tile keys / 64 rounded up is the drafted one
+  int tree, node0, split, n, keys, t0, t1;   // tiles [t0, t1) of the cached keys
+  bool drafted, whole;                       // the range has the drafted tile too; is the tree's only one
   int64_t base, slot;
 };
+
+// Work-group b's share: item (b % 8) ceil(items / 8) + b / 8 of the list, in which
+// the nodes of a (tree, range) are next to each other.  False behind its end.
+template <bool F32>
 __device__ __forceinline__ bool find_work(const MlaTreeArgs &a, Work &w) {
-  // unit (tree, range) u: work-groups 8 (groups (u / 8) + group) + u % 8
-  const int b = blockIdx.x, r = b >> 3;
-  const int unit = (r / a.groups) * 8 + (b & 7);
-  if (unit >= a.n_trees * a.splits) return false;
-  w.tree = unit / a.splits;
-  w.split = unit % a.splits;
-  w.node0 = (r % a.groups) * kGroup;
-  w.n = tree_nodes(a.trees, w.tree, w.base);
-  if (w.node0 >= w.n) return false;
-  w.keys = cached_keys(a, w.tree, w.slot);
+  const int lane = threadIdx.x & 63;
+  // The tree of this lane: its nodes, keys and ranges, and the items up to it.
+  int64_t base = 0, slot = 0;
+  int n = 0, keys = 0, used = 0, mine = 0, sum = 0;
+  const auto look = [&](int tree) {
+    mine = 0;
+    if (tree < a.n_trees) {
+      keys = cached_keys(a, tree, slot);
+      n = tree_nodes(a.trees, tree, base);
+      used = keys < 0 ? 1 : ranges(a, (keys + kTile - 1) / kTile + 1);
+      mine = used * ((n + kGroup<F32> - 1) / kGroup<F32>);
+    }
+    sum = wave_scan(mine);
+    return __builtin_amdgcn_readlane(sum, 63);
+  };
+  int all = look(lane), items = all;
+  for (int t0 = 64; t0 < a.n_trees; t0 += 64) items += look(t0 + lane);
+  const int share = (items + 7) >> 3, b = blockIdx.x;
+  int item = (b & 7) * share + (b >> 3);
+  if ((b >> 3) >= share || item >= items) return false;
+  int t0 = 0;
+  if (a.n_trees > 64) all = look(lane);   // (the last trees' otherwise)
+  while (item >= all) {
+    item -= all;
+    t0 += 64;
+    if (t0 >= a.n_trees) return false;
+    all = look(t0 + lane);
+  }
+  const int at = __ffsll(static_cast<unsigned long long>(__ballot(item < sum))) - 1;
+  const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+  const auto of64 = [&](int64_t v) {
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(of(static_cast<int>(v >> 32)))) << 32 |
+                                static_cast<uint32_t>(of(static_cast<int>(v))));
+  };
+  item -= of(sum - mine);
+  w.tree = t0 + at;
+  w.keys = of(keys);
+  w.n = of(n);
+  w.base = of64(base);
+  w.slot = of64(slot);
+  const int ranges_of = of(used);
+  const int groups = (w.n + kGroup<F32> - 1) / kGroup<F32>;
   const int tiles = (w.keys + kTile - 1) / kTile + 1;
-  const int per = tiles_per_split(tiles, a.splits);
-  w.t0 = w.split * per;
-  w.t1 = min(tiles, w.t0 + per);
-  return w.keys < 0 ? w.split == 0 : w.t0 < tiles;
+  w.split = item / groups;
+  w.node0 = (item - w.split * groups) * kGroup<F32>;
+  w.t0 = static_cast<int>(static_cast<int64_t>(tiles) * w.split / ranges_of);
+  w.t1 = static_cast<int>(static_cast<int64_t>(tiles) * (w.split + 1) / ranges_of);
+  w.drafted = w.split + 1 == ranges_of;
+  if (w.drafted) --w.t1;
+  w.whole = ranges_of == 1;
+  return true;
+}
+
+// Partials: of each (group of nodes, range) and wavefront, four ranks of a lane's
+// column at a time, [R / 8 or R / 16 of them][64 lanes], then maximum and sum [64 lanes].
+// Groups are counted over the packed rows: a tree's are (first row) / nodes + tree + 0, 1, ..
+template <int R, bool F32>
+constexpr int kQuads = F32 ? R / 16 : R / 8;
+template <int R, bool F32>
+constexpr int kPart = 4 * 64 * (4 * kQuads<R, F32> + 2);
+template <int R, bool F32>
+__device__ __forceinline__ float *partial(const MlaTreeArgs &a, int64_t base, int tree, int node0, int split, int wave) {
+  const int64_t group = base / kGroup<F32> + tree + node0 / kGroup<F32>;
+  return a.part + (group * a.splits + split) * kPart<R, F32> + wave * (kPart<R, F32> / 4);
 }
 
 template <bool F32>
 __device__ __forceinline__ void zero_rows(const MlaTreeArgs &a, const Work &w, int rank) {
-  const int rows = min(kGroup, w.n - w.node0), width = a.heads * rank;
+  const int rows = min(kGroup<F32>, w.n - w.node0), width = a.heads * rank;
   for (int i = threadIdx.x; i < rows * width; i += 256) {
     const int64_t at = (w.base + w.node0 + i / width) * a.out_stride + i % width;
     if constexpr (F32)
@@ -93,18 +159,23 @@ __device__ __forceinline__ void zero_rows(const MlaTreeArgs &a, const Work &w, i
   }
 }
 
-// Four ranks from `rank` on of (row, head): the result, or a partial with its
-// running maximum and sum behind it.
-template <int R, bool F32>
-__device__ __forceinline__ void put4(const MlaTreeArgs &a, const Work &w, int64_t row, int head, int rank, f4 v, float m,
-                                     float l) {
-  if (a.splits > 1) {
-    float *p = a.part + ((row * a.splits + w.split) * 16 + head) * (R + 4);
-    *reinterpret_cast<f4 *>(p + rank) = v;
-    if (rank == 0) *reinterpret_cast<f2 *>(p + R) = f2{m, l};
-  } else {
-    store4(a.out, row * a.out_stride + static_cast<int64_t>(head) * R + rank,
-           F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, v * (1.0f / l));
+// The lane's column (head `head` of row `row`, `real`) of a range, quad j being four
+// ranks from rank(j) on: the result, or a partial.
+template <int R, bool F32, typename V, typename K>
+__device__ __forceinline__ void put(const MlaTreeArgs &a, const Work &w, int64_t row, int head, bool real, float m, float l,
+                                    V value, K rank) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (!w.whole) {
+    float *p = partial<R, F32>(a, w.base, w.tree, w.node0, w.split, wave);
+#pragma unroll
+    for (int j = 0; j < kQuads<R, F32>; ++j) reinterpret_cast<f4 *>(p)[64 * j + lane] = value(j);
+    reinterpret_cast<f2 *>(p + 256 * kQuads<R, F32>)[lane] = f2{m, l};
+  } else if (real) {
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < kQuads<R, F32>; ++j)
+      store4(a.out, row * a.out_stride + static_cast<int64_t>(head) * R + rank(j),
+             F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, value(j) * inv);
   }
 }
 
@@ -115,23 +186,22 @@ template <int R, bool F32>
 struct Stage {
   static constexpr int kQuads = R / 4, kRows = 256 / kQuads, kSteps = kTile / kRows;
   f4 v[kSteps];
+  // A tile of cached keys: a scalar base and 32-bit offsets.
   __device__ __forceinline__ void load(const MlaTreeArgs &a, const Work &w, int t) {
     const int q = threadIdx.x % kQuads, r0 = threadIdx.x / kQuads;
-    if (kTile * t < w.keys) {
-      const float *p = a.cache + w.slot * a.slot_stride + 4 * q;
+    const float *p = a.cache + (w.slot * a.slot_stride + static_cast<int64_t>(kTile * t) * R);
+    const int last = w.keys - 1 - kTile * t;
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i)
-        v[i] = *reinterpret_cast<const f4 *>(p + static_cast<int64_t>(min(kTile * t + r0 + kRows * i, w.keys - 1)) * R);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i)
-        v[i] = load4(a.latent, (w.base + min(r0 + kRows * i, w.n - 1)) * a.latent_stride + 4 * q,
-                     F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16);
-    }
+    for (int i = 0; i < kSteps; ++i)
+      v[i] = *reinterpret_cast<const f4 *>(p + static_cast<uint32_t>(min(r0 + kRows * i, last) * R + 4 * q));
   }
-  // Of the drafted tile: zeros for what is not finite, and which rows held it.
-  __device__ __forceinline__ void clean(int (&bad)[kTile]) {
+  // The drafted tile: zeros for what is not finite, and which rows held it.
+  __device__ __forceinline__ void load_drafted(const MlaTreeArgs &a, const Work &w, int (&bad)[kTile]) {
     const int q = threadIdx.x % kQuads, r0 = threadIdx.x / kQuads, lane0 = (threadIdx.x & 63) - q;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      v[i] = load4(a.latent, (w.base + min(r0 + kRows * i, w.n - 1)) * a.latent_stride + 4 * q,
+                   F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       bool any = false;
@@ -146,6 +216,16 @@ struct Stage {
     }
   }
 };
+
+// The path of a node, which may differ from lane to lane (0 behind the tree's nodes);
+// `parent` is that of node `lane`.
+__device__ __forceinline__ uint64_t path_of(const Work &w, int parent, int node) {
+  const int lane = threadIdx.x & 63, from = min(node, kTreeNodes - 1);
+  const uint64_t paths = tree_paths(parent, w.n, lane, [](int, int) {});
+  const uint32_t lo = __shfl(static_cast<uint32_t>(paths), from, 64);
+  const uint32_t hi = __shfl(static_cast<uint32_t>(paths >> 32), from, 64);
+  return node < w.n ? static_cast<uint64_t>(hi) << 32 | lo : 0;
+}
 
 // ---- bf16: 32x32x16 MFMAs, as the causal attention uses them ---------------------
 // The cached latents are rounded to bf16 on their way into LDS (a bf16 model wrote
@@ -164,15 +244,19 @@ __device__ __forceinline__ int place(int row, int chunk) {
 template <int R>
 __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTreeArgs a) {
   constexpr int KS = R / 16, DT = R / 32;
-  __shared__ __attribute__((aligned(1024))) uint16_t s_lat[2][kTile * R];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_lat[kTile * R];
   __shared__ int s_bad[kTile];
   Work w;
-  if (!find_work(a, w)) return;
+  if (!find_work<false>(a, w)) return;
   if (w.keys < 0) return zero_rows<false>(a, w, R);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int ln = lane & 31, half = lane >> 5, l16 = lane & 15;
+  const int parent = w.drafted ? tree_parent(a.trees, w.base, w.n, lane) : -1;
   Stage<R, false> next;
-  next.load(a, w, w.t0);
+  if (w.drafted)
+    next.load_drafted(a, w, s_bad);
+  else
+    next.load(a, w, w.t0);
   const int node = w.node0 + 2 * wave + (ln >> 4);   // this lane's column: (node, head)
   const int64_t row = w.base + min(node, w.n - 1);
   bf8 qf[KS];
@@ -182,32 +266,35 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = bits_to_bf8(*reinterpret_cast<const u4 *>(qp + 16 * ks));
   }
-  const uint64_t paths = tree_paths(tree_parent(a.trees, w.base, w.n, lane), w.n, lane, [](int, int) {});
-  const uint64_t path = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(paths >> 32), min(node, 63), 64)) << 32 |
-                        __shfl(static_cast<uint32_t>(paths), min(node, 63), 64);
+  const uint64_t path = w.drafted ? path_of(w, parent, node) : 0;
   const bool idle = w.node0 + 2 * wave >= w.n;   // (of the whole wavefront)
 
+  // This lane's places within a tile: K row ln (32 kt rows on: a constant), V rows
+  // 4 half + l16 / 4 (16 kp rows on: a constant; 8 rows on: the chunk's lowest bit turns).
+  int ko[KS], vo[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) ko[ks] = place<R>(ln, 2 * ks + half);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    vo[dt] = place<R>(4 * half + (l16 >> 2), 4 * dt + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1)) + 4 * (l16 & 1);
   f16v ot[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) ot[dt][i] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;   // l_run over this lane's keys alone
-  for (int t = w.t0; t < w.t1; ++t) {
-    uint16_t *lat = s_lat[(t - w.t0) & 1];
-    const bool drafted = kTile * t >= w.keys;
-    if (drafted) next.clean(s_bad);
-    {
-      using St = Stage<R, false>;
-      const int q = tid % St::kQuads, r0 = tid / St::kQuads;
+  const auto stage = [&]() {
+    using St = Stage<R, false>;
+    const int q = tid % St::kQuads, r0 = tid / St::kQuads;
 #pragma unroll
-      for (int i = 0; i < St::kSteps; ++i)
-        *reinterpret_cast<u2 *>(lat + place<R>(r0 + St::kRows * i, q >> 1) + 4 * (q & 1)) =
-            u2{pack_bf16x2(next.v[i].x, next.v[i].y), pack_bf16x2(next.v[i].z, next.v[i].w)};
-    }
-    lds_barrier();   // (the other buffer's reads ended before each wavefront's last barrier)
-    if (t + 1 < w.t1) next.load(a, w, t + 1);
-    if (idle) continue;
+    for (int i = 0; i < St::kSteps; ++i)
+      *reinterpret_cast<u2 *>(s_lat + place<R>(r0 + St::kRows * i, q >> 1) + 4 * (q & 1)) =
+          u2{pack_bf16x2(next.v[i].x, next.v[i].y), pack_bf16x2(next.v[i].z, next.v[i].w)};
+    lds_barrier();
+  };
+  // One tile from LDS, of which this lane's column sees the keys `seen` (`all`: every
+  // key; one copy of this code, as three held more than the registers there are).
+  const auto block = [&](bool all, uint64_t seen) {
     // st[kt][i] = score(key 32 kt + 8 (i / 4) + 4 half + i % 4 of the tile, column ln)
     f16v st[2];
 #pragma unroll
@@ -218,19 +305,22 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
-        st[kt] = mfma32x32(
-            bits_to_bf8(*reinterpret_cast<const u4 *>(lat + place<R>(32 * kt + ln, 2 * ks + half))), qf[ks], st[kt]);
-    if (kTile * (t + 1) > w.keys) {
-      const uint64_t seen = drafted ? path : (1ull << (w.keys - kTile * t)) - 1;
+        st[kt] = mfma32x32(bits_to_bf8(*reinterpret_cast<const u4 *>(s_lat + ko[ks] + 32 * kt * R)), qf[ks], st[kt]);
+    if (!all) {
+      const uint32_t bits[2] = {static_cast<uint32_t>(seen) >> (4 * half), static_cast<uint32_t>(seen >> 32) >> (4 * half)};
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          st[kt][i] = (seen >> (32 * kt + 8 * (i >> 2) + 4 * half + (i & 3))) & 1 ? st[kt][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) st[kt][i] = bits[kt] & (1u << (8 * (i >> 2) + (i & 3))) ? st[kt][i] : -INFINITY;
     }
-    float mx = st[0][0];
+    float top[4];   // (four chains: one of 32 waits for every step of it)
 #pragma unroll
-    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, st[i >> 4][i & 15]);
+    for (int i = 0; i < 4; ++i) {
+      top[i] = st[i >> 1][8 * (i & 1)];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top[i] = fmaxf(top[i], st[i >> 1][8 * (i & 1) + j]);
+    }
+    float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     mx = fmaxf(mx, lane_xor32(mx)) * a.scale_log2;
     if (__any(mx > m_run)) {
       const float m_new = fmaxf(m_run, mx);
@@ -240,16 +330,15 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) ot[dt] *= alpha;
     }
-    float ps = 0.f;
+    float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         st[kt][i] = __builtin_amdgcn_exp2f(fmaf(st[kt][i], a.scale_log2, -m_run));
-        ps += st[kt][i];
+        ps[i & 3] += st[kt][i];
       }
-    l_run += ps;
-    if (drafted && (__ballot(s_bad[lane] != 0) & path)) l_run = NAN;
+    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 #pragma unroll
     for (int kp = 0; kp < 4; ++kp) {   // 16 keys from 16 kp on
       const f16v &sv = st[kp >> 1];
@@ -257,25 +346,34 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 #pragma unroll
       for (int i = 0; i < 4; ++i) pw[i] = pack_bf16x2(sv[8 * (kp & 1) + 2 * i], sv[8 * (kp & 1) + 2 * i + 1]);
       const bf8 pf = bits_to_bf8(pw);
-      const int vr = 16 * kp + 4 * half + (l16 >> 2);
-      const int vc = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const u2 lo = lds_read_tr(lat + place<R>(vr, 4 * dt + vc) + 4 * (l16 & 1));
-        const u2 hi = lds_read_tr(lat + place<R>(vr + 8, 4 * dt + vc) + 4 * (l16 & 1));
+        const u2 lo = lds_read_tr(s_lat + vo[dt] + 16 * kp * R);
+        const u2 hi = lds_read_tr(s_lat + (vo[dt] ^ 8) + (16 * kp + 8) * R);
         ot[dt] = mfma32x32(bits_to_bf8(u4{lo.x, lo.y, hi.x, hi.y}), pf, ot[dt]);
       }
     }
+  };
+  for (int t = w.t0 - (w.drafted ? 1 : 0); t < w.t1; ++t) {
+    stage();
+    if (t + 1 < w.t1) next.load(a, w, t + 1);
+    if (!idle) {
+      const int left = t < w.t0 ? 0 : w.keys - kTile * t;
+      block(left >= kTile, t < w.t0 ? path : (1ull << (left & 63)) - 1);
+    }
+    lds_barrier();
   }
+  if (w.drafted && (__ballot(s_bad[lane] != 0) & path)) l_run = NAN;
   // ot[dt][i] = O[column ln][rank 32 dt + 8 (i / 4) + 4 half + i % 4] before the 1 / l
   l_run += lane_xor32(l_run);
-  if (node >= w.n || l16 >= a.heads) return;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      put4<R, false>(a, w, row, l16, 32 * dt + 8 * i + 4 * half,
-                     f4{ot[dt][4 * i], ot[dt][4 * i + 1], ot[dt][4 * i + 2], ot[dt][4 * i + 3]}, m_run, l_run);
+  put<R, false>(
+      a, w, row, l16, node < w.n && l16 < a.heads, m_run, l_run,
+      [&](int j) {
+        const f16v &v = ot[j >> 2];
+        const int i = 4 * (j & 3);
+        return f4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+      },
+      [&](int j) { return 8 * j + 4 * half; });
 }
 
 // ---- fp32 ----------------------------------------------------------------------
@@ -284,149 +382,157 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 // steps (the k index runs 4 (lane / 16) + step), and the scores' accumulator, keys
 // 4 (lane / 16) + i, is the B operand of the value product in the same order.
 template <int R>
-__global__ __launch_bounds__(256, 1) void mla_tree_f32_kernel(MlaTreeArgs a) {
+__global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(MlaTreeArgs a) {
   constexpr int KB = R / 16, LD = R + 4;
   __shared__ __attribute__((aligned(16))) float s_lat[kTile][LD];
   __shared__ int s_bad[kTile];
   Work w;
-  if (!find_work(a, w)) return;
+  if (!find_work<true>(a, w)) return;
   if (w.keys < 0) return zero_rows<true>(a, w, R);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int l16 = lane & 15, grp = lane >> 4;
+  const int parent = w.drafted ? tree_parent(a.trees, w.base, w.n, lane) : -1;
   Stage<R, true> next;
-  next.load(a, w, w.t0);
-  const uint64_t paths = tree_paths(tree_parent(a.trees, w.base, w.n, lane), w.n, lane, [](int, int) {});
-  f4 qf[2][KB], ot[2][KB];
-  uint64_t path[2];
-  float m_run[2], l_run[2];
+  if (w.drafted)
+    next.load_drafted(a, w, s_bad);
+  else
+    next.load(a, w, w.t0);
+  const int node = w.node0 + wave;   // (the same for the whole wavefront)
+  const int64_t row = w.base + min(node, w.n - 1);
+  f4 qf[KB], ot[KB];
+  const float *qp = static_cast<const float *>(a.qa) + row * a.qa_stride +
+                    static_cast<int64_t>(min(l16, a.heads - 1)) * R + 4 * grp;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int node = min(w.node0 + 2 * wave + e, w.n - 1);
-    const float *qp = static_cast<const float *>(a.qa) + (w.base + node) * a.qa_stride +
-                      static_cast<int64_t>(min(l16, a.heads - 1)) * R + 4 * grp;
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      qf[e][b] = *reinterpret_cast<const f4 *>(qp + 16 * b);
-      ot[e][b] = f4{0.f, 0.f, 0.f, 0.f};
-    }
-    path[e] = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(paths >> 32), node, 64)) << 32 |
-              __shfl(static_cast<uint32_t>(paths), node, 64);
-    m_run[e] = -INFINITY;
-    l_run[e] = 0.f;
+  for (int b = 0; b < KB; ++b) {
+    qf[b] = *reinterpret_cast<const f4 *>(qp + 16 * b);
+    ot[b] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  const bool idle = w.node0 + 2 * wave >= w.n;
-  for (int t = w.t0; t < w.t1; ++t) {
+  const uint64_t path = w.drafted ? path_of(w, parent, node) : 0;
+  float m_run = -INFINITY, l_run = 0.f;   // l_run over this lane's keys alone
+  const auto stage = [&]() {
     using St = Stage<R, true>;
-    if (t > w.t0) lds_barrier();
-    const bool drafted = kTile * t >= w.keys;
-    if (drafted) next.clean(s_bad);
 #pragma unroll
     for (int i = 0; i < St::kSteps; ++i)
       *reinterpret_cast<f4 *>(&s_lat[tid / St::kQuads + St::kRows * i][4 * (tid % St::kQuads)]) = next.v[i];
     lds_barrier();
-    if (t + 1 < w.t1) next.load(a, w, t + 1);
-    if (idle) continue;
-    f4 st[2][4];   // score(key 16 kt + 4 grp + i, head l16 of node e)
+  };
+  const auto block = [&](uint64_t seen) {
+    f4 st[4];   // score(key 16 kt + 4 grp + i, head l16)
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      st[0][kt] = st[1][kt] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int kt = 0; kt < 4; ++kt) st[kt] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
         const f4 k = *reinterpret_cast<const f4 *>(&s_lat[16 * kt + l16][16 * b + 4 * grp]);
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) st[e][kt] = mfma_f32(k[s], qf[e][b][s], st[e][kt]);
+        for (int s = 0; s < 4; ++s) st[kt] = mfma_f32(k[s], qf[b][s], st[kt]);
       }
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      uint64_t seen = ~0ull;
-      if (drafted)
-        seen = path[e];
-      else if (kTile * (t + 1) > w.keys)
-        seen = (1ull << (w.keys - kTile * t)) - 1;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          st[e][kt][i] = (seen >> (16 * kt + 4 * grp + i)) & 1 ? st[e][kt][i] * a.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, st[e][kt][i]);
-        }
-      mx = fmaxf(mx, lane_xor16(mx));
-      mx = fmaxf(mx, lane_xor32(mx));
-      const float m_new = fmaxf(m_run[e], mx);
-      const float alpha = m_run[e] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[e] - m_new);
-      m_run[e] = m_new;
-      float ps = 0.f;
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          st[e][kt][i] = __builtin_amdgcn_exp2f(st[e][kt][i] - m_new);
-          ps += st[e][kt][i];
-        }
-      l_run[e] = l_run[e] * alpha + ps;
-      if (drafted && (__ballot(s_bad[lane] != 0) & path[e])) l_run[e] = NAN;
-#pragma unroll
-      for (int b = 0; b < KB; ++b) ot[e][b] *= alpha;
-    }
+    float mx = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
+      for (int i = 0; i < 4; ++i) {
+        st[kt][i] = (seen >> (16 * kt + 4 * grp + i)) & 1 ? st[kt][i] * a.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, st[kt][i]);
+      }
+    mx = fmaxf(mx, lane_xor16(mx));
+    mx = fmaxf(mx, lane_xor32(mx));
+    const float m_new = fmaxf(m_run, mx);
+    const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+    m_run = m_new;
+    float ps = 0.f;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const float v = s_lat[16 * kt + 4 * grp + s][16 * b + l16];
+    for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) ot[e][b] = mfma_f32(v, st[e][kt][s], ot[e][b]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        st[kt][i] = __builtin_amdgcn_exp2f(st[kt][i] - m_new);
+        ps += st[kt][i];
+      }
+    l_run = l_run * alpha + ps;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) ot[b] *= alpha;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int b = 0; b < KB; ++b) ot[b] = mfma_f32(s_lat[16 * kt + 4 * grp + s][16 * b + l16], st[kt][s], ot[b]);
+  };
+  for (int t = w.t0 - (w.drafted ? 1 : 0); t < w.t1; ++t) {
+    stage();
+    if (t + 1 < w.t1) next.load(a, w, t + 1);
+    if (node < w.n) {
+      const int left = t < w.t0 ? 0 : w.keys - kTile * t;
+      block(t < w.t0 ? path : left >= kTile ? ~0ull : (1ull << left) - 1);
+    }
+    lds_barrier();
   }
-  // ot[e][b][i] = O[head l16 of node e][rank 16 b + 4 grp + i] before the 1 / l
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    float l = l_run[e];
-    l += lane_xor16(l);
-    l += lane_xor32(l);
-    const int node = w.node0 + 2 * wave + e;
-    if (node >= w.n || l16 >= a.heads) continue;
-#pragma unroll
-    for (int b = 0; b < KB; ++b)
-      put4<R, true>(a, w, w.base + node, l16, 16 * b + 4 * grp, ot[e][b], m_run[e], l);
-  }
+  if (w.drafted && (__ballot(s_bad[lane] != 0) & path)) l_run = NAN;
+  // ot[b][i] = O[head l16][rank 16 b + 4 grp + i] before the 1 / l
+  l_run += lane_xor16(l_run);
+  l_run += lane_xor32(l_run);
+  put<R, true>(
+      a, w, row, l16, node < w.n && l16 < a.heads, m_run, l_run, [&](int j) { return ot[j]; },
+      [&](int j) { return 16 * j + 4 * grp; });
 }
 
-// Joins the ranges of a tree's rows: work-group per (node, tree), a thread four
-// ranks of a head.
+// Joins the ranges of a tree: work-groups (group of nodes and an eighth of the
+// quads, tree), a wavefront as in the attention, a thread four ranks at a time.  Eight partials
+// are loaded before the first is used.
+constexpr int kMergeParts = 8;
 template <int R, bool F32>
 __global__ __launch_bounds__(256) void mla_tree_merge_kernel(MlaTreeArgs a) {
+  constexpr int kParts = kQuads<R, F32> < 8 ? kQuads<R, F32> : 8, QW = kQuads<R, F32> / kParts;   // quads per work-group
+  const int tree = blockIdx.y, node0 = static_cast<int>(blockIdx.x / kMergeParts) * kGroup<F32>;
+  if (blockIdx.x % kMergeParts >= kParts) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
   int64_t base, slot;
-  const int n = tree_nodes(a.trees, blockIdx.y, base);
-  if (static_cast<int>(blockIdx.x) >= n) return;
-  const int keys = cached_keys(a, blockIdx.y, slot);
-  if (keys < 0) return;   // (zeros already)
-  const int tiles = (keys + kTile - 1) / kTile + 1;
-  const int per = tiles_per_split(tiles, a.splits);
-  const int used = (tiles + per - 1) / per;
-  const int64_t row = base + blockIdx.x;
-  for (int i = threadIdx.x; i < a.heads * (R / 4); i += 256) {
-    const int h = i / (R / 4), r = 4 * (i % (R / 4));
-    const float *p = a.part + (row * a.splits * 16 + h) * (R + 4);
-    float m = -INFINITY, l = 0.f;
-    f4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < used; ++s, p += 16 * (R + 4)) {
-      const f2 ml = *reinterpret_cast<const f2 *>(p + R);
-      const f4 v = *reinterpret_cast<const f4 *>(p + r);
-      const float m_new = fmaxf(m, ml.x);
-      const float e0 = __builtin_amdgcn_exp2f(m - m_new), e1 = __builtin_amdgcn_exp2f(ml.x - m_new);
-      acc = acc * e0 + v * e1;
-      l = l * e0 + ml.y * e1;
-      m = m_new;
+  const int keys = cached_keys(a, tree, slot);
+  const int n = tree_nodes(a.trees, tree, base);
+  const int used = ranges(a, (keys + kTile - 1) / kTile + 1);
+  const int node = node0 + (F32 ? wave : 2 * wave + ((lane >> 4) & 1));
+  if (node >= n || l16 >= a.heads || keys < 0 || used == 1) return;   // (one range: written already)
+  const float *p = partial<R, F32>(a, base, tree, node0, 0, wave);
+  const int j0 = static_cast<int>(blockIdx.x % kMergeParts) * QW;
+  float m = -INFINITY, l = 0.f;
+  f4 acc[QW];
+#pragma unroll
+  for (int j = 0; j < QW; ++j) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
+  constexpr int kAhead = 8;
+  for (int s0 = 0; s0 < used; s0 += kAhead) {
+    f2 ml[kAhead];
+    f4 v[kAhead][QW];
+    float top = m;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const float *ps = p + static_cast<int64_t>(min(s0 + s, used - 1)) * kPart<R, F32>;   // the last one again, unused
+      ml[s] = reinterpret_cast<const f2 *>(ps + 256 * kQuads<R, F32>)[lane];
+#pragma unroll
+      for (int j = 0; j < QW; ++j) v[s][j] = reinterpret_cast<const f4 *>(ps)[64 * (j0 + j) + lane];
     }
-    store4(a.out, row * a.out_stride + static_cast<int64_t>(h) * R + r, F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16,
-           acc * (1.0f / l));
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) top = fmaxf(top, ml[s].x);
+    const float e0 = __builtin_amdgcn_exp2f(m - top);
+    l *= e0;
+#pragma unroll
+    for (int j = 0; j < QW; ++j) acc[j] *= e0;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+      if (s0 + s < used) {
+        const float e = __builtin_amdgcn_exp2f(ml[s].x - top);
+        l = fmaf(ml[s].y, e, l);
+#pragma unroll
+        for (int j = 0; j < QW; ++j) acc[j] += v[s][j] * e;
+      }
+    m = top;
   }
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int j = 0; j < QW; ++j)
+    store4(a.out, (base + node) * a.out_stride + static_cast<int64_t>(l16) * R + (F32 ? 16 * (j0 + j) + 4 * (lane >> 4)
+                                                                                      : 8 * (j0 + j) + 4 * (lane >> 5)),
+           F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, acc[j] * inv);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -436,23 +542,26 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 using namespace sophia;
 
-extern "C" size_t sophia_mla_tree_workspace_size(int64_t rows, int rank, int splits) {
-  if (rows < 0 || rank <= 0 || splits < 1) return 0;
-  return splits > 1 ? static_cast<size_t>(rows) * splits * 16 * (rank + 4) * sizeof(float) : 0;
+extern "C" size_t sophia_mla_tree_workspace_size(int64_t rows, int n_trees, int rank, int splits) {
+  if (rows < 0 || n_trees < 0 || rank <= 0 || splits < 2) return 0;
+  const size_t bf16 = static_cast<size_t>(rows / kGroup<false> + n_trees + 1) * (rank / 2 + 2);
+  const size_t f32 = static_cast<size_t>(rows / kGroup<true> + n_trees + 1) * (rank / 4 + 2);
+  return (bf16 > f32 ? bf16 : f32) * splits * 4 * 64 * sizeof(float);
 }
 
 extern "C" int sophia_mla_tree_attn(const void *qa, int64_t qa_stride, const void *latent, int64_t latent_stride,
                                     int dtype, const float *cache, int64_t slot_stride, int n_slots, int max_seq,
                                     const int32_t *slots, const int64_t *cached, const int32_t *cu_nodes,
                                     const int32_t *parents, int n_trees, int64_t rows, int max_nodes, float scale,
-                                    void *out, int64_t out_stride, int heads, int rank, int splits, void *workspace,
-                                    size_t workspace_bytes, void *stream) {
+                                    void *out, int64_t out_stride, int heads, int rank, int splits, int split_keys,
+                                    void *workspace, size_t workspace_bytes, void *stream) {
   SOPHIA_REQUIRE(dtype == SOPHIA_DTYPE_F32 || dtype == SOPHIA_DTYPE_BF16, "mla_tree_attn: dtype not supported");
   SOPHIA_REQUIRE(rank == 32 || rank == 64 || rank == 128 || rank == 256,
                  "mla_tree_attn: rank %d not supported (32, 64, 128 or 256)", rank);
   SOPHIA_REQUIRE(heads >= 1 && heads <= 16, "mla_tree_attn: heads must be in [1, 16]");
   SOPHIA_REQUIRE(n_trees >= 0 && n_trees <= 65535 && rows >= 0 && splits >= 1 && splits <= 1024,
                  "mla_tree_attn: n_trees must be 0..65535, rows >= 0 and splits 1..1024");
+  SOPHIA_REQUIRE(split_keys > 0 && split_keys % kTile == 0, "mla_tree_attn: split_keys must be a multiple of %d", kTile);
   SOPHIA_REQUIRE(max_nodes >= 1 && max_nodes <= kTreeNodes, "mla_tree_attn: max_nodes must be in [1, %d]", kTreeNodes);
   SOPHIA_REQUIRE(scale > 0.f, "mla_tree_attn: scale must be > 0");
   SOPHIA_REQUIRE(n_slots >= 0 && max_seq >= 0 && slot_stride >= static_cast<int64_t>(max_seq) * rank,
@@ -466,16 +575,17 @@ extern "C" int sophia_mla_tree_attn(const void *qa, int64_t qa_stride, const voi
   SOPHIA_REQUIRE(aligned16(qa) && aligned16(latent) && aligned16(cache) && aligned16(out),
                  "mla_tree_attn: qa, latent, cache and out must be 16-byte aligned");
   SOPHIA_REQUIRE(splits == 1 || (workspace && aligned16(workspace) &&
-                                 workspace_bytes >= sophia_mla_tree_workspace_size(rows, rank, splits)),
+                                 workspace_bytes >= sophia_mla_tree_workspace_size(rows, n_trees, rank, splits)),
                  "mla_tree_attn: workspace too small");
-  const int groups = (max_nodes + kGroup - 1) / kGroup;
-  const int64_t blocks = (static_cast<int64_t>(n_trees) * splits + 7) / 8 * 8 * groups;
+  const int group = dtype == SOPHIA_DTYPE_F32 ? kGroup<true> : kGroup<false>;
+  const int groups = (max_nodes + group - 1) / group;
+  const int64_t blocks = (static_cast<int64_t>(n_trees) * splits * groups + 7) / 8 * 8;   // the longest list there may be
   SOPHIA_REQUIRE(blocks <= 0x7fffffff, "mla_tree_attn: too many trees and splits");
   const MlaTreeArgs a{{cu_nodes, parents, rows, max_nodes}, qa, qa_stride, latent, latent_stride, cache, slot_stride,
                       max_seq, n_slots, slots, cached, scale * 1.44269504088896341f, out, out_stride,
-                      static_cast<float *>(workspace), heads, splits, groups, n_trees};
+                      static_cast<float *>(workspace), heads, splits, split_keys / kTile, n_trees};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(blocks)), merge(max_nodes, n_trees);
+  const dim3 grid(static_cast<unsigned>(blocks)), merge(kMergeParts * groups, n_trees);
   switch (rank) {
 #define SOPHIA_MLA_TREE(r)                                                                      \
   case r:                                                                                       \

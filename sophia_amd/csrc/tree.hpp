@@ -66,4 +66,19 @@ __device__ __forceinline__ float row_sum16(float v) {
   return v + dpp_rotate<0x121>(v);
 }
 
+// Sum over this lane and those before it, without the LDS crossbar: shifts within
+// the rows of 16 lanes, then each row's last sum on to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xf>(v);   // row_shr:1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);   // row_bcast:15 into rows 1 and 3
+  return dpp_add<0x143, 0xc>(v);   // row_bcast:31 into rows 2 and 3
+}
+
 }  // namespace sophia

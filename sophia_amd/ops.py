@@ -1710,26 +1710,38 @@ def mla_tree_attn(qa: torch.Tensor, latent: torch.Tensor, latent_cache: torch.Te
     _nrows(y, "out", rows)
     if y.dtype != qa.dtype:
         raise RuntimeError("out must have qa's dtype")
+    bound = max_seq if max_len is None else max(0, min(int(max_len), max_seq))
     if splits is None:
-        bound = max_seq if max_len is None else min(int(max_len), max_seq)
-        splits = mla_tree_splits(n, int(max_nodes), bound)
+        splits = mla_tree_splits(n, int(max_nodes), bound, qa.dtype)
+    # whole 64-key tiles, the drafted latents being one more at the end
+    split_keys = max(1, -(-(-(-bound // 64) + 1) // max(int(splits), 1))) * 64
     lib = nat.lib()
     with _on(device):
-        ws_bytes = int(lib.sophia_mla_tree_workspace_size(rows, rank, int(splits)))
+        ws_bytes = int(lib.sophia_mla_tree_workspace_size(rows, n, rank, int(splits)))
         ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
         rc = lib.sophia_mla_tree_attn(
             nat.ptr(qa), qs, nat.ptr(latent), ls, nat.dtype_code(qa.dtype), nat.ptr(latent_cache), slot_stride, n_slots,
             max_seq, nat.ptr(sl), nat.ptr(cached), nat.ptr(cu_nodes), nat.ptr(parents), n, rows, int(max_nodes),
-            float(scale), nat.ptr(y), os_, heads, rank, int(splits), nat.ptr(ws), ws_bytes, nat.stream_handle(device))
+            float(scale), nat.ptr(y), os_, heads, rank, int(splits), split_keys, nat.ptr(ws), ws_bytes, nat.stream_handle(device))
     nat.check(rc, "sophia_mla_tree_attn")
     return y
 
 
-def mla_tree_splits(trees: int, max_nodes: int, max_len: int) -> int:
-    """Key splits of ``mla_tree_attn``: about two work-groups per CU, at least
-    four 64-key tiles each."""
-    groups = max(trees, 1) * -(-max_nodes // 8)
-    return max(1, min(2 * _CUS // groups, -(-max_len // 256), 32))
+def mla_tree_splits(trees: int, max_nodes: int, max_len: int, dtype: torch.dtype) -> int:
+    """Key ranges of ``mla_tree_attn`` at most, the longest context's: of how many
+    64-key tiles one is.  A range costs a work-group about three tiles' time before
+    and after its tiles and a partial of each node in the merge, so long lists of
+    work take 8 (us with the merge, bf16: 32 trees of 24 to 64 nodes after up to
+    4,000 keys 38 with 8, 44 with 6, 67 with 2), and where they do not fill the chip
+    each tile more is latency (one tree after 523 keys 12.4 with 2, 13.5 with 3,
+    16.5 with 8).  An fp32 tile takes three times as long: 2 (5 trees after up to
+    3,000 keys 23 with 2, 27 with 3 and with 1)."""
+    tiles = -(-max_len // 64) + 1
+    work = max(trees, 1) * -(-max_nodes // 8) * tiles   # at the bounds; a ragged batch has about half
+    least = 2 if dtype == torch.float32 else min(8, max(2, work // 2048))
+    # at most 128 ranges for the merge to join one after the other, and no workspace
+    # past what keeps the chip busy
+    return -(-tiles // max(least, -(-work // 8192), -(-tiles // 128)))
 
 
 def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: torch.Tensor | None, g: torch.Tensor,

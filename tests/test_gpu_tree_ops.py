@@ -569,3 +569,17 @@ def test_operators_refuse_wrong_shapes_types_and_layouts():
     refused(ops.tree_accept, k, parents=s["parents"][:2])
     refused(ops.tree_accept, k, logits=x[:, :0])
     refused(ops.tree_accept, k, logits=x.half())
+
+
+def test_tree_attention_of_many_trees():
+    """More trees than a wavefront has lanes, of all sizes, some without nodes, some without slots."""
+    from sophia_amd import ops
+    lens = [(7 * i) % 19 for i in range(150)]
+    tr, qa, latent, cache, slots, cached = _attn_case(lens, [(37 * i) % 200 for i in range(150)], max_seq=200, heads=2, rank=32)
+    slots[70], slots[149] = -1, 500
+    for dtype in (BF, F32):
+        for splits in (1, 4):
+            got = ops.mla_tree_attn(*_dev(qa.to(dtype), latent.to(dtype), cache, tr.cu, tr.par, slots, cached), 0.1,
+                                    max_nodes=18, splits=splits)
+            want, mass, size = ref.attention(tr, qa, latent, cache, slots, cached, 0.1)
+            _within(got, want, _attn_tol(tr, want, mass, size, dtype, 32))

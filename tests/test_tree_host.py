@@ -43,9 +43,9 @@ def _call(nat, name, args, order, **change):
     return rc, nat.last_error()
 
 
-ATTN = "qa qs latent ls dt cache ss slots_n seq slots cached cu par n rows nodes scale out os heads rank splits ws wsb st"
+ATTN = "qa qs latent ls dt cache ss slots_n seq slots cached cu par n rows nodes scale out os heads rank splits sk ws wsb st"
 ATTN_OK = dict(qa=P, qs=2048, latent=P, ls=128, dt=1, cache=P, ss=1024 * 128, slots_n=4, seq=1024, slots=P, cached=P, cu=P,
-               par=P, n=2, rows=9, nodes=5, scale=0.1, out=P, os=2048, heads=16, rank=128, splits=1, ws=None, wsb=0, st=None)
+               par=P, n=2, rows=9, nodes=5, scale=0.1, out=P, os=2048, heads=16, rank=128, splits=1, sk=64, ws=None, wsb=0, st=None)
 
 
 @pytest.mark.parametrize("change,word", [
@@ -55,6 +55,7 @@ ATTN_OK = dict(qa=P, qs=2048, latent=P, ls=128, dt=1, cache=P, ss=1024 * 128, sl
     (dict(ls=127), "strides"), (dict(ls=132), "strides"), (dict(os=100), "strides"), (dict(qa=P + 8), "aligned"),
     (dict(cache=P + 4), "aligned"), (dict(out=P + 2), "aligned"), (dict(cached=None), "NULL"), (dict(par=None), "NULL"),
     (dict(splits=2), "workspace"), (dict(splits=2, ws=P, wsb=16), "workspace"), (dict(splits=0), "splits"),
+    (dict(sk=0), "split_keys"), (dict(sk=96), "split_keys"),
     (dict(n=-1), "n_trees"), (dict(n=70000), "n_trees"), (dict(rows=-1), "rows"), (dict(seq=-1), "slot stride")])
 def test_tree_attention_refuses(nat, change, word):
     rc, msg = _call(nat, "sophia_mla_tree_attn", ATTN_OK, ATTN, **change)
@@ -149,9 +150,10 @@ def test_accept_refuses(nat, change, word):
 
 def test_sizes_and_empty_calls(nat):
     lib = nat.lib()
-    assert lib.sophia_mla_tree_workspace_size(10, 128, 1) == 0
-    assert lib.sophia_mla_tree_workspace_size(10, 128, 3) == 10 * 3 * 16 * 132 * 4
-    assert lib.sophia_mla_tree_workspace_size(-1, 128, 3) == 0
+    assert lib.sophia_mla_tree_workspace_size(10, 2, 128, 1) == 0
+    # three groups of 4 or two of 8 nodes in two trees, 3 ranges, 16 columns a node
+    assert lib.sophia_mla_tree_workspace_size(10, 2, 128, 3) >= 4 * 3 * 4 * 16 * (128 + 2) * 4
+    assert lib.sophia_mla_tree_workspace_size(-1, 2, 128, 3) == 0
     assert lib.sophia_tree_accept_workspace_size(-1, 5) == 0 and lib.sophia_tree_accept_workspace_size(0, 5) == 0
     assert lib.sophia_tree_accept_workspace_size(3, 5) >= 3 * 8
     # nothing to do: no pointer is needed
@@ -183,9 +185,10 @@ def test_operators_reject_cpu_tensors():
 
 def test_tree_attention_splits_rule():
     from sophia_amd import ops
-    for trees in (0, 1, 7, 64, 5000):
-        for nodes in (1, 8, 9, 64):
-            for length in (0, 1, 255, 257, 4096, 10 ** 6):
-                s = ops.mla_tree_splits(trees, nodes, length)
-                assert 1 <= s <= 1024
-                assert s == 1 or (s - 1) * 256 < length    # no split without keys at the longest length
+    for dtype in (torch.bfloat16, torch.float32):
+        for trees in (0, 1, 7, 64, 5000):
+            for nodes in (1, 8, 9, 64):
+                for length in (0, 1, 255, 257, 4096, 10 ** 5):
+                    s = ops.mla_tree_splits(trees, nodes, length, dtype)
+                    assert 1 <= s <= 1024
+                    assert s <= -(-length // 64) + 1    # no range without keys at the longest length
