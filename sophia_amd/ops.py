@@ -16,7 +16,6 @@ FlashKDA seam (sm120_concurrent_ffn.py:375-423), so they drop into
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import torch
 
@@ -33,20 +32,24 @@ def _gpu(t: torch.Tensor, name: str) -> None:
 
 def _rows(t: torch.Tensor, name: str, width: int) -> int:
     """Row stride (elements) of a [N, width] view whose rows are dense."""
-    if t.dim() != 2 or t.size(1) != width:
-        raise RuntimeError(f"{name} must be [N, {width}], got {tuple(t.shape)}")
-    if t.size(1) > 1 and t.stride(1) != 1:
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width:
+        raise RuntimeError(f"{name} must be [N, {width}], got {tuple(shape)}")
+    rows, cols = t.stride()
+    if width > 1 and cols != 1:
         raise RuntimeError(f"{name} rows must be contiguous")
-    return int(t.stride(0)) if t.size(0) > 1 else width
+    return rows if shape[0] > 1 else width
 
 
 def _heads_rows(t: torch.Tensor, name: str, heads: int, dim: int) -> int:
     """Row stride of a [N, H, D] view with dense [H, D] rows."""
-    if t.dim() != 3 or t.size(1) != heads or t.size(2) != dim:
-        raise RuntimeError(f"{name} must be [N, {heads}, {dim}], got {tuple(t.shape)}")
-    if (heads > 1 and t.stride(1) != dim) or t.stride(2) != 1:
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise RuntimeError(f"{name} must be [N, {heads}, {dim}], got {tuple(shape)}")
+    rows, head, cols = t.stride()
+    if (heads > 1 and head != dim) or cols != 1:
         raise RuntimeError(f"{name} must have dense [heads, dim] rows")
-    return int(t.stride(0)) if t.size(0) > 1 else heads * dim
+    return rows if shape[0] > 1 else heads * dim
 
 
 def _int32(t: torch.Tensor | None, name: str, device) -> torch.Tensor | None:
@@ -218,13 +221,19 @@ def _flags(use_qk_l2norm: bool, use_gate: bool, use_beta_sigmoid: bool) -> int:
             | (nat.BETA_SIGMOID if use_beta_sigmoid else 0))
 
 
+def _f32_values(t: torch.Tensor, device) -> torch.Tensor:
+    """The tensor's values as the kernels read them (itself when they lie so)."""
+    if t.dtype == torch.float32 and t.device == device and t.is_contiguous():
+        return t
+    return t.detach().to(device=device, dtype=torch.float32).reshape(-1).contiguous()
+
+
 def _gate_params(use_gate, A_log, dt_bias, heads, device):
     if not use_gate:
         return None, None
     if A_log is None or dt_bias is None:
         raise RuntimeError("use_gate_in_kernel needs A_log and dt_bias")
-    a = A_log.detach().to(device=device, dtype=torch.float32).reshape(-1).contiguous()
-    b = dt_bias.detach().to(device=device, dtype=torch.float32).reshape(-1).contiguous()
+    a, b = _f32_values(A_log, device), _f32_values(dt_bias, device)
     if a.numel() != heads or b.numel() != heads * HEAD_DIM:
         raise RuntimeError(f"A_log must have {heads} and dt_bias {heads * HEAD_DIM} elements")
     return a, b
@@ -1619,20 +1628,21 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 TREE_NODES = nat.TREE_NODES   # nodes of a tree of drafted tokens, at most
 
 
-def _same_device(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None:
+def _on_device(index: int, device, *named) -> None:
+    """(tensor or None, name) pairs: each tensor lies on GPU ``index``."""
+    for t, name in named:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != index):
             _gpu(t, name)
-            if t.device != device:
-                raise RuntimeError(f"{name} must be on {device}, got {t.device}")
+            raise RuntimeError(f"{name} must be on {device}, got {t.device}")
 
 
-def _on(device):
-    """The device as the current one for a launch (a stream handle alone does
-    not name it)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(device, fn, *args) -> int:
+    """``fn(*args, stream)`` with ``device`` as the current one (a stream handle
+    alone does not name it)."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args, nat.stream_handle(device))
+    with torch.cuda.device(device):
+        return fn(*args, nat.stream_handle(device))
 
 
 def _trees(cu_nodes: torch.Tensor, parents: torch.Tensor, max_nodes: int, rows: int, device) -> int:
@@ -1641,11 +1651,11 @@ def _trees(cu_nodes: torch.Tensor, parents: torch.Tensor, max_nodes: int, rows: 
     par = _int32(parents, "parents", device)
     if cu is None or cu.dim() != 1 or cu.numel() < 1:
         raise RuntimeError("cu_nodes must hold one offset per tree and the end of the last")
-    if par is None or int(par.numel()) != rows:
+    if par is None or par.numel() != rows:
         raise RuntimeError(f"parents must hold one entry per node, {rows}")
     if not 1 <= int(max_nodes) <= TREE_NODES:
         raise RuntimeError(f"max_nodes must be in [1, {TREE_NODES}], got {max_nodes}")
-    return int(cu.numel()) - 1
+    return cu.numel() - 1
 
 
 def _int64(t: torch.Tensor, name: str, n: int, device) -> torch.Tensor:
@@ -1693,8 +1703,8 @@ def mla_tree_attn(qa: torch.Tensor, latent: torch.Tensor, latent_cache: torch.Te
     if qa.dim() != 3:
         raise RuntimeError(f"qa must be [rows, heads, rank], got {tuple(qa.shape)}")
     device = qa.device
-    rows, heads, rank = (int(v) for v in qa.shape)
-    _same_device(device, latent=latent, latent_cache=latent_cache, cached=cached, out=out)
+    rows, heads, rank = qa.shape
+    _on_device(qa.get_device(), device, (latent, "latent"), (latent_cache, "latent_cache"), (out, "out"))
     qs = _heads_rows(qa, "qa", heads, rank)
     ls = _rows(latent, "latent", rank)
     _nrows(latent, "latent", rows)
@@ -1716,13 +1726,12 @@ def mla_tree_attn(qa: torch.Tensor, latent: torch.Tensor, latent_cache: torch.Te
     # whole 64-key tiles, the drafted latents being one more at the end
     split_keys = max(1, -(-(-(-bound // 64) + 1) // max(int(splits), 1))) * 64
     lib = nat.lib()
-    with _on(device):
-        ws_bytes = int(lib.sophia_mla_tree_workspace_size(rows, n, rank, int(splits)))
-        ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
-        rc = lib.sophia_mla_tree_attn(
-            nat.ptr(qa), qs, nat.ptr(latent), ls, nat.dtype_code(qa.dtype), nat.ptr(latent_cache), slot_stride, n_slots,
-            max_seq, nat.ptr(sl), nat.ptr(cached), nat.ptr(cu_nodes), nat.ptr(parents), n, rows, int(max_nodes),
-            float(scale), nat.ptr(y), os_, heads, rank, int(splits), split_keys, nat.ptr(ws), ws_bytes, nat.stream_handle(device))
+    ws_bytes = lib.sophia_mla_tree_workspace_size(rows, n, rank, int(splits))
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
+    rc = _launch(device, lib.sophia_mla_tree_attn, qa.data_ptr(), qs, latent.data_ptr(), ls, nat.dtype_code(qa.dtype),
+                 latent_cache.data_ptr(), slot_stride, n_slots, max_seq, nat.ptr(sl), cached.data_ptr(),
+                 cu_nodes.data_ptr(), parents.data_ptr(), n, rows, int(max_nodes), float(scale), y.data_ptr(), os_, heads,
+                 rank, int(splits), split_keys, nat.ptr(ws), ws_bytes)
     nat.check(rc, "sophia_mla_tree_attn")
     return y
 
@@ -1767,13 +1776,14 @@ def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: to
     _gpu(x_qkv, "x_qkv")
     _gpu(g, "g")
     device = x_qkv.device
-    rows = int(x_qkv.size(0))
-    heads = int(g.size(1)) if g.dim() == 3 else 0
+    rows = x_qkv.size(0)
+    heads = g.size(1) if g.dim() == 3 else 0
     inner = heads * HEAD_DIM
+    _on_device(x_qkv.get_device(), device, (conv_weight, "conv_weight"), (conv_state, "conv_state"), (g, "g"),
+               (beta, "beta"), (state, "state"), (out, "out"), (tape, "tape"))
     xs = _rows(x_qkv, "x_qkv", 3 * inner)
     gs = _heads_rows(g, "g", heads, HEAD_DIM)
     bs = _rows(beta, "beta", heads)
-    _same_device(device, conv_weight=conv_weight, conv_state=conv_state, g=g, beta=beta, state=state, out=out, tape=tape)
     for t, name in ((g, "g"), (beta, "beta")):
         _nrows(t, name, rows)
     n = _trees(cu_nodes, parents, max_nodes, rows, device)
@@ -1793,14 +1803,13 @@ def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: to
         tape = torch.empty((rows, heads, 3, HEAD_DIM), dtype=torch.float32, device=device)
     _tape(tape, rows, heads)
     base, esz = x_qkv.data_ptr(), x_qkv.element_size()
-    with _on(device):
-        rc = nat.lib().sophia_kda_tree_step(
-            base, base + inner * esz, base + 2 * inner * esz, xs, nat.dtype_code(x_qkv.dtype), nat.ptr(conv_weight),
-            nat.ptr(conv_state), taps, nat.ptr(g), gs, nat.dtype_code(g.dtype), nat.ptr(beta), bs,
-            nat.dtype_code(beta.dtype), nat.ptr(a_log), nat.ptr(dtb), float(HEAD_DIM ** -0.5 if scale is None else scale),
-            float(lower_bound), _flags(use_qk_l2norm, use_gate, use_beta_sigmoid), nat.ptr(state), n_slots,
-            nat.ptr(slots), nat.ptr(cu_nodes), nat.ptr(parents), n, rows, int(max_nodes), heads, HEAD_DIM, nat.ptr(o),
-            os_, nat.ptr(tape), nat.stream_handle(device))
+    rc = _launch(device, nat.lib().sophia_kda_tree_step, base, base + inner * esz, base + 2 * inner * esz, xs,
+                 nat.dtype_code(x_qkv.dtype), conv_weight.data_ptr(), nat.ptr(conv_state), taps, g.data_ptr(), gs,
+                 nat.dtype_code(g.dtype), beta.data_ptr(), bs, nat.dtype_code(beta.dtype), nat.ptr(a_log), nat.ptr(dtb),
+                 float(HEAD_DIM ** -0.5 if scale is None else scale), float(lower_bound),
+                 _flags(use_qk_l2norm, use_gate, use_beta_sigmoid), state.data_ptr(), n_slots, nat.ptr(slots),
+                 cu_nodes.data_ptr(), parents.data_ptr(), n, rows, int(max_nodes), heads, HEAD_DIM, o.data_ptr(), os_,
+                 tape.data_ptr())
     nat.check(rc, "sophia_kda_tree_step")
     return o, tape
 
@@ -1849,64 +1858,66 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
     n, max_path = int(path.size(0)), int(path.size(1))
     if not 1 <= max_path <= TREE_NODES:
         raise RuntimeError(f"path rows must hold 1..{TREE_NODES} entries, got {max_path}")
-    _same_device(device, n_path=n_path, cu_nodes=cu_nodes, slots=slots, cached=cached)
+    index = path.get_device()
     count = _int32(n_path, "n_path", device)
     cu = _int32(cu_nodes, "cu_nodes", device)
-    if int(count.numel()) != n or int(cu.numel()) != n + 1:
+    if count.numel() != n or cu.numel() != n + 1:
         raise RuntimeError(f"n_path must hold {n} and cu_nodes {n + 1} entries")
     kda, mla = list(kda), list(mla)
-    rows = n_slots = None
-    heads, taps, x_dtype = 1, 1, torch.float32
-
-    def agree(what, got, want):
-        if want is not None and got != want:
-            raise RuntimeError(f"every layer must have the same {what}, got {got} and {want}")
-        return got
-
-    kda_args = (nat.CommitKda * max(len(kda), 1))()
-    for i, (tape, x, conv_state, state) in enumerate(kda):
-        _same_device(device, tape=tape, x_qkv=x, conv_state=conv_state, state=state)
-        h = int(tape.size(1)) if tape.dim() == 4 else 0
-        t = int(conv_state.size(-1)) + 1 if conv_state is not None else 1
-        if i:
-            agree("heads, conv taps and x_qkv type", (h, t, x.dtype), (heads, taps, x_dtype))
-        heads, taps, x_dtype = h, t, x.dtype
+    if not kda and not mla:
+        return
+    for layer in kda:
+        _on_device(index, device, *zip(layer, ("tape", "x_qkv", "conv_state", "state")))
+    for layer in mla:
+        _on_device(index, device, *zip(layer, ("latent", "latent_cache")))
+    # What the first layer of a kind is, all of them are.
+    heads, taps, x_dtype, f32 = 1, 1, torch.float32, torch.float32
+    rank = max_seq = 0
+    rows, n_slots = (kda[0][1].size(0), kda[0][3].size(0)) if kda else (mla[0][0].size(0), mla[0][1].size(0))
+    flat = []
+    if kda:
+        tape, x, conv_state, state = kda[0]
+        heads, x_dtype = tape.size(1) if tape.dim() == 4 else 0, x.dtype
+        inner = heads * HEAD_DIM
+        taps = conv_state.size(-1) + 1 if conv_state is not None else 1
         if not 1 <= taps <= 4:
             raise RuntimeError("conv_state must hold at most 3 samples")
-        xs = _rows(x, "x_qkv", 3 * heads * HEAD_DIM)
-        rows = agree("rows", int(x.size(0)), rows)
-        _tape(tape, rows, heads)
-        _state(state, "state", heads, device)
-        _conv_history(conv_state, heads * HEAD_DIM, taps)
-        n_slots = agree("slots", int(state.size(0)), n_slots)
-        if conv_state is not None:
-            agree("slots", int(conv_state.size(0)), n_slots)
-        kda_args[i] = nat.CommitKda(tape.data_ptr(), x.data_ptr(), xs, nat.ptr(conv_state), state.data_ptr())
-    rank = max_seq = lat_dtype = None
-    mla_args = (nat.CommitMla * max(len(mla), 1))()
-    for i, (latent, cache) in enumerate(mla):
-        _same_device(device, latent=latent, latent_cache=cache)
-        rank = agree("rank", int(latent.size(-1)), rank)
-        lat_dtype = agree("latent type", latent.dtype, lat_dtype)
-        ls = _rows(latent, "latent", rank)
-        ss = _latents(cache, rank, "latent_cache")
-        rows = agree("rows", int(latent.size(0)), rows)
-        n_slots = agree("slots", int(cache.size(0)), n_slots)
-        max_seq = agree("cache length", int(cache.size(1)), max_seq)
-        mla_args[i] = nat.CommitMla(latent.data_ptr(), ls, cache.data_ptr(), ss)
-    if rows is None:
-        return
-    sl = _tree_slots(slots, n, n_slots, device)
+        tape_shape, x_shape = (rows, heads, 3, HEAD_DIM), (rows, 3 * inner)
+        state_shape, hist_shape = (n_slots, heads, HEAD_DIM, HEAD_DIM), (n_slots, 3 * inner, taps - 1)
+        for i, (tape, x, conv_state, state) in enumerate(kda):
+            if (tape.shape != tape_shape or tape.dtype is not f32 or not tape.is_contiguous()
+                    or state.shape != state_shape or state.dtype is not f32 or not state.is_contiguous()
+                    or x.shape != x_shape or x.dtype is not x_dtype or x.stride(1) != 1
+                    or (taps > 1 if conv_state is None else (conv_state.shape != hist_shape or conv_state.dtype is not f32
+                                                             or not conv_state.is_contiguous()))):
+                raise RuntimeError(
+                    f"KDA layer {i}: tape must be contiguous fp32 {list(tape_shape)}, x_qkv {x_dtype} {list(x_shape)} with "
+                    f"dense rows, conv_state contiguous fp32 {list(hist_shape)} and state contiguous fp32 "
+                    f"{list(state_shape)}, as in every layer")
+            flat += (tape.data_ptr(), x.data_ptr(), x.stride(0) if rows > 1 else 3 * inner,
+                     0 if conv_state is None else conv_state.data_ptr(), state.data_ptr())
+    kda_args = (ctypes.c_int64 * max(len(flat), 1))(*flat)   # (sophia_commit_kda: five words a layer)
+    flat = []
+    lat_dtype = f32
     if mla:
         if cached is None:
             raise RuntimeError("MLA layers need cached")
         _int64(cached, "cached", n, device)
-    with _on(device):
-        rc = nat.lib().sophia_tree_commit(
-            nat.ptr(path), int(path.stride(0)) if n > 1 else max_path, nat.ptr(count), max_path, nat.ptr(cu), n, rows,
-            nat.ptr(sl), n_slots, kda_args, len(kda), heads, HEAD_DIM, taps, nat.dtype_code(x_dtype), mla_args, len(mla),
-            nat.ptr(cached) if mla else None, max_seq or 0, rank or 0, nat.dtype_code(lat_dtype or torch.float32),
-            nat.stream_handle(device))
+        latent, cache = mla[0]
+        rank, max_seq, lat_dtype = latent.size(-1), cache.size(1) if cache.dim() == 3 else 0, latent.dtype
+        for i, (latent, cache) in enumerate(mla):
+            if (latent.shape != (rows, rank) or latent.dtype is not lat_dtype or latent.stride(1) != 1
+                    or cache.shape != (n_slots, max_seq, rank)):
+                raise RuntimeError(f"MLA layer {i}: latent must be {lat_dtype} [{rows}, {rank}] with dense rows and "
+                                   f"latent_cache fp32 [{n_slots}, {max_seq}, {rank}], as in every layer")
+            flat += (latent.data_ptr(), latent.stride(0) if rows > 1 else rank, cache.data_ptr(),
+                     _latents(cache, rank, "latent_cache"))
+    mla_args = (ctypes.c_int64 * max(len(flat), 1))(*flat)   # (sophia_commit_mla: four)
+    sl = _tree_slots(slots, n, n_slots, device)
+    rc = _launch(device, nat.lib().sophia_tree_commit, path.data_ptr(), path.stride(0) if n > 1 else max_path,
+                 count.data_ptr(), max_path, cu.data_ptr(), n, rows, nat.ptr(sl), n_slots, kda_args, len(kda), heads,
+                 HEAD_DIM, taps, nat.dtype_code(x_dtype), mla_args, len(mla), cached.data_ptr() if mla else None, max_seq,
+                 rank, nat.dtype_code(lat_dtype))
     nat.check(rc, "sophia_tree_commit")
 
 
@@ -1941,11 +1952,11 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     device = logits.device
     if logits.dim() != 2:
         raise RuntimeError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
-    rows, vocab = (int(v) for v in logits.shape)
+    rows, vocab = logits.shape
     xs = _rows(logits, "logits", vocab)
-    _same_device(device, history=history, history_len=history_len, prompt_len=prompt_len, repetition=repetition,
-                 presence=presence, frequency=frequency, bias_ids=bias_ids, bias=bias, allowed=allowed,
-                 allowed_rows=allowed_rows, tokens=tokens, out=out)
+    _on_device(logits.get_device(), device, (history, "history"), (repetition, "repetition"), (presence, "presence"),
+               (frequency, "frequency"), (bias_ids, "bias_ids"), (bias, "bias"), (allowed, "allowed"), (tokens, "tokens"),
+               (out, "out"))
     if cu_nodes is not None:
         if parents is None or tokens is None:
             raise RuntimeError("trees need parents and tokens")
@@ -2000,13 +2011,11 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
         x0, y0, e = logits.data_ptr(), y.data_ptr(), logits.element_size()
         if x0 < y0 + ((rows - 1) * ys + vocab) * e and y0 < x0 + ((rows - 1) * xs + vocab) * e:
             raise RuntimeError("out must be logits itself or not overlap it")
-    with _on(device):
-        rc = nat.lib().sophia_adjust_logits(
-            nat.ptr(logits), xs, nat.ptr(y), ys, nat.dtype_code(logits.dtype), rows, vocab, nat.ptr(history), hist_stride,
-            nat.ptr(history_len), nat.ptr(prompt_len), hist_max, nat.ptr(repetition), nat.ptr(presence),
-            nat.ptr(frequency), nat.ptr(bias_ids), nat.ptr(bias), n_bias, nat.ptr(allowed), n_masks,
-            nat.ptr(allowed_rows), nat.ptr(cu_nodes), nat.ptr(parents), nat.ptr(tokens), n, int(max_nodes),
-            nat.stream_handle(device))
+    rc = _launch(device, nat.lib().sophia_adjust_logits, logits.data_ptr(), xs, y.data_ptr(), ys,
+                 nat.dtype_code(logits.dtype), rows, vocab, nat.ptr(history), hist_stride, nat.ptr(history_len),
+                 nat.ptr(prompt_len), hist_max, nat.ptr(repetition), nat.ptr(presence), nat.ptr(frequency),
+                 nat.ptr(bias_ids), nat.ptr(bias), n_bias, nat.ptr(allowed), n_masks, nat.ptr(allowed_rows),
+                 nat.ptr(cu_nodes), nat.ptr(parents), nat.ptr(tokens), n, int(max_nodes))
     nat.check(rc, "sophia_adjust_logits")
     return y
 
@@ -2028,24 +2037,22 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tens
     device = logits.device
     if logits.dim() != 2 or int(logits.size(1)) < 1:
         raise RuntimeError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
-    rows, vocab = (int(v) for v in logits.shape)
+    rows, vocab = logits.shape
     xs = _rows(logits, "logits", vocab)
-    _same_device(device, tokens=tokens)
+    _on_device(logits.get_device(), device, (tokens, "tokens"))
     n = _trees(cu_nodes, parents, max_nodes, rows, device)
     _int64(tokens, "tokens", rows, device)
     lib = nat.lib()
-    with _on(device):
-        path = torch.empty((n, int(max_nodes)), dtype=torch.int32, device=device)
-        n_path = torch.empty(n, dtype=torch.int32, device=device)
-        next_token = torch.empty(n, dtype=torch.int64, device=device)
-        chosen = torch.empty(rows, dtype=torch.int64, device=device)
-        buf, addr, nbytes = _workspace(int(lib.sophia_tree_accept_workspace_size(rows, vocab)), device)
-        rc = lib.sophia_tree_accept(
-            nat.ptr(logits), xs, nat.dtype_code(logits.dtype), rows, vocab, nat.ptr(tokens), nat.ptr(cu_nodes),
-            nat.ptr(parents), n, int(max_nodes), nat.ptr(path), int(max_nodes), nat.ptr(n_path), nat.ptr(next_token),
-            nat.ptr(chosen), addr, nbytes, nat.stream_handle(device))
+    nbytes = lib.sophia_tree_accept_workspace_size(rows, vocab)
+    path = torch.empty((n, int(max_nodes)), dtype=torch.int32, device=device)
+    n_path = torch.empty(n, dtype=torch.int32, device=device)
+    next_token = torch.empty(n, dtype=torch.int64, device=device)
+    chosen = torch.empty(rows, dtype=torch.int64, device=device)
+    ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device)
+    rc = _launch(device, lib.sophia_tree_accept, logits.data_ptr(), xs, nat.dtype_code(logits.dtype), rows, vocab,
+                 tokens.data_ptr(), cu_nodes.data_ptr(), parents.data_ptr(), n, int(max_nodes), path.data_ptr(),
+                 int(max_nodes), n_path.data_ptr(), next_token.data_ptr(), chosen.data_ptr(), ws.data_ptr(), nbytes)
     nat.check(rc, "sophia_tree_accept")
-    del buf
     return path, n_path, next_token, chosen
 
 
