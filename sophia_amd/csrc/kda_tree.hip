@@ -28,7 +28,6 @@
 // A node with an input that is not finite would reach its siblings through the
 // products (0 times infinity): its rows enter them as zeros, and what lies on a
 // path with it ends as NaN.
-#include <cstdlib>
 #include <type_traits>
 
 #include "common.hpp"
@@ -722,20 +721,10 @@ extern "C" int sophia_kda_tree_step(const void *x_q, const void *x_k, const void
     hipLaunchKernelGGL((kda_tree_step_kernel<MT, NT, SOPHIA_DTYPE_BF16>), grid, dim3(NT), 0, st, a);        \
   else                                                                                                      \
     hipLaunchKernelGGL((kda_tree_step_kernel<MT, NT, SOPHIA_DTYPE_F32>), grid, dim3(NT), 0, st, a);
-  const bool wide = static_cast<int64_t>(num_heads) * n_trees <= 256;
-  static const bool narrow = getenv("TREE_NARROW") != nullptr;
   if (max_nodes <= 16) {
-    if (wide || !narrow) {
-      SOPHIA_TREE_STEP(1, 512)
-    } else {
-      SOPHIA_TREE_STEP(1, 256)
-    }
+    SOPHIA_TREE_STEP(1, 512)
   } else if (max_nodes <= 32) {
-    if (wide || !narrow) {
-      SOPHIA_TREE_STEP(2, 512)
-    } else {
-      SOPHIA_TREE_STEP(2, 256)
-    }
+    SOPHIA_TREE_STEP(2, 512)
   } else {
     SOPHIA_TREE_STEP(4, 512)
   }
