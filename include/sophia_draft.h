@@ -51,7 +51,7 @@ extern "C" {
  *   o             : [rows, heads, 128] of x's type.
  *   tape          : [rows, heads, 3, 128] fp32: u, k and G of each node, for sophia_tree_commit.
  * flags: SOPHIA_KDA_QK_L2NORM, SOPHIA_KDA_GATE_IN_KERNEL, SOPHIA_KDA_BETA_SIGMOID.
- * x, g and o: 16-byte aligned, row strides multiples of 8; state and tape 16-byte aligned.
+ * x, g and o: 16-byte aligned, row strides multiples of 8; state, tape and dt_bias 16-byte aligned.
  */
 int sophia_kda_tree_step(const void *x_q, const void *x_k, const void *x_v, int64_t x_row_stride, int x_dtype,
                          const float *conv_weight, const float *conv_state, int kernel_size, const void *g,

@@ -41,6 +41,7 @@ namespace {
 constexpr int kD = 128;
 constexpr int kLd = kD + 4;     // row stride of the LDS matrices: 16 rows 4 banks apart
 constexpr int kTape = 3 * kD;   // floats of a node's tape per head
+constexpr int kStateParts = 4;
 
 struct TreeStepArgs {
   Trees trees;
@@ -71,32 +72,35 @@ struct TreeStepArgs {
 // k stays a normal fp32 number down to 1.3e-12.
 constexpr float kFactored = 60.f;
 
-// Eight consecutive elements as they lie, and as floats.
+// Eight elements of a row as they lie, and as floats: four from p on and the four 64
+// places behind them.  Over 16 threads each half is contiguous, which eight in a row
+// per thread are not (two of them then meet in every LDS bank).
+constexpr int kHalf = kD / 2;
 template <int DT>
 struct Raw8 {
-  u4 w[DT == SOPHIA_DTYPE_BF16 ? 1 : 2];
+  typename std::conditional<DT == SOPHIA_DTYPE_BF16, u2, u4>::type w[2];
 };
-template <int DT>
-__device__ __forceinline__ Raw8<DT> raw8(const void *p) {
-  Raw8<DT> r;
-  r.w[0] = static_cast<const u4 *>(p)[0];
-  if constexpr (DT == SOPHIA_DTYPE_F32) r.w[1] = static_cast<const u4 *>(p)[1];
-  return r;
+template <int DT, typename E>
+__device__ __forceinline__ Raw8<DT> raw8(const E *p) {
+  using V = decltype(Raw8<DT>::w[0] + 0);
+  return {{*reinterpret_cast<const V *>(p), *reinterpret_cast<const V *>(p + kHalf)}};
 }
 template <int DT>
 __device__ __forceinline__ void to_float(const Raw8<DT> &r, float (&f)[8]) {
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
-    if constexpr (DT == SOPHIA_DTYPE_BF16)
-      f[c] = __uint_as_float(c & 1 ? r.w[0][c >> 1] & 0xffff0000u : r.w[0][c >> 1] << 16);
-    else
+    if constexpr (DT == SOPHIA_DTYPE_BF16) {
+      const uint32_t w = r.w[c >> 2][(c & 3) >> 1];
+      f[c] = __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16);
+    } else {
       f[c] = __uint_as_float(r.w[c >> 2][c & 3]);
+    }
   }
 }
 __device__ __forceinline__ void read8(const float *p, float (&f)[8]) { to_float(raw8<SOPHIA_DTYPE_F32>(p), f); }
 __device__ __forceinline__ void write8(float *p, const float (&f)[8]) {
   reinterpret_cast<f4 *>(p)[0] = f4{f[0], f[1], f[2], f[3]};
-  reinterpret_cast<f4 *>(p)[1] = f4{f[4], f[5], f[6], f[7]};
+  reinterpret_cast<f4 *>(p + kHalf)[0] = f4{f[4], f[5], f[6], f[7]};
 }
 
 // LDS of the step: first the rows before the conv, then the matrices.
@@ -153,22 +157,26 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
 
   // ---- loads
   const int64_t inner = static_cast<int64_t>(a.heads) * kD;
-  const int r0 = t >> 4, seg = 8 * (t & 15);            // this thread's nodes r0 + RP p, channels seg .. + 7
+  const int r0 = t >> 4, seg = 4 * (t & 15);            // this thread's nodes r0 + RP p, channels seg .. + 3, seg + 64 ..
   const int64_t hc = static_cast<int64_t>(h) * kD + seg;
-  constexpr int kEsz = DT == SOPHIA_DTYPE_BF16 ? 2 : 4;
+  using Elem = typename Lds::Elem;
   const int parent = tree_parent(a.trees, base, n, lane);
   Raw8<DT> raw[P][3];
-  Raw8<SOPHIA_DTYPE_F32> raw_g[P];
+  u2 raw_g[P][4];
   const bool g16 = a.g_dtype == SOPHIA_DTYPE_BF16;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int64_t row = base + min(r0 + RP * p, n - 1);
 #pragma unroll
     for (int part = 0; part < 3; ++part)
-      raw[p][part] = raw8<DT>(static_cast<const uint8_t *>(a.x[part]) + (row * a.x_stride + hc) * kEsz);
-    const u4 *gp = reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(a.g) + (row * a.g_stride + hc) * (g16 ? 2 : 4));
-    raw_g[p].w[0] = gp[0];
-    raw_g[p].w[1] = gp[g16 ? 0 : 1];   // (bf16: the same again, no branch around a load)
+      raw[p][part] = raw8<DT>(static_cast<const Elem *>(a.x[part]) + row * a.x_stride + hc);
+    // (of bf16 the first half of what is loaded; no branch around a load)
+    const int gsz = g16 ? 2 : 4;
+    const uint8_t *gp = static_cast<const uint8_t *>(a.g) + (row * a.g_stride + hc) * gsz;
+    raw_g[p][0] = *reinterpret_cast<const u2 *>(gp);
+    raw_g[p][1] = *reinterpret_cast<const u2 *>(gp + (g16 ? 0 : 8));
+    raw_g[p][2] = *reinterpret_cast<const u2 *>(gp + kHalf * gsz);
+    raw_g[p][3] = *reinterpret_cast<const u2 *>(gp + kHalf * gsz + (g16 ? 0 : 8));
   }
   // Taps by distance and history samples of channels t, t + NT of the head's 384;
   // those that a shorter conv lacks are zeros.
@@ -190,19 +198,22 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
   Raw8<SOPHIA_DTYPE_F32> raw_bias = {};
   if (gate) raw_bias = raw8<SOPHIA_DTYPE_F32>(a.dt_bias + hc);
   const float a_log = gate ? a.A_log[h] : 0.f;
-  // S rows 16 blk + 4 grp + s of the lane's columns, the state last: the waits for
-  // the others do not include it.
-  asm volatile("" ::: "memory");
+  // S rows 16 blk + 4 grp + s of the lane's columns: behind the other loads, whose waits
+  // do not include them, and a quarter at a time between the steps below, as a
+  // wavefront stands still while the memory queue takes no more.
   using St = typename std::conditional<CE == 2, f2, float>::type;
   St st[kD / 4];
   const int col = CW * wave + CE * c16;
-  {
+  const auto load_state = [&](auto part) {
+    constexpr int kPer = kD / 4 / kStateParts, i0 = decltype(part)::value * kPer;
     const float *S = a.state + (static_cast<int64_t>(slot) * a.heads + h) * kD * kD + col;
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < kD / 4; ++i)
+    for (int i = i0; i < i0 + kPer; ++i)
       st[i] = __builtin_nontemporal_load(reinterpret_cast<const St *>(S + (16 * (i >> 2) + 4 * grp + (i & 3)) * kD));
-  }
-  __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  load_state(std::integral_constant<int, 0>{});
   const auto sval = [&](int i, int e) {
     if constexpr (CE == 2)
       return st[i][e];
@@ -211,6 +222,7 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
   };
 
   // ---- paths, and the raw rows into LDS
+  if (wave == 0) s_up[0][lane] = parent;
   const uint64_t path = tree_paths(parent, n, lane, [&](int r, int up) {
     if (wave == 0) s_up[r][lane] = up;
   });
@@ -223,9 +235,10 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
     if (r0 + RP * p < T)
 #pragma unroll
       for (int part = 0; part < 3; ++part) {
-        u4 *d = reinterpret_cast<u4 *>(&lds.conv.x[3 + r0 + RP * p][part * kD + seg]);
-        d[0] = raw[p][part].w[0];
-        if constexpr (DT == SOPHIA_DTYPE_F32) d[1] = raw[p][part].w[1];
+        using V = decltype(raw[p][part].w[0] + 0);
+        Elem *d = &lds.conv.x[3 + r0 + RP * p][part * kD + seg];
+        *reinterpret_cast<V *>(d) = raw[p][part].w[0];
+        *reinterpret_cast<V *>(d + kHalf) = raw[p][part].w[1];
       }
 #pragma unroll
   for (int j = 0; j < kCh; ++j) {
@@ -245,6 +258,7 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
     s_bad[t] = !ok;
   }
   if (t == 0) s_far = 0;
+  load_state(std::integral_constant<int, 1>{});
   lds_barrier();
 
   // ---- conv, norms, log-decay: in registers
@@ -308,8 +322,9 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
     for (int c = 0; c < 8; ++c) {
       q[p][c] *= qs;
       k[p][c] *= ks;
-      const uint32_t w = raw_g[p].w[0][c >> 1];
-      const float z = g16 ? __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16) : __uint_as_float(raw_g[p].w[c >> 2][c & 3]);
+      const uint32_t w = raw_g[p][2 * (c >> 2)][(c & 3) >> 1];
+      const float z = g16 ? __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16)
+                          : __uint_as_float(raw_g[p][2 * (c >> 2) + ((c & 3) >> 1)][c & 1]);
       g[p][c] = gate ? kda_log_decay(z, head_scale, bias[c], a.lower_bound) : z;
       ok &= is_finite(q[p][c]) && is_finite(k[p][c]) && is_finite(v[p][c]) && is_finite(g[p][c]);
     }
@@ -319,6 +334,7 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
       s_bad[node] = 1;
     }
   }
+  load_state(std::integral_constant<int, 2>{});
   lds_barrier();
 
   // ---- G: sums of the log-decay along the paths, by doubling (as many rounds as the
@@ -335,6 +351,7 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
       }
   };
   put_g(mat.g);
+  load_state(std::integral_constant<int, 3>{});
   lds_barrier();
   for (int r = 0; (1 << r) < depth; ++r) {
     float (*from)[kLd] = r & 1 ? mat.q : mat.g, (*to)[kLd] = r & 1 ? mat.g : mat.q;
@@ -438,9 +455,9 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
     for (int i = wave; i < n; i += NW) {
       uint64_t left = s_path[i];
       float qi[8], ki[8], gi[8];
-      read8(&mat.q[i][8 * c16], qi);
-      read8(&mat.k[i][8 * c16], ki);
-      read8(&mat.g[i][8 * c16], gi);
+      read8(&mat.q[i][4 * c16], qi);
+      read8(&mat.k[i][4 * c16], ki);
+      read8(&mat.g[i][4 * c16], gi);
       while (left) {
         int j = -1;
 #pragma unroll
@@ -452,8 +469,8 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
         float kk = 0.f, qk = 0.f;
         if (j >= 0) {
           float kj[8], gj[8];
-          read8(&mat.k[j][8 * c16], kj);
-          read8(&mat.g[j][8 * c16], gj);
+          read8(&mat.k[j][4 * c16], kj);
+          read8(&mat.g[j][4 * c16], gj);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             const float w = kj[c] * __expf(gi[c] - gj[c]);
@@ -709,8 +726,8 @@ extern "C" int sophia_kda_tree_step(const void *x_q, const void *x_k, const void
   SOPHIA_REQUIRE(!(flags & SOPHIA_KDA_GATE_IN_KERNEL) || (A_log && dt_bias),
                  "kda_tree_step: gate in kernel needs A_log and dt_bias");
   SOPHIA_REQUIRE(aligned(x_q, 16) && aligned(x_k, 16) && aligned(x_v, 16) && aligned(g, 16) && aligned(o, 16) &&
-                     aligned(state, 16) && aligned(tape, 16),
-                 "kda_tree_step: x, g, o, state and tape must be 16-byte aligned");
+                     aligned(state, 16) && aligned(tape, 16) && aligned(dt_bias, 16),
+                 "kda_tree_step: x, g, o, state, tape and dt_bias must be 16-byte aligned");
   const TreeStepArgs a{{cu_nodes, parents, rows, max_nodes}, {x_q, x_k, x_v}, x_row_stride, conv_weight, conv_state,
                        kernel_size, g, g_row_stride, g_dtype, beta, beta_row_stride, beta_dtype, A_log, dt_bias, scale,
                        lower_bound, flags, state, n_slots, slots, num_heads, o, o_row_stride, tape};

@@ -33,14 +33,16 @@ __device__ __forceinline__ int tree_parent(const Trees &t, int64_t base, int n, 
 }
 
 // Every node's path (itself and its ancestors) as bits, in the lane of the node:
-// six doublings, after r of them `mask` holds the 2^r nodes next to the node on
-// its path and `up` the one above those.  `jump(r, up)` sees each round's `up`.
+// doublings, after r of them `mask` holds the 2^r nodes next to the node on its path
+// and `up` the one above those.  `jump(r, up)` sees each round's `up`, of as many
+// rounds as the deepest path needs.
 template <typename F>
 __device__ __forceinline__ uint64_t tree_paths(int parent, int n, int lane, F jump) {
   uint64_t mask = lane < n ? 1ull << lane : 0;
   int up = parent;
 #pragma unroll
   for (int r = 0; r < 6; ++r) {
+    if (!__any(up >= 0)) break;
     jump(r, up);
     const int from = up < 0 ? lane : up;
     const uint32_t lo = __shfl(static_cast<uint32_t>(mask), from, 64);

@@ -1794,6 +1794,8 @@ def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: to
         raise RuntimeError("conv_state and state must have the same number of slots")
     slots = _tree_slots(state_slots, n, n_slots, device)
     a_log, dtb = _gate_params(use_gate, A_log, dt_bias, heads, device)
+    if dtb is not None and dtb.data_ptr() % 16:
+        dtb = dtb.clone()
     o = out if out is not None else torch.empty((rows, heads, HEAD_DIM), dtype=x_qkv.dtype, device=device)
     os_ = _heads_rows(o, "out", heads, HEAD_DIM)
     _nrows(o, "out", rows)

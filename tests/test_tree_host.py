@@ -75,7 +75,8 @@ STEP_OK = dict(xq=P, xk=P, xv=P, xs=6144, xdt=1, w=P, hist=P, taps=4, g=P, gs=20
     (dict(bdt=-1), "dtype"), (dict(slots_n=-1), "n_slots"), (dict(xs=2000), "stride"), (dict(gs=2000), "stride"),
     (dict(bs=15), "stride"), (dict(os=2044), "stride"), (dict(xs=6148), "multiples"), (dict(hist=None), "NULL"),
     (dict(tape=None), "NULL"), (dict(alog=None), "A_log"), (dict(dtb=None), "A_log"), (dict(xq=P + 2), "aligned"),
-    (dict(state=P + 8), "aligned"), (dict(o=P + 8), "aligned"), (dict(g=P + 8), "aligned")])
+    (dict(state=P + 8), "aligned"), (dict(o=P + 8), "aligned"), (dict(g=P + 8), "aligned"),
+    (dict(dtb=P + 4), "aligned")])
 def test_tree_step_refuses(nat, change, word):
     rc, msg = _call(nat, "sophia_kda_tree_step", STEP_OK, STEP, **change)
     assert rc == nat.SOPHIA_ERR_INVALID and word in msg, msg
