@@ -8,15 +8,15 @@
 //   (I + A) U = beta (V - (K e^G) S),   O = (Q e^G) S + B U.
 // The state is read once and not written; a node's own state is never formed.
 //
-// One work-group per (tree, head).  A wavefront owns 16 or 32 value columns, of
-// which its lanes hold S as B operands of v_mfma_f32_16x16x4_f32 from the start;
-// every load is issued before the first is waited for, the state last.  q, k, v and
-// the log-decay of a node are then 8 channels in each of 16 threads, in registers;
-// the conv's samples, G along the paths, and the operands of the matrix products go
-// through LDS.  From the products with S on no wavefront waits for another but
-// once: an accumulator holds rows 4 (lane / 16) + i of a 16-row tile, which is a B
-// operand whose k index runs 4 (lane / 16) + step, so U goes from one product to
-// the next in registers.
+// One work-group of 8 wavefronts per (tree, head).  A wavefront owns 16 value columns,
+// of which its lanes hold S as B operands of v_mfma_f32_16x16x4_f32; loads are asked
+// for long before they are used, the state behind the rest, a quarter at a time.  q,
+// k, v and the log-decay of a node are then 8 channels in each of 16 threads, in
+// registers; the conv's samples, G along the paths, and the operands of the matrix
+// products go through LDS.  From the products with S on no wavefront waits for another
+// but once: an accumulator holds rows 4 (lane / 16) + i of a 16-row tile, which is a B
+// operand whose k index runs 4 (lane / 16) + step, so U goes from one product to the
+// next in registers.
 //
 // Everything is fp32 (the matrix products too): u enters the cached state with
 // the accepted path, and the decode step that the state otherwise comes from
@@ -24,6 +24,17 @@
 // where |G| stays below kFactored; beyond it e^-G would leave the range of fp32, and
 // they are formed per pair of a node and an ancestor on the vector unit, from
 // e^(G_i - G_j), whose argument is never positive.
+//
+// What bounds it: the steps' latency.  One tree of 7 nodes takes 13 us (16 heads on
+// as many CUs, 25,000 cycles from the first load to the last store), 64 trees of 8 to
+// 24 nodes 55 us, two work-groups per CU in two rounds, where their 114 MB take 22 us
+// at the rate of a copy; there the matrix pipes are busy a quarter of the time, the
+// vector unit and LDS about as much.  8 fp32 chains of 17 to 64 nodes take 55 us.  On
+// the way (us, these three cases): samples gathered from memory tap by tap 21, 128, 121;
+// samples through LDS, pairs on the vector unit 23, 83, 59; conv taps by distance in
+// LDS, where by channel all 16 threads of a node met in one bank, tiles without nodes
+// left out 13, 57, 56.  Not kept: 4 wavefronts of 32 columns (58 for the second), the
+// solve step by step along shallow paths in place of the inverse (58), taps in bf16 (57).
 //
 // A node with an input that is not finite would reach its siblings through the
 // products (0 times infinity): its rows enter them as zeros, and what lies on a
@@ -41,7 +52,7 @@ namespace {
 constexpr int kD = 128;
 constexpr int kLd = kD + 4;     // row stride of the LDS matrices: 16 rows 4 banks apart
 constexpr int kTape = 3 * kD;   // floats of a node's tape per head
-constexpr int kStateParts = 4;
+constexpr int kStateParts = 4;  // (all of S at once: 57 us in place of 55 for the 64 trees)
 
 struct TreeStepArgs {
   Trees trees;
@@ -69,7 +80,9 @@ struct TreeStepArgs {
 };
 
 // |G| up to which A and B are formed from e^G and e^-G: e^-60 times a component of
-// k stays a normal fp32 number down to 1.3e-12.
+// k stays a normal fp32 number down to 1.3e-12.  The exponentials are then off by up to
+// 2.6e-6, where e^(G_i - G_j) is not; a channel that has come that far within 64
+// nodes has lost e^-1 and more at every one of them, and its part in A and B with it.
 constexpr float kFactored = 60.f;
 
 // Eight elements of a row as they lie, and as floats: four from p on and the four 64
@@ -124,13 +137,15 @@ struct StepLds {
   };
 };
 
-// MT: tiles of 16 nodes; NT: threads.
-template <int MT, int NT, int DT>
-__global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2))) void kda_tree_step_kernel(TreeStepArgs a) {
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+static_assert(kWaves * 16 == kD, "16 value columns per wavefront");
+
+// MT: tiles of 16 nodes.
+template <int MT, int DT>
+__global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kernel(TreeStepArgs a) {
   using Lds = StepLds<MT, DT>;
-  constexpr int T = Lds::T, NW = NT / 64;
-  constexpr int CW = kD / NW, CE = CW / 16;             // columns of a wavefront, and per lane
-  constexpr int RP = NT / 16, P = (T + RP - 1) / RP;    // nodes at a time, and how often
+  constexpr int T = Lds::T;
+  constexpr int RP = kThreads / 16, P = (T + RP - 1) / RP;    // nodes at a time, and how often
   __shared__ __align__(16) Lds lds;
   __shared__ float s_beta[T];
   __shared__ uint64_t s_path[kTreeNodes];
@@ -146,7 +161,7 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
   const int slot = a.slots ? a.slots[tree] : tree;
   if (n == 0) return;
   if (slot < 0 || slot >= a.n_slots) {
-    for (int i = t; i < n * kD; i += NT) {
+    for (int i = t; i < n * kD; i += kThreads) {
       const int64_t row = base + i / kD;
       store_elem(a.o, row * a.o_stride + static_cast<int64_t>(h) * kD + i % kD, DT, 0.f);
       float *tp = a.tape + (row * a.heads + h) * kTape + i % kD;
@@ -178,14 +193,14 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
     raw_g[p][2] = *reinterpret_cast<const u2 *>(gp + kHalf * gsz);
     raw_g[p][3] = *reinterpret_cast<const u2 *>(gp + kHalf * gsz + (g16 ? 0 : 8));
   }
-  // Taps by distance and history samples of channels t, t + NT of the head's 384;
+  // Taps by distance and history samples of channels t, t + kThreads of the head's 384;
   // those that a shorter conv lacks are zeros.
-  constexpr int kCh = (3 * kD + NT - 1) / NT;
+  constexpr int kCh = (3 * kD + kThreads - 1) / kThreads;
   float taps[kCh][4], past[kCh][3];
   const int hist = a.taps - 1;
 #pragma unroll
   for (int j = 0; j < kCh; ++j) {
-    const int i = min(t + NT * j, 3 * kD - 1);
+    const int i = min(t + kThreads * j, 3 * kD - 1);
     const int64_t ch = (i / kD) * inner + static_cast<int64_t>(h) * kD + i % kD;
 #pragma unroll
     for (int d = 0; d < 4; ++d) taps[j][d] = d <= hist ? a.conv_w[ch * a.taps + hist - d] : 0.f;
@@ -201,26 +216,18 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
   // S rows 16 blk + 4 grp + s of the lane's columns: behind the other loads, whose waits
   // do not include them, and a quarter at a time between the steps below, as a
   // wavefront stands still while the memory queue takes no more.
-  using St = typename std::conditional<CE == 2, f2, float>::type;
-  St st[kD / 4];
-  const int col = CW * wave + CE * c16;
+  float st[kD / 4];
+  const int col = 16 * wave + c16;
   const auto load_state = [&](auto part) {
     constexpr int kPer = kD / 4 / kStateParts, i0 = decltype(part)::value * kPer;
     const float *S = a.state + (static_cast<int64_t>(slot) * a.heads + h) * kD * kD + col;
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = i0; i < i0 + kPer; ++i)
-      st[i] = __builtin_nontemporal_load(reinterpret_cast<const St *>(S + (16 * (i >> 2) + 4 * grp + (i & 3)) * kD));
+      st[i] = __builtin_nontemporal_load(S + (16 * (i >> 2) + 4 * grp + (i & 3)) * kD);
     __builtin_amdgcn_sched_barrier(0);
   };
   load_state(std::integral_constant<int, 0>{});
-  const auto sval = [&](int i, int e) {
-    if constexpr (CE == 2)
-      return st[i][e];
-    else
-      return st[i];
-  };
-
   // ---- paths, and the raw rows into LDS
   if (wave == 0) s_up[0][lane] = parent;
   const uint64_t path = tree_paths(parent, n, lane, [&](int r, int up) {
@@ -242,7 +249,7 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
       }
 #pragma unroll
   for (int j = 0; j < kCh; ++j) {
-    const int i = t + NT * j;
+    const int i = t + kThreads * j;
     if (i >= 3 * kD) continue;
 #pragma unroll
     for (int d = 0; d < 4; ++d) lds.conv.w[d][i] = taps[j][d];
@@ -416,7 +423,7 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
     }
     lds_barrier();
     // Units (row tile, column tile, A or B), one wavefront each.
-    for (int u = wave; u < mt * (mt + 1); u += NW) {
+    for (int u = wave; u < mt * (mt + 1); u += kWaves) {
       int ti = 0, tj = u >> 1;
       while (tj > ti) tj -= ++ti;
       const float (*left)[kLd] = u & 1 ? mat.q : mat.k;
@@ -449,10 +456,10 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
         write8(&mat.k[r0 + RP * p][seg], k[p]);
         write8(&mat.g[r0 + RP * p][seg], g[p]);
       }
-    for (int i = t; i < T * Lds::LA; i += NT) (&mat.a[0][0])[i] = (&mat.b[0][0])[i] = 0.f;
+    for (int i = t; i < T * Lds::LA; i += kThreads) (&mat.a[0][0])[i] = (&mat.b[0][0])[i] = 0.f;
     lds_barrier();
     // A wavefront takes a node, 16 lanes one of its ancestors.
-    for (int i = wave; i < n; i += NW) {
+    for (int i = wave; i < n; i += kWaves) {
       uint64_t left = s_path[i];
       float qi[8], ki[8], gi[8];
       read8(&mat.q[i][4 * c16], qi);
@@ -496,7 +503,7 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
 #pragma unroll
   for (int p = 0; p < P; ++p)
     if (r0 + RP * p < T) write8(&mat.g[r0 + RP * p][seg], v[p]);
-  if (wave == NW - 1 && grp < MT) {
+  if (wave == kWaves - 1 && grp < MT) {
     float inv[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -509,11 +516,9 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
     for (int i = 0; i < 16; ++i) mat.a[16 * grp + i][16 * grp + c16] = inv[i];
   }
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  f4 u[MT][CE], o[MT][CE];
+  f4 u[MT], o[MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int e = 0; e < CE; ++e) u[m][e] = o[m][e] = zero;
+  for (int m = 0; m < MT; ++m) u[m] = o[m] = zero;
 #pragma unroll
   for (int blk = 0; blk < kD / 16; ++blk)
 #pragma unroll
@@ -522,12 +527,10 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
       const f4 ak = *reinterpret_cast<const f4 *>(&mat.k[16 * m + c16][16 * blk + 4 * grp]);
       const f4 aq = *reinterpret_cast<const f4 *>(&mat.q[16 * m + c16][16 * blk + 4 * grp]);
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int e = 0; e < CE; ++e) {
-          u[m][e] = mfma_f32(ak[s], sval(4 * blk + s, e), u[m][e]);
-          o[m][e] = mfma_f32(aq[s], sval(4 * blk + s, e), o[m][e]);
-        }
+      for (int s = 0; s < 4; ++s) {
+        u[m] = mfma_f32(ak[s], st[4 * blk + s], u[m]);
+        o[m] = mfma_f32(aq[s], st[4 * blk + s], o[m]);
+      }
     }
   lds_barrier();
 
@@ -536,35 +539,27 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     if (m >= mt) break;
-    f4 rhs[CE];
+    f4 rhs;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int node = 16 * m + 4 * grp + i;
-#pragma unroll
-      for (int e = 0; e < CE; ++e) rhs[e][i] = s_beta[node] * (mat.g[node][col + e] - u[m][e][i]);
+      rhs[i] = s_beta[node] * (mat.g[node][col] - u[m][i]);
     }
 #pragma unroll
     for (int p = 0; p < m; ++p) {
       const f4 l = *reinterpret_cast<const f4 *>(&mat.a[16 * m + c16][16 * p + 4 * grp]);
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int e = 0; e < CE; ++e) rhs[e] = mfma_f32(l[s], u[p][e][s], rhs[e]);
+      for (int s = 0; s < 4; ++s) rhs = mfma_f32(l[s], u[p][s], rhs);
     }
     const f4 inv = *reinterpret_cast<const f4 *>(&mat.a[16 * m + c16][16 * m + 4 * grp]);
+    u[m] = zero;
 #pragma unroll
-    for (int e = 0; e < CE; ++e) u[m][e] = zero;
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int e = 0; e < CE; ++e) u[m][e] = mfma_f32(inv[s], rhs[e][s], u[m][e]);
+    for (int s = 0; s < 4; ++s) u[m] = mfma_f32(inv[s], rhs[s], u[m]);
 #pragma unroll
     for (int p = 0; p <= m; ++p) {
       const f4 b = *reinterpret_cast<const f4 *>(&mat.b[16 * m + c16][16 * p + 4 * grp]);
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int e = 0; e < CE; ++e) o[m][e] = mfma_f32(b[s], u[p][e][s], o[m][e]);
+      for (int s = 0; s < 4; ++s) o[m] = mfma_f32(b[s], u[p][s], o[m]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -572,18 +567,8 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
       if (node >= n) continue;
       const int64_t row = base + node;
       const float nan = s_path[node] & bad ? NAN : 0.f;
-      const int64_t at = row * a.o_stride + vc;
-      float *tp = a.tape + (row * a.heads + h) * kTape + col;
-      if constexpr (CE == 2) {
-        if constexpr (DT == SOPHIA_DTYPE_BF16)
-          *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.o) + at) = pack_bf16x2(o[m][0][i] + nan, o[m][1][i] + nan);
-        else
-          *reinterpret_cast<f2 *>(static_cast<float *>(a.o) + at) = f2{o[m][0][i] + nan, o[m][1][i] + nan};
-        *reinterpret_cast<f2 *>(tp) = f2{u[m][0][i] + nan, u[m][1][i] + nan};
-      } else {
-        store_elem(a.o, at, DT, o[m][0][i] + nan);
-        *tp = u[m][0][i] + nan;
-      }
+      store_elem(a.o, row * a.o_stride + vc, DT, o[m][i] + nan);
+      a.tape[(row * a.heads + h) * kTape + col] = u[m][i] + nan;
     }
   }
 }
@@ -593,7 +578,8 @@ __global__ __launch_bounds__(NT, MT == 4 ? 2 : (NT == 512 ? 4 : (MT == 1 ? 3 : 2
 // layers, (layer) x tree for the MLA layers, all layers in one launch: the few
 // trees of a small batch then still fill the chip, and 28 launches become one.
 // Bound by the state: 64 KiB read and written per (layer, tree, head), in place,
-// as the decode step moves it (thread: 4 columns of every 16th row).
+// as the decode step moves it (thread: 4 columns of every 16th row).  28 layers of 48
+// trees: 2.3 GB in 393 us, 5.9 TB/s (a copy of 1 GiB: 5.2); of 4 trees: 192 MB in 41 us.
 struct CommitArgs {
   Trees trees;
   const int32_t *path;
@@ -733,17 +719,17 @@ extern "C" int sophia_kda_tree_step(const void *x_q, const void *x_k, const void
                        lower_bound, flags, state, n_slots, slots, num_heads, o, o_row_stride, tape};
   const dim3 grid(num_heads, n_trees);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-#define SOPHIA_TREE_STEP(MT, NT)                                                                            \
-  if (x_dtype == SOPHIA_DTYPE_BF16)                                                                         \
-    hipLaunchKernelGGL((kda_tree_step_kernel<MT, NT, SOPHIA_DTYPE_BF16>), grid, dim3(NT), 0, st, a);        \
-  else                                                                                                      \
-    hipLaunchKernelGGL((kda_tree_step_kernel<MT, NT, SOPHIA_DTYPE_F32>), grid, dim3(NT), 0, st, a);
+#define SOPHIA_TREE_STEP(MT)                                                                            \
+  if (x_dtype == SOPHIA_DTYPE_BF16)                                                                     \
+    hipLaunchKernelGGL((kda_tree_step_kernel<MT, SOPHIA_DTYPE_BF16>), grid, dim3(kThreads), 0, st, a);        \
+  else                                                                                                  \
+    hipLaunchKernelGGL((kda_tree_step_kernel<MT, SOPHIA_DTYPE_F32>), grid, dim3(kThreads), 0, st, a);
   if (max_nodes <= 16) {
-    SOPHIA_TREE_STEP(1, 512)
+    SOPHIA_TREE_STEP(1)
   } else if (max_nodes <= 32) {
-    SOPHIA_TREE_STEP(2, 512)
+    SOPHIA_TREE_STEP(2)
   } else {
-    SOPHIA_TREE_STEP(4, 512)
+    SOPHIA_TREE_STEP(4)
   }
 #undef SOPHIA_TREE_STEP
   return check_launch("kda_tree_step");

@@ -7,10 +7,15 @@
 // sequence.  It counts the sequence's history into LDS (integer atomics, whose
 // order does not matter), lays the biases of the tile beside the counts, and then
 // streams its rows through both.  Tokens of a tree are few and mostly in other
-// tiles, so a row's ancestors are compared one by one.
+// tiles, so a row's own ones are taken one by one, by the thread that has each.
+// 362 rows of 24 trees, 65,536 tokens, bf16, histories of up to 4,000 tokens: 96 MB in
+// 30 us (18.6 at the rate of a copy; about a third of a work-group's time is its
+// setup); 8 rows in fp32: 4.2 MB in 5.2 us, latency.
 //
 // Accept: the chosen tokens of all rows in parts, then one wavefront per tree,
-// whose lanes are the nodes, joins the parts and walks: a step is one ballot.
+// whose lanes are the nodes, joins the parts and walks: a step is one ballot.  1,061
+// rows of 64 trees, bf16: 139 MB in 22 us, 6.3 TB/s, and 4 for the walk; 7 rows 3.3
+// and 2.5.
 #include "common.hpp"
 #include "tree.hpp"
 

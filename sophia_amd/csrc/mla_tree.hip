@@ -18,6 +18,18 @@
 // with a mask per column.  A drafted latent that is not finite would reach every
 // node through the products (0 times infinity): it enters them as zeros, and the
 // nodes that do see it end as NaN.
+//
+// What bounds it: 32 trees of 24 to 64 nodes after 60 to 4,000 keys (11.7 GFLOP, 11 us at
+// the rate of a large product) take 29 us and 9 for the merge: a tile of 8 nodes is
+// 32 MFMAs per wavefront, 1,024 cycles, and about 330 vector instructions, mostly the
+// softmax, and two wavefronts per SIMD (216 registers) do one in 2,300 cycles each;
+// before and after its tiles a work-group spends as much as three of them take.  One
+// tree of 7 nodes after 523 keys takes 9 us and 4, all of it latency.  On the way, for
+// the 32 trees: ranges by number instead of length 79; three copies of the tile's code
+// for masked and whole tiles, whose spilled registers were waited for together with
+// the next tile 50 + 8; one copy 42 + 8; shares from a list of what there is, instead
+// of a grid over the bounds, which left CUs without work beside others with two shares,
+// and partials stored as the lanes hold them 29 + 9.
 #include <type_traits>
 
 #include "common.hpp"
@@ -59,10 +71,11 @@ __device__ __forceinline__ f16v mfma32x32(const bf8 &a, const bf8 &b, const f16v
 }
 
 // Cached keys of a tree: -1 when its slot is out of range (its rows are then zeros).
+// No branch: both loads are then under way together.
 __device__ __forceinline__ int cached_keys(const MlaTreeArgs &a, int tree, int64_t &slot) {
+  const int64_t keys = iclamp64(a.cached[tree], 0, a.max_seq);
   slot = a.slots ? a.slots[tree] : tree;
-  if (slot < 0 || slot >= a.n_slots) return -1;
-  return static_cast<int>(iclamp64(a.cached[tree], 0, a.max_seq));
+  return slot >= 0 && slot < a.n_slots ? static_cast<int>(keys) : -1;
 }
 
 // Ranges of a tree with `tiles` tiles.
@@ -86,13 +99,11 @@ __device__ __forceinline__ bool find_work(const MlaTreeArgs &a, Work &w) {
   int64_t base = 0, slot = 0;
   int n = 0, keys = 0, used = 0, mine = 0, sum = 0;
   const auto look = [&](int tree) {
-    mine = 0;
-    if (tree < a.n_trees) {
-      keys = cached_keys(a, tree, slot);
-      n = tree_nodes(a.trees, tree, base);
-      used = keys < 0 ? 1 : ranges(a, (keys + kTile - 1) / kTile + 1);
-      mine = used * ((n + kGroup<F32> - 1) / kGroup<F32>);
-    }
+    const int in = min(tree, a.n_trees - 1);
+    keys = cached_keys(a, in, slot);
+    n = tree_nodes(a.trees, in, base);
+    used = keys < 0 ? 1 : ranges(a, (keys + kTile - 1) / kTile + 1);
+    mine = tree == in ? used * ((n + kGroup<F32> - 1) / kGroup<F32>) : 0;
     sum = wave_scan(mine);
     return __builtin_amdgcn_readlane(sum, 63);
   };
@@ -269,6 +280,10 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
   const uint64_t path = w.drafted ? path_of(w, parent, node) : 0;
   const bool idle = w.node0 + 2 * wave >= w.n;   // (of the whole wavefront)
 
+  // Q is waited for here: a wait for it inside the loop would be one for the next
+  // tile's loads too, every time.
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
   // This lane's places within a tile: K row ln (32 kt rows on: a constant), V rows
   // 4 half + l16 / 4 (16 kp rows on: a constant; 8 rows on: the chunk's lowest bit turns).
   int ko[KS], vo[DT];
@@ -378,7 +393,9 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 
 // ---- fp32 ----------------------------------------------------------------------
 // 16x16x4 MFMAs in fp32 throughout: an fp32 model's latents have more bits than
-// bf16 holds.  A lane's four consecutive ranks of a key are the A operands of four
+// bf16 holds.  5 trees of 1 to 32 nodes after up to 3,001 keys: 18 us and 6 for the
+// merge; a tile takes a wavefront 256 MFMAs of 32 cycles, and only the keys divide it
+// further.  A lane's four consecutive ranks of a key are the A operands of four
 // steps (the k index runs 4 (lane / 16) + step), and the scores' accumulator, keys
 // 4 (lane / 16) + i, is the B operand of the value product in the same order.
 template <int R>
@@ -408,6 +425,8 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(Mla
     ot[b] = f4{0.f, 0.f, 0.f, 0.f};
   }
   const uint64_t path = w.drafted ? path_of(w, parent, node) : 0;
+#pragma unroll
+  for (int b = 0; b < KB; ++b) asm volatile("" : "+v"(qf[b]));   // (waited for here, not in the loop)
   float m_run = -INFINITY, l_run = 0.f;   // l_run over this lane's keys alone
   const auto stage = [&]() {
     using St = Stage<R, true>;
@@ -478,8 +497,8 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(Mla
 }
 
 // Joins the ranges of a tree: work-groups (group of nodes and an eighth of the
-// quads, tree), a wavefront as in the attention, a thread four ranks at a time.  Eight partials
-// are loaded before the first is used.
+// quads, tree), a wavefront as in the attention, a thread four ranks at a time.  Eight
+// partials are loaded before the first is used.
 constexpr int kMergeParts = 8;
 template <int R, bool F32>
 __global__ __launch_bounds__(256) void mla_tree_merge_kernel(MlaTreeArgs a) {

@@ -1742,12 +1742,12 @@ def mla_tree_splits(trees: int, max_nodes: int, max_len: int, dtype: torch.dtype
     and after its tiles and a partial of each node in the merge, so long lists of
     work take 8 (us with the merge, bf16: 32 trees of 24 to 64 nodes after up to
     4,000 keys 38 with 8, 44 with 6, 67 with 2), and where they do not fill the chip
-    each tile more is latency (one tree after 523 keys 12.4 with 2, 13.5 with 3,
-    16.5 with 8).  An fp32 tile takes three times as long: 2 (5 trees after up to
-    3,000 keys 23 with 2, 27 with 3 and with 1)."""
+    each tile more is latency (one tree after 523 keys 13 with 2, 14 with 3, 17 with
+    8).  An fp32 tile takes three times as long: 2 (5 trees after up to 3,001 keys 24
+    with 2, 27 with 3, 28 with 1)."""
     tiles = -(-max_len // 64) + 1
     work = max(trees, 1) * -(-max_nodes // 8) * tiles   # at the bounds; a ragged batch has about half
-    least = 2 if dtype == torch.float32 else min(8, max(2, work // 2048))
+    least = 2 if dtype == torch.float32 else min(8, max(2, work // 1024))
     # at most 128 ranges for the merge to join one after the other, and no workspace
     # past what keeps the chip busy
     return -(-tiles // max(least, -(-work // 8192), -(-tiles // 128)))
