@@ -38,7 +38,7 @@ extern "C" {
  *   q, k, v = silu(conv) of the q | k | v channels, whose earlier samples are the
  *             node's ancestors and then the cached history (rounded to x's type, as the
  *             decode step rounds it); q, k normalised (flag), q times scale
- *   G_i = sum over anc(i) of the log-decay
+ *   G_i = sum over anc(i) of the log-decay (below -104, where e^x is 0 in fp32: -104)
  *   u_i = beta_i (v_i - S^T (k_i e^G_i) - sum_{j in anc(i), j != i} (k_i . k_j e^(G_i - G_j)) u_j)
  *   o_i = S^T (q_i e^G_i) + sum_{j in anc(i)} (q_i . k_j e^(G_i - G_j)) u_j
  * All of it in fp32; o is rounded once.
@@ -150,7 +150,7 @@ int sophia_adjust_logits(const void *logits, int64_t logits_stride, void *out, i
  * The model's choice at every node, and the walk along the drafted tokens that
  * agree with it:
  *   chosen[r]   = the index of row r's greatest logit, of equal ones the lowest (NaN is
- *                 never chosen; a row without a value above -inf gives 0)
+ *                 never chosen; a row without a value above -inf gives 0); of all rows
  *   path[s]     = node 0, then again and again the first child whose token is the choice of
  *                 the node before it; -1 behind the path (max_nodes entries, stride path_stride)
  *   n_path[s]   = its length (0 for a tree without nodes)

@@ -85,6 +85,10 @@ struct TreeStepArgs {
 // nodes has lost e^-1 and more at every one of them, and its part in A and B with it.
 constexpr float kFactored = 60.f;
 
+// Log-decays below this one count as it: e^-104 is 0 in fp32 as theirs is, and a G that
+// holds them still tells apart what is added to it (-inf and the lowest float do not).
+constexpr float kForgotten = -104.f;
+
 // Eight elements of a row as they lie, and as floats: four from p on and the four 64
 // places behind them.  Over 16 threads each half is contiguous, which eight in a row
 // per thread are not (two of them then meet in every LDS bank).
@@ -333,6 +337,7 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
       const float z = g16 ? __uint_as_float(c & 1 ? w & 0xffff0000u : w << 16)
                           : __uint_as_float(raw_g[p][2 * (c >> 2) + ((c & 3) >> 1)][c & 1]);
       g[p][c] = gate ? kda_log_decay(z, head_scale, bias[c], a.lower_bound) : z;
+      g[p][c] = g[p][c] < kForgotten ? kForgotten : g[p][c];   // (NaN stays)
       ok &= is_finite(q[p][c]) && is_finite(k[p][c]) && is_finite(v[p][c]) && is_finite(g[p][c]);
     }
     if (((__ballot(!ok) >> (lane & 48)) & 0xffff) != 0) {   // (of the node's 16 threads alike)
@@ -724,6 +729,9 @@ extern "C" int sophia_kda_tree_step(const void *x_q, const void *x_k, const void
     hipLaunchKernelGGL((kda_tree_step_kernel<MT, SOPHIA_DTYPE_BF16>), grid, dim3(kThreads), 0, st, a);        \
   else                                                                                                  \
     hipLaunchKernelGGL((kda_tree_step_kernel<MT, SOPHIA_DTYPE_F32>), grid, dim3(kThreads), 0, st, a);
+  // By the bound on a tree's nodes: the least that holds it has the least LDS and registers,
+  // so more of its work-groups run together.  us, 16 heads, bf16: 64 trees of 32 nodes 62 as
+  // 32, 86 as 64; 64 of 8 nodes 38 as 16 or 32, 59 as 64; 8 of 16 nodes 17 as any.
   if (max_nodes <= 16) {
     SOPHIA_TREE_STEP(1)
   } else if (max_nodes <= 32) {

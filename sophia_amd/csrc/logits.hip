@@ -266,7 +266,7 @@ struct AcceptArgs {
   int64_t *next, *chosen;
 };
 
-// The greater logit, of equal ones the lower index.
+// The greater logit, of equal ones the lower index (of -inf any: join_parts).
 __device__ __forceinline__ void better(float &v, int &i, float v2, int i2) {
   const bool take = v2 > v || (v2 == v && i2 < i);
   v = take ? v2 : v;
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256) void argmax_part_kernel(AcceptArgs a) {
   const int v0 = part * a.per_part, v1 = min(a.vocab, v0 + a.per_part);
   const int64_t xr = row * a.x_stride;
   float best = -INFINITY;
-  int at = 0x7fffffff;   // nothing above -inf
+  int at = 0x7fffffff;
   const auto see = [&](float v, int i) {
     if (v > best) {      // (never for NaN; indices rise, so an equal one is not lower)
       best = v;
@@ -342,7 +342,7 @@ __device__ __forceinline__ int join_parts(const AcceptArgs &a, int64_t row) {
   for (int p = 0; p < kParts; ++p) v[p] = a.part[row * a.parts + min(p, a.parts - 1)];   // the last one again
 #pragma unroll
   for (int p = 0; p < kParts; ++p) better(best, at, v[p].x, __float_as_int(v[p].y));
-  return at == 0x7fffffff ? 0 : at;
+  return best > -INFINITY ? at : 0;
 }
 
 // Work-group per tree (the walk), then one per 64 rows (`chosen`, of all rows).
@@ -456,8 +456,9 @@ extern "C" int sophia_tree_accept(const void *logits, int64_t logits_stride, int
   SOPHIA_REQUIRE(max_nodes >= 1 && max_nodes <= kTreeNodes && path_stride >= max_nodes,
                  "tree_accept: max_nodes must be in [1, %d] and path rows at least as long", kTreeNodes);
   SOPHIA_REQUIRE(logits_stride >= vocab, "tree_accept: row stride smaller than a row");
-  if (n_trees == 0) return SOPHIA_OK;
-  SOPHIA_REQUIRE((rows == 0 || (logits && tokens && parents && chosen)) && cu_nodes && path && n_path && next_token,
+  if (n_trees == 0 && rows == 0) return SOPHIA_OK;
+  SOPHIA_REQUIRE((rows == 0 || (logits && tokens && parents && chosen)) &&
+                     (n_trees == 0 || (cu_nodes && path && n_path && next_token)),
                  "tree_accept: NULL pointer");
   SOPHIA_REQUIRE(rows == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0 &&
                                workspace_bytes >= sophia_tree_accept_workspace_size(rows, vocab)),

@@ -1768,8 +1768,8 @@ def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: to
     a multiple of 8, 16-byte aligned); conv_weight: [3 * H * 128, K] fp32 taps
     rounded to x_qkv.dtype, K in 1..4; conv_state: fp32 [slots, 3 * H * 128,
     K - 1] (None for K = 1); g: [rows, H, 128] decay logits, or with
-    ``use_gate=False`` finite log-decays; beta: [rows, H]; state: fp32 [slots, H,
-    128, 128]; cu_nodes, parents, max_nodes: as in ``mla_tree_attn``.  q, k and v
+    ``use_gate=False`` log-decays (-inf: the state is forgotten); beta: [rows, H];
+    state: fp32 [slots, H, 128, 128]; cu_nodes, parents, max_nodes: as in ``mla_tree_attn``.  q, k and v
     stay in fp32 from the conv on.  Returns (o [rows, H, 128] in x_qkv.dtype,
     tape [rows, H, 3, 128] fp32: what ``tree_commit`` takes to advance the state
     along an accepted path)."""
@@ -1863,7 +1863,7 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
     index = path.get_device()
     count = _int32(n_path, "n_path", device)
     cu = _int32(cu_nodes, "cu_nodes", device)
-    if count.numel() != n or cu.numel() != n + 1:
+    if count is None or cu is None or count.numel() != n or cu.numel() != n + 1:
         raise RuntimeError(f"n_path must hold {n} and cu_nodes {n + 1} entries")
     kda, mla = list(kda), list(mla)
     if not kda and not mla:
@@ -1948,8 +1948,9 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
 
     A token seen before has x / repetition (x > 0) or x * repetition, less
     frequency * count and presence; then the biases are added; tokens that are
-    not allowed get -inf (a row whose mask allows nothing is all -inf).  Returns
-    ``out`` (may be ``logits``; default a new tensor of logits' dtype)."""
+    not allowed get -inf (a row whose mask allows nothing is all -inf).  Rows of
+    no tree are left as they are.  Returns ``out`` (may be ``logits``; default a
+    new tensor of logits' dtype)."""
     _gpu(logits, "logits")
     device = logits.device
     if logits.dim() != 2:
@@ -2032,9 +2033,10 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tens
     starts at node 0 of its tree (the token that was known already) and goes on to
     the first child whose token is its parent's choice.  Returns (path int32 [N,
     max_nodes], -1 behind its end; n_path int32 [N]; next_token int64 [N], the
-    choice at the path's end; chosen int64 [rows], the lowest index of each row's
-    greatest logit, NaN never, and of rows without a value above -inf 0).  A tree
-    without nodes has an empty path and next_token -1.  To sample instead of choosing, add Gumbel noise to the logits."""
+    choice at the path's end; chosen int64 [rows], of rows of no tree too, the
+    lowest index of each row's greatest logit, NaN never, and of rows without a
+    value above -inf 0).  A tree without nodes has an empty path and next_token
+    -1.  To sample instead of choosing, add Gumbel noise to the logits."""
     _gpu(logits, "logits")
     device = logits.device
     if logits.dim() != 2 or int(logits.size(1)) < 1:

@@ -260,6 +260,38 @@ def test_tree_step_of_a_chain_is_the_decode_steps():
     _within(state2, state.double().cpu(), torch.full_like(state2, 2 * float(tol_o.max())).double().cpu())
 
 
+@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.float32).min, -1e5])
+def test_tree_step_log_decays_that_forget_the_state(low):
+    """Log-decays whose exponential is 0 in fp32 count as -104, the last whole number of that kind (e^-104 = 7e-46): what
+    follows a forgotten state keeps its own decays, and so does a commit."""
+    from sophia_amd import ops
+    tr, c = _step_case([18, 40, 5], kind="wide", dtype=F32, gate=False, seed=17)
+    gen = torch.Generator().manual_seed(3)
+    hit = torch.rand(c["g"].shape, generator=gen) < 0.1
+    hit[tr.offsets[1] + 1] = True      # a whole row, near the root
+    o, want, states = ref.kda_step(tr, **{**c, "g": torch.where(hit, -104.0, c["g"])}, gate=False)
+    c["g"] = torch.where(hit, low, c["g"])
+    got, tape = _run_step(tr, c, gate=False)
+    tol_o, tol = _step_tol(tr, o, want, F32)
+    n = torch.zeros(tr.total, 1, 1, dtype=torch.float64)
+    for _, row, path, _ in tr.nodes():
+        n[row] = len(path)
+    tol[:, :, 2] = n * want[:, :, 2].abs() * E32     # (sums beyond the bound of 5 that _step_tol counts)
+    _within(tape, want, tol)
+    _within(got, o, tol_o)
+    last = [tr.paths[s][-1] for s in range(3)]
+    path = torch.full((3, max(map(len, last))), -1, dtype=torch.int32)
+    for s, nodes in enumerate(last):
+        path[s, :len(nodes)] = torch.tensor(nodes, dtype=torch.int32)
+    state = c["state"].cuda()
+    ops.tree_commit(path.cuda(), torch.tensor([len(p) for p in last], dtype=torch.int32, device="cuda"), tr.cu.cuda(),
+                    c["slots"].cuda(), kda=[(tape, c["x"].cuda(), c["conv_state"].cuda(), state)])
+    for s in range(3):
+        row = tr.offsets[s] + last[s][-1]
+        full = torch.full_like(states[row], float(tol[row, :, 0].max()) * 4)
+        _within(state[int(c["slots"][s])], states[row], full)
+
+
 def test_tree_step_nan_stays_on_its_paths():
     tr, c = _step_case([40, 12], kind="wide", dtype=F32, seed=9)
     o, want, _ = ref.kda_step(tr, **c)
@@ -453,6 +485,38 @@ def test_accept_matches_reference(lens, kind, vocab, dtype):
         path, n_path, following, said = ops.tree_accept(logits, tokens.cuda(), tr.cu.cuda(), tr.par.cuda(), max_nodes=bound)
         assert (path.tolist(), n_path.tolist(), following.tolist(), said.tolist()) == want
         assert path.dtype == n_path.dtype == torch.int32 and following.dtype == said.dtype == torch.int64
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [4, 13, 2051, 9003])
+def test_accept_of_padded_rows_without_a_choice(vocab, dtype):
+    """Rows of -inf and NaN alone choose 0, whatever the alignment of the row's last logits; values behind a row are not
+    its own."""
+    from sophia_amd import ops
+    tr = ref.Trees([6], "wide", 0)
+    wide = torch.full((6, -(-vocab // 8) * 8), 9.0, dtype=dtype)
+    x = wide[:, :vocab]
+    x[:] = float("-inf")
+    x[1] = float("nan")
+    x[2, -1] = float("nan")
+    x[3, -1] = -3.0
+    x[4, -2:] = 1.0
+    x[5, 0] = torch.finfo(dtype).min
+    tokens = torch.zeros(6, dtype=torch.int64)
+    want = ref.accept(tr, x, tokens, 6)
+    assert want[3] == [0, 0, 0, vocab - 1, vocab - 2, 0]
+    got = ops.tree_accept(wide.cuda()[:, :vocab], tokens.cuda(), tr.cu.cuda(), tr.par.cuda(), max_nodes=6)
+    assert tuple(t.tolist() for t in got) == want
+
+
+def test_accept_chooses_for_rows_of_no_tree_too():
+    from sophia_amd import ops
+    x = torch.randn(70, 33, generator=torch.Generator().manual_seed(1)).cuda()
+    tokens, par = torch.zeros(70, dtype=torch.int64, device="cuda"), torch.full((70,), -1, dtype=torch.int32, device="cuda")
+    for cu in ([0], [0, 3], [5, 5, 5]):
+        path, n_path, following, said = ops.tree_accept(x, tokens, torch.tensor(cu, dtype=torch.int32, device="cuda"), par,
+                                                        max_nodes=3)
+        assert torch.equal(said, x.argmax(-1)) and path.shape == (len(cu) - 1, 3)
 
 
 def test_no_trees_and_no_rows():
