@@ -588,8 +588,11 @@ class DraftTrees:
     the tree (before the node; -1: a root).  Node 0 is the sequence's last known
     token, which is in no cache yet, the others are drafted continuations.
     ``slots`` [N] int32 are the (different) cache slots, ``cached`` [N] int64
-    the tokens in them.  ``max_nodes`` (at most 64) bounds the nodes of a tree,
-    ``max_len`` bounds ``cached``: host ints."""
+    the tokens in them; with the tree's deepest path they fit max_seq_len.
+    ``max_nodes`` (at most 64) bounds the nodes of a tree, ``max_len`` bounds
+    ``cached``: host ints.  Trees without nodes and rows behind the last tree
+    are allowed (their logits mean nothing): a captured step of a fixed number of
+    rows then takes trees of any size within it, copied into its tensors."""
 
     token_ids: torch.Tensor
     cu_nodes: torch.Tensor
@@ -934,7 +937,7 @@ class Transformer(nn.Module):
         rows, n = int(trees.token_ids.numel()), int(trees.slots.numel())
         if rows == 0 or n == 0:
             raise ValueError("empty step")
-        if int(trees.max_len) < 0 or int(trees.max_len) + int(trees.max_nodes) > int(self.args.max_seq_len):
+        if not 0 <= int(trees.max_len) < int(self.args.max_seq_len):
             raise ValueError("sequence exceeds max_seq_len")
         if not self.args.use_cache:
             raise RuntimeError("forward_tree needs use_cache=True (it reads cache slots)")

@@ -157,7 +157,8 @@ def pack_trees(model: Transformer, trees, slots, cached) -> DraftTrees:
     """``DraftTrees`` on the model's device from host lists: ``trees[s]`` =
     (tokens, parents) of sequence s, node 0 its last known token (parent -1),
     each other node after its parent (an index into the tree); ``slots[s]`` its
-    cache slot and ``cached[s]`` the tokens in it."""
+    cache slot and ``cached[s]`` the tokens in it, to which the deepest path is
+    added within max_seq_len."""
     dev = model.tok_embeddings.weight.device
     slots, cached = ([int(v) for v in (t.tolist() if isinstance(t, torch.Tensor) else t)] for t in (slots, cached))
     if not len(trees) == len(slots) == len(cached):
@@ -168,18 +169,21 @@ def pack_trees(model: Transformer, trees, slots, cached) -> DraftTrees:
     if any(not 0 <= s < capacity for s in slots):
         raise ValueError(f"cache slots must be in [0, {capacity})")
     tokens, parents, offsets = [], [], [0]
-    for toks, pars in trees:
+    for (toks, pars), length in zip(trees, cached):
         if len(toks) != len(pars) or not 1 <= len(toks) <= ops.TREE_NODES:
             raise ValueError(f"a tree has 1..{ops.TREE_NODES} nodes, each with a token and a parent")
         if int(pars[0]) != -1 or any(not 0 <= int(p) < i for i, p in enumerate(pars) if i):
             raise ValueError("node 0 is the root (parent -1), and every other node comes after its parent")
         if any(not 0 <= int(t) < int(model.args.vocab_size) for t in toks):
             raise ValueError("a token is outside the vocabulary")
+        depth = [length + 1]
+        for p in pars[1:]:
+            depth.append(depth[int(p)] + 1)
+        if length < 0 or max(depth) > int(model.args.max_seq_len):
+            raise ValueError("cached token counts must be >= 0" if length < 0 else "sequence exceeds max_seq_len")
         tokens += [int(t) for t in toks]
         parents += [int(p) for p in pars]
         offsets.append(len(tokens))
-    if any(c < 0 for c in cached):
-        raise ValueError("cached token counts must be >= 0")
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
     i64 = lambda v: torch.tensor(v, dtype=torch.int64, device=dev)  # noqa: E731
     return DraftTrees(i64(tokens), i32(offsets), i32(parents), i32(slots), i64(cached),

@@ -204,6 +204,126 @@ def test_verify_step_captured_replays_as_it_runs_eager():
             assert torch.equal(a, b)
 
 
+def _pad(trees, n, rows):
+    """``trees`` with trees without nodes up to ``n`` (their slots are taken by nobody), and rows of no tree up to ``rows``."""
+    from dataclasses import replace
+    grow = lambda t, size, v: torch.cat([t, t.new_full((size - t.numel(),), v)])  # noqa: E731
+    return replace(trees, token_ids=grow(trees.token_ids, rows, 0), parents=grow(trees.parents, rows, -1),
+                   cu_nodes=grow(trees.cu_nodes, n + 1, int(trees.cu_nodes[-1])), slots=grow(trees.slots, n, -1),
+                   cached=grow(trees.cached, n, 0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_captured_step_takes_padded_batches_of_any_trees(dtype):
+    """One captured step of 40 rows and 4 trees, with trees of other sizes, sequences and contexts at every replay, is what
+    the step of those trees alone gives, and leaves all other slots as they were."""
+    from dataclasses import replace
+    from sophia_amd.runtime import pack_trees, verify_trees
+    model = _model(seed=6, dtype=dtype, mla_kv_rank=64)
+    lens = [90, 1, 300, 64, 7, 129]
+    _prefill(model, list(range(6)), lens)
+    start = _caches(model)
+    rng = random.Random(4)
+
+    def batch(sizes):
+        trees = [([rng.randrange(512) for _ in range(n)], [-1] + [rng.randrange(i) for i in range(1, n)]) for n in sizes]
+        slots = rng.sample(range(6), len(sizes))
+        return pack_trees(model, trees, slots, [lens[s] for s in slots])
+    static = replace(_pad(batch([3]), 4, 40), max_nodes=24, max_len=320)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        verify_trees(model, static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = verify_trees(model, static)
+    for sizes in ([24, 1, 9, 6], [5], [13, 17], []):
+        if sizes:
+            trees = batch(sizes)
+            padded = _pad(trees, 4, 40)
+        else:
+            padded = _pad(replace(trees, cu_nodes=trees.cu_nodes[:1], slots=trees.slots[:0], cached=trees.cached[:0]), 4, 40)
+        for name in ("token_ids", "parents", "cu_nodes", "slots", "cached"):
+            getattr(static, name).copy_(getattr(padded, name))
+        _load(model, start)
+        want = verify_trees(model, replace(padded, max_nodes=24, max_len=320))
+        eager = _caches(model)
+        _load(model, start)
+        graph.replay()
+        torch.cuda.synchronize()
+        n, rows = len(sizes), sum(sizes)
+        for name in ("path", "n_path", "next_token", "cached"):
+            assert torch.equal(getattr(out, name), getattr(want, name)), name
+        assert torch.equal(out.logits[:rows], want.logits[:rows])
+        for a, b in zip(_caches(model), eager):
+            assert torch.equal(a, b)
+        assert out.n_path[n:].tolist() == [0] * (4 - n) and out.next_token[n:].tolist() == [-1] * (4 - n)
+        used = trees.slots.tolist() if sizes else []
+        for a, b in zip(eager, start):
+            for slot in set(range(6)) - set(used):
+                assert torch.equal(a[slot], b[slot])
+        if sizes:     # the trees alone: other bounds, so other divisions of the work
+            _load(model, start)
+            alone = verify_trees(model, trees)
+            assert _rel(out.logits[:rows].float(), alone.logits.float()) <= (1e-4 if dtype == torch.float32 else 6e-2)
+            if dtype == torch.float32:
+                assert alone.n_path.tolist() == out.n_path[:n].tolist() and alone.next_token.tolist() == out.next_token[:n].tolist()
+
+
+def test_caches_may_grow_between_a_drafted_step_and_its_commit():
+    from sophia_amd.runtime import pack_trees
+    model, other = _model(seed=4), _model(seed=4)
+    paths = torch.tensor([[0, 1], [0, -1]], dtype=torch.int32, device="cuda"), torch.tensor([2, 1], dtype=torch.int32, device="cuda")
+    for m in (model, other):
+        _prefill(m, [5, 1], [33, 60])
+        draft = m.forward_tree(pack_trees(m, TREES[:2], [5, 1], [33, 60]))
+        if m is other:
+            m.ensure_batch_capacity(9)
+        m.commit_tree(draft, *paths)
+    for a, b in zip(_caches(model), _caches(other)):
+        assert b.size(0) == 9 and torch.equal(a, b[:6]) and not b[6:].any()
+
+
+def test_two_drafted_steps_of_different_sequences_on_two_streams():
+    """Two steps under way at once, each on its stream, of different slots: as one after the other."""
+    from sophia_amd.runtime import pack_trees, verify_trees
+    model = _model(seed=5, dtype=torch.bfloat16, mla_kv_rank=128)
+    slots, lens = [0, 3, 4], [200, 17, 80]
+    _prefill(model, slots, lens)
+    start = _caches(model)
+    batches = [pack_trees(model, TREES[:2], slots[:2], lens[:2]), pack_trees(model, TREES[2:], slots[2:], lens[2:])]
+    want = [verify_trees(model, b) for b in batches]
+    after = _caches(model)
+    _load(model, start)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in batches]
+    got = []
+    for b, s in zip(batches, streams):
+        with torch.cuda.stream(s):
+            got.append(verify_trees(model, b))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for name in ("path", "n_path", "next_token", "cached", "logits"):
+            assert torch.equal(getattr(g, name), getattr(w, name)), name
+    for a, b in zip(_caches(model), after):
+        assert torch.equal(a, b)
+
+
+def test_trees_reach_the_end_of_the_context():
+    """A short tree at the cache's last positions beside a long one elsewhere."""
+    from sophia_amd.runtime import pack_trees, verify_trees
+    model = _model()
+    _prefill(model, [0, 1], [398, 5])
+    trees = pack_trees(model, [([1, 2, 3], [-1, 0, 0]), ([4] * 64, [-1] + [0] * 63)], [0, 1], [398, 5])
+    out = verify_trees(model, trees)
+    assert out.cached.tolist()[0] in (399, 400)
+    mla = next(layer.attn for layer in model.layers if layer.layer_type == "mla")
+    assert mla.latent_cache[0, :int(out.cached[0])].abs().sum(-1).gt(0).all()
+    with pytest.raises(ValueError, match="max_seq_len"):
+        pack_trees(model, [([1, 2, 3], [-1, 0, 1])], [0], [398])
+
+
 def test_tree_step_refusals():
     from sophia_amd.runtime import pack_trees
     model = _model()
