@@ -21,9 +21,10 @@
 // Everything is fp32 (the matrix products too): u enters the cached state with
 // the accepted path, and the decode step that the state otherwise comes from
 // is fp32 as well.  A and B are (K e^G) (K e^-G)^T and (Q e^G) (K e^-G)^T on MFMAs
-// where |G| stays below kFactored; beyond it e^-G would leave the range of fp32, and
-// they are formed per pair of a node and an ancestor on the vector unit, from
-// e^(G_i - G_j), whose argument is never positive.
+// where |G| stays below kFactored.  Beyond it e^-G would leave the range of fp32: then
+// tile by tile of 16 nodes with a reference near both (K e^(G - R)) (K e^(R - G))^T, and
+// tiles whose nodes have lost too different parts for any one reference per pair of a node
+// and an ancestor on the vector unit, from e^(G_i - G_j), whose argument is never positive.
 //
 // What bounds it: the steps' latency.  One tree of 7 nodes takes 13 us (16 heads on
 // as many CUs, 25,000 cycles from the first load to the last store), 64 trees of 8 to
@@ -84,6 +85,11 @@ struct TreeStepArgs {
 // 2.6e-6, where e^(G_i - G_j) is not; a channel that has come that far within 64
 // nodes has lost e^-1 and more at every one of them, and its part in A and B with it.
 constexpr float kFactored = 60.f;
+// Beyond it the exponents are G_i - R and R - G_j, R the largest G of i's 16 nodes, so the
+// first is never positive.  The second may reach kFar, where e^x is in the range of fp32
+// still; past kNear the first must stay in that range too, as e^(G_i - G_j) may then be
+// large although e^(G_i - R) is lost (below kNear it is under e^-60).
+constexpr float kFar = 80.f, kNear = 20.f;
 
 // Log-decays below this one count as it: e^-104 is 0 in fp32 as theirs is, and a G that
 // holds them still tells apart what is added to it (-inf and the lowest float do not).
@@ -461,40 +467,78 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
         write8(&mat.k[r0 + RP * p][seg], k[p]);
         write8(&mat.g[r0 + RP * p][seg], g[p]);
       }
-    for (int i = t; i < T * Lds::LA; i += kThreads) (&mat.a[0][0])[i] = (&mat.b[0][0])[i] = 0.f;
     lds_barrier();
-    // A wavefront takes a node, 16 lanes one of its ancestors.
-    for (int i = wave; i < n; i += kWaves) {
-      uint64_t left = s_path[i];
-      float qi[8], ki[8], gi[8];
-      read8(&mat.q[i][4 * c16], qi);
-      read8(&mat.k[i][4 * c16], ki);
-      read8(&mat.g[i][4 * c16], gi);
-      while (left) {
-        int j = -1;
+    // Tiles (ti, tj) of A and of B, one wavefront each.
+    for (int u = wave; u < mt * (mt + 1) / 2; u += kWaves) {
+      int ti = 0, tj = u;
+      while (tj > ti) tj -= ++ti;
+      const uint64_t mine = s_path[16 * ti + c16] >> (16 * tj) & 0xffff;
+      bool seen = false;        // node c16 of tile tj is on the path of one of tile ti
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int low = left ? __ffsll(static_cast<unsigned long long>(left)) - 1 : -1;
-          if (grp == e) j = low;
-          left &= left - 1;   // (0 stays 0)
-        }
-        float kk = 0.f, qk = 0.f;
-        if (j >= 0) {
-          float kj[8], gj[8];
-          read8(&mat.k[j][4 * c16], kj);
-          read8(&mat.g[j][4 * c16], gj);
+      for (int i = 0; i < 16; ++i) seen |= (s_path[16 * ti + i] >> (16 * tj + c16)) & 1;
+      f4 acc_a = {0.f, 0.f, 0.f, 0.f}, acc_b = acc_a;
+      float low = 0.f, high = 0.f;   // of the exponents
+      if (__any(mine != 0)) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float w = kj[c] * __expf(gi[c] - gj[c]);
-            kk = fmaf(ki[c], w, kk);
-            qk = fmaf(qi[c], w, qk);
+        for (int blk = 0; blk < kD / 16; ++blk) {
+          const int at = 16 * blk + 4 * grp, i = 16 * ti + c16, j = 16 * tj + c16;
+          const f4 ki = *reinterpret_cast<const f4 *>(&mat.k[i][at]), qi = *reinterpret_cast<const f4 *>(&mat.q[i][at]);
+          const f4 gi = *reinterpret_cast<const f4 *>(&mat.g[i][at]);
+          const f4 kj = *reinterpret_cast<const f4 *>(&mat.k[j][at]), gj = *reinterpret_cast<const f4 *>(&mat.g[j][at]);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const float r = row_max16(i < n ? gi[s] : -INFINITY);
+            const float ei = gi[s] - r, ej = r - gj[s];
+            if (i < n) low = fminf(low, ei);
+            if (seen) high = fmaxf(high, ej);
+            const float e = __expf(ei), right = kj[s] * __expf(ej);
+            acc_a = mfma_f32(ki[s] * e, right, acc_a);
+            acc_b = mfma_f32(qi[s] * e, right, acc_b);
           }
         }
-        kk = row_sum16(kk);
-        qk = row_sum16(qk);
-        if (j >= 0 && c16 == 0) {
-          mat.b[i][j] = qk;
-          if (j != i) mat.a[i][j] = -s_beta[i] * kk;
+      }
+      const bool in_range = !__any(high > kFar) && !(__any(high > kNear) && __any(low < -kFar));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * ti + 4 * grp + i, j = 16 * tj + c16;
+        const bool on = in_range && ((s_path[row] >> j) & 1);
+        mat.a[row][j] = on && row != j ? -s_beta[row] * acc_a[i] : 0.f;
+        mat.b[row][j] = on ? acc_b[i] : 0.f;
+      }
+      if (in_range) continue;
+      // Pair by pair, 16 lanes each.
+      for (int i = 16 * ti; i < min(n, 16 * ti + 16); ++i) {
+        uint64_t left = s_path[i] & 0xffffull << 16 * tj;
+        float qi[8], ki[8], gi[8];
+        read8(&mat.q[i][4 * c16], qi);
+        read8(&mat.k[i][4 * c16], ki);
+        read8(&mat.g[i][4 * c16], gi);
+        while (left) {
+          int j = -1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int next = left ? __ffsll(static_cast<unsigned long long>(left)) - 1 : -1;
+            if (grp == e) j = next;
+            left &= left - 1;   // (0 stays 0)
+          }
+          float kk = 0.f, qk = 0.f;
+          if (j >= 0) {
+            float kj[8], gj[8];
+            read8(&mat.k[j][4 * c16], kj);
+            read8(&mat.g[j][4 * c16], gj);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const float w = kj[c] * __expf(gi[c] - gj[c]);
+              kk = fmaf(ki[c], w, kk);
+              qk = fmaf(qi[c], w, qk);
+            }
+          }
+          kk = row_sum16(kk);
+          qk = row_sum16(qk);
+          if (j >= 0 && c16 == 0) {
+            mat.b[i][j] = qk;
+            if (j != i) mat.a[i][j] = -s_beta[i] * kk;
+          }
         }
       }
     }

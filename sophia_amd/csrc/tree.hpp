@@ -60,12 +60,19 @@ __device__ __forceinline__ f4 mfma_f32(float a, float b, const f4 &c) {
 
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
 
-// Sum over the 16 lanes of a row, in each of them.
+// Sum, and maximum, over the 16 lanes of a row, in each of them.
 __device__ __forceinline__ float row_sum16(float v) {
   v += dpp_rotate<0x128>(v);
   v += dpp_rotate<0x124>(v);
   v += dpp_rotate<0x122>(v);
   return v + dpp_rotate<0x121>(v);
+}
+
+__device__ __forceinline__ float row_max16(float v) {
+  v = fmaxf(v, dpp_rotate<0x128>(v));
+  v = fmaxf(v, dpp_rotate<0x124>(v));
+  v = fmaxf(v, dpp_rotate<0x122>(v));
+  return fmaxf(v, dpp_rotate<0x121>(v));
 }
 
 // Sum over this lane and those before it, without the LDS crossbar: shifts within

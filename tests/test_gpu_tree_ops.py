@@ -186,6 +186,10 @@ STEP = [
     dict(lens=[48], taps=3, gate=False),
     dict(lens=[15, 8], kind="chain", gate=False, g_dtype=F32),
     dict(lens=[64, 30, 16], kind="chain", strong=True),
+    dict(lens=[64, 41, 26], kind="branches", strong=True),
+    dict(lens=[64, 20, 15], strong=True, g_dtype=F32),
+    dict(lens=[64, 50], kind="branches", gate=False, g_dtype=F32),
+    dict(lens=[31, 64], kind="odd", strong=True, taps=1),
     dict(lens=[13], g_dtype=F32, heads=16),
 ]
 

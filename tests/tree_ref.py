@@ -8,7 +8,7 @@ import torch
 
 
 def parents_of(n: int, kind: str, rng: random.Random) -> list[int]:
-    """Parents of one tree: a chain, a wide tree, random ones, several roots, or entries that the operators read as
+    """Parents of one tree: a chain, a wide tree, random ones, long branches, several roots, or entries that the operators read as
     roots (not an earlier node)."""
     if kind == "chain":
         return [i - 1 for i in range(n)]
@@ -16,6 +16,8 @@ def parents_of(n: int, kind: str, rng: random.Random) -> list[int]:
         return [(i - 1) // 4 if i else -1 for i in range(n)]
     if kind == "forest":
         return [rng.randint(-1, i - 1) if rng.random() < 0.7 else -1 for i in range(n)]
+    if kind == "branches":     # one after the other, each from the root down
+        return [-1 if i == 0 else 0 if i % 21 == 0 else i - 1 for i in range(n)]
     if kind == "odd":
         return [rng.choice([i, i + 1, 70, -5, 2 ** 31 - 1, -2 ** 31, rng.randint(-1, i - 1)]) for i in range(n)]
     return [rng.randint(max(0, i - 5), i - 1) if i else -1 for i in range(n)]
