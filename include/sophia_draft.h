@@ -112,10 +112,11 @@ int sophia_tree_commit(const int32_t *path, int64_t path_stride, const int32_t *
  * product; fp32: fp32 products.  Scores, softmax and sums are fp32; out is rounded once.
  * rank in {32, 64, 128, 256}; heads <= 16; scale > 0; row strides multiples of 8, every
  * pointer 16-byte aligned.  With splits > 1 a tree's keys are divided into equal
- * ranges of about split_keys (a multiple of 64), at most `splits` of them; this needs a
- * workspace of sophia_mla_tree_workspace_size(rows, n_trees, rank, splits) bytes.
+ * ranges of split_keys (a multiple of 64) or more, as long as keeps the chip full, at most
+ * `splits` of them; this needs a workspace of sophia_mla_tree_workspace_size(n_trees,
+ * max_nodes, rank, dtype, splits) bytes.
  */
-size_t sophia_mla_tree_workspace_size(int64_t rows, int n_trees, int rank, int splits);
+size_t sophia_mla_tree_workspace_size(int n_trees, int max_nodes, int rank, int dtype, int splits);
 int sophia_mla_tree_attn(const void *qa, int64_t qa_stride, const void *latent, int64_t latent_stride, int dtype,
                          const float *cache, int64_t slot_stride, int n_slots, int max_seq, const int32_t *slots,
                          const int64_t *cached, const int32_t *cu_nodes, const int32_t *parents, int n_trees,

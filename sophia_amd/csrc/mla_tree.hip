@@ -9,7 +9,7 @@
 // holds 2 nodes in bf16, 1 in fp32.  Contexts and trees of a batch differ by far, and
 // the host does not know them: every work-group finds its share in the list of all
 // (tree, range, nodes), which it counts itself, a tree per lane.  A tree's ranges are
-// equally long, and all have about the same length.  Neighbours in the list, which
+// equally long, and all have about the same length, which follows from the whole work.  Neighbours in the list, which
 // read the same keys, run on one XCD, whose L2 serves all but the first of them.  A
 // tree of one range writes its result at once, the others partials that a second
 // kernel joins, both in the order in which the lanes hold them.
@@ -20,16 +20,19 @@
 // nodes that do see it end as NaN.
 //
 // What bounds it: 32 trees of 24 to 64 nodes after 60 to 4,000 keys (11.7 GFLOP, 11 us at
-// the rate of a large product) take 29 us and 9 for the merge: a tile of 8 nodes is
-// 32 MFMAs per wavefront, 1,024 cycles, and about 330 vector instructions, mostly the
-// softmax, and two wavefronts per SIMD (216 registers) do one in 2,300 cycles each;
-// before and after its tiles a work-group spends as much as three of them take.  One
-// tree of 7 nodes after 523 keys takes 9 us and 4, all of it latency.  On the way, for
-// the 32 trees: ranges by number instead of length 79; three copies of the tile's code
-// for masked and whole tiles, whose spilled registers were waited for together with
-// the next tile 50 + 8; one copy 42 + 8; shares from a list of what there is, instead
-// of a grid over the bounds, which left CUs without work beside others with two shares,
-// and partials stored as the lanes hold them 29 + 9.
+// the rate of a large product) take 27 us and 10 for the merge.  A tile of 8 nodes is 32
+// MFMAs per wavefront, 1,024 cycles; 128 KB of LDS reads for its four wavefronts, 1,024
+// cycles of the CU; and about 230 vector instructions, mostly the softmax, with 32
+// exponentials, 1,200.  Two wavefronts per SIMD (226 registers) do one each in about 3,300
+// cycles, so all three units are busy for two thirds of the time.  Before its first tile and
+// after its last a work-group spends 8,000.  One tree of 7 nodes after 523 keys takes 9 us
+// and 4, all of it latency.  On the way, for the 32 trees: ranges by number instead of
+// length 79; three copies of the tile's code for masked and whole tiles, whose spilled
+// registers were waited for together with the next tile 50 + 8; one copy 42 + 8; shares from
+// a list of what there is, instead of a grid over the bounds, which left CUs without work
+// beside others with two shares, and partials stored as the lanes hold them 29 + 9; K rows
+// read ahead of their products and a reference that seldom moves 27.  Not kept: two tiles in
+// LDS and one barrier a tile (28), lines of the tiles ahead loaded early (28).
 #include <type_traits>
 
 #include "common.hpp"
@@ -43,6 +46,7 @@ namespace {
 template <bool F32>
 constexpr int kGroup = F32 ? 4 : 8;   // nodes per work-group
 constexpr int kTile = 64;        // keys per tile (a whole tree)
+constexpr float kSlack = 8.f;    // (powers of 2)
 static_assert(kTile == kTreeNodes, "the drafted latents are one tile");
 
 struct MlaTreeArgs {
@@ -59,9 +63,14 @@ struct MlaTreeArgs {
   float scale_log2;
   void *out;
   int64_t out_stride;
-  float *part;             // when splits > 1: kPart<R, F32> floats per (group, range)
+  float *part;             // when splits > 1: `part_cap` partials of kPart<R, F32> floats
+  int part_cap;
   int heads, splits, split_tiles, n_trees;
 };
+
+// Work-groups that run at a time.
+template <int R>
+constexpr int kSlots = R <= 128 ? 512 : 256;
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
@@ -78,47 +87,87 @@ __device__ __forceinline__ int cached_keys(const MlaTreeArgs &a, int tree, int64
   return slot >= 0 && slot < a.n_slots ? static_cast<int>(keys) : -1;
 }
 
-// Ranges of a tree with `tiles` tiles.
-__device__ __forceinline__ int ranges(const MlaTreeArgs &a, int tiles) {
-  return min(a.splits, (tiles + a.split_tiles - 1) / a.split_tiles);
-}
-
 // What a work-group does.
 struct Work {
   int tree, node0, split, n, keys, t0, t1;   // tiles [t0, t1) of the cached keys
+  int part;                                  // its partial
   bool drafted, whole;                       // the range has the drafted tile too; is the tree's only one
   int64_t base, slot;
 };
 
-// Work-group b's share: item (b % 8) ceil(items / 8) + b / 8 of the list, in which
-// the nodes of a (tree, range) are next to each other.  False behind its end.
-template <bool F32>
-__device__ __forceinline__ bool find_work(const MlaTreeArgs &a, Work &w) {
-  const int lane = threadIdx.x & 63;
-  // The tree of this lane: its nodes, keys and ranges, and the items up to it.
+// A tree per lane, 64 at a time.
+template <int R, bool F32>
+struct Lanes {
+  const MlaTreeArgs &a;
   int64_t base = 0, slot = 0;
-  int n = 0, keys = 0, used = 0, mine = 0, sum = 0;
-  const auto look = [&](int tree) {
+  int n = 0, keys = 0, groups = 0, tiles = 0;   // of this lane's tree; groups 0 behind the last one
+  int used = 0, items = 0, parts = 0;           // its ranges, (range, group) items, those of them that are partials
+  __device__ __forceinline__ explicit Lanes(const MlaTreeArgs &args) : a(args) {}
+  __device__ __forceinline__ void look(int tree) {
     const int in = min(tree, a.n_trees - 1);
     keys = cached_keys(a, in, slot);
     n = tree_nodes(a.trees, in, base);
-    used = keys < 0 ? 1 : ranges(a, (keys + kTile - 1) / kTile + 1);
-    mine = tree == in ? used * ((n + kGroup<F32> - 1) / kGroup<F32>) : 0;
-    sum = wave_scan(mine);
-    return __builtin_amdgcn_readlane(sum, 63);
-  };
-  int all = look(lane), items = all;
-  for (int t0 = 64; t0 < a.n_trees; t0 += 64) items += look(t0 + lane);
+    groups = tree == in ? (n + kGroup<F32> - 1) / kGroup<F32> : 0;
+    tiles = keys < 0 ? 1 : (keys + kTile - 1) / kTile + 1;
+  }
+  __device__ __forceinline__ void divide(int length) {
+    used = min(a.splits, (tiles + length - 1) / length);
+    items = used * groups;
+    parts = used > 1 ? items : 0;
+  }
+  // Tiles of a range at most.  With W = sum of groups x tiles and G = sum of groups there
+  // are about W / length + G / 2 items, as many as run at a time if that can be: one more
+  // takes as long as all of them.  At least split_tiles.  A tree of two ranges or more has
+  // fewer than 2 tiles / length of them, so there are at most 2 kSlots partials.  Looks at
+  // the first 64 trees last.
+  __device__ __forceinline__ int range_tiles(int lane) {
+    float work = 0.f;
+    int all = 0;
+    for (int t0 = (a.n_trees - 1) & ~63; t0 >= 0; t0 -= 64) {
+      look(t0 + lane);
+      work += static_cast<float>(groups) * static_cast<float>(tiles);
+      all += groups;
+    }
+    all = __builtin_amdgcn_readlane(wave_scan(all), 63);
+    work = row_sum16(work);
+    work += lane_xor16(work);
+    work = (work + lane_xor32(work)) * 1.0001f + 1.f;   // (not less than it is, by rounding)
+    const int fill = max(kSlots<R> - all / 2, kSlots<R> / 2);
+    return static_cast<int>(fmaxf(static_cast<float>(a.split_tiles), ceilf(work / static_cast<float>(fill))));
+  }
+};
+
+// Work-group b's share: item (b % 8) ceil(items / 8) + b / 8 of the list, in which
+// the nodes of a (tree, range) are next to each other.  False behind its end.
+template <int R, bool F32>
+__device__ __forceinline__ bool find_work(const MlaTreeArgs &a, Work &w) {
+  const int lane = threadIdx.x & 63;
+  Lanes<R, F32> l(a);
+  const int length = l.range_tiles(lane);
+  l.divide(length);
+  int sum = wave_scan(l.items), all = __builtin_amdgcn_readlane(sum, 63), items = all;
+  if (a.n_trees > 64) {
+    for (int t0 = 64; t0 < a.n_trees; t0 += 64) {
+      l.look(t0 + lane);
+      l.divide(length);
+      items += __builtin_amdgcn_readlane(wave_scan(l.items), 63);
+    }
+    l.look(lane);
+    l.divide(length);
+  }
   const int share = (items + 7) >> 3, b = blockIdx.x;
   int item = (b & 7) * share + (b >> 3);
   if ((b >> 3) >= share || item >= items) return false;
-  int t0 = 0;
-  if (a.n_trees > 64) all = look(lane);   // (the last trees' otherwise)
+  int t0 = 0, parts = 0;
   while (item >= all) {
     item -= all;
+    parts += __builtin_amdgcn_readlane(wave_scan(l.parts), 63);
     t0 += 64;
     if (t0 >= a.n_trees) return false;
-    all = look(t0 + lane);
+    l.look(t0 + lane);
+    l.divide(length);
+    sum = wave_scan(l.items);
+    all = __builtin_amdgcn_readlane(sum, 63);
   }
   const int at = __ffsll(static_cast<unsigned long long>(__ballot(item < sum))) - 1;
   const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
@@ -126,36 +175,35 @@ __device__ __forceinline__ bool find_work(const MlaTreeArgs &a, Work &w) {
     return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(of(static_cast<int>(v >> 32)))) << 32 |
                                 static_cast<uint32_t>(of(static_cast<int>(v))));
   };
-  item -= of(sum - mine);
+  item -= of(sum - l.items);
+  w.part = parts + of(wave_scan(l.parts) - l.parts) + item;
   w.tree = t0 + at;
-  w.keys = of(keys);
-  w.n = of(n);
-  w.base = of64(base);
-  w.slot = of64(slot);
-  const int ranges_of = of(used);
-  const int groups = (w.n + kGroup<F32> - 1) / kGroup<F32>;
-  const int tiles = (w.keys + kTile - 1) / kTile + 1;
+  w.keys = of(l.keys);
+  w.n = of(l.n);
+  w.base = of64(l.base);
+  w.slot = of64(l.slot);
+  const int used = of(l.used), groups = of(l.groups), tiles = of(l.tiles);
   w.split = item / groups;
   w.node0 = (item - w.split * groups) * kGroup<F32>;
-  w.t0 = static_cast<int>(static_cast<int64_t>(tiles) * w.split / ranges_of);
-  w.t1 = static_cast<int>(static_cast<int64_t>(tiles) * (w.split + 1) / ranges_of);
-  w.drafted = w.split + 1 == ranges_of;
+  const int each = tiles / used, more = tiles - each * used;   // the first `more` ranges have one more
+  w.t0 = each * w.split + min(w.split, more);
+  w.t1 = w.t0 + each + (w.split < more ? 1 : 0);
+  w.drafted = w.split + 1 == used;
   if (w.drafted) --w.t1;
-  w.whole = ranges_of == 1;
-  return true;
+  w.whole = used == 1;
+  return w.whole || w.part < a.part_cap;   // (there is always room, see range_tiles)
 }
 
-// Partials: of each (group of nodes, range) and wavefront, four ranks of a lane's
-// column at a time, [R / 8 or R / 16 of them][64 lanes], then maximum and sum [64 lanes].
-// Groups are counted over the packed rows: a tree's are (first row) / nodes + tree + 0, 1, ..
+// Partials: of each item and wavefront, four ranks of a lane's column at a time,
+// [R / 8 or R / 16 of them][64 lanes], then maximum and sum [64 lanes].  They lie in the
+// order of the list, those of a group `groups` apart.
 template <int R, bool F32>
 constexpr int kQuads = F32 ? R / 16 : R / 8;
 template <int R, bool F32>
 constexpr int kPart = 4 * 64 * (4 * kQuads<R, F32> + 2);
 template <int R, bool F32>
-__device__ __forceinline__ float *partial(const MlaTreeArgs &a, int64_t base, int tree, int node0, int split, int wave) {
-  const int64_t group = base / kGroup<F32> + tree + node0 / kGroup<F32>;
-  return a.part + (group * a.splits + split) * kPart<R, F32> + wave * (kPart<R, F32> / 4);
+__device__ __forceinline__ float *partial(const MlaTreeArgs &a, int64_t part, int wave) {
+  return a.part + part * kPart<R, F32> + wave * (kPart<R, F32> / 4);
 }
 
 template <bool F32>
@@ -177,7 +225,7 @@ __device__ __forceinline__ void put(const MlaTreeArgs &a, const Work &w, int64_t
                                     V value, K rank) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (!w.whole) {
-    float *p = partial<R, F32>(a, w.base, w.tree, w.node0, w.split, wave);
+    float *p = partial<R, F32>(a, w.part, wave);
 #pragma unroll
     for (int j = 0; j < kQuads<R, F32>; ++j) reinterpret_cast<f4 *>(p)[64 * j + lane] = value(j);
     reinterpret_cast<f2 *>(p + 256 * kQuads<R, F32>)[lane] = f2{m, l};
@@ -200,11 +248,11 @@ struct Stage {
   // A tile of cached keys: a scalar base and 32-bit offsets.
   __device__ __forceinline__ void load(const MlaTreeArgs &a, const Work &w, int t) {
     const int q = threadIdx.x % kQuads, r0 = threadIdx.x / kQuads;
-    const float *p = a.cache + (w.slot * a.slot_stride + static_cast<int64_t>(kTile * t) * R);
+    const char *p = reinterpret_cast<const char *>(a.cache + (w.slot * a.slot_stride + static_cast<int64_t>(kTile * t) * R));
     const int last = w.keys - 1 - kTile * t;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
-      v[i] = *reinterpret_cast<const f4 *>(p + static_cast<uint32_t>(min(r0 + kRows * i, last) * R + 4 * q));
+      v[i] = *reinterpret_cast<const f4 *>(p + static_cast<uint32_t>(min(r0 + kRows * i, last) * (4 * R) + 16 * q));
   }
   // The drafted tile: zeros for what is not finite, and which rows held it.
   __device__ __forceinline__ void load_drafted(const MlaTreeArgs &a, const Work &w, int (&bad)[kTile]) {
@@ -258,7 +306,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
   __shared__ __attribute__((aligned(1024))) uint16_t s_lat[kTile * R];
   __shared__ int s_bad[kTile];
   Work w;
-  if (!find_work<false>(a, w)) return;
+  if (!find_work<R, false>(a, w)) return;
   if (w.keys < 0) return zero_rows<false>(a, w, R);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int ln = lane & 31, half = lane >> 5, l16 = lane & 15;
@@ -321,6 +369,13 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
         st[kt] = mfma32x32(bits_to_bf8(*reinterpret_cast<const u4 *>(s_lat + ko[ks] + 32 * kt * R)), qf[ks], st[kt]);
+    // (K rows two steps ahead of their products)
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+      if (ks + 3 < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
     if (!all) {
       const uint32_t bits[2] = {static_cast<uint32_t>(seen) >> (4 * half), static_cast<uint32_t>(seen >> 32) >> (4 * half)};
 #pragma unroll
@@ -337,7 +392,9 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
     }
     float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     mx = fmaxf(mx, lane_xor32(mx)) * a.scale_log2;
-    if (__any(mx > m_run)) {
+    // The reference follows the maximum where that has risen by more than kSlack: until
+    // then probabilities are up to 2^kSlack, as exact as below 1.
+    if (__any(mx > m_run + kSlack)) {
       const float m_new = fmaxf(m_run, mx);
       const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
@@ -404,7 +461,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(Mla
   __shared__ __attribute__((aligned(16))) float s_lat[kTile][LD];
   __shared__ int s_bad[kTile];
   Work w;
-  if (!find_work<true>(a, w)) return;
+  if (!find_work<R, true>(a, w)) return;
   if (w.keys < 0) return zero_rows<true>(a, w, R);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int l16 = lane & 15, grp = lane >> 4;
@@ -506,13 +563,24 @@ __global__ __launch_bounds__(256) void mla_tree_merge_kernel(MlaTreeArgs a) {
   const int tree = blockIdx.y, node0 = static_cast<int>(blockIdx.x / kMergeParts) * kGroup<F32>;
   if (blockIdx.x % kMergeParts >= kParts) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
-  int64_t base, slot;
-  const int keys = cached_keys(a, tree, slot);
-  const int n = tree_nodes(a.trees, tree, base);
-  const int used = ranges(a, (keys + kTile - 1) / kTile + 1);
+  Lanes<R, F32> trees(a);
+  const int length = trees.range_tiles(lane);
+  trees.divide(length);
+  int64_t part = 0;     // the tree's first
+  for (int t0 = 64; t0 <= tree; t0 += 64) {
+    part += __builtin_amdgcn_readlane(wave_scan(trees.parts), 63);
+    trees.look(t0 + lane);
+    trees.divide(length);
+  }
+  const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, tree & 63); };
+  part += of(wave_scan(trees.parts) - trees.parts);
+  const int used = of(trees.used), n = of(trees.n), groups = of(trees.groups);
+  const int64_t base = iclamp64(a.trees.cu[tree], 0, a.trees.rows);
   const int node = node0 + (F32 ? wave : 2 * wave + ((lane >> 4) & 1));
-  if (node >= n || l16 >= a.heads || keys < 0 || used == 1) return;   // (one range: written already)
-  const float *p = partial<R, F32>(a, base, tree, node0, 0, wave);
+  // (one range: written already; and there is always room, see range_tiles)
+  if (node >= n || l16 >= a.heads || used == 1 || part + used * groups > a.part_cap) return;
+  const float *p = partial<R, F32>(a, part + node0 / kGroup<F32>, wave);
+  const int64_t step = static_cast<int64_t>(groups) * kPart<R, F32>;
   const int j0 = static_cast<int>(blockIdx.x % kMergeParts) * QW;
   float m = -INFINITY, l = 0.f;
   f4 acc[QW];
@@ -525,7 +593,7 @@ __global__ __launch_bounds__(256) void mla_tree_merge_kernel(MlaTreeArgs a) {
     float top = m;
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
-      const float *ps = p + static_cast<int64_t>(min(s0 + s, used - 1)) * kPart<R, F32>;   // the last one again, unused
+      const float *ps = p + min(s0 + s, used - 1) * step;   // the last one again, unused
       ml[s] = reinterpret_cast<const f2 *>(ps + 256 * kQuads<R, F32>)[lane];
 #pragma unroll
       for (int j = 0; j < QW; ++j) v[s][j] = reinterpret_cast<const f4 *>(ps)[64 * (j0 + j) + lane];
@@ -561,11 +629,22 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 using namespace sophia;
 
-extern "C" size_t sophia_mla_tree_workspace_size(int64_t rows, int n_trees, int rank, int splits) {
-  if (rows < 0 || n_trees < 0 || rank <= 0 || splits < 2) return 0;
-  const size_t bf16 = static_cast<size_t>(rows / kGroup<false> + n_trees + 1) * (rank / 2 + 2);
-  const size_t f32 = static_cast<size_t>(rows / kGroup<true> + n_trees + 1) * (rank / 4 + 2);
-  return (bf16 > f32 ? bf16 : f32) * splits * 4 * 64 * sizeof(float);
+namespace {
+// Items of a list at most, were every range one of its own; how many partials there can
+// be (Lanes::range_tiles), and the floats of one.
+int64_t tree_items(int n_trees, int max_nodes, bool f32, int splits) {
+  const int group = f32 ? kGroup<true> : kGroup<false>;
+  return static_cast<int64_t>(n_trees) * ((max_nodes + group - 1) / group) * splits;
+}
+constexpr int64_t kMostParts = 2 * 512;
+int64_t part_floats(int rank, bool f32) { return 4 * 64 * (4 * (rank / (f32 ? 16 : 8)) + 2); }
+}  // namespace
+
+extern "C" size_t sophia_mla_tree_workspace_size(int n_trees, int max_nodes, int rank, int dtype, int splits) {
+  if (n_trees < 0 || max_nodes < 1 || rank <= 0 || splits < 2) return 0;
+  const bool f32 = dtype == SOPHIA_DTYPE_F32;
+  return static_cast<size_t>(imin64(kMostParts, tree_items(n_trees, max_nodes, f32, splits)) * part_floats(rank, f32)) *
+         sizeof(float);
 }
 
 extern "C" int sophia_mla_tree_attn(const void *qa, int64_t qa_stride, const void *latent, int64_t latent_stride,
@@ -594,17 +673,17 @@ extern "C" int sophia_mla_tree_attn(const void *qa, int64_t qa_stride, const voi
   SOPHIA_REQUIRE(aligned16(qa) && aligned16(latent) && aligned16(cache) && aligned16(out),
                  "mla_tree_attn: qa, latent, cache and out must be 16-byte aligned");
   SOPHIA_REQUIRE(splits == 1 || (workspace && aligned16(workspace) &&
-                                 workspace_bytes >= sophia_mla_tree_workspace_size(rows, n_trees, rank, splits)),
+                                 workspace_bytes >= sophia_mla_tree_workspace_size(n_trees, max_nodes, rank, dtype, splits)),
                  "mla_tree_attn: workspace too small");
-  const int group = dtype == SOPHIA_DTYPE_F32 ? kGroup<true> : kGroup<false>;
-  const int groups = (max_nodes + group - 1) / group;
-  const int64_t blocks = (static_cast<int64_t>(n_trees) * splits * groups + 7) / 8 * 8;   // the longest list there may be
-  SOPHIA_REQUIRE(blocks <= 0x7fffffff, "mla_tree_attn: too many trees and splits");
+  const bool f32 = dtype == SOPHIA_DTYPE_F32;
+  const int64_t items = tree_items(n_trees, max_nodes, f32, splits), groups = tree_items(1, max_nodes, f32, 1);
+  const int64_t most = imin64(items, groups * n_trees + 512);   // of the list: no more than run at a time, or a group each
+  const int part_cap = splits > 1 ? static_cast<int>(imin64(kMostParts, items)) : 0;
   const MlaTreeArgs a{{cu_nodes, parents, rows, max_nodes}, qa, qa_stride, latent, latent_stride, cache, slot_stride,
                       max_seq, n_slots, slots, cached, scale * 1.44269504088896341f, out, out_stride,
-                      static_cast<float *>(workspace), heads, splits, split_keys / kTile, n_trees};
+                      static_cast<float *>(workspace), part_cap, heads, splits, split_keys / kTile, n_trees};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(blocks)), merge(kMergeParts * groups, n_trees);
+  const dim3 grid(static_cast<unsigned>((most + 7) / 8 * 8)), merge(static_cast<unsigned>(kMergeParts * groups), n_trees);
   switch (rank) {
 #define SOPHIA_MLA_TREE(r)                                                                      \
   case r:                                                                                       \

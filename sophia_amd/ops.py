@@ -1721,36 +1721,35 @@ def mla_tree_attn(qa: torch.Tensor, latent: torch.Tensor, latent_cache: torch.Te
     if y.dtype != qa.dtype:
         raise RuntimeError("out must have qa's dtype")
     bound = max_seq if max_len is None else max(0, min(int(max_len), max_seq))
-    if splits is None:
-        splits = mla_tree_splits(n, int(max_nodes), bound, qa.dtype)
     # whole 64-key tiles, the drafted latents being one more at the end
-    split_keys = max(1, -(-(-(-bound // 64) + 1) // max(int(splits), 1))) * 64
+    tiles = -(-bound // 64) + 1
+    if splits is None:
+        splits, least = mla_tree_splits(bound), TREE_RANGE
+    else:
+        least = max(1, -(-tiles // max(int(splits), 1)))
     lib = nat.lib()
-    ws_bytes = lib.sophia_mla_tree_workspace_size(rows, n, rank, int(splits))
+    code = nat.dtype_code(qa.dtype)
+    ws_bytes = lib.sophia_mla_tree_workspace_size(n, int(max_nodes), rank, code, int(splits))
     ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
-    rc = _launch(device, lib.sophia_mla_tree_attn, qa.data_ptr(), qs, latent.data_ptr(), ls, nat.dtype_code(qa.dtype),
+    rc = _launch(device, lib.sophia_mla_tree_attn, qa.data_ptr(), qs, latent.data_ptr(), ls, code,
                  latent_cache.data_ptr(), slot_stride, n_slots, max_seq, nat.ptr(sl), cached.data_ptr(),
                  cu_nodes.data_ptr(), parents.data_ptr(), n, rows, int(max_nodes), float(scale), y.data_ptr(), os_, heads,
-                 rank, int(splits), split_keys, nat.ptr(ws), ws_bytes)
+                 rank, int(splits), 64 * least, nat.ptr(ws), ws_bytes)
     nat.check(rc, "sophia_mla_tree_attn")
     return y
 
 
-def mla_tree_splits(trees: int, max_nodes: int, max_len: int, dtype: torch.dtype) -> int:
-    """Key ranges of ``mla_tree_attn`` at most, the longest context's: of how many
-    64-key tiles one is.  A range costs a work-group about three tiles' time before
-    and after its tiles and a partial of each node in the merge, so long lists of
-    work take 8 (us with the merge, bf16: 32 trees of 24 to 64 nodes after up to
-    4,000 keys 38 with 8, 44 with 6, 67 with 2), and where they do not fill the chip
-    each tile more is latency (one tree after 523 keys 13 with 2, 14 with 3, 17 with
-    8).  An fp32 tile takes three times as long: 2 (5 trees after up to 3,001 keys 24
-    with 2, 27 with 3, 28 with 1)."""
-    tiles = -(-max_len // 64) + 1
-    work = max(trees, 1) * -(-max_nodes // 8) * tiles   # at the bounds; a ragged batch has about half
-    least = 2 if dtype == torch.float32 else min(8, max(2, work // 1024))
-    # at most 128 ranges for the merge to join one after the other, and no workspace
-    # past what keeps the chip busy
-    return -(-tiles // max(least, -(-work // 8192), -(-tiles // 128)))
+TREE_RANGE = 2    # 64-key tiles of a key range of mla_tree_attn at least
+
+
+def mla_tree_splits(max_len: int) -> int:
+    """Key ranges of ``mla_tree_attn`` at most, of a context of ``max_len`` keys: of
+    TREE_RANGE tiles as long as there are few (where the work does not fill the
+    chip each tile more is latency, and a range costs about three tiles' time before
+    and after its tiles: one tree after 523 keys 13 us with 2, 14 with 3, 17 with 8;
+    the kernel makes them longer where it does), and 128, which the merge joins one
+    after the other."""
+    return min(128, -(-(-(-max_len // 64) + 1) // TREE_RANGE))
 
 
 def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: torch.Tensor | None, g: torch.Tensor,

@@ -646,8 +646,24 @@ def test_tree_attention_of_many_trees():
     tr, qa, latent, cache, slots, cached = _attn_case(lens, [(37 * i) % 200 for i in range(150)], max_seq=200, heads=2, rank=32)
     slots[70], slots[149] = -1, 500
     for dtype in (BF, F32):
-        for splits in (1, 4):
+        for splits in (1, 4, None):
             got = ops.mla_tree_attn(*_dev(qa.to(dtype), latent.to(dtype), cache, tr.cu, tr.par, slots, cached), 0.1,
                                     max_nodes=18, splits=splits)
             want, mass, size = ref.attention(tr, qa, latent, cache, slots, cached, 0.1)
             _within(got, want, _attn_tol(tr, want, mass, size, dtype, 32))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rank,heads,trees", [(32, 2, 90), (128, 3, 30), (256, 1, 66)])
+def test_tree_attention_of_more_work_than_fits_at_once(rank, heads, trees, dtype):
+    """Ranges as long as the kernel makes them, long contexts beside short ones, partials of some trees alone."""
+    from sophia_amd import ops
+    lens, seq = [1 + (11 * i) % 40 for i in range(trees)], 2500
+    cached = [(997 * i) % seq if i % 3 else i for i in range(trees)]
+    tr, qa, latent, cache, slots, cached = _attn_case(lens, cached, max_seq=seq, heads=heads, rank=rank, dtype=dtype, q_std=0.5)
+    slots[7] = -1
+    want, mass, size = ref.attention(tr, qa, latent, cache, slots, cached, 0.1)
+    tol = _attn_tol(tr, want, mass, size, dtype, rank) + 1800 * E32 * mass     # (sums of up to 2,500 keys)
+    dev = _dev(qa, latent, cache, tr.cu, tr.par, slots, cached)
+    for kw in (dict(), dict(max_len=64), dict(splits=7)):
+        _within(ops.mla_tree_attn(*dev, 0.1, max_nodes=64, **kw), want, tol)

@@ -151,10 +151,6 @@ def test_accept_refuses(nat, change, word):
 
 def test_sizes_and_empty_calls(nat):
     lib = nat.lib()
-    assert lib.sophia_mla_tree_workspace_size(10, 2, 128, 1) == 0
-    # three groups of 4 or two of 8 nodes in two trees, 3 ranges, 16 columns a node
-    assert lib.sophia_mla_tree_workspace_size(10, 2, 128, 3) >= 4 * 3 * 4 * 16 * (128 + 2) * 4
-    assert lib.sophia_mla_tree_workspace_size(-1, 2, 128, 3) == 0
     assert lib.sophia_tree_accept_workspace_size(-1, 5) == 0 and lib.sophia_tree_accept_workspace_size(0, 5) == 0
     assert lib.sophia_tree_accept_workspace_size(3, 5) >= 3 * 8
     # nothing to do: no pointer is needed
@@ -164,7 +160,8 @@ def test_sizes_and_empty_calls(nat):
         assert _call(nat, "sophia_kda_tree_step", STEP_OK, STEP, xq=None, tape=None, cu=None, **empty)[0] == nat.SOPHIA_OK
         assert _call(nat, "sophia_tree_commit", COMMIT_OK, COMMIT, path=None, cu=None, **empty)[0] == nat.SOPHIA_OK
     assert _call(nat, "sophia_adjust_logits", ADJUST_OK, ADJUST, x=None, rows=0)[0] == nat.SOPHIA_OK
-    assert _call(nat, "sophia_tree_accept", ACCEPT_OK, ACCEPT, x=None, n=0)[0] == nat.SOPHIA_OK
+    assert _call(nat, "sophia_tree_accept", ACCEPT_OK, ACCEPT, x=None, path=None, rows=0, n=0)[0] == nat.SOPHIA_OK
+    assert _call(nat, "sophia_tree_accept", ACCEPT_OK, ACCEPT, x=None, n=0)[0] == nat.SOPHIA_ERR_INVALID   # (rows of no tree)
 
 
 def test_operators_reject_cpu_tensors():
@@ -184,12 +181,15 @@ def test_operators_reject_cpu_tensors():
         ops.tree_accept(f(4, 10), f(4, dtype=i64), cu, par, max_nodes=4)
 
 
-def test_tree_attention_splits_rule():
+def test_tree_attention_splits_rule(nat):
     from sophia_amd import ops
-    for dtype in (torch.bfloat16, torch.float32):
-        for trees in (0, 1, 7, 64, 5000):
-            for nodes in (1, 8, 9, 64):
-                for length in (0, 1, 255, 257, 4096, 10 ** 5):
-                    s = ops.mla_tree_splits(trees, nodes, length, dtype)
-                    assert 1 <= s <= 1024
-                    assert s <= -(-length // 64) + 1    # no range without keys at the longest length
+    for length in (0, 1, 255, 257, 4096, 10 ** 5, 2 ** 31 - 1):
+        s = ops.mla_tree_splits(length)
+        assert 1 <= s <= 128
+        assert s <= -(-length // 64) + 1    # no range without keys at the longest length
+    size = nat.lib().sophia_mla_tree_workspace_size
+    part = 4 * 64 * (128 // 2 + 2) * 4      # of 8 nodes in bf16
+    assert size(1, 7, 128, nat.DTYPE_BF16, 5) == 5 * part and size(1, 9, 128, nat.DTYPE_BF16, 5) == 10 * part
+    assert size(65535, 64, 128, nat.DTYPE_BF16, 128) == 1024 * part
+    assert size(3, 64, 256, nat.DTYPE_F32, 1) == size(0, 64, 256, nat.DTYPE_F32, 4) == size(-1, 64, 256, nat.DTYPE_F32, 4) == 0
+    assert size(2, 5, 128, nat.DTYPE_F32, 4) == 16 * 4 * 64 * (128 // 4 + 2) * 4
