@@ -1645,6 +1645,17 @@ def _launch(device, fn, *args) -> int:
         return fn(*args, nat.stream_handle(device))
 
 
+def _heads_out(out: torch.Tensor | None, rows: int, heads: int, dim: int, dtype, device) -> tuple[torch.Tensor, int]:
+    """``out`` as the caller has it, checked, or a new [rows, heads, dim]; and its row stride."""
+    if out is None:
+        return torch.empty((rows, heads, dim), dtype=dtype, device=device), heads * dim
+    stride = _heads_rows(out, "out", heads, dim)
+    _nrows(out, "out", rows)
+    if out.dtype != dtype:
+        raise RuntimeError(f"out must be {dtype}, as the input")
+    return out, stride
+
+
 def _trees(cu_nodes: torch.Tensor, parents: torch.Tensor, max_nodes: int, rows: int, device) -> int:
     """Checks the trees over ``rows`` packed nodes; returns their number."""
     cu = _int32(cu_nodes, "cu_nodes", device)
@@ -1715,11 +1726,7 @@ def mla_tree_attn(qa: torch.Tensor, latent: torch.Tensor, latent_cache: torch.Te
     n_slots, max_seq = int(latent_cache.size(0)), int(latent_cache.size(1))
     sl = _tree_slots(slots, n, n_slots, device)
     _int64(cached, "cached", n, device)
-    y = out if out is not None else torch.empty((rows, heads, rank), dtype=qa.dtype, device=device)
-    os_ = _heads_rows(y, "out", heads, rank)
-    _nrows(y, "out", rows)
-    if y.dtype != qa.dtype:
-        raise RuntimeError("out must have qa's dtype")
+    y, os_ = _heads_out(out, rows, heads, rank, qa.dtype, device)
     bound = max_seq if max_len is None else max(0, min(int(max_len), max_seq))
     # whole 64-key tiles, the drafted latents being one more at the end
     tiles = -(-bound // 64) + 1
@@ -1795,14 +1802,11 @@ def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: to
     a_log, dtb = _gate_params(use_gate, A_log, dt_bias, heads, device)
     if dtb is not None and dtb.data_ptr() % 16:
         dtb = dtb.clone()
-    o = out if out is not None else torch.empty((rows, heads, HEAD_DIM), dtype=x_qkv.dtype, device=device)
-    os_ = _heads_rows(o, "out", heads, HEAD_DIM)
-    _nrows(o, "out", rows)
-    if o.dtype != x_qkv.dtype:
-        raise RuntimeError("out must have x_qkv's dtype")
+    o, os_ = _heads_out(out, rows, heads, HEAD_DIM, x_qkv.dtype, device)
     if tape is None:
         tape = torch.empty((rows, heads, 3, HEAD_DIM), dtype=torch.float32, device=device)
-    _tape(tape, rows, heads)
+    else:
+        _tape(tape, rows, heads)
     base, esz = x_qkv.data_ptr(), x_qkv.element_size()
     rc = _launch(device, nat.lib().sophia_kda_tree_step, base, base + inner * esz, base + 2 * inner * esz, xs,
                  nat.dtype_code(x_qkv.dtype), conv_weight.data_ptr(), nat.ptr(conv_state), taps, g.data_ptr(), gs,
@@ -1867,10 +1871,6 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
     kda, mla = list(kda), list(mla)
     if not kda and not mla:
         return
-    for layer in kda:
-        _on_device(index, device, *zip(layer, ("tape", "x_qkv", "conv_state", "state")))
-    for layer in mla:
-        _on_device(index, device, *zip(layer, ("latent", "latent_cache")))
     # What the first layer of a kind is, all of them are.
     heads, taps, x_dtype, f32 = 1, 1, torch.float32, torch.float32
     rank = max_seq = 0
@@ -1886,17 +1886,24 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
         tape_shape, x_shape = (rows, heads, 3, HEAD_DIM), (rows, 3 * inner)
         state_shape, hist_shape = (n_slots, heads, HEAD_DIM, HEAD_DIM), (n_slots, 3 * inner, taps - 1)
         for i, (tape, x, conv_state, state) in enumerate(kda):
-            if (tape.shape != tape_shape or tape.dtype is not f32 or not tape.is_contiguous()
-                    or state.shape != state_shape or state.dtype is not f32 or not state.is_contiguous()
-                    or x.shape != x_shape or x.dtype is not x_dtype or x.stride(1) != 1
-                    or (taps > 1 if conv_state is None else (conv_state.shape != hist_shape or conv_state.dtype is not f32
-                                                             or not conv_state.is_contiguous()))):
+            bad = (tape.shape != tape_shape or tape.dtype is not f32 or not tape.is_contiguous() or tape.get_device() != index
+                   or state.shape != state_shape or state.dtype is not f32 or not state.is_contiguous()
+                   or state.get_device() != index or x.shape != x_shape or x.dtype is not x_dtype or x.get_device() != index
+                   or x.stride(1) != 1)
+            hist = 0
+            if conv_state is None:
+                bad = bad or taps > 1
+            else:
+                bad = (bad or conv_state.shape != hist_shape or conv_state.dtype is not f32 or not conv_state.is_contiguous()
+                       or conv_state.get_device() != index)
+                hist = conv_state.data_ptr()
+            if bad:
+                _on_device(index, device, (tape, "tape"), (x, "x_qkv"), (conv_state, "conv_state"), (state, "state"))
                 raise RuntimeError(
                     f"KDA layer {i}: tape must be contiguous fp32 {list(tape_shape)}, x_qkv {x_dtype} {list(x_shape)} with "
                     f"dense rows, conv_state contiguous fp32 {list(hist_shape)} and state contiguous fp32 "
                     f"{list(state_shape)}, as in every layer")
-            flat += (tape.data_ptr(), x.data_ptr(), x.stride(0) if rows > 1 else 3 * inner,
-                     0 if conv_state is None else conv_state.data_ptr(), state.data_ptr())
+            flat += (tape.data_ptr(), x.data_ptr(), x.stride(0) if rows > 1 else 3 * inner, hist, state.data_ptr())
     kda_args = (ctypes.c_int64 * max(len(flat), 1))(*flat)   # (sophia_commit_kda: five words a layer)
     flat = []
     lat_dtype = f32
@@ -1907,6 +1914,8 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
         latent, cache = mla[0]
         rank, max_seq, lat_dtype = latent.size(-1), cache.size(1) if cache.dim() == 3 else 0, latent.dtype
         for i, (latent, cache) in enumerate(mla):
+            if latent.get_device() != index or cache.get_device() != index:
+                _on_device(index, device, (latent, "latent"), (cache, "latent_cache"))
             if (latent.shape != (rows, rank) or latent.dtype is not lat_dtype or latent.stride(1) != 1
                     or cache.shape != (n_slots, max_seq, rank)):
                 raise RuntimeError(f"MLA layer {i}: latent must be {lat_dtype} [{rows}, {rank}] with dense rows and "
@@ -2004,15 +2013,17 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
             raise RuntimeError(f"allowed_rows must hold {rows} entries")
     elif allowed_rows is not None:
         raise RuntimeError("allowed_rows belongs to allowed")
-    y = out if out is not None else torch.empty((rows, vocab), dtype=logits.dtype, device=device)
-    ys = _rows(y, "out", vocab)
-    _nrows(y, "out", rows)
-    if y.dtype != logits.dtype:
-        raise RuntimeError("out must have logits' dtype")
-    if out is not None and rows and vocab and (y.data_ptr() != logits.data_ptr() or ys != xs):
-        x0, y0, e = logits.data_ptr(), y.data_ptr(), logits.element_size()
-        if x0 < y0 + ((rows - 1) * ys + vocab) * e and y0 < x0 + ((rows - 1) * xs + vocab) * e:
-            raise RuntimeError("out must be logits itself or not overlap it")
+    if out is None:
+        y, ys = torch.empty((rows, vocab), dtype=logits.dtype, device=device), vocab
+    else:
+        y, ys = out, _rows(out, "out", vocab)
+        _nrows(y, "out", rows)
+        if y.dtype != logits.dtype:
+            raise RuntimeError("out must have logits' dtype")
+        if rows and vocab and (y.data_ptr() != logits.data_ptr() or ys != xs):
+            x0, y0, e = logits.data_ptr(), y.data_ptr(), logits.element_size()
+            if x0 < y0 + ((rows - 1) * ys + vocab) * e and y0 < x0 + ((rows - 1) * xs + vocab) * e:
+                raise RuntimeError("out must be logits itself or not overlap it")
     rc = _launch(device, nat.lib().sophia_adjust_logits, logits.data_ptr(), xs, y.data_ptr(), ys,
                  nat.dtype_code(logits.dtype), rows, vocab, nat.ptr(history), hist_stride, nat.ptr(history_len),
                  nat.ptr(prompt_len), hist_max, nat.ptr(repetition), nat.ptr(presence), nat.ptr(frequency),
