@@ -20,10 +20,10 @@
 // nodes that do see it end as NaN.
 //
 // What bounds it: 32 trees of 24 to 64 nodes after 60 to 4,000 keys (11.7 GFLOP, 11 us at
-// the rate of a large product) take 27 us and 10 for the merge.  A tile of 8 nodes is 32
-// MFMAs per wavefront, 1,024 cycles; 128 KB of LDS reads for its four wavefronts, 1,024
-// cycles of the CU; and about 230 vector instructions, mostly the softmax, with 32
-// exponentials, 1,200.  Two wavefronts per SIMD (226 registers) do one each in about 3,300
+// the rate of a large product) take 28 us and 10 for the merge.  A tile of 8 nodes is 36
+// MFMAs per wavefront, 1,152 cycles; 128 KB of LDS reads for its four wavefronts, 1,024
+// cycles of the CU; and about 200 vector instructions, mostly the softmax, with 32
+// exponentials, 1,100.  Two wavefronts per SIMD (242 registers) do one each in about 3,300
 // cycles, so all three units are busy for two thirds of the time.  Before its first tile and
 // after its last a work-group spends 8,000.  One tree of 7 nodes after 523 keys takes 9 us
 // and 4, all of it latency.  On the way, for the 32 trees: ranges by number instead of
@@ -31,8 +31,8 @@
 // registers were waited for together with the next tile 50 + 8; one copy 42 + 8; shares from
 // a list of what there is, instead of a grid over the bounds, which left CUs without work
 // beside others with two shares, and partials stored as the lanes hold them 29 + 9; K rows
-// read ahead of their products and a reference that seldom moves 27.  Not kept: two tiles in
-// LDS and one barrier a tile (28), lines of the tiles ahead loaded early (28).
+// read ahead of their products and a reference that seldom moves 28.  Not kept, as no faster: two tiles
+// in LDS and one barrier a tile, lines of the tiles ahead loaded early.
 #include <type_traits>
 
 #include "common.hpp"
@@ -345,7 +345,13 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) ot[dt][i] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;   // l_run over this lane's keys alone
+  // The sums of the probabilities, as they are rounded for the value product (a key that
+  // takes everything then has weight 1): a product with ones, all of whose rows are alike.
+  f16v lt;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) lt[i] = 0.f;
+  const bf8 ones = bits_to_bf8(u4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  float m_run = -INFINITY;
   const auto stage = [&]() {
     using St = Stage<R, false>;
     const int q = tid % St::kQuads, r0 = tid / St::kQuads;
@@ -398,19 +404,14 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
       const float m_new = fmaxf(m_run, mx);
       const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
-      l_run *= alpha;
+      lt *= alpha;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) ot[dt] *= alpha;
     }
-    float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        st[kt][i] = __builtin_amdgcn_exp2f(fmaf(st[kt][i], a.scale_log2, -m_run));
-        ps[i & 3] += st[kt][i];
-      }
-    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      for (int i = 0; i < 16; ++i) st[kt][i] = __builtin_amdgcn_exp2f(fmaf(st[kt][i], a.scale_log2, -m_run));
 #pragma unroll
     for (int kp = 0; kp < 4; ++kp) {   // 16 keys from 16 kp on
       const f16v &sv = st[kp >> 1];
@@ -418,6 +419,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 #pragma unroll
       for (int i = 0; i < 4; ++i) pw[i] = pack_bf16x2(sv[8 * (kp & 1) + 2 * i], sv[8 * (kp & 1) + 2 * i + 1]);
       const bf8 pf = bits_to_bf8(pw);
+      lt = mfma32x32(ones, pf, lt);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const u2 lo = lds_read_tr(s_lat + vo[dt] + 16 * kp * R);
@@ -435,11 +437,10 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
     }
     lds_barrier();
   }
-  if (w.drafted && (__ballot(s_bad[lane] != 0) & path)) l_run = NAN;
+  if (w.drafted && (__ballot(s_bad[lane] != 0) & path)) lt[0] = NAN;
   // ot[dt][i] = O[column ln][rank 32 dt + 8 (i / 4) + 4 half + i % 4] before the 1 / l
-  l_run += lane_xor32(l_run);
   put<R, false>(
-      a, w, row, l16, node < w.n && l16 < a.heads, m_run, l_run,
+      a, w, row, l16, node < w.n && l16 < a.heads, m_run, lt[0],
       [&](int j) {
         const f16v &v = ot[j >> 2];
         const int i = 4 * (j & 3);
