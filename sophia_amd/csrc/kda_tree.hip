@@ -30,12 +30,15 @@
 // as many CUs, 25,000 cycles from the first load to the last store), 64 trees of 8 to
 // 24 nodes 55 us, two work-groups per CU in two rounds, where their 114 MB take 22 us
 // at the rate of a copy; there the matrix pipes are busy a quarter of the time, the
-// vector unit and LDS about as much.  8 fp32 chains of 17 to 64 nodes take 55 us.  On
-// the way (us, these three cases): samples gathered from memory tap by tap 21, 128, 121;
-// samples through LDS, pairs on the vector unit 23, 83, 59; conv taps by distance in
-// LDS, where by channel all 16 threads of a node met in one bank, tiles without nodes
-// left out 13, 57, 56.  Not kept: 4 wavefronts of 32 columns (58 for the second), the
-// solve step by step along shallow paths in place of the inverse (58), taps in bf16 (57).
+// vector unit and LDS about as much.  8 fp32 chains of 17 to 64 nodes take 39 us: half
+// the CUs, 72,000 cycles for 64 nodes, of which the products with S, at the fp32 MFMA
+// rate, are 20,000.  On the way (us, these three cases): samples gathered from memory tap
+// by tap 21, 128, 121; samples through LDS, pairs on the vector unit 23, 83, 59; conv taps
+// by distance in LDS, where by channel all 16 threads of a node met in one bank, tiles
+// without nodes left out 13, 57, 56; strong decays by tiles in place of pairs (62,000 of
+// the slowest head's cycles, 23,000 since) 13, 55, 39.  Not kept: 4 wavefronts of 32
+// columns (58 for the second), the solve step by step along shallow paths in place of the
+// inverse (58), taps in bf16 (57).
 //
 // A node with an input that is not finite would reach its siblings through the
 // products (0 times infinity): its rows enter them as zeros, and what lies on a

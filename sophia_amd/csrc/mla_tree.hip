@@ -31,8 +31,8 @@
 // registers were waited for together with the next tile 50 + 8; one copy 42 + 8; shares from
 // a list of what there is, instead of a grid over the bounds, which left CUs without work
 // beside others with two shares, and partials stored as the lanes hold them 29 + 9; K rows
-// read ahead of their products and a reference that seldom moves 28.  Not kept, as no faster: two tiles
-// in LDS and one barrier a tile, lines of the tiles ahead loaded early.
+// read ahead of their products and a reference that seldom moves 28 + 10.  Not kept, as no
+// faster: two tiles in LDS and one barrier a tile, lines of the tiles ahead loaded early.
 #include <type_traits>
 
 #include "common.hpp"
@@ -451,7 +451,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 
 // ---- fp32 ----------------------------------------------------------------------
 // 16x16x4 MFMAs in fp32 throughout: an fp32 model's latents have more bits than
-// bf16 holds.  5 trees of 1 to 32 nodes after up to 3,001 keys: 18 us and 6 for the
+// bf16 holds.  5 trees of 1 to 32 nodes after up to 3,001 keys: 18 us and 7 for the
 // merge; a tile takes a wavefront 256 MFMAs of 32 cycles, and only the keys divide it
 // further.  A lane's four consecutive ranks of a key are the A operands of four
 // steps (the k index runs 4 (lane / 16) + step), and the scores' accumulator, keys
