@@ -572,10 +572,10 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
 #pragma unroll
   for (int m = 0; m < MT; ++m) u[m] = o[m] = zero;
 #pragma unroll
-  for (int blk = 0; blk < kD / 16; ++blk)
+  for (int m = 0; m < MT; ++m) {
+    if (m >= mt) break;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (m >= mt) break;
+    for (int blk = 0; blk < kD / 16; ++blk) {
       const f4 ak = *reinterpret_cast<const f4 *>(&mat.k[16 * m + c16][16 * blk + 4 * grp]);
       const f4 aq = *reinterpret_cast<const f4 *>(&mat.q[16 * m + c16][16 * blk + 4 * grp]);
 #pragma unroll
@@ -584,6 +584,13 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
         o[m] = mfma_f32(aq[s], st[4 * blk + s], o[m]);
       }
     }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);   // (reads ahead of their products)
+#pragma unroll
+    for (int blk = 0; blk < kD / 16; ++blk) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
+      if (blk + 2 < kD / 16) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  }
   lds_barrier();
 
   // ---- block forward substitution, and the outputs

@@ -20,7 +20,7 @@
 // nodes that do see it end as NaN.
 //
 // What bounds it: 32 trees of 24 to 64 nodes after 60 to 4,000 keys (11.7 GFLOP, 11 us at
-// the rate of a large product) take 28 us and 10 for the merge.  A tile of 8 nodes is 36
+// the rate of a large product) take 27 us and 10 for the merge.  A tile of 8 nodes is 36
 // MFMAs per wavefront, 1,152 cycles; 128 KB of LDS reads for its four wavefronts, 1,024
 // cycles of the CU; and about 200 vector instructions, mostly the softmax, with 32
 // exponentials, 1,100.  Two wavefronts per SIMD (242 registers) do one each in about 3,300
@@ -30,8 +30,8 @@
 // length 79; three copies of the tile's code for masked and whole tiles, whose spilled
 // registers were waited for together with the next tile 50 + 8; one copy 42 + 8; shares from
 // a list of what there is, instead of a grid over the bounds, which left CUs without work
-// beside others with two shares, and partials stored as the lanes hold them 29 + 9; K rows
-// read ahead of their products and a reference that seldom moves 28 + 10.  Not kept, as no
+// beside others with two shares, and partials stored as the lanes hold them 29 + 9; rows
+// read ahead of their products and a reference that seldom moves 27 + 10.  Not kept, as no
 // faster: two tiles in LDS and one barrier a tile, lines of the tiles ahead loaded early.
 #include <type_traits>
 
@@ -133,7 +133,8 @@ struct Lanes {
     work += lane_xor16(work);
     work = (work + lane_xor32(work)) * 1.0001f + 1.f;   // (not less than it is, by rounding)
     const int fill = max(kSlots<R> - all / 2, kSlots<R> / 2);
-    return static_cast<int>(fmaxf(static_cast<float>(a.split_tiles), ceilf(work / static_cast<float>(fill))));
+    work = fminf(ceilf(work / static_cast<float>(fill)), 1 << 29);
+    return max(a.split_tiles, static_cast<int>(work));
   }
 };
 
@@ -427,6 +428,13 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
         ot[dt] = mfma32x32(bits_to_bf8(u4{lo.x, lo.y, hi.x, hi.y}), pf, ot[dt]);
       }
     }
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 1);
+#pragma unroll
+    for (int i = 0; i < 4 * DT; ++i) {
+      if (i % DT == 0) __builtin_amdgcn_sched_group_barrier(0x8, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 1);
+      if (i + 3 < 4 * DT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+    }
   };
   for (int t = w.t0 - (w.drafted ? 1 : 0); t < w.t1; ++t) {
     stage();
@@ -451,9 +459,9 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 
 // ---- fp32 ----------------------------------------------------------------------
 // 16x16x4 MFMAs in fp32 throughout: an fp32 model's latents have more bits than
-// bf16 holds.  5 trees of 1 to 32 nodes after up to 3,001 keys: 18 us and 7 for the
-// merge; a tile takes a wavefront 256 MFMAs of 32 cycles, and only the keys divide it
-// further.  A lane's four consecutive ranks of a key are the A operands of four
+// bf16 holds.  5 trees of 1 to 32 nodes after up to 3,001 keys: 16 us and 7 for the
+// merge; a tile takes a wavefront 256 MFMAs of 32 cycles (9,700 in all; 12,100 while the
+// compiler read V right before each product), and only the keys divide it further.  A lane's four consecutive ranks of a key are the A operands of four
 // steps (the k index runs 4 (lane / 16) + step), and the scores' accumulator, keys
 // 4 (lane / 16) + i, is the B operand of the value product in the same order.
 template <int R>
@@ -498,13 +506,22 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(Mla
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) st[kt] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+    for (int b = 0; b < KB; ++b) {
+      f4 k[4];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        const f4 k = *reinterpret_cast<const f4 *>(&s_lat[16 * kt + l16][16 * b + 4 * grp]);
+      for (int kt = 0; kt < 4; ++kt) k[kt] = *reinterpret_cast<const f4 *>(&s_lat[16 * kt + l16][16 * b + 4 * grp]);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) st[kt] = mfma_f32(k[s], qf[b][s], st[kt]);
-      }
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) st[kt] = mfma_f32(k[kt][s], qf[b][s], st[kt]);
+    }
+    // (LDS reads ahead of their products, here and below)
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 16, 0);
+      if (b + 2 < KB) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    }
     float mx = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
@@ -535,6 +552,12 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(Mla
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int b = 0; b < KB; ++b) ot[b] = mfma_f32(s_lat[16 * kt + 4 * grp + s][16 * b + l16], st[kt][s], ot[b]);
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);   // (two values each)
+#pragma unroll
+    for (int i = 0; i < 8 * KB; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+      if (i + 8 < 8 * KB) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
   };
   for (int t = w.t0 - (w.drafted ? 1 : 0); t < w.t1; ++t) {
     stage();
