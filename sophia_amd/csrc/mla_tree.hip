@@ -505,22 +505,22 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(Mla
     f4 st[4];   // score(key 16 kt + 4 grp + i, head l16)
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) st[kt] = f4{0.f, 0.f, 0.f, 0.f};
+    // LDS reads a step ahead of their products, here and below: by hand, as scheduling groups
+    // over that many products take the compiler a minute.
+    f4 k[2][4];
+    const auto read_k = [&](int b) {
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) k[b & 1][kt] = *reinterpret_cast<const f4 *>(&s_lat[16 * kt + l16][16 * b + 4 * grp]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read_k(0);
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-      f4 k[4];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) k[kt] = *reinterpret_cast<const f4 *>(&s_lat[16 * kt + l16][16 * b + 4 * grp]);
+      if (b + 1 < KB) read_k(b + 1);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) st[kt] = mfma_f32(k[kt][s], qf[b][s], st[kt]);
-    }
-    // (LDS reads ahead of their products, here and below)
-    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 16, 0);
-      if (b + 2 < KB) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        for (int kt = 0; kt < 4; ++kt) st[kt] = mfma_f32(k[b & 1][kt][s], qf[b][s], st[kt]);
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -546,17 +546,18 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(Mla
     l_run = l_run * alpha + ps;
 #pragma unroll
     for (int b = 0; b < KB; ++b) ot[b] *= alpha;
+    float v[2][KB];
+    const auto read_v = [&](int i) {   // of key 16 (i / 4) + 4 grp + i % 4
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+      for (int b = 0; b < KB; ++b) v[i & 1][b] = s_lat[16 * (i >> 2) + 4 * grp + (i & 3)][16 * b + l16];
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read_v(0);
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+    for (int i = 0; i < 16; ++i) {
+      if (i + 1 < 16) read_v(i + 1);
 #pragma unroll
-        for (int b = 0; b < KB; ++b) ot[b] = mfma_f32(s_lat[16 * kt + 4 * grp + s][16 * b + l16], st[kt][s], ot[b]);
-    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);   // (two values each)
-#pragma unroll
-    for (int i = 0; i < 8 * KB; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
-      if (i + 8 < 8 * KB) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      for (int b = 0; b < KB; ++b) ot[b] = mfma_f32(v[i & 1][b], st[i >> 2][i & 3], ot[b]);
     }
   };
   for (int t = w.t0 - (w.drafted ? 1 : 0); t < w.t1; ++t) {
