@@ -108,8 +108,8 @@ int sophia_tree_commit(const int32_t *path, int64_t path_stride, const int32_t *
  *   cache           : [n_slots, max_seq, rank] fp32, slot_stride between slots; tree s uses
  *                     slot slots[s] (NULL: s).  A tree whose slot is out of range gets zeros.
  *   cached          : [n_trees] int64, taken into [0, max_seq].
- * bf16: the cached latents are rounded to bf16, and the probabilities for the value
- * product; fp32: fp32 products.  Scores, softmax and sums are fp32; out is rounded once.
+ * bf16: the cached latents are rounded to bf16, the probabilities enter the value product
+ * to 2^-16; fp32: fp32 products.  Scores, softmax and sums are fp32; out is rounded once.
  * rank in {32, 64, 128, 256}; heads <= 16; scale > 0; row strides multiples of 8, every
  * pointer 16-byte aligned.  With splits > 1 a tree's keys are divided into equal
  * ranges of split_keys (a multiple of 64) or more, as long as keeps the chip full, at most

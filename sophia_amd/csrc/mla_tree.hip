@@ -20,18 +20,19 @@
 // nodes that do see it end as NaN.
 //
 // What bounds it: 32 trees of 24 to 64 nodes after 60 to 4,000 keys (11.7 GFLOP, 11 us at
-// the rate of a large product) take 27 us and 10 for the merge.  A tile of 8 nodes is 36
-// MFMAs per wavefront, 1,152 cycles; 128 KB of LDS reads for its four wavefronts, 1,024
-// cycles of the CU; and about 200 vector instructions, mostly the softmax, with 32
-// exponentials, 1,100.  Two wavefronts per SIMD (242 registers) do one each in about 3,300
-// cycles, so all three units are busy for two thirds of the time.  Before its first tile and
-// after its last a work-group spends 8,000.  One tree of 7 nodes after 523 keys takes 9 us
-// and 4, all of it latency.  On the way, for the 32 trees: ranges by number instead of
+// the rate of a large product) take 32 us and 10 for the merge.  A tile of 8 nodes is 48
+// MFMAs per wavefront, 1,536 cycles (a third of them for what the probabilities lose when
+// rounded once); 128 KB of LDS reads for its four wavefronts, 1,024 cycles of the CU; and
+// about 300 vector instructions, mostly the softmax, with 32 exponentials.  Two wavefronts
+// per SIMD (226 registers) share these.  Before its first tile and after its last a
+// work-group spends 8,000 cycles.  One tree of 7 nodes after 523 keys takes 10 us and 4, all
+// of it latency.  On the way, for the 32 trees: ranges by number instead of
 // length 79; three copies of the tile's code for masked and whole tiles, whose spilled
 // registers were waited for together with the next tile 50 + 8; one copy 42 + 8; shares from
 // a list of what there is, instead of a grid over the bounds, which left CUs without work
 // beside others with two shares, and partials stored as the lanes hold them 29 + 9; rows
-// read ahead of their products and a reference that seldom moves 27 + 10.  Not kept, as no
+// read ahead of their products and a reference that seldom moves 27 + 10; probabilities in
+// two parts 32 + 10.  Not kept, as no
 // faster: two tiles in LDS and one barrier a tile, lines of the tiles ahead loaded early.
 #include <type_traits>
 
@@ -288,9 +289,12 @@ __device__ __forceinline__ uint64_t path_of(const Work &w, int parent, int node)
 }
 
 // ---- bf16: 32x32x16 MFMAs, as the causal attention uses them ---------------------
-// The cached latents are rounded to bf16 on their way into LDS (a bf16 model wrote
-// them from bf16 values, so nothing is lost), probabilities to bf16 for the value
-// product; scores, maxima and sums are fp32.
+// The cached latents are rounded to bf16 on their way into LDS: a bf16 model wrote
+// them from bf16 values, so nothing is lost.  A probability enters the value product
+// as two bf16 numbers, the second what the first has lost (2^-16 of it remains lost):
+// as one, the outputs of 32 trees were 0.0020 off a float64 form, of which their own
+// rounding is 0.0017; as two 0.0017, for 38.6 us in place of 34.3 (with the merge).
+// Scores, maxima and sums are fp32.
 //
 // An LDS row is R / 8 chunks of 16 bytes, chunk c of row r at place c ^ f(r), f =
 // r % 16 rotated left by one bit: eight rows of one chunk (K) and four rows of two
@@ -346,12 +350,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) ot[dt][i] = 0.f;
-  // The sums of the probabilities, as they are rounded for the value product (a key that
-  // takes everything then has weight 1): a product with ones, all of whose rows are alike.
-  f16v lt;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) lt[i] = 0.f;
-  const bf8 ones = bits_to_bf8(u4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  float l_run = 0.f;   // over this lane's keys alone
   float m_run = -INFINITY;
   const auto stage = [&]() {
     using St = Stage<R, false>;
@@ -405,7 +404,7 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
       const float m_new = fmaxf(m_run, mx);
       const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
-      lt *= alpha;
+      l_run *= alpha;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) ot[dt] *= alpha;
     }
@@ -413,26 +412,37 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) st[kt][i] = __builtin_amdgcn_exp2f(fmaf(st[kt][i], a.scale_log2, -m_run));
+    float ps[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ps[i] = st[i >> 1][8 * (i & 1)];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) ps[i] += st[i >> 1][8 * (i & 1) + j];
+    }
+    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 #pragma unroll
     for (int kp = 0; kp < 4; ++kp) {   // 16 keys from 16 kp on
       const f16v &sv = st[kp >> 1];
-      u4 pw;
+      u4 pw, pr;   // rounded, and the rest
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pw[i] = pack_bf16x2(sv[8 * (kp & 1) + 2 * i], sv[8 * (kp & 1) + 2 * i + 1]);
-      const bf8 pf = bits_to_bf8(pw);
-      lt = mfma32x32(ones, pf, lt);
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = sv[8 * (kp & 1) + 2 * i], p1 = sv[8 * (kp & 1) + 2 * i + 1];
+        pw[i] = pack_bf16x2(p0, p1);
+        pr[i] = pack_bf16x2(p0 - __uint_as_float(pw[i] << 16), p1 - __uint_as_float(pw[i] & 0xffff0000u));
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const u2 lo = lds_read_tr(s_lat + vo[dt] + 16 * kp * R);
         const u2 hi = lds_read_tr(s_lat + (vo[dt] ^ 8) + (16 * kp + 8) * R);
-        ot[dt] = mfma32x32(bits_to_bf8(u4{lo.x, lo.y, hi.x, hi.y}), pf, ot[dt]);
+        const bf8 vf = bits_to_bf8(u4{lo.x, lo.y, hi.x, hi.y});
+        ot[dt] = mfma32x32(vf, bits_to_bf8(pw), ot[dt]);
+        ot[dt] = mfma32x32(vf, bits_to_bf8(pr), ot[dt]);
       }
     }
     __builtin_amdgcn_sched_group_barrier(0x100, 6, 1);
 #pragma unroll
     for (int i = 0; i < 4 * DT; ++i) {
-      if (i % DT == 0) __builtin_amdgcn_sched_group_barrier(0x8, 1, 1);
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x8, 2, 1);
       if (i + 3 < 4 * DT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
     }
   };
@@ -445,10 +455,11 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
     }
     lds_barrier();
   }
-  if (w.drafted && (__ballot(s_bad[lane] != 0) & path)) lt[0] = NAN;
+  if (w.drafted && (__ballot(s_bad[lane] != 0) & path)) l_run = NAN;
+  l_run += lane_xor32(l_run);
   // ot[dt][i] = O[column ln][rank 32 dt + 8 (i / 4) + 4 half + i % 4] before the 1 / l
   put<R, false>(
-      a, w, row, l16, node < w.n && l16 < a.heads, m_run, lt[0],
+      a, w, row, l16, node < w.n && l16 < a.heads, m_run, l_run,
       [&](int j) {
         const f16v &v = ot[j >> 2];
         const int i = 4 * (j & 3);
