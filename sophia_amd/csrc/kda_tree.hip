@@ -84,9 +84,12 @@ struct TreeStepArgs {
 };
 
 // |G| up to which A and B are formed from e^G and e^-G: e^-60 times a component of
-// k stays a normal fp32 number down to 1.3e-12.  The exponentials are then off by up to
-// 2.6e-6, where e^(G_i - G_j) is not; a channel that has come that far within 64
-// nodes has lost e^-1 and more at every one of them, and its part in A and B with it.
+// k stays a normal fp32 number down to 1.3e-12.  Each exponential is then off by up to
+// 2.6e-6, the rounding of its argument, and a pair's weight by up to 5.3e-6.  That counts
+// where a weight is near 1 far down, in a channel that lost e^-50 at one node and little
+// since (one that lost it evenly has small weights); the roundings of G itself, 1.9e-6 a
+// sum at 60, are in e^(G_i - G_j) too.  With the references below up to 1.3e-5: both
+// exponents are up to 80 then, and rounded differences.
 constexpr float kFactored = 60.f;
 // Beyond it the exponents are G_i - R and R - G_j, R the largest G of i's 16 nodes, so the
 // first is never positive.  The second may reach kFar, where e^x is in the range of fp32
