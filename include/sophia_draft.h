@@ -164,6 +164,15 @@ int sophia_tree_accept(const void *logits, int64_t logits_stride, int dtype, int
                        int max_nodes, int32_t *path, int64_t path_stride, int32_t *n_path, int64_t *next_token,
                        int64_t *chosen, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * The same, but a row without a value above -inf (its mask allows nothing, or it is NaN)
+ * has no choice: chosen is -1, a path ends at such a node, and next_token is -1 there.
+ */
+int sophia_tree_accept_strict(const void *logits, int64_t logits_stride, int dtype, int64_t rows, int vocab,
+                              const int64_t *tokens, const int32_t *cu_nodes, const int32_t *parents, int n_trees,
+                              int max_nodes, int32_t *path, int64_t path_stride, int32_t *n_path, int64_t *next_token,
+                              int64_t *chosen, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -117,6 +117,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sophia_tree_accept_workspace_size": (_sz, [_i64, _i32]),
     "sophia_tree_accept": (_i32, [_vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _vp, _vp, _vp,
                                   _vp, _sz, _vp]),
+    "sophia_tree_accept_strict": (_i32, [_vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _vp, _vp, _vp,
+                                         _vp, _sz, _vp]),
 }
 
 

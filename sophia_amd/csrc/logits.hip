@@ -264,6 +264,7 @@ struct AcceptArgs {
   int64_t path_stride;
   int32_t *n_path;
   int64_t *next, *chosen;
+  int none;                 // what a row without a value above -inf says
 };
 
 // The greater logit, of equal ones the lower index (of -inf any: join_parts).
@@ -342,7 +343,7 @@ __device__ __forceinline__ int join_parts(const AcceptArgs &a, int64_t row) {
   for (int p = 0; p < kParts; ++p) v[p] = a.part[row * a.parts + min(p, a.parts - 1)];   // the last one again
 #pragma unroll
   for (int p = 0; p < kParts; ++p) better(best, at, v[p].x, __float_as_int(v[p].y));
-  return best > -INFINITY ? at : 0;
+  return best > -INFINITY ? at : a.none;
 }
 
 // Work-group per tree (the walk), then one per 64 rows (`chosen`, of all rows).
@@ -361,6 +362,7 @@ __global__ __launch_bounds__(64) void tree_walk_kernel(AcceptArgs a, int n_trees
   int cur = 0, len = n > 0 ? 1 : 0, mine = n > 0 && lane == 0 ? 0 : -1;   // mine: path entry `lane`
   while (len > 0) {   // (a child is a later node: at most n steps)
     const int want = __shfl(at, cur, 64);
+    if (want < 0) break;
     const uint64_t next = __ballot(lane < n && parent == cur && token == want);
     if (next == 0) break;
     cur = __ffsll(static_cast<unsigned long long>(next)) - 1;
@@ -446,10 +448,11 @@ extern "C" size_t sophia_tree_accept_workspace_size(int64_t rows, int vocab) {
   return static_cast<size_t>(rows) * argmax_parts(rows, vocab) * sizeof(f2);
 }
 
-extern "C" int sophia_tree_accept(const void *logits, int64_t logits_stride, int dtype, int64_t rows, int vocab,
-                                  const int64_t *tokens, const int32_t *cu_nodes, const int32_t *parents, int n_trees,
-                                  int max_nodes, int32_t *path, int64_t path_stride, int32_t *n_path, int64_t *next_token,
-                                  int64_t *chosen, void *workspace, size_t workspace_bytes, void *stream) {
+namespace {
+int tree_accept(const void *logits, int64_t logits_stride, int dtype, int64_t rows, int vocab, const int64_t *tokens,
+                const int32_t *cu_nodes, const int32_t *parents, int n_trees, int max_nodes, int32_t *path,
+                int64_t path_stride, int32_t *n_path, int64_t *next_token, int64_t *chosen, int none, void *workspace,
+                size_t workspace_bytes, void *stream) {
   SOPHIA_REQUIRE(dtype_ok(dtype), "tree_accept: dtype not supported");
   SOPHIA_REQUIRE(rows >= 0 && rows <= 0x7fffffff && vocab >= 1 && vocab <= 1 << 30 && n_trees >= 0 && n_trees <= 65535,
                  "tree_accept: vocab must be 1..2^30, rows >= 0 and n_trees 0..65535");
@@ -467,7 +470,7 @@ extern "C" int sophia_tree_accept(const void *logits, int64_t logits_stride, int
   const int tiles = (vocab + kTileV - 1) / kTileV;
   const int per_part = (tiles + parts - 1) / parts * kTileV;
   AcceptArgs a{{cu_nodes, parents, rows, max_nodes}, logits, logits_stride, vocab, tokens, parts, per_part,
-               static_cast<f2 *>(workspace), path, path_stride, n_path, next_token, chosen};
+               static_cast<f2 *>(workspace), path, path_stride, n_path, next_token, chosen, none};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool vec = logits_stride % 8 == 0 && aligned16(logits);
   // rows beyond the grid's y limit in further launches
@@ -492,4 +495,22 @@ extern "C" int sophia_tree_accept(const void *logits, int64_t logits_stride, int
   const int64_t blocks = n_trees + (rows + 63) / 64;
   hipLaunchKernelGGL(tree_walk_kernel, dim3(static_cast<unsigned>(blocks)), dim3(64), 0, st, a, n_trees);
   return check_launch("tree_accept");
+}
+}  // namespace
+
+extern "C" int sophia_tree_accept(const void *logits, int64_t logits_stride, int dtype, int64_t rows, int vocab,
+                                  const int64_t *tokens, const int32_t *cu_nodes, const int32_t *parents, int n_trees,
+                                  int max_nodes, int32_t *path, int64_t path_stride, int32_t *n_path, int64_t *next_token,
+                                  int64_t *chosen, void *workspace, size_t workspace_bytes, void *stream) {
+  return tree_accept(logits, logits_stride, dtype, rows, vocab, tokens, cu_nodes, parents, n_trees, max_nodes, path,
+                     path_stride, n_path, next_token, chosen, 0, workspace, workspace_bytes, stream);
+}
+
+extern "C" int sophia_tree_accept_strict(const void *logits, int64_t logits_stride, int dtype, int64_t rows, int vocab,
+                                         const int64_t *tokens, const int32_t *cu_nodes, const int32_t *parents,
+                                         int n_trees, int max_nodes, int32_t *path, int64_t path_stride, int32_t *n_path,
+                                         int64_t *next_token, int64_t *chosen, void *workspace, size_t workspace_bytes,
+                                         void *stream) {
+  return tree_accept(logits, logits_stride, dtype, rows, vocab, tokens, cu_nodes, parents, n_trees, max_nodes, path,
+                     path_stride, n_path, next_token, chosen, -1, workspace, workspace_bytes, stream);
 }

@@ -2034,7 +2034,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
 
 
 def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tensor, parents: torch.Tensor, *,
-                max_nodes: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+                max_nodes: int, strict: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """The greedy choice at every node of the trees, and the walk along the
     drafted tokens that agree with it (sophia_tree_accept).
 
@@ -2045,8 +2045,11 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tens
     max_nodes], -1 behind its end; n_path int32 [N]; next_token int64 [N], the
     choice at the path's end; chosen int64 [rows], of rows of no tree too, the
     lowest index of each row's greatest logit, NaN never, and of rows without a
-    value above -inf 0).  A tree without nodes has an empty path and next_token
-    -1.  To sample instead of choosing, add Gumbel noise to the logits."""
+    value above -inf 0).  With ``strict`` such a row, whose mask allows nothing or
+    which is NaN, has no choice: chosen is -1, a path ends at its node, and
+    next_token is -1 there (sophia_tree_accept_strict).  A tree without nodes has
+    an empty path and next_token -1.  To sample instead of choosing, add Gumbel
+    noise to the logits."""
     _gpu(logits, "logits")
     device = logits.device
     if logits.dim() != 2 or int(logits.size(1)) < 1:
@@ -2063,7 +2066,7 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tens
     next_token = torch.empty(n, dtype=torch.int64, device=device)
     chosen = torch.empty(rows, dtype=torch.int64, device=device)
     ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device)
-    rc = _launch(device, lib.sophia_tree_accept, logits.data_ptr(), xs, nat.dtype_code(logits.dtype), rows, vocab,
+    rc = _launch(device, lib.sophia_tree_accept_strict if strict else lib.sophia_tree_accept, logits.data_ptr(), xs, nat.dtype_code(logits.dtype), rows, vocab,
                  tokens.data_ptr(), cu_nodes.data_ptr(), parents.data_ptr(), n, int(max_nodes), path.data_ptr(),
                  int(max_nodes), n_path.data_ptr(), next_token.data_ptr(), chosen.data_ptr(), ws.data_ptr(), nbytes)
     nat.check(rc, "sophia_tree_accept")

@@ -194,8 +194,9 @@ def pack_trees(model: Transformer, trees, slots, cached) -> DraftTrees:
 class Verified:
     """The outcome of ``verify_trees``, on the device: ``path`` int32 [N,
     max_nodes] (the kept nodes, -1 behind them), ``n_path`` int32 [N],
-    ``next_token`` int64 [N] (the token after the path: the next tree's node 0),
-    ``cached`` int64 [N] (tokens in the caches now), ``logits`` [rows, vocab] of
+    ``next_token`` int64 [N] (the token after the path: the next tree's node 0;
+    -1: there is none, as the last node's logits are all masked or NaN, and the
+    sequence ends),     ``cached`` int64 [N] (tokens in the caches now), ``logits`` [rows, vocab] of
     every node, adjusted."""
 
     path: torch.Tensor
@@ -220,7 +221,7 @@ def verify_trees(model: Transformer, trees: DraftTrees, **controls) -> Verified:
         logits = ops.adjust_logits(logits, cu_nodes=trees.cu_nodes, parents=trees.parents, tokens=trees.token_ids,
                                    max_nodes=trees.max_nodes, out=logits, **controls)
     path, n_path, next_token, _ = ops.tree_accept(logits, trees.token_ids, trees.cu_nodes, trees.parents,
-                                                  max_nodes=trees.max_nodes)
+                                                  max_nodes=trees.max_nodes, strict=True)
     model.commit_tree(draft, path, n_path)
     return Verified(path, n_path, next_token, trees.cached + n_path, logits)
 

@@ -1,0 +1,80 @@
+"""Calls that a server makes of the drafted-token step beside the ordinary ones."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import tree_ref as ref
+from test_gpu_tree_decode import _caches, _load, _model, _prefill
+
+pytestmark = pytest.mark.gpu
+
+
+def _strict(tr, logits, tokens, bound):
+    """tree_ref.accept with -1 for rows without a choice, at which walks end."""
+    chosen = ref.accept(tr, logits, tokens, bound)[3]
+    clean = torch.where(torch.isnan(logits.double()), float("-inf"), logits.double())
+    chosen = [c if float(r.max()) > float("-inf") else -1 for c, r in zip(chosen, clean)]
+    paths, counts, following = [], [], []
+    for s, parents in enumerate(tr.parents):
+        base, path = tr.offsets[s], [0] if parents else []
+        while path and chosen[base + path[-1]] >= 0:
+            nxt = [i for i, p in enumerate(parents) if 0 <= p < i and p == path[-1] and int(tokens[base + i]) == chosen[base + p]]
+            if not nxt:
+                break
+            path.append(nxt[0])
+        paths.append(path + [-1] * (bound - len(path)))
+        counts.append(len(path))
+        following.append(chosen[base + path[-1]] if path else -1)
+    return paths, counts, following, chosen
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [1, 3, 2048, 4099])
+def test_strict_walks_end_at_rows_without_a_choice(vocab, dtype):
+    """Rows of -inf, of NaN and of both say -1 (also where a token is -1); the others, and walks that meet none, are as ever."""
+    from sophia_amd import ops
+    tr = ref.Trees([20, 0, 64, 7, 1], "wide", 2, behind=2)
+    gen = torch.Generator().manual_seed(vocab)
+    x = torch.randn(tr.rows, vocab, generator=gen).to(dtype)
+    none = torch.rand(tr.rows, generator=gen) < 0.3
+    none[20], none[0] = False, False
+    x[none] = float("-inf")
+    x[none.nonzero()[::2, 0], 0] = float("nan")
+    tokens = torch.randint(-1, 1, (tr.rows,), generator=gen)
+    chosen = ref.accept(tr, x, tokens, 64)[3]
+    for _, row, path, _ in tr.nodes():
+        if len(path) > 1 and torch.rand((), generator=gen) < 0.8:
+            tokens[row] = chosen[path[-2]]      # (0 after a row without a choice)
+    want = _strict(tr, x, tokens, 64)
+    assert -1 in want[3] and max(want[1]) > 1 and want != ref.accept(tr, x, tokens, 64)
+    got = ops.tree_accept(x.cuda(), tokens.cuda(), tr.cu.cuda(), tr.par.cuda(), max_nodes=64, strict=True)
+    assert tuple(t.tolist() for t in got) == want
+
+
+def test_a_mask_that_allows_nothing_ends_the_sequence():
+    """A drafted child of token 0 below a node whose mask allows nothing is not kept, and no token follows; a sequence beside it
+    goes on."""
+    from sophia_amd.runtime import pack_trees, verify_trees
+    model = _model(seed=9)
+    slots, lens = [2, 0], [30, 11]
+    _prefill(model, slots, lens)
+    start = _caches(model)
+    trees = pack_trees(model, [([5, 0, 0], [-1, 0, 1]), ([7, 0], [-1, 0])], slots, lens)
+    one = torch.zeros(1, 16, dtype=torch.int32, device="cuda")      # nothing; the other rows have no mask
+    rows = torch.tensor([0, -1, -1, -1, -1], dtype=torch.int32, device="cuda")
+    only0 = torch.zeros(1, 16, dtype=torch.int32, device="cuda")
+    only0[0, 0] = 1
+    out = verify_trees(model, trees, allowed=torch.cat([one, only0]), allowed_rows=rows)
+    assert out.n_path[0] == 1 and out.next_token[0] == -1 and out.path[0].tolist() == [0, -1, -1] and out.cached[0] == 31
+    assert out.next_token[1] >= 0
+    got = _caches(model)
+    _load(model, start)
+    model.commit_tree(model.forward_tree(trees), out.path, torch.minimum(out.n_path, out.n_path.new_tensor([1, 2])))
+    for a, b in zip(got, _caches(model)):
+        assert torch.equal(a, b)
+    # where the mask allows token 0 alone, the child of token 0 is kept
+    _load(model, start)
+    out = verify_trees(model, trees, allowed=torch.cat([one, only0]), allowed_rows=rows + (rows == 0).int())
+    assert out.n_path[0] >= 2 and out.path[0, :2].tolist() == [0, 1]
