@@ -131,7 +131,8 @@ int sophia_mla_tree_attn(const void *qa, int64_t qa_stride, const void *latent, 
  *   y = seen ? (x > 0 ? x / repetition[s] : x repetition[s]) - frequency[s] count - presence[s] (count > 0) : x
  *   out = allowed ? y + sum of bias[s, j] with bias_ids[s, j] = v : -inf
  *   logits, out : [rows, vocab] of one type, out may be logits itself.
- *   history     : [n_seqs, history_stride] int64 or NULL; ids outside the vocabulary are not
+ *   history     : [n_seqs, history_stride] int64 or NULL, with trees without the nodes' tokens
+ *                 (node 0's neither); ids outside the vocabulary are not
  *                 looked at, in bias_ids neither; history_len is taken into [0, history_max].
  *   repetition (> 0), presence, frequency : [n_seqs] fp32 or NULL (1, 0, 0).
  *   bias_ids, bias : [n_seqs, n_bias].

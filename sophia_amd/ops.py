@@ -1944,9 +1944,11 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
 
     Row r is sequence r, or with ``cu_nodes`` int32 [N + 1], ``parents`` int32
     [rows], ``tokens`` int64 [rows] and ``max_nodes`` (as in ``mla_tree_attn``)
-    a node of a tree: its ancestors' tokens and its own count as generated ones.
+    a node of a tree: its ancestors' tokens and its own count as generated ones
+    (node 0's too, also where it is a prompt's last token).
     Of each sequence (all optional): ``history`` int64 [N, L] with
-    ``history_len`` int32 [N], the tokens so far, of which the first
+    ``history_len`` int32 [N], the tokens so far (with trees: those in the caches,
+    without node 0, which would count twice), of which the first
     ``prompt_len`` int32 [N] (None: none) count for the repetition penalty only;
     ``repetition`` (> 0), ``presence``, ``frequency`` fp32 [N]; ``bias_ids``
     int64 [N, M] with ``bias`` fp32 [N, M], ids outside the vocabulary ignored,

@@ -209,7 +209,9 @@ class Verified:
 def verify_trees(model: Transformer, trees: DraftTrees, **controls) -> Verified:
     """One step of greedy decoding with drafted tokens: the nodes of all trees
     through the model, their logits adjusted (``controls``: the penalties, biases
-    and masks of ``ops.adjust_logits``, per sequence; allowed_rows per node), the
+    and masks of ``ops.adjust_logits``, per sequence; allowed_rows per node;
+    ``history`` holds the tokens in the caches, history_len == cached: node 0 is a
+    node of every path already, and counts as generated), the
     drafted tokens walked as far as they are the model's own choices, and the
     caches advanced along that path.  A sequence gains n_path tokens in its
     caches and knows the next one: what decoding them one at a time gives, at

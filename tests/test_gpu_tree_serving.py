@@ -78,3 +78,27 @@ def test_a_mask_that_allows_nothing_ends_the_sequence():
     _load(model, start)
     out = verify_trees(model, trees, allowed=torch.cat([one, only0]), allowed_rows=rows + (rows == 0).int())
     assert out.n_path[0] >= 2 and out.path[0, :2].tolist() == [0, 1]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_adjusted_nodes_are_the_single_rows_of_the_texts_that_they_end(dtype):
+    """With the cached tokens as history, each node's logits are what a row of decoding gets whose history is the cached tokens
+    and its path, node 0 counted once."""
+    from sophia_amd import ops
+    tr, vocab, width = ref.Trees([9, 1, 30], "mixed", 4), 777, 50
+    gen = torch.Generator().manual_seed(1)
+    ri = lambda *s: torch.randint(0, 40, s, generator=gen)  # noqa: E731
+    x = (torch.randn(tr.rows, vocab, generator=gen) * 3).to(dtype)
+    cached, prompt, text, tokens = [50, 7, 0], [20, 7, 0], ri(3, width), ri(tr.rows)
+    pens = dict(repetition=torch.tensor([1.3, 1.1, 0.8]), presence=torch.tensor([0.4, 0.0, 0.2]),
+                frequency=torch.tensor([0.1, 0.3, 0.25]))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = ops.adjust_logits(x.cuda(), history=text.cuda(), history_len=i32(cached), prompt_len=i32(prompt), tokens=tokens.cuda(),
+                            cu_nodes=tr.cu.cuda(), parents=tr.par.cuda(), max_nodes=30, **{k: v.cuda() for k, v in pens.items()})
+    of = [(s, path) for s, _, path, _ in tr.nodes()]
+    full = [text[s, :cached[s]].tolist() + tokens[path].tolist() for s, path in of]
+    hist = torch.tensor([t + [0] * (width + 30 - len(t)) for t in full])
+    rows = ops.adjust_logits(x.cuda(), history=hist.cuda(), history_len=i32([len(t) for t in full]),
+                             prompt_len=i32([prompt[s] for s, _ in of]),
+                             **{k: v[[s for s, _ in of]].cuda() for k, v in pens.items()})
+    assert torch.equal(got, rows)
