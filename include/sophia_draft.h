@@ -99,6 +99,17 @@ int sophia_tree_commit(const int32_t *path, int64_t path_stride, const int32_t *
                        int latent_dtype, void *stream);
 
 /*
+ * The same for trees of which only the first max_nodes nodes were looked at (the step's
+ * max_nodes; sophia_tree_commit: SOPHIA_TREE_NODES): the tape holds nothing of the
+ * others, and an index of one of them ends the path too.
+ */
+int sophia_tree_commit_within(const int32_t *path, int64_t path_stride, const int32_t *n_path, int max_path,
+                              const int32_t *cu_nodes, int n_trees, int64_t rows, int max_nodes, const int32_t *slots,
+                              int n_slots, const sophia_commit_kda *kda, int n_kda, int num_heads, int head_dim,
+                              int kernel_size, int x_dtype, const sophia_commit_mla *mla, int n_mla, const int64_t *cached,
+                              int max_seq, int rank, int latent_dtype, void *stream);
+
+/*
  * MLA attention in latent space of every node of the trees over the cached latents
  * of its sequence and the drafted ones of itself and its ancestors (beside
  * sophia_mla_decode_attn, attention.py:609-657 of the reference):

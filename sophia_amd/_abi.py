@@ -109,6 +109,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                     _i32, _vp, _i64, _vp, _vp]),
     "sophia_tree_commit": (_i32, [_vp, _i64, _vp, _i32, _vp, _i32, _i64, _vp, _i32, _vp, _i32, _i32, _i32, _i32,
                                   _i32, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),
+    "sophia_tree_commit_within": (_i32, [_vp, _i64, _vp, _i32, _vp, _i32, _i64, _i32, _vp, _i32, _vp, _i32, _i32, _i32,
+                                         _i32, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),
     "sophia_mla_tree_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32]),
     "sophia_mla_tree_attn": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32,
                                     _i64, _i32, _f32, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _sz, _vp]),

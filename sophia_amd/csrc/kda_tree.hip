@@ -805,10 +805,22 @@ extern "C" int sophia_tree_commit(const int32_t *path, int64_t path_stride, cons
                                   const sophia_commit_kda *kda, int n_kda, int num_heads, int head_dim, int kernel_size,
                                   int x_dtype, const sophia_commit_mla *mla, int n_mla, const int64_t *cached,
                                   int max_seq, int rank, int latent_dtype, void *stream) {
+  return sophia_tree_commit_within(path, path_stride, n_path, max_path, cu_nodes, n_trees, rows, kTreeNodes, slots, n_slots,
+                                   kda, n_kda, num_heads, head_dim, kernel_size, x_dtype, mla, n_mla, cached, max_seq, rank,
+                                   latent_dtype, stream);
+}
+
+extern "C" int sophia_tree_commit_within(const int32_t *path, int64_t path_stride, const int32_t *n_path, int max_path,
+                                         const int32_t *cu_nodes, int n_trees, int64_t rows, int max_nodes,
+                                         const int32_t *slots, int n_slots, const sophia_commit_kda *kda, int n_kda,
+                                         int num_heads, int head_dim, int kernel_size, int x_dtype,
+                                         const sophia_commit_mla *mla, int n_mla, const int64_t *cached, int max_seq,
+                                         int rank, int latent_dtype, void *stream) {
   SOPHIA_REQUIRE(n_trees >= 0 && n_trees <= 65535 && rows >= 0 && n_slots >= 0 && n_kda >= 0 && n_mla >= 0,
                  "tree_commit: n_trees must be 0..65535, rows, n_slots and layer counts >= 0");
   SOPHIA_REQUIRE(max_path >= 1 && max_path <= kTreeNodes && path_stride >= max_path,
                  "tree_commit: max_path must be in [1, %d] and path rows at least as long", kTreeNodes);
+  SOPHIA_REQUIRE(max_nodes >= 1 && max_nodes <= kTreeNodes, "tree_commit: max_nodes must be in [1, %d]", kTreeNodes);
   SOPHIA_REQUIRE((n_kda == 0 || kda) && (n_mla == 0 || mla), "tree_commit: NULL layer list");
   if (n_kda > 0) {
     SOPHIA_REQUIRE(head_dim == kD, "tree_commit: head_dim must be 128 (got %d)", head_dim);
@@ -838,7 +850,7 @@ extern "C" int sophia_tree_commit(const int32_t *path, int64_t path_stride, cons
   for (int k0 = 0, m0 = 0; k0 < n_kda || m0 < n_mla;) {
     const int nk = n_kda - k0 < SOPHIA_COMMIT_KDA ? n_kda - k0 : SOPHIA_COMMIT_KDA;
     const int nm = n_mla - m0 < SOPHIA_COMMIT_MLA ? n_mla - m0 : SOPHIA_COMMIT_MLA;
-    CommitArgs a{{cu_nodes, nullptr, rows, kTreeNodes}, path, path_stride, n_path, max_path, slots, n_slots, num_heads,
+    CommitArgs a{{cu_nodes, nullptr, rows, max_nodes}, path, path_stride, n_path, max_path, slots, n_slots, num_heads,
                  kernel_size, x_dtype, cached, max_seq, rank, latent_dtype, nk, {}, {}};
     for (int l = 0; l < nk; ++l) a.kda[l] = kda[k0 + l];
     for (int l = 0; l < nm; ++l) a.mla[l] = mla[m0 + l];

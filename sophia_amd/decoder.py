@@ -964,7 +964,8 @@ class Transformer(nn.Module):
                 mla.append((kept, attn.latent_cache))
             else:
                 kda.append((*kept, attn.conv_history(), attn.recurrent_state))
-        ops.tree_commit(path, n_path, trees.cu_nodes, trees.slots, kda=kda, mla=mla, cached=trees.cached)
+        ops.tree_commit(path, n_path, trees.cu_nodes, trees.slots, kda=kda, mla=mla, cached=trees.cached,
+                        max_nodes=trees.max_nodes)
         draft.committed = True
 
     def forward_mixed(self, prefill_ids: torch.Tensor, decode_ids: torch.Tensor, *,

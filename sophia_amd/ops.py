@@ -1843,17 +1843,18 @@ def _tape(tape: torch.Tensor, rows: int, heads: int) -> None:
 
 
 def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor, slots: torch.Tensor | None, *,
-                kda=(), mla=(), cached: torch.Tensor | None = None) -> None:
+                kda=(), mla=(), cached: torch.Tensor | None = None, max_nodes: int = TREE_NODES) -> None:
     """Writes an accepted path of every tree into the caches of all layers, in
-    place and in one launch (sophia_tree_commit): what the path's tokens, decoded
-    one by one, would have left there.
+    place and in one launch: what the path's tokens, decoded one by one, would
+    have left there (sophia_tree_commit_within).
 
     path: int32 [N, max_path], node indices within the tree from a root
     downwards; n_path: int32 [N], how many of them count (0: the tree's caches
     stay as they are; an index that is no node of the tree ends the path);
-    cu_nodes, slots: as in ``mla_tree_attn``; the trees of one call have different
-    slots.  kda: for each KDA layer (tape, x_qkv, conv_state, state), the tape
-    and the arguments of its ``kda_tree_step``; mla: for each MLA layer (latent,
+    cu_nodes, slots, max_nodes: as in the step that made the tape, which holds
+    nothing of nodes past max_nodes; the trees of one call have different slots.
+    kda: for each KDA layer (tape, x_qkv, conv_state, state), the tape and the
+    arguments of its ``kda_tree_step``; mla: for each MLA layer (latent,
     latent_cache) of its ``mla_tree_attn``, and ``cached`` int64 [N]: node t of
     the path goes to position cached[s] + t (past the cache's end: left out)."""
     _gpu(path, "path")
@@ -1863,6 +1864,8 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
     n, max_path = int(path.size(0)), int(path.size(1))
     if not 1 <= max_path <= TREE_NODES:
         raise RuntimeError(f"path rows must hold 1..{TREE_NODES} entries, got {max_path}")
+    if not 1 <= int(max_nodes) <= TREE_NODES:
+        raise RuntimeError(f"max_nodes must be in [1, {TREE_NODES}], got {max_nodes}")
     index = path.get_device()
     count = _int32(n_path, "n_path", device)
     cu = _int32(cu_nodes, "cu_nodes", device)
@@ -1924,9 +1927,9 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
                      _latents(cache, rank, "latent_cache"))
     mla_args = (ctypes.c_int64 * max(len(flat), 1))(*flat)   # (sophia_commit_mla: four)
     sl = _tree_slots(slots, n, n_slots, device)
-    rc = _launch(device, nat.lib().sophia_tree_commit, path.data_ptr(), path.stride(0) if n > 1 else max_path,
-                 count.data_ptr(), max_path, cu.data_ptr(), n, rows, nat.ptr(sl), n_slots, kda_args, len(kda), heads,
-                 HEAD_DIM, taps, nat.dtype_code(x_dtype), mla_args, len(mla), cached.data_ptr() if mla else None, max_seq,
+    rc = _launch(device, nat.lib().sophia_tree_commit_within, path.data_ptr(), path.stride(0) if n > 1 else max_path,
+                 count.data_ptr(), max_path, cu.data_ptr(), n, rows, int(max_nodes), nat.ptr(sl), n_slots, kda_args,
+                 len(kda), heads, HEAD_DIM, taps, nat.dtype_code(x_dtype), mla_args, len(mla), cached.data_ptr() if mla else None, max_seq,
                  rank, nat.dtype_code(lat_dtype))
     nat.check(rc, "sophia_tree_commit")
 

@@ -102,3 +102,45 @@ def test_adjusted_nodes_are_the_single_rows_of_the_texts_that_they_end(dtype):
                              prompt_len=i32([prompt[s] for s, _ in of]),
                              **{k: v[[s for s, _ in of]].cuda() for k, v in pens.items()})
     assert torch.equal(got, rows)
+
+
+def test_a_path_past_the_steps_bound_ends_there():
+    """A tree with more nodes than the step's max_nodes: its tape holds nothing of the others (NaN here), and a commit along them
+    takes the part before them."""
+    from sophia_amd import ops
+    from test_gpu_tree_ops import _run_step, _step_case
+    tr, c = _step_case([20, 6], kind="chain", dtype=torch.float32, seed=2)
+    tape = torch.full((tr.rows, 2, 3, 128), float("nan"), device="cuda")
+    _run_step(tr, c, max_nodes=12, tape=tape)
+    path = torch.arange(20, dtype=torch.int32, device="cuda").repeat(2, 1)
+    latent, cached = torch.randn(tr.rows, 32, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    slots, x = c["slots"].cuda(), c["x"].cuda()
+    left = []
+    for count, bound in ((20, 12), (12, 64)):     # the whole path within the bound, and the part before it
+        hist, state, cache = c["conv_state"].cuda(), c["state"].cuda(), torch.zeros(c["state"].size(0), 40, 32, device="cuda")
+        ops.tree_commit(path, torch.tensor([count, 6], dtype=torch.int32, device="cuda"), tr.cu.cuda(), slots,
+                        kda=[(tape, x, hist, state)], mla=[(latent, cache)], cached=cached, max_nodes=bound)
+        left.append((hist, state, cache))
+    for a, b in zip(*left):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    for bound in (0, 65):
+        with pytest.raises(RuntimeError, match="max_nodes"):
+            ops.tree_commit(path, torch.tensor([1, 1], dtype=torch.int32, device="cuda"), tr.cu.cuda(), slots,
+                            kda=[(tape, x, *left[0][:2])], max_nodes=bound)
+
+
+def test_commit_tree_keeps_to_the_steps_bound():
+    from dataclasses import replace
+    from sophia_amd.runtime import pack_trees
+    model = _model(seed=12)
+    _prefill(model, [1], [25])
+    start = _caches(model)
+    trees = replace(pack_trees(model, [([3, 4, 5, 6, 7], [-1, 0, 1, 2, 3])], [1], [25]), max_nodes=3)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    left = []
+    for count in (5, 3):
+        _load(model, start)
+        model.commit_tree(model.forward_tree(trees), i32([[0, 1, 2, 3, 4]]), i32([count]))
+        left.append(_caches(model))
+    for a, b in zip(*left):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
