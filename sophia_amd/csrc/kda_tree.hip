@@ -42,7 +42,8 @@
 //
 // A node with an input that is not finite would reach its siblings through the
 // products (0 times infinity): its rows enter them as zeros, and what lies on a
-// path with it ends as NaN.
+// path with it ends as NaN; where that is its q alone, which no other node reads, its
+// own output.
 #include <type_traits>
 
 #include "common.hpp"
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
   __shared__ float s_beta[T];
   __shared__ uint64_t s_path[kTreeNodes];
   __shared__ int s_up[6][kTreeNodes];                   // s_up[0]: parents
-  __shared__ int s_bad[kTreeNodes], s_far;
+  __shared__ int s_bad[kTreeNodes], s_bad_q[kTreeNodes], s_far;
   auto &mat = lds.mat;
 
   const int h = blockIdx.x, tree = blockIdx.y;
@@ -279,6 +280,7 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
     const bool ok = is_finite(b);
     if (t < T) s_beta[t] = t < n && ok ? b : 0.f;
     s_bad[t] = !ok;
+    s_bad_q[t] = 0;
   }
   if (t == 0) s_far = 0;
   load_state(std::integral_constant<int, 1>{});
@@ -286,6 +288,8 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
 
   // ---- conv, norms, log-decay: in registers
   // Predecessors, counted from the oldest history sample: 0, 1, 2, then node i as 3 + i.
+  // Where a shorter conv has none, the node itself: its tap is 0, and 0 times another
+  // node's sample need not be.
   float qkv[3][P][8], g[P][8], bias[8];
   to_float(raw_bias, bias);
   const float head_scale = __expf(a_log);
@@ -298,7 +302,7 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
 #pragma unroll
     for (int d = 1; d < 4; ++d) {
       const int at = e[p][d - 1], up = s_up[0][max(at - 3, 0)];
-      e[p][d] = at < 3 ? at - 1 : (up < 0 ? 2 : up + 3);
+      e[p][d] = d > hist ? e[p][0] : at < 3 ? at - 1 : (up < 0 ? 2 : up + 3);
     }
   }
 #pragma unroll
@@ -340,7 +344,7 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
       qs = a.scale / fmaxf(sqrtf(row_sum16(sq)), 1e-12f);
       ks = 1.f / fmaxf(sqrtf(row_sum16(sk)), 1e-12f);
     }
-    bool ok = true;
+    bool ok = true, ok_q = true;
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       q[p][c] *= qs;
@@ -350,12 +354,19 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
                           : __uint_as_float(raw_g[p][2 * (c >> 2) + ((c & 3) >> 1)][c & 1]);
       g[p][c] = gate ? kda_log_decay(z, head_scale, bias[c], a.lower_bound) : z;
       g[p][c] = g[p][c] < kForgotten ? kForgotten : g[p][c];   // (NaN stays)
-      ok &= is_finite(q[p][c]) && is_finite(k[p][c]) && is_finite(v[p][c]) && is_finite(g[p][c]);
+      ok &= is_finite(k[p][c]) && is_finite(v[p][c]) && is_finite(g[p][c]);
+      ok_q &= is_finite(q[p][c]);
     }
-    if (((__ballot(!ok) >> (lane & 48)) & 0xffff) != 0) {   // (of the node's 16 threads alike)
+    const auto any16 = [&](bool x) { return ((__ballot(x) >> (lane & 48)) & 0xffff) != 0; };   // (of the node's 16 threads)
+    if (any16(!ok)) {
 #pragma unroll
-      for (int c = 0; c < 8; ++c) q[p][c] = k[p][c] = v[p][c] = g[p][c] = 0.f;
+      for (int c = 0; c < 8; ++c) k[p][c] = v[p][c] = g[p][c] = 0.f;
       s_bad[node] = 1;
+    }
+    if (any16(!ok_q)) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) q[p][c] = 0.f;
+      s_bad_q[node] = 1;
     }
   }
   load_state(std::integral_constant<int, 2>{});
@@ -392,7 +403,7 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
     put_g(to);
     lds_barrier();
   }
-  const uint64_t bad = __ballot(s_bad[lane] != 0);
+  const uint64_t bad = __ballot(s_bad[lane] != 0), bad_q = __ballot(s_bad_q[lane] != 0);
   const bool far = s_far != 0;
   const int mt = MT == 1 ? 1 : (n + 15) >> 4;   // tiles that hold nodes
 
@@ -629,7 +640,7 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
       if (node >= n) continue;
       const int64_t row = base + node;
       const float nan = s_path[node] & bad ? NAN : 0.f;
-      store_elem(a.o, row * a.o_stride + vc, DT, o[m][i] + nan);
+      store_elem(a.o, row * a.o_stride + vc, DT, o[m][i] + ((bad_q >> node) & 1 ? NAN : nan));
       a.tape[(row * a.heads + h) * kTape + col] = u[m][i] + nan;
     }
   }

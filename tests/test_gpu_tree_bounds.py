@@ -80,3 +80,23 @@ def test_tree_step_after_one_strong_decay(drop):
     got, tape = _run_step(tr, c, gate=False)
     _within(tape, want["tape"], want["tol_tape"])
     _within(got, want["o"], want["tol_o"])
+
+
+@pytest.mark.parametrize("taps", [1, 4])
+def test_a_q_that_is_not_finite_is_its_own_nodes_output_alone(taps):
+    """As in the decode step: q enters no state, so the tape and the other nodes' outputs are as without it (but for those whose
+    conv reads the sample)."""
+    tr, c = _step_case([40, 12], kind="mixed", dtype=F32, seed=11, taps=taps)
+    want = tree_bounds.step(tr, **c)
+    hit = {3: (0, float("nan")), 17: (1, float("inf")), 41: (0, float("-inf"))}     # row: head, value (of q)
+    for row, (head, value) in hit.items():
+        c["x"][row, head * 128 + 9] = value
+    got, tape = _run_step(tr, c)
+    _within(tape, want["tape"], want["tol_tape"])
+    for _, row, path, _ in tr.nodes():
+        for head in range(2):
+            read = [r for r in path[-taps:] if r in hit and hit[r][0] == head]
+            if read:
+                assert torch.isnan(got[row, head]).all()
+            else:
+                _within(got[row, head], want["o"][row, head], want["tol_o"][row, head])
