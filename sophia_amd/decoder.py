@@ -931,8 +931,11 @@ class Transformer(nn.Module):
         own path through the tree, and the caches are left as they are.
         ``DraftStep.logits`` [rows, vocab] are those of a decode step that had
         taken each node's path token by token; ``commit_tree`` then advances
-        the caches along one path of each tree.  Nothing is read back on the
-        host, so the step is capturable.  Values only (no gradient)."""
+        the caches along one path of each tree.  Like that step (``forward_step``)
+        it attends to every cached latent of its slot, so a prompt whose padding
+        is masked (``set_pad_mask``) is refused until the mask is cleared.
+        Nothing is read back on the host, so the step is capturable.  Values only
+        (no gradient)."""
         _require_gpu(trees.token_ids)
         rows, n = int(trees.token_ids.numel()), int(trees.slots.numel())
         if rows == 0 or n == 0:
@@ -941,6 +944,9 @@ class Transformer(nn.Module):
             raise ValueError("sequence exceeds max_seq_len")
         if not self.args.use_cache:
             raise RuntimeError("forward_tree needs use_cache=True (it reads cache slots)")
+        if any(getattr(layer.attn, "_prompt_mask", None) is not None for layer in self.layers):
+            raise RuntimeError("a padded prompt is in the caches, whose pad keys this step would attend to; "
+                               "set_pad_mask(model, None) when none of its slots is used")
         hidden = self.tok_embeddings(trees.token_ids.reshape(-1))
         completed = depth_store(hidden, self.args.n_layers, self.args.attn_res_block_size)
         pending, kept = None, []

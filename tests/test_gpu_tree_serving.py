@@ -144,3 +144,26 @@ def test_commit_tree_keeps_to_the_steps_bound():
         left.append(_caches(model))
     for a, b in zip(*left):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_padded_prompts_are_refused_until_their_mask_is_cleared():
+    """The step has no mask over cached keys: a left-padded prompt's pads would be attended to."""
+    from sophia_amd.kda import set_pad_mask
+    from sophia_amd.runtime import pack_trees, verify_trees
+    model = _model(seed=13)
+    ids = torch.randint(0, 512, (2, 20), generator=torch.Generator().manual_seed(1)).cuda()
+    mask = torch.ones(2, 20, dtype=torch.bool, device="cuda")
+    mask[0, :7] = False
+    set_pad_mask(model, mask)
+    with torch.no_grad():
+        model(ids)
+    before = _caches(model)
+    trees = pack_trees(model, [([1, 2], [-1, 0]), ([3], [-1])], [0, 1], [20, 20])
+    with pytest.raises(RuntimeError, match="set_pad_mask"):
+        verify_trees(model, trees)
+    for a, b in zip(before, _caches(model)):
+        assert torch.equal(a, b)
+    set_pad_mask(model, None)
+    with torch.no_grad():
+        model(ids)
+    assert verify_trees(model, trees).n_path.min() >= 1
