@@ -929,11 +929,14 @@ class Transformer(nn.Module):
         reference cannot express (one token per sequence after the prompt,
         transformer.py:146-160): every node sees its sequence's caches and its
         own path through the tree, and the caches are left as they are.
-        ``DraftStep.logits`` [rows, vocab] are those of a decode step that had
-        taken each node's path token by token; ``commit_tree`` then advances
-        the caches along one path of each tree.  Like that step (``forward_step``)
-        it attends to every cached latent of its slot, so a prompt whose padding
-        is masked (``set_pad_mask``) is refused until the mask is cleared.
+        ``DraftStep.logits`` [rows, vocab] are those of a decode step
+        (``forward_step``) that had taken each node's path token by token, but for
+        roundings: this step keeps conv outputs in fp32, which a bf16 model's
+        decode step rounds, and an fp32 model's latent attention in fp32, which
+        its decode step has in bf16.  ``commit_tree`` then advances the caches
+        along one path of each tree.  Like the decode step it attends to every
+        cached latent of its slot, so a prompt whose padding is masked
+        (``set_pad_mask``) is refused until the mask is cleared.
         Nothing is read back on the host, so the step is capturable.  Values only
         (no gradient)."""
         _require_gpu(trees.token_ids)

@@ -15,7 +15,7 @@ only at start_pos 0, runtime_host.py:146-170); here every step is one
 
 ``pack_trees`` and ``verify_trees`` are greedy decoding with drafted tokens: a
 server proposes a tree of continuations for each running sequence, one step runs
-all of them, and the longest part that the model itself would have said is kept.
+all of them, and the longest part that the model itself says is kept.
 """
 
 from __future__ import annotations
@@ -211,12 +211,13 @@ def verify_trees(model: Transformer, trees: DraftTrees, **controls) -> Verified:
     through the model, their logits adjusted (``controls``: the penalties, biases
     and masks of ``ops.adjust_logits``, per sequence; allowed_rows per node;
     ``history`` holds the tokens in the caches, history_len == cached: node 0 is a
-    node of every path already, and counts as generated), the
-    drafted tokens walked as far as they are the model's own choices, and the
-    caches advanced along that path.  A sequence gains n_path tokens in its
-    caches and knows the next one: what decoding them one at a time gives, at
-    least one token per step.  Nothing is read back on the host, so the step is
-    capturable."""
+    node of every path already, and counts as generated), the drafted tokens
+    walked as far as they are the model's own choices, and the caches advanced
+    along that path.  A sequence gains n_path tokens in its caches, at least one,
+    and knows the next: what steps over trees of one node give.  Decode steps
+    (``forward_step``) round elsewhere (``Transformer.forward_tree``), so where two
+    logits are closer than that, they may choose the other.  Nothing is read back
+    on the host, so the step is capturable."""
     draft = model.forward_tree(trees)
     logits = draft.logits
     if controls:

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import tree_ref as ref
-from test_gpu_tree_decode import _caches, _load, _model, _prefill
+from test_gpu_tree_decode import _caches, _decode, _load, _model, _prefill
 
 pytestmark = pytest.mark.gpu
 
@@ -167,3 +167,32 @@ def test_padded_prompts_are_refused_until_their_mask_is_cleared():
     with torch.no_grad():
         model(ids)
     assert verify_trees(model, trees).n_path.min() >= 1
+
+
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 2e-2), (torch.bfloat16, 6e-2)], ids=["f32", "bf16"])
+def test_drafted_decoding_chooses_greatest_logits_of_decode_steps(dtype, tol):
+    """Every token that decoding with drafted trees keeps or says has, in decode steps over the same text, a logit as great as
+    any but for the roundings that the steps do not share (the tolerances of the decoder's own tests, relative to the greatest
+    magnitude, on either logit)."""
+    from sophia_amd.runtime import pack_trees, verify_trees
+    model = _model(seed=14, dtype=dtype)
+    _, first = _prefill(model, [3], [37])
+    start = _caches(model)
+    text, cached, known = [], 37, first[0]
+    while len(text) < 24:      # drafts from the model itself: what it says after its last choice, and a wrong token beside
+        probe = _caches(model)
+        guess = [known]
+        for _ in range(3):
+            out = verify_trees(model, pack_trees(model, [([guess[-1]], [-1])], [3], [cached + len(guess) - 1]))
+            guess.append(int(out.next_token[0]))
+        _load(model, probe)
+        tree = (guess[:1] + [(guess[1] + 1) % 512] + guess[1:], [-1, 0, 0, 2, 3])
+        out = verify_trees(model, pack_trees(model, [tree], [3], [cached]))
+        text += [tree[0][i] for i in out.path[0, :int(out.n_path[0])].tolist()]
+        cached, known = int(out.cached[0]), int(out.next_token[0])
+        assert cached == 37 + len(text)
+    _load(model, start)
+    rows = _decode(model, text, 3, 37)
+    for said, row in zip(text[1:] + [known], rows):
+        row = row.double()
+        assert float(row.max() - row[said]) <= 2 * tol * float(row.abs().max())
