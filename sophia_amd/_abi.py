@@ -41,6 +41,15 @@ class CommitMla(ctypes.Structure):
                 ("slot_stride", ctypes.c_int64)]
 
 
+def packed(struct, words: list[int]):
+    """An array of ``struct``, whose fields are 8 bytes each, from all its fields in a row (None: of
+    nothing); field by field it would be a Python object for each."""
+    if not words:
+        return None
+    flat = (ctypes.c_int64 * len(words))(*words)
+    return (struct * (ctypes.sizeof(flat) // ctypes.sizeof(struct))).from_buffer(flat)
+
+
 # Every symbol of include/sophia_kda.h, include/sophia_decoder.h and
 # include/sophia_draft.h, with its ctypes signature.
 _vp = ctypes.c_void_p

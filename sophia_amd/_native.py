@@ -33,6 +33,7 @@ from ._abi import (  # noqa: F401
     TREE_NODES,
     CommitKda,
     CommitMla,
+    packed,
 )
 
 _HERE = os.path.dirname(os.path.abspath(__file__))

@@ -1907,7 +1907,7 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
                     f"dense rows, conv_state contiguous fp32 {list(hist_shape)} and state contiguous fp32 "
                     f"{list(state_shape)}, as in every layer")
             flat += (tape.data_ptr(), x.data_ptr(), x.stride(0) if rows > 1 else 3 * inner, hist, state.data_ptr())
-    kda_args = (ctypes.c_int64 * max(len(flat), 1))(*flat)   # (sophia_commit_kda: five words a layer)
+    kda_args = nat.packed(nat.CommitKda, flat)
     flat = []
     lat_dtype = f32
     if mla:
@@ -1925,7 +1925,7 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
                                    f"latent_cache fp32 [{n_slots}, {max_seq}, {rank}], as in every layer")
             flat += (latent.data_ptr(), latent.stride(0) if rows > 1 else rank, cache.data_ptr(),
                      _latents(cache, rank, "latent_cache"))
-    mla_args = (ctypes.c_int64 * max(len(flat), 1))(*flat)   # (sophia_commit_mla: four)
+    mla_args = nat.packed(nat.CommitMla, flat)
     sl = _tree_slots(slots, n, n_slots, device)
     rc = _launch(device, nat.lib().sophia_tree_commit_within, path.data_ptr(), path.stride(0) if n > 1 else max_path,
                  count.data_ptr(), max_path, cu.data_ptr(), n, rows, int(max_nodes), nat.ptr(sl), n_slots, kda_args,

@@ -31,3 +31,19 @@ def test_commit_within_of_nothing(nat):  # noqa: F811
 def test_strict_accept_refuses(nat, change, word):  # noqa: F811
     rc, msg = host._call(nat, "sophia_tree_accept_strict", host.ACCEPT_OK, host.ACCEPT, **change)
     assert rc == nat.SOPHIA_ERR_INVALID and word in msg, msg
+
+
+def test_layer_lists_are_the_structures_of_the_header():
+    """What tree_commit hands over: field by field the words it was made of, none left."""
+    import ctypes
+    from sophia_amd import _abi
+    for struct in (_abi.CommitKda, _abi.CommitMla):
+        fields = [f for f, _ in struct._fields_]
+        assert ctypes.sizeof(struct) == 8 * len(fields)
+        words = [(1 << 40) + 3 * i for i in range(7 * len(fields))]
+        made = _abi.packed(struct, words)
+        assert len(made) == 7 and made._type_ is struct
+        assert [getattr(layer, f) for layer in made for f in fields] == words
+        assert _abi.packed(struct, []) is None
+    nulls = _abi.packed(_abi.CommitKda, [1, 2, 3, 0, 5])
+    assert nulls[0].conv_state is None and nulls[0].state == 5
