@@ -592,7 +592,9 @@ class DraftTrees:
     ``max_nodes`` (at most 64) bounds the nodes of a tree, ``max_len`` bounds
     ``cached``: host ints.  Trees without nodes and rows behind the last tree
     are allowed (their logits mean nothing): a captured step of a fixed number of
-    rows then takes trees of any size within it, copied into its tensors."""
+    rows then takes trees of any size within it, copied into its tensors.  A token
+    outside the vocabulary is run as the nearest one in it: the next_token -1 of a
+    sequence that has ended may come back before the host knows of it."""
 
     token_ids: torch.Tensor
     cu_nodes: torch.Tensor
@@ -950,7 +952,8 @@ class Transformer(nn.Module):
         if any(getattr(layer.attn, "_prompt_mask", None) is not None for layer in self.layers):
             raise RuntimeError("a padded prompt is in the caches, whose pad keys this step would attend to; "
                                "set_pad_mask(model, None) when none of its slots is used")
-        hidden = self.tok_embeddings(trees.token_ids.reshape(-1))
+        ids = trees.token_ids.reshape(-1).clamp(0, int(self.args.vocab_size) - 1)
+        hidden = self.tok_embeddings(ids)
         completed = depth_store(hidden, self.args.n_layers, self.args.attn_res_block_size)
         pending, kept = None, []
         for layer in self.layers:

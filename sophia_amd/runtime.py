@@ -196,8 +196,8 @@ class Verified:
     max_nodes] (the kept nodes, -1 behind them), ``n_path`` int32 [N],
     ``next_token`` int64 [N] (the token after the path: the next tree's node 0;
     -1: there is none, as the last node's logits are all masked or NaN, and the
-    sequence ends),     ``cached`` int64 [N] (tokens in the caches now), ``logits`` [rows, vocab] of
-    every node, adjusted."""
+    sequence ends), ``cached`` int64 [N] (tokens in the caches now), ``logits``
+    [rows, vocab] of every node, adjusted."""
 
     path: torch.Tensor
     n_path: torch.Tensor

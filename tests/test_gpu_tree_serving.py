@@ -196,3 +196,20 @@ def test_drafted_decoding_chooses_greatest_logits_of_decode_steps(dtype, tol):
     for said, row in zip(text[1:] + [known], rows):
         row = row.double()
         assert float(row.max() - row[said]) <= 2 * tol * float(row.abs().max())
+
+
+def test_an_ended_sequences_token_may_come_back():
+    """next_token -1 as node 0 of the next tree (a step whose tokens stay on the device): run as a token of the vocabulary, and
+    the trees beside it are as they are without it."""
+    from dataclasses import replace
+    from sophia_amd.runtime import pack_trees, verify_trees
+    model = _model(seed=15)
+    _prefill(model, [0, 4], [12, 50])
+    start = _caches(model)
+    trees = pack_trees(model, [([0, 3], [-1, 0]), ([7, 1, 511], [-1, 0, 0])], [0, 4], [12, 50])
+    want, kept = verify_trees(model, trees), _caches(model)
+    _load(model, start)
+    out = verify_trees(model, replace(trees, token_ids=torch.tensor([-1, 3, 7, 1, 600], device="cuda")))
+    assert torch.equal(out.logits, want.logits) and torch.equal(out.n_path, want.n_path)
+    for a, b in zip(_caches(model), kept):
+        assert torch.equal(a, b)
