@@ -1702,7 +1702,8 @@ def mla_tree_attn(qa: torch.Tensor, latent: torch.Tensor, latent_cache: torch.Te
 
     qa: [rows, heads, rank] (bf16 or fp32, heads <= 16, rank in 32/64/128/256),
     the nodes of all trees; latent: [rows, rank] of qa's dtype; latent_cache:
-    [n_slots, max_seq, rank] fp32 with dense rows; cu_nodes int32 [N + 1], the
+    [n_slots, max_seq, rank] fp32 with dense rows (all of these and out: 16-byte
+    aligned, row strides multiples of 8); cu_nodes int32 [N + 1], the
     rows of each tree; parents int32 [rows], a node's parent as an index into
     its own tree, before the node (else, -1 say, the node is a root, which
     follows the cached tokens); slots int32 [N] (None: s); cached int64 [N].
@@ -1774,9 +1775,10 @@ def kda_tree_step(x_qkv: torch.Tensor, conv_weight: torch.Tensor, conv_state: to
     a multiple of 8, 16-byte aligned); conv_weight: [3 * H * 128, K] fp32 taps
     rounded to x_qkv.dtype, K in 1..4; conv_state: fp32 [slots, 3 * H * 128,
     K - 1] (None for K = 1); g: [rows, H, 128] decay logits, or with
-    ``use_gate=False`` log-decays (-inf: the state is forgotten); beta: [rows, H];
-    state: fp32 [slots, H, 128, 128]; cu_nodes, parents, max_nodes: as in ``mla_tree_attn``.  q, k and v
-    stay in fp32 from the conv on.  Returns (o [rows, H, 128] in x_qkv.dtype,
+    ``use_gate=False`` log-decays (-inf: the state is forgotten), aligned as x_qkv
+    is (out too); beta: [rows, H]; state: fp32 [slots, H, 128, 128]; cu_nodes,
+    parents, max_nodes: as in ``mla_tree_attn``.  q, k and v stay in fp32 from the
+    conv on.  Returns (o [rows, H, 128] in x_qkv.dtype,
     tape [rows, H, 3, 128] fp32: what ``tree_commit`` takes to advance the state
     along an accepted path)."""
     _gpu(x_qkv, "x_qkv")
