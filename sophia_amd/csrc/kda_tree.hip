@@ -29,8 +29,8 @@
 // What bounds it: the steps' latency.  One tree of 7 nodes takes 13 us (16 heads on
 // as many CUs, 25,000 cycles from the first load to the last store), 64 trees of 8 to
 // 24 nodes 55 us, two work-groups per CU in two rounds, where their 114 MB take 22 us
-// at the rate of a copy; there the matrix pipes are busy a quarter of the time, the
-// vector unit and LDS about as much.  8 fp32 chains of 17 to 64 nodes take 39 us: half
+// at the rate of a copy; there the matrix pipes are busy 27 % of the time, the
+// vector unit 31 and LDS 20.  8 fp32 chains of 17 to 64 nodes take 39 us: half
 // the CUs, 72,000 cycles for 64 nodes, of which the products with S, at the fp32 MFMA
 // rate, are 20,000.  On the way (us, these three cases): samples gathered from memory tap
 // by tap 21, 128, 121; samples through LDS, pairs on the vector unit 23, 83, 59; conv taps
@@ -652,7 +652,7 @@ __global__ __launch_bounds__(kThreads, MT == 4 ? 2 : 4) void kda_tree_step_kerne
 // trees of a small batch then still fill the chip, and 28 launches become one.
 // Bound by the state: 64 KiB read and written per (layer, tree, head), in place,
 // as the decode step moves it (thread: 4 columns of every 16th row).  28 layers of 48
-// trees: 2.3 GB in 393 us, 5.9 TB/s (a copy of 1 GiB: 5.2); of 4 trees: 192 MB in 41 us.
+// trees: 2.3 GB in 410 us, 5.6 TB/s (a copy of 1 GiB: 5.15); of 4 trees: 192 MB in 38 us.
 struct CommitArgs {
   Trees trees;
   const int32_t *path;

@@ -9,13 +9,14 @@
 // streams its rows through both.  Tokens of a tree are few and mostly in other
 // tiles, so a row's own ones are taken one by one, by the thread that has each.
 // 362 rows of 24 trees, 65,536 tokens, bf16, histories of up to 4,000 tokens: 96 MB in
-// 30 us (18.6 at the rate of a copy; about a third of a work-group's time is its
-// setup); 8 rows in fp32: 4.2 MB in 5.2 us, latency.
+// 29 us (18.6 at the rate of a copy; about a third of a work-group's time is its
+// setup); 8 rows in fp32: 4.2 MB in 5.3 us, latency.
 //
 // Accept: the chosen tokens of all rows in parts, then one wavefront per tree,
 // whose lanes are the nodes, joins the parts and walks: a step is one ballot.  1,061
-// rows of 64 trees, bf16: 139 MB in 22 us, 6.3 TB/s, and 4 for the walk; 7 rows 3.3
-// and 2.5.
+// rows of 64 trees, bf16: 139 MB in 22 us, 6.2 TB/s, and 4 for the walk; 7 rows 3.5
+// and 2.4.  Rows off 16 bytes, one logit per lane at a time, are far from that: as many
+// rows of 50,257 tokens 86 us with the walk, 1.2 TB/s.
 #include "common.hpp"
 #include "tree.hpp"
 
@@ -381,7 +382,10 @@ bool dtype_ok(int dtype) { return dtype == SOPHIA_DTYPE_F32 || dtype == SOPHIA_D
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Parts of a row's argmax: enough work-groups to fill the chip several times,
-// whole tiles each, and no more than the join loads at once.
+// whole tiles each, and no more than the join loads at once.  us with 1,024, 2,048, 4,096
+// and 8,192 of them (bf16, with the walk): 1,061 rows of 65,536 logits 34, 31, 30, 29; of
+// 32,000 17.1, 16.3, 16.1, 18.7; 362 rows of 65,536 14.4, 14.3, 13.3, 13.3; 64 rows and
+// fewer alike.
 int argmax_parts(int64_t rows, int vocab) {
   const int64_t tiles = (static_cast<int64_t>(vocab) + kTileV - 1) / kTileV;
   const int64_t want = (4096 + rows - 1) / (rows > 0 ? rows : 1);
@@ -421,8 +425,10 @@ extern "C" int sophia_adjust_logits(const void *logits, int64_t logits_stride, v
                n_bias ? bias_ids : nullptr, bias, n_bias, allowed, allowed_rows, n_masks, (vocab + 31) / 32, 0};
   // Rows of a sequence per work-group: every one of them counts the history again,
   // but fewer than 1,536 of them leave the slow ones (a tile with the tokens that
-  // repeat most) behind the others: 24 trees of 8 to 24 nodes, 65,536 tokens, bf16,
-  // 34.6 us with 768, 30.3 with 1,536, 32.5 with 2,304.
+  // repeat most) behind the others.  us with 768, 1,536 and 2,304: 24 trees of 8 to 24
+  // nodes, 65,536 tokens, bf16, 38, 30, 35; 32,000 tokens 22, 24, 23; 8 trees of 24 to 64
+  // nodes 41, 38, 39; in fp32, 128,256 tokens, 99, 89, 90; 64 trees of 16 to 24, which
+  // have as many without a division, 81, 81, 82.
   const int64_t fill = static_cast<int64_t>(tiles) * n_seqs;
   const int groups = static_cast<int>(iclamp64((1536 + fill - 1) / fill, 1, (a.trees.max_nodes + kRows - 1) / kRows));
   a.rows_per_group = (a.trees.max_nodes + groups - 1) / groups;

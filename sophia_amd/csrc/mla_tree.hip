@@ -24,15 +24,17 @@
 // MFMAs per wavefront, 1,536 cycles (a third of them for what the probabilities lose when
 // rounded once); 128 KB of LDS reads for its four wavefronts, 1,024 cycles of the CU; and
 // about 300 vector instructions, mostly the softmax, with 32 exponentials.  Two wavefronts
-// per SIMD (226 registers) share these.  Before its first tile and after its last a
-// work-group spends 8,000 cycles.  One tree of 7 nodes after 523 keys takes 10 us and 4, all
-// of it latency.  On the way, for the 32 trees: ranges by number instead of
-// length 79; three copies of the tile's code for masked and whole tiles, whose spilled
-// registers were waited for together with the next tile 50 + 8; one copy 42 + 8; shares from
-// a list of what there is, instead of a grid over the bounds, which left CUs without work
-// beside others with two shares, and partials stored as the lanes hold them 29 + 9; rows
-// read ahead of their products and a reference that seldom moves 27 + 10; probabilities in
-// two parts 32 + 10.  Not kept, as no
+// per SIMD (226 registers) share these; over the whole kernel the matrix pipes are busy 35 %
+// of the time, the vector unit 42 and LDS 21, as a work-group spends 8,000 cycles before its
+// first tile and after its last, and some have a tile more than others.  One tree of 7 nodes
+// after 523 keys takes 10 us and 4, all of it latency.  The same 32 trees at other ranks, with
+// the merge: 32 27 us, 64 32, 128 42, 256 150 (76 bytes of a lane's state in scratch).
+// On the way, for the 32 trees: ranges by number instead of length 79; three copies of the
+// tile's code for masked and whole tiles, whose spilled registers were waited for together
+// with the next tile 50 + 8; one copy 42 + 8; shares from a list of what there is, instead of
+// a grid over the bounds, which left CUs without work beside others with two shares, and
+// partials stored as the lanes hold them 29 + 9; rows read ahead of their products and a
+// reference that seldom moves 27 + 10; probabilities in two parts 32 + 10.  Not kept, as no
 // faster: two tiles in LDS and one barrier a tile, lines of the tiles ahead loaded early.
 #include <type_traits>
 
@@ -472,8 +474,8 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_kernel(MlaTree
 // 16x16x4 MFMAs in fp32 throughout: an fp32 model's latents have more bits than
 // bf16 holds.  5 trees of 1 to 32 nodes after up to 3,001 keys: 16 us and 7 for the
 // merge; a tile takes a wavefront 256 MFMAs of 32 cycles (9,700 in all; 12,100 while the
-// compiler read V right before each product), and only the keys divide it further.  A lane's four consecutive ranks of a key are the A operands of four
-// steps (the k index runs 4 (lane / 16) + step), and the scores' accumulator, keys
+// compiler read V right before each product), and only the keys divide it further.  A
+// lane's four consecutive ranks of a key are the A operands of four steps (the k index runs 4 (lane / 16) + step), and the scores' accumulator, keys
 // 4 (lane / 16) + i, is the B operand of the value product in the same order.
 template <int R>
 __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_tree_f32_kernel(MlaTreeArgs a) {

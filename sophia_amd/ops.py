@@ -1754,9 +1754,12 @@ def mla_tree_splits(max_len: int) -> int:
     """Key ranges of ``mla_tree_attn`` at most, of a context of ``max_len`` keys: of
     TREE_RANGE tiles as long as there are few (where the work does not fill the
     chip each tile more is latency, and a range costs about three tiles' time before
-    and after its tiles: one tree after 523 keys 13 us with 2, 14 with 3, 17 with 8;
-    the kernel makes them longer where it does), and 128, which the merge joins one
-    after the other."""
+    and after its tiles; the kernel makes them longer where it does), and 128, which
+    the merge joins one after the other.  us with ranges of 1, 2, 3, 4 and 8 tiles,
+    bf16: a tree of 7 nodes after 523 keys 12.5, 13.0, 13.1, 14.3, 17.1, after 4,000
+    21.5, 17.6, 16.8, 17.6, 21.7; of 64 nodes after 4,000 25, 25, 22, 20, 22; 8 trees
+    of 16 21, 17, 18, 19, 21; 32 of 24 to 64 44, 42, 42, 42, 42; fp32, 5 trees after
+    up to 3,001 keys 29, 23, 25, 28, 44, one of 7 after 523 14, 18, 21, 26, 30."""
     return min(128, -(-(-(-max_len // 64) + 1) // TREE_RANGE))
 
 
@@ -1931,8 +1934,8 @@ def tree_commit(path: torch.Tensor, n_path: torch.Tensor, cu_nodes: torch.Tensor
     sl = _tree_slots(slots, n, n_slots, device)
     rc = _launch(device, nat.lib().sophia_tree_commit_within, path.data_ptr(), path.stride(0) if n > 1 else max_path,
                  count.data_ptr(), max_path, cu.data_ptr(), n, rows, int(max_nodes), nat.ptr(sl), n_slots, kda_args,
-                 len(kda), heads, HEAD_DIM, taps, nat.dtype_code(x_dtype), mla_args, len(mla), cached.data_ptr() if mla else None, max_seq,
-                 rank, nat.dtype_code(lat_dtype))
+                 len(kda), heads, HEAD_DIM, taps, nat.dtype_code(x_dtype), mla_args, len(mla),
+                 cached.data_ptr() if mla else None, max_seq, rank, nat.dtype_code(lat_dtype))
     nat.check(rc, "sophia_tree_commit")
 
 
@@ -2073,8 +2076,8 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tens
     next_token = torch.empty(n, dtype=torch.int64, device=device)
     chosen = torch.empty(rows, dtype=torch.int64, device=device)
     ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device)
-    rc = _launch(device, lib.sophia_tree_accept_strict if strict else lib.sophia_tree_accept, logits.data_ptr(), xs, nat.dtype_code(logits.dtype), rows, vocab,
-                 tokens.data_ptr(), cu_nodes.data_ptr(), parents.data_ptr(), n, int(max_nodes), path.data_ptr(),
+    rc = _launch(device, lib.sophia_tree_accept_strict if strict else lib.sophia_tree_accept, logits.data_ptr(), xs,
+                 nat.dtype_code(logits.dtype), rows, vocab, tokens.data_ptr(), cu_nodes.data_ptr(), parents.data_ptr(), n, int(max_nodes), path.data_ptr(),
                  int(max_nodes), n_path.data_ptr(), next_token.data_ptr(), chosen.data_ptr(), ws.data_ptr(), nbytes)
     nat.check(rc, "sophia_tree_accept")
     return path, n_path, next_token, chosen
