@@ -2077,8 +2077,9 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tens
     chosen = torch.empty(rows, dtype=torch.int64, device=device)
     ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device)
     rc = _launch(device, lib.sophia_tree_accept_strict if strict else lib.sophia_tree_accept, logits.data_ptr(), xs,
-                 nat.dtype_code(logits.dtype), rows, vocab, tokens.data_ptr(), cu_nodes.data_ptr(), parents.data_ptr(), n, int(max_nodes), path.data_ptr(),
-                 int(max_nodes), n_path.data_ptr(), next_token.data_ptr(), chosen.data_ptr(), ws.data_ptr(), nbytes)
+                 nat.dtype_code(logits.dtype), rows, vocab, tokens.data_ptr(), cu_nodes.data_ptr(), parents.data_ptr(), n,
+                 int(max_nodes), path.data_ptr(), int(max_nodes), n_path.data_ptr(), next_token.data_ptr(),
+                 chosen.data_ptr(), ws.data_ptr(), nbytes)
     nat.check(rc, "sophia_tree_accept")
     return path, n_path, next_token, chosen
 
