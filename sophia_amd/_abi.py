@@ -1,8 +1,8 @@
 """The C ABI of ``libsophia_kda.so`` as a ctypes table, with no torch import.
 
 Status codes, element types and flag bits of include/sophia_kda.h and every
-entry point of include/sophia_kda.h, include/sophia_decoder.h and
-include/sophia_draft.h with its ctypes signature.  ``sophia_amd._native`` binds the library through this
+entry point of include/sophia_kda.h, include/sophia_decoder.h,
+include/sophia_draft.h and include/sophia_pages.h with its ctypes signature.  ``sophia_amd._native`` binds the library through this
 table; the CPU tests also bind a host-sanitized build of the library with it
 (torch is not loaded into that process).
 """
@@ -27,6 +27,8 @@ BWD_RECURRENT = 16
 BWD_GRAD_BF16 = 32
 
 TREE_NODES = 64          # SOPHIA_TREE_NODES of include/sophia_draft.h
+BEAMS = 64               # SOPHIA_BEAMS, SOPHIA_MOVES of include/sophia_pages.h
+MOVES = 4096
 
 
 class CommitKda(ctypes.Structure):
@@ -50,8 +52,8 @@ def packed(struct, words: list[int]):
     return (struct * (ctypes.sizeof(flat) // ctypes.sizeof(struct))).from_buffer(flat)
 
 
-# Every symbol of include/sophia_kda.h, include/sophia_decoder.h and
-# include/sophia_draft.h, with its ctypes signature.
+# Every symbol of include/sophia_kda.h, include/sophia_decoder.h,
+# include/sophia_draft.h and include/sophia_pages.h, with its ctypes signature.
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
@@ -128,6 +130,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sophia_tree_accept_workspace_size": (_sz, [_i64, _i32]),
     "sophia_tree_accept": (_i32, [_vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _vp, _vp, _vp,
                                   _vp, _sz, _vp]),
+    "sophia_mla_paged_workspace_size": (_sz, [_i32, _i64, _i32, _i64, _i32, _i32, _i32, _i32]),
+    "sophia_mla_paged_attn": (_i32, [_vp, _i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32,
+                                     _i64, _i32, _i64, _f32, _vp, _i64, _i32, _i32, _i32, _vp, _sz, _vp]),
+    "sophia_mla_latent_norms_paged": (_i32, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _f32, _vp, _f32, _vp, _i64,
+                                             _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _vp]),
+    "sophia_beam_select_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "sophia_beam_select": (_i32, [_vp, _i64, _i32, _i64, _i32, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "sophia_move_workspace_size": (_sz, [_i32]),
+    "sophia_cache_fork": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _i64,
+                                 _i64, _i32, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _sz, _vp]),
+    "sophia_page_copy": (_i32, [_vp, _vp, _i32, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _sz, _vp]),
     "sophia_tree_accept_strict": (_i32, [_vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _vp, _vp, _vp,
                                          _vp, _sz, _vp]),
 }

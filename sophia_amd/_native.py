@@ -1,7 +1,8 @@
 """ctypes binding of the HIP library ``sophia_amd/_lib/libsophia_kda.so``.
 
 The library exports the C ABI declared in ``include/sophia_kda.h``,
-``include/sophia_decoder.h`` and ``include/sophia_draft.h``.  torch is
+``include/sophia_decoder.h``, ``include/sophia_draft.h`` and
+``include/sophia_pages.h``.  torch is
 imported first so that the library binds to the HIP runtime torch already
 loaded (same soname), which keeps torch streams and device pointers valid for
 the kernels.  There is no fallback: if the library is missing or fails to
@@ -31,6 +32,8 @@ from ._abi import (  # noqa: F401
     BWD_RECURRENT,
     BWD_GRAD_BF16,
     TREE_NODES,
+    BEAMS,
+    MOVES,
     CommitKda,
     CommitMla,
     packed,

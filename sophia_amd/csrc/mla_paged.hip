@@ -1,0 +1,921 @@
+// MLA attention in latent space over paged latents, and the latent norms that write
+// them (include/sophia_pages.h).
+//
+// Keys and values are the same rows, so a tile of them is staged in LDS once and read
+// twice, as K rows and, transposed, as V, under a running maximum and sum.  The columns of
+// the products are the (token, head) pairs of a sequence, packed: with 16 heads 32 columns
+// are two tokens.  Two forms of one kernel:
+//   wide   : a work-group takes 4 x 32 columns (fp32: 4 x 16) and a range of their keys; its
+//            wavefronts share tiles of 64 keys and differ in their columns.
+//   narrow : a sequence of at most 32 (16) columns, so one token of it, or two: a work-group
+//            takes a range of its keys, and the wavefronts differ in their keys, each with tiles
+//            of its own and no barrier until they join through LDS at the end.
+// A sequence of several ranges leaves partials, which a second kernel joins.
+#include "common.hpp"
+#include "pages.hpp"
+#include "tree.hpp"
+
+#include "../../include/sophia_pages.h"
+
+namespace sophia {
+namespace {
+
+constexpr float kSlack = 8.f;    // (powers of 2)
+constexpr int kWideKeys = 64;    // keys of a tile of the wide form
+
+struct PagedArgs {
+  Pages p;
+  const void *qa;
+  int64_t qa_stride;
+  void *out;
+  int64_t out_stride;
+  float scale_log2;
+  int heads, max_new;
+  int splits, range_keys;   // key ranges of a sequence at most, and keys of one
+  float *part;              // partials (splits > 1)
+  int64_t units;            // 32 (16) columns each: how many there is room for in a range's partials
+  int both;                 // narrow sequences are left to the narrow kernel
+};
+
+template <int R, bool F32, bool NARROW>
+struct Form {
+  static constexpr int kCols = F32 ? 16 : 32;                     // of a wavefront
+  static constexpr int kGroup = NARROW ? kCols : 4 * kCols;       // of a work-group
+  static constexpr int kKeys = !NARROW ? kWideKeys : F32 && R == 256 ? 16 : 32;   // of a tile
+  static constexpr int kBytes = R * (F32 ? 4 : 2);                // of a row
+  static constexpr int kChunks = kBytes / 16;
+  static constexpr int kTile = kKeys * kBytes;
+  static constexpr int kQuads = F32 ? R / 16 : R / 8;             // four ranks each, of a lane's column
+  static constexpr int kOwn = NARROW ? kKeys : kKeys / 4;         // rows that a wavefront stages
+  static constexpr int kLoads = kOwn * kChunks / 64;
+};
+
+// Floats of a wavefront's partial: [kQuads][64 lanes] times four, then maximum and sum [64 lanes].
+template <int R, bool F32>
+constexpr int kPart = 64 * (4 * (F32 ? R / 16 : R / 8) + 2);
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ bf8 bits_to_bf8(const u4 &v) { return __builtin_bit_cast(bf8, v); }
+__device__ __forceinline__ f16v mfma32x32(const bf8 &a, const bf8 &b, const f16v &c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ const u4 zero_chunk = {0u, 0u, 0u, 0u};   // what a key that is not there is read from
+
+// Chunk c (16 bytes) of an LDS row lies at place c ^ turn(row): in bf16 eight rows of one chunk
+// (K) and four rows of two chunks (V, transposing reads), in fp32 sixteen rows of one chunk and
+// four rows of four, touch all banks.
+template <bool F32>
+__device__ __forceinline__ int turn(int row) {
+  return F32 ? row & 15 : ((row & 7) << 1) | ((row >> 3) & 1);
+}
+template <int R, bool F32>
+__device__ __forceinline__ int place(int row, int chunk) {   // in bytes
+  constexpr int kChunks = R * (F32 ? 4 : 2) / 16;
+  return 16 * (row * kChunks + (chunk ^ (turn<F32>(row) & (kChunks - 1))));
+}
+
+// What a work-group does.
+struct Work {
+  Sequence q;
+  int col0, cols;           // its first column, and the sequence's
+  int first, last;          // tokens of its first and its last column
+  int keys;                 // that its last token sees
+  int k0, k1;               // its range
+  int split, used;
+  int64_t unit;             // of its first wavefront
+};
+
+__device__ __forceinline__ bool narrow_cols(const PagedArgs &a, int n, int cols) {
+  return n <= cols / a.heads;
+}
+
+// The part of find() that both forms share: false if the range is behind the last.
+__device__ __forceinline__ bool range(const PagedArgs &a, Work &w, int group, int split) {
+  const int heads = a.heads;
+  w.cols = w.q.n * heads;
+  w.first = w.col0 / heads;
+  w.last = (min(w.col0 + group, w.cols) - 1) / heads;
+  w.keys = max(0, min(w.q.pos0 + w.last + 1, w.q.keys));
+  // (the last range has what max_len did not tell of)
+  w.used = max(1, min((w.keys + a.range_keys - 1) / a.range_keys, a.splits));
+  w.split = split;
+  w.k0 = split * a.range_keys;
+  w.k1 = split == a.splits - 1 ? w.keys : min(w.keys, w.k0 + a.range_keys);
+  return split < w.used;
+}
+
+// Narrow: work-group (split, sequence).  Wide: work-group b has split b % splits of group
+// (all - 1 - b / splits) of the list of all groups of all sequences, so that a sequence's last
+// tokens, which see most keys, come first.
+template <int R, bool F32, bool NARROW>
+__device__ __forceinline__ bool find(const PagedArgs &a, Work &w, int block, int split) {
+  using F = Form<R, F32, NARROW>;
+  if constexpr (NARROW) {
+    w.q = sequence(a.p, block);
+    if (w.q.n == 0 || !narrow_cols(a, w.q.n, F::kCols)) return false;
+    w.q.n = min(w.q.n, a.max_new);
+    w.col0 = 0;
+    w.unit = block;
+  } else {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int s0 = 0;; s0 += 64) {
+      if (s0 >= a.p.n_seqs) return false;
+      const int s = min(s0 + lane, a.p.n_seqs - 1);
+      const int64_t base = iclamp64(a.p.cu[s], 0, a.p.rows);
+      const int n = static_cast<int>(iclamp64(imin64(a.p.cu[s + 1], a.p.rows) - base, 0, 1 << 29));
+      const bool mine = s == s0 + lane && !(a.both && narrow_cols(a, n, F::kCols));
+      const int groups = mine ? (min(n, a.max_new) * a.heads + F::kGroup - 1) / F::kGroup : 0;
+      const int sum = wave_scan(groups), all = __builtin_amdgcn_readlane(sum, 63);
+      if (block < before + all) {
+        const int at = __ffsll(static_cast<unsigned long long>(__ballot(block < before + sum))) - 1;
+        const int g = __builtin_amdgcn_readlane(groups, at);
+        // (late groups first)
+        const int in = block - before - (__builtin_amdgcn_readlane(sum, at) - g);
+        w.q = sequence(a.p, s0 + at);
+        w.q.n = min(w.q.n, a.max_new);
+        w.col0 = (g - 1 - in) * F::kGroup;
+        w.unit = 4 * static_cast<int64_t>(block);
+        break;
+      }
+      before += all;
+    }
+  }
+  // (positions are of all of a sequence's rows, also of those past max_new)
+  return range(a, w, F::kGroup, split);
+}
+
+// The lane's column `col` of a range: the result, or a partial.
+template <int R, bool F32, typename V, typename K>
+__device__ __forceinline__ void put(const PagedArgs &a, const Work &w, int64_t unit, int col, float m, float l, V value, K rank) {
+  constexpr int kQuads = F32 ? R / 16 : R / 8;
+  const int lane = threadIdx.x & 63;
+  if (w.used > 1) {
+    if (unit >= a.units) return;   // (there is always room, see plan())
+    float *p = a.part + (unit * a.splits + w.split) * kPart<R, F32>;
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j) reinterpret_cast<f4 *>(p)[64 * j + lane] = value(j);
+    reinterpret_cast<f2 *>(p + 256 * kQuads)[lane] = f2{m, l};
+  } else if (col < w.cols) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;   // (no key: zeros)
+    const int token = col / a.heads, head = col - token * a.heads;
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j)
+      store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(head) * R + rank(j),
+             F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, value(j) * inv);
+  }
+}
+
+// A tile on its way into LDS: the ids of its pages, a key per lane, and the copies.
+template <int R, bool F32, bool NARROW>
+struct Stage {
+  using F = Form<R, F32, NARROW>;
+  const PagedArgs &a;
+  const Work &w;
+  int lane, row0;      // this wavefront's first row
+  __device__ __forceinline__ Stage(const PagedArgs &args, const Work &work)
+      : a(args), w(work), lane(threadIdx.x & 63), row0(NARROW ? 0 : F::kOwn * static_cast<int>(threadIdx.x >> 6)) {}
+  // The page of key k0 + lane (of the tile's keys, lanes past them repeat), -1 if it is not there.
+  __device__ __forceinline__ int ids(int k0) const {
+    const int j = k0 + (lane & (F::kKeys - 1));
+    return j < w.k1 ? page_of(a.p, w.q.slot, j) : -1;
+  }
+  __device__ __forceinline__ void copy(char *tile, int k0, int id) const {
+#pragma unroll
+    for (int t = 0; t < F::kLoads; ++t) {
+      const int i = 64 * t + lane, row = row0 + i / F::kChunks, c = (i % F::kChunks) ^ (turn<F32>(row) & (F::kChunks - 1));
+      const int page = __shfl(id, row, 64);
+      const char *from = static_cast<const char *>(a.p.pages) +
+                         (page * a.p.page_stride * (F32 ? 4 : 2) +
+                          static_cast<int64_t>((k0 + row) & ((1 << a.p.shift) - 1)) * F::kBytes + 16 * c);
+      __builtin_amdgcn_global_load_lds(page >= 0 ? from : reinterpret_cast<const char *>(&zero_chunk),
+                                       tile + 16 * (row0 * F::kChunks + 64 * t), 16, 0, 0);
+    }
+  }
+  // Chunks that hold a value that is not finite become zeros; returns the rows that had one, of
+  // those that this wavefront copied.
+  __device__ __forceinline__ uint64_t clean(char *tile) const {
+    uint64_t rows = 0;
+#pragma unroll
+    for (int t = 0; t < F::kLoads; ++t) {
+      u4 *at = reinterpret_cast<u4 *>(tile + 16 * (row0 * F::kChunks + 64 * t) + 16 * lane);
+      const u4 v = *at;
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (F32)
+          any |= (v[i] & 0x7f800000u) == 0x7f800000u;
+        else
+          any |= (v[i] & 0x7f800000u) == 0x7f800000u || (v[i] & 0x7f80u) == 0x7f80u;
+      }
+      if (any) *at = u4{0u, 0u, 0u, 0u};
+      const uint64_t hit = __ballot(any);
+#pragma unroll
+      for (int r = 0; r < 64 / F::kChunks; ++r)
+        if ((hit >> (r * F::kChunks)) & (~0ull >> (64 - F::kChunks))) rows |= 1ull << (row0 + 64 / F::kChunks * t + r);
+    }
+    return rows;
+  }
+};
+
+// The softmax and value product of a wavefront's columns: bf16 in 32x32x16 MFMAs.  A
+// probability enters the value product as two bf16 numbers, the second what the first has
+// lost (2^-16 of it remains lost), so that outputs are as close as their own rounding;
+// scores, maxima and sums are fp32.
+template <int R, bool NARROW>
+struct Bf16Columns {
+  using F = Form<R, false, NARROW>;
+  static constexpr int KS = R / 16, DT = R / 32, KT = F::kKeys / 32;
+  const PagedArgs &a;
+  bf8 qf[KS];
+  f16v ot[DT];
+  float m, l;          // l over this lane's keys alone
+  int lane, half;
+  int ko[KS], vo[DT];  // places of this lane's reads in a tile
+  __device__ __forceinline__ explicit Bf16Columns(const PagedArgs &args) : a(args), m(-INFINITY), l(0.f) {
+    lane = threadIdx.x & 63;
+    half = lane >> 5;
+    const int l16 = lane & 15;
+    // K row lane % 32 (32 kt rows on: a constant); V rows 4 half + l16 / 4 (16 kp rows on: a
+    // constant; 8 rows on: the chunk's lowest bit turns).
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ko[ks] = place<R, false>(lane & 31, 2 * ks + half);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      vo[dt] = place<R, false>(4 * half + (l16 >> 2), 4 * dt + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1)) + 8 * (l16 & 1);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ot[dt][i] = 0.f;
+  }
+  __device__ __forceinline__ int column() const { return lane & 31; }
+  __device__ __forceinline__ void queries(int64_t row, int head) {
+    const uint16_t *qp = static_cast<const uint16_t *>(a.qa) + row * a.qa_stride + static_cast<int64_t>(head) * R + 8 * half;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = bits_to_bf8(*reinterpret_cast<const u4 *>(qp + 16 * ks));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));   // (waited for here, not in the loop)
+  }
+  // One tile, of which this lane's column sees the keys `seen` (`all`: every key).
+  __device__ __forceinline__ void tile(const char *lds, bool all, uint64_t seen) {
+    // st[kt][i] = score(key 32 kt + 8 (i / 4) + 4 half + i % 4 of the tile, this column)
+    f16v st[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+        st[kt] = mfma32x32(bits_to_bf8(*reinterpret_cast<const u4 *>(lds + ko[ks] + 32 * kt * F::kBytes)), qf[ks], st[kt]);
+    if (!all) {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const uint32_t bits = static_cast<uint32_t>(seen >> (32 * kt)) >> (4 * half);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[kt][i] = bits & (1u << (8 * (i >> 2) + (i & 3))) ? st[kt][i] : -INFINITY;
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      float top[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = st[kt][8 * i];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top[i] = fmaxf(top[i], st[kt][8 * i + j]);
+      }
+      mx = fmaxf(mx, fmaxf(top[0], top[1]));
+    }
+    mx = fmaxf(mx, lane_xor32(mx)) * a.scale_log2;
+    // The reference follows the maximum where that has risen by more than kSlack: until
+    // then probabilities are up to 2^kSlack, as exact as below 1.
+    if (__any(mx > m + kSlack)) {
+      const float m_new = fmaxf(m, mx);
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) ot[dt] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;   // (a column without a key so far)
+    float ps = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[kt][i] = __builtin_amdgcn_exp2f(fmaf(st[kt][i], a.scale_log2, -ref));
+      float s2[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s2[i] = st[kt][8 * i];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) s2[i] += st[kt][8 * i + j];
+      }
+      ps += s2[0] + s2[1];
+    }
+    l += ps;
+#pragma unroll
+    for (int kp = 0; kp < 2 * KT; ++kp) {   // 16 keys from 16 kp on
+      const f16v &sv = st[kp >> 1];
+      u4 pw, pr;   // rounded, and the rest
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = sv[8 * (kp & 1) + 2 * i], p1 = sv[8 * (kp & 1) + 2 * i + 1];
+        pw[i] = pack_bf16x2(p0, p1);
+        pr[i] = pack_bf16x2(p0 - __uint_as_float(pw[i] << 16), p1 - __uint_as_float(pw[i] & 0xffff0000u));
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const u2 lo = lds_read_tr(reinterpret_cast<const uint16_t *>(lds + vo[dt] + 16 * kp * F::kBytes));
+        const u2 hi = lds_read_tr(reinterpret_cast<const uint16_t *>(lds + (vo[dt] ^ 16) + (16 * kp + 8) * F::kBytes));
+        const bf8 vf = bits_to_bf8(u4{lo.x, lo.y, hi.x, hi.y});
+        ot[dt] = mfma32x32(vf, bits_to_bf8(pw), ot[dt]);
+        ot[dt] = mfma32x32(vf, bits_to_bf8(pr), ot[dt]);
+      }
+    }
+  }
+  __device__ __forceinline__ void finish(bool poison) {
+    l += lane_xor32(l);
+    if (poison) l = NAN;
+  }
+  // ot[dt][i] = O[this column][rank 32 dt + 8 (i / 4) + 4 half + i % 4] before the 1 / l
+  __device__ __forceinline__ f4 quad(int j) const {
+    const f16v &v = ot[j >> 2];
+    const int i = 4 * (j & 3);
+    return f4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+  }
+  __device__ __forceinline__ int rank(int j) const { return 8 * j + 4 * half; }
+};
+
+// The same in fp32, 16x16x4 MFMAs: a lane's four consecutive ranks of a key are the A
+// operands of four steps (the k index runs 4 (lane / 16) + step), and the scores'
+// accumulator, keys 4 (lane / 16) + i, is the B operand of the value product in the same order.
+template <int R, bool NARROW>
+struct F32Columns {
+  using F = Form<R, true, NARROW>;
+  static constexpr int KB = R / 16, KT = F::kKeys / 16;
+  const PagedArgs &a;
+  f4 qf[KB], ot[KB];
+  float m, l;
+  int lane, grp, l16;
+  __device__ __forceinline__ explicit F32Columns(const PagedArgs &args) : a(args), m(-INFINITY), l(0.f) {
+    lane = threadIdx.x & 63;
+    grp = lane >> 4;
+    l16 = lane & 15;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) ot[b] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ int column() const { return l16; }
+  __device__ __forceinline__ void queries(int64_t row, int head) {
+    const float *qp = static_cast<const float *>(a.qa) + row * a.qa_stride + static_cast<int64_t>(head) * R + 4 * grp;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) qf[b] = *reinterpret_cast<const f4 *>(qp + 16 * b);
+#pragma unroll
+    for (int b = 0; b < KB; ++b) asm volatile("" : "+v"(qf[b]));
+  }
+  __device__ __forceinline__ void tile(const char *lds, bool, uint64_t seen) {
+    f4 st[KT];   // score(key 16 kt + 4 grp + i, this column)
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) st[kt] = f4{0.f, 0.f, 0.f, 0.f};
+    // LDS reads a step ahead of their products, here and below: by hand, as scheduling groups
+    // over that many products take the compiler a minute.
+    f4 k[2][KT];
+    const auto read_k = [&](int b) {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+        k[b & 1][kt] = *reinterpret_cast<const f4 *>(lds + place<R, true>(l16, 4 * b + grp) + 16 * kt * F::kBytes);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read_k(0);
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      if (b + 1 < KB) read_k(b + 1);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) st[kt] = mfma_f32(k[b & 1][kt][s], qf[b][s], st[kt]);
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        st[kt][i] = (seen >> (16 * kt + 4 * grp + i)) & 1 ? st[kt][i] * a.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, st[kt][i]);
+      }
+    mx = fmaxf(mx, lane_xor16(mx));
+    mx = fmaxf(mx, lane_xor32(mx));
+    const float m_new = fmaxf(m, mx);
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    const float ref = m == -INFINITY ? 0.f : m;
+    float ps = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        st[kt][i] = __builtin_amdgcn_exp2f(st[kt][i] - ref);
+        ps += st[kt][i];
+      }
+    l = l * alpha + ps;
+#pragma unroll
+    for (int b = 0; b < KB; ++b) ot[b] *= alpha;
+    float v[2][KB];
+    const auto read_v = [&](int i) {   // of key 16 (i / 4) + 4 grp + i % 4
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+        v[i & 1][b] = *reinterpret_cast<const float *>(lds + place<R, true>(4 * grp + (i & 3), 4 * b + (l16 >> 2)) +
+                                                       16 * (i >> 2) * F::kBytes + 4 * (l16 & 3));
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read_v(0);
+#pragma unroll
+    for (int i = 0; i < 4 * KT; ++i) {
+      if (i + 1 < 4 * KT) read_v(i + 1);
+#pragma unroll
+      for (int b = 0; b < KB; ++b) ot[b] = mfma_f32(v[i & 1][b], st[i >> 2][i & 3], ot[b]);
+    }
+  }
+  __device__ __forceinline__ void finish(bool poison) {
+    l += lane_xor16(l);
+    l += lane_xor32(l);
+    if (poison) l = NAN;
+  }
+  // ot[b][i] = O[this column][rank 16 b + 4 grp + i] before the 1 / l
+  __device__ __forceinline__ f4 quad(int j) const { return ot[j]; }
+  __device__ __forceinline__ int rank(int j) const { return 16 * j + 4 * grp; }
+};
+
+template <int R, bool F32, bool NARROW>
+struct ColumnsOf {
+  using type = Bf16Columns<R, NARROW>;
+};
+template <int R, bool NARROW>
+struct ColumnsOf<R, true, NARROW> {
+  using type = F32Columns<R, NARROW>;
+};
+
+// Keys of the tile from k0 on that a column at position pos sees, of those there are.
+__device__ __forceinline__ uint64_t seen_keys(uint64_t there, int pos, int k0) {
+  const int n = pos + 1 - k0;
+  return n >= 64 ? there : n <= 0 ? 0 : there & ((1ull << n) - 1);
+}
+
+template <int R, bool F32>
+__global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_wide_kernel(PagedArgs a) {
+  using F = Form<R, F32, false>;
+  __shared__ __attribute__((aligned(1024))) char s_tile[2][F::kTile];
+  __shared__ uint64_t s_bad[4];
+  Work w;
+  const int splits = a.splits;
+  if (!find<R, F32, false>(a, w, blockIdx.x / splits, blockIdx.x % splits)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Stage<R, F32, false> stage(a, w);
+  typename ColumnsOf<R, F32, false>::type c(a);
+  const int col = w.col0 + F::kCols * wave + c.column(), in = min(col, w.cols - 1);
+  const int token = in / a.heads, pos = w.q.pos0 + token;
+  const int wave_col = w.col0 + F::kCols * wave;
+  const bool idle = wave_col >= w.cols;   // (of the whole wavefront)
+  const int wave_last = w.q.pos0 + (min(wave_col + F::kCols, w.cols) - 1) / a.heads, wave_first = w.q.pos0 + wave_col / a.heads;
+  int id = stage.ids(w.k0);
+  uint64_t there = __ballot(id >= 0);
+  if (w.k0 < w.k1) stage.copy(s_tile[0], w.k0, id);
+  c.queries(w.q.base + token, in - token * a.heads);
+  if (w.k0 + F::kKeys < w.k1) id = stage.ids(w.k0 + F::kKeys);
+  uint64_t poison = 0;
+  int buf = 0;
+  for (int k0 = w.k0; k0 < w.k1; k0 += F::kKeys, buf ^= 1) {
+    // This wavefront's copies, then the others'.  The next tile's go out only after that, into
+    // the buffer that all have left.
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    const uint64_t now = there;
+    if (k0 + F::kKeys < w.k1) {
+      there = __ballot(id >= 0);
+      stage.copy(s_tile[buf ^ 1], k0 + F::kKeys, id);
+      if (k0 + 2 * F::kKeys < w.k1) id = stage.ids(k0 + 2 * F::kKeys);
+    }
+    // A key that not every column sees would reach all of them through the products (0 times
+    // infinity): it enters them as zeros where it is not finite, and the columns that do see it
+    // end as NaN.
+    uint64_t bad = 0;
+    if (k0 + F::kKeys - 1 > w.q.pos0 + w.first && w.first != w.last) {
+      const uint64_t mine = stage.clean(s_tile[buf]);
+      if (lane == 0) s_bad[wave] = mine;
+      lds_barrier();
+      bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+    }
+    if (!idle && wave_last >= k0) {
+      const uint64_t seen = seen_keys(now, pos, k0);
+      poison |= bad & seen;
+      c.tile(s_tile[buf], now == ~0ull && wave_first >= k0 + F::kKeys - 1, seen);
+    }
+  }
+  if (idle) return;
+  c.finish(poison != 0);
+  put<R, F32>(a, w, w.unit + wave, col, c.m, c.l, [&](int j) { return c.quad(j); }, [&](int j) { return c.rank(j); });
+}
+
+template <int R, bool F32>
+__global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_narrow_kernel(PagedArgs a) {
+  using F = Form<R, F32, true>;
+  constexpr int kQuads = F::kQuads;
+  // Two tiles of each wavefront; then the wavefronts' sums.
+  __shared__ __attribute__((aligned(1024))) char s_tile[4][2][F::kTile];
+  __shared__ f2 s_ml[4][64];
+  static_assert(sizeof(s_tile) >= 4 * kQuads * 64 * sizeof(f4), "the sums fit the tiles");
+  Work w;
+  if (!find<R, F32, true>(a, w, blockIdx.y, blockIdx.x)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Stage<R, F32, true> stage(a, w);
+  typename ColumnsOf<R, F32, true>::type c(a);
+  const int col = c.column(), in = min(col, w.cols - 1);
+  const int token = in / a.heads, pos = w.q.pos0 + token;
+  constexpr uint64_t kAll = ~0ull >> (64 - F::kKeys);
+  constexpr int kStep = 4 * F::kKeys;
+  const int first = w.k0 + F::kKeys * wave;
+  int id = stage.ids(first);
+  uint64_t there = __ballot(id >= 0) & kAll;
+  if (first < w.k1) stage.copy(s_tile[wave][0], first, id);
+  c.queries(w.q.base + token, in - token * a.heads);
+  if (first + kStep < w.k1) id = stage.ids(first + kStep);
+  uint64_t poison = 0;
+  int buf = 0;
+  for (int k0 = first; k0 < w.k1; k0 += kStep, buf ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // (its own copies; nobody else reads them)
+    const uint64_t now = there;
+    char *tile = s_tile[wave][buf];
+    if (k0 + kStep < w.k1) {
+      there = __ballot(id >= 0) & kAll;
+      stage.copy(s_tile[wave][buf ^ 1], k0 + kStep, id);
+      if (k0 + 2 * kStep < w.k1) id = stage.ids(k0 + 2 * kStep);
+    }
+    const uint64_t seen = seen_keys(now, pos, k0);
+    if (k0 + F::kKeys - 1 > w.q.pos0 && w.last != 0) {   // (as in the wide form)
+      poison |= stage.clean(tile) & seen;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+    }
+    c.tile(tile, now == kAll && w.q.pos0 >= k0 + F::kKeys - 1, seen);
+  }
+  c.finish(poison != 0);
+  // The wavefronts' columns joined: each scaled to the common maximum, then summed four ranks a thread.
+  __syncthreads();
+  s_ml[wave][lane] = f2{c.m, c.l};
+  __syncthreads();
+  float m = s_ml[0][lane].x;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = fmaxf(m, s_ml[i][lane].x);
+  const auto weight = [&](int i) {
+    const float mi = s_ml[i][lane].x;
+    return mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m);
+  };
+  float l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) l = fmaf(s_ml[i][lane].y, weight(i), l);
+  f4 *sums = reinterpret_cast<f4 *>(&s_tile[0][0][0]);   // [wave][kQuads][64]
+  const float own = weight(wave);
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j) sums[(wave * kQuads + j) * 64 + lane] = c.quad(j) * own;
+  __syncthreads();
+  constexpr int kMine = (kQuads + 3) / 4;
+  f4 v[kMine];
+#pragma unroll
+  for (int t = 0; t < kMine; ++t) {
+    const int j = wave + 4 * t;
+    v[t] = f4{0.f, 0.f, 0.f, 0.f};
+    if (j < kQuads)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[t] += sums[(i * kQuads + j) * 64 + lane];
+  }
+  if (w.used > 1) {
+    if (w.unit >= a.units) return;
+    float *p = a.part + (w.unit * a.splits + w.split) * kPart<R, F32>;
+#pragma unroll
+    for (int t = 0; t < kMine; ++t)
+      if (wave + 4 * t < kQuads) reinterpret_cast<f4 *>(p)[64 * (wave + 4 * t) + lane] = v[t];
+    if (wave == 0) reinterpret_cast<f2 *>(p + 256 * kQuads)[lane] = f2{m, l};
+  } else if (col < w.cols) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int t = 0; t < kMine; ++t)
+      if (wave + 4 * t < kQuads)
+        store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(in - token * a.heads) * R + c.rank(wave + 4 * t),
+               F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, v[t] * inv);
+  }
+}
+
+// Joins the ranges of 32 (16) columns: a wavefront four ranks of each, the partials one after
+// the other, several loaded before the first is used.
+template <int R, bool F32, bool NARROW>
+__global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a) {
+  using F = Form<R, F32, NARROW>;
+  const int lane = threadIdx.x & 63, j = 4 * blockIdx.y + (threadIdx.x >> 6);
+  const int sub = NARROW ? 0 : blockIdx.x & 3;
+  Work w;
+  if (!find<R, F32, NARROW>(a, w, NARROW ? blockIdx.x : blockIdx.x >> 2, 0)) return;
+  const int col = w.col0 + F::kCols * sub + (lane & (F::kCols - 1));
+  if (w.used == 1 || j >= F::kQuads || w.col0 + F::kCols * sub >= w.cols || w.unit + sub >= a.units) return;
+  const float *p = a.part + (w.unit + sub) * a.splits * kPart<R, F32>;
+  float m = -INFINITY, l = 0.f;
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
+  constexpr int kAhead = 8;
+  for (int s0 = 0; s0 < w.used; s0 += kAhead) {
+    f2 ml[kAhead];
+    f4 v[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const float *ps = p + static_cast<int64_t>(min(s0 + s, w.used - 1)) * kPart<R, F32>;   // the last one again, unused
+      ml[s] = reinterpret_cast<const f2 *>(ps + 256 * F::kQuads)[lane];
+      v[s] = reinterpret_cast<const f4 *>(ps)[64 * j + lane];
+    }
+    float top = m;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) top = fmaxf(top, ml[s].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float e0 = __builtin_amdgcn_exp2f(m - ref);
+    l *= e0;
+    acc *= e0;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+      if (s0 + s < w.used) {
+        const float e = __builtin_amdgcn_exp2f(ml[s].x - ref);
+        l = fmaf(ml[s].y, e, l);
+        acc += v[s] * e;
+      }
+    m = top;
+  }
+  if (col >= w.cols) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const int token = col / a.heads, head = col - token * a.heads;
+  const int rank = F32 ? 16 * j + 4 * (lane >> 4) : 8 * j + 4 * (lane >> 5);
+  store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(head) * R + rank,
+         F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, acc * inv);
+}
+
+// ---- norms ---------------------------------------------------------------------
+// The normalisations that follow MLA's down projections, in place, and the latents into
+// their pages: a wavefront per row, lanes [0, q_rank / 8) hold 8 elements of q each, the
+// next kv_rank / 8 lanes 8 of the latent.
+struct PagedNormArgs {
+  Pages p;
+  void *q;
+  int64_t q_stride;
+  void *kv;
+  int64_t kv_stride;
+  int q_rank, kv_rank;
+  const float *q_w, *kv_w;
+  float q_eps, kv_eps;
+};
+
+// Of n ascending offsets, how many are <= row: by 64ths, a step per factor of 64.
+__device__ __forceinline__ int count_not_above(const int32_t *cu, int n, int64_t row, int lane) {
+  int lo = 0, hi = n;   // the count lies within [lo, hi]
+  while (hi > lo) {
+    const int step = (hi - lo + 63) >> 6;
+    const int at = lo + (lane + 1) * step - 1;
+    const uint64_t not_above = __ballot(at < hi && cu[min(at, hi - 1)] <= row);
+    const int first = __popcll(not_above & ~(not_above + 1));   // lanes from 0 on
+    const int from = lo + first * step;
+    hi = min(hi, from + step - 1);
+    lo = min(from, hi);
+    if (step == 1) hi = lo;
+  }
+  return lo;
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const void *base, float (&v)[8]) {
+  const f4 a = load4(base, 0, DT), b = load4(base, 4, DT);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+}
+template <int DT>
+__device__ __forceinline__ void store8(void *base, const float (&v)[8]) {
+  store4(base, 0, DT, f4{v[0], v[1], v[2], v[3]});
+  store4(base, 4, DT, f4{v[4], v[5], v[6], v[7]});
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void mla_paged_norm_kernel(PagedNormArgs a) {
+  constexpr int kEsz = DT == SOPHIA_DTYPE_BF16 ? 2 : 4;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= a.p.rows) return;  // uniform over the wavefront
+  const int l = threadIdx.x & 63;
+  const int qc = a.q_rank / 8, kc = a.kv_rank / 8;
+  const bool isq = l < qc, iskv = l >= qc && l < qc + kc;
+  const int c = isq ? l : l - qc;  // 8-element chunk within its part
+  uint8_t *base = isq ? static_cast<uint8_t *>(a.q) + (row * a.q_stride + 8 * c) * kEsz
+                      : static_cast<uint8_t *>(a.kv) + (row * a.kv_stride + 8 * c) * kEsz;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (isq || iskv) load8<DT>(base, v);
+  const int s = count_not_above(a.p.cu + 1, a.p.n_seqs, row, l);
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+  const float sq = wave_sum_dpp(isq ? ss : 0.f), sk = wave_sum_dpp(iskv ? ss : 0.f);
+  if (!(isq || iskv)) return;
+  const float r = isq ? rsqrtf(sq / static_cast<float>(a.q_rank) + a.q_eps)
+                      : rsqrtf(sk / static_cast<float>(a.kv_rank) + a.kv_eps);
+  const float *w = (isq ? a.q_w : a.kv_w) + 8 * c;
+  float o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = v[i] * r * as_dtype(w[i], DT);
+  store8<DT>(base, o);
+  if (!iskv || s >= a.p.n_seqs) return;
+  const Sequence q = sequence(a.p, s);
+  const int64_t pos = q.pos0 + (row - q.base);
+  if (row < q.base || row >= q.base + q.n || pos < 0 || pos >= q.keys) return;
+  const int page = page_of(a.p, q.slot, static_cast<int>(pos));
+  if (page < 0) return;
+  uint8_t *to = static_cast<uint8_t *>(const_cast<void *>(a.p.pages)) +
+                (page * a.p.page_stride + (pos & ((1 << a.p.shift) - 1)) * a.kv_rank + 8 * c) * kEsz;
+  store8<DT>(to, o);
+}
+
+// ---- the host's side -------------------------------------------------------------
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int log2_of(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+// How the work is divided: which of the two kernels run, their groups and key ranges.
+struct Plan {
+  bool narrow, wide;
+  int64_t wide_groups;      // at most
+  int narrow_splits, wide_splits, narrow_range, wide_range;
+  size_t narrow_bytes, wide_bytes;   // of their partials
+};
+
+Plan plan(int n_seqs, int64_t rows, int max_new, int64_t max_len, int heads, int rank, int dtype, int splits) {
+  const bool f32 = dtype == SOPHIA_DTYPE_F32;
+  if (max_new > rows) max_new = static_cast<int>(rows);
+  const int cols = f32 ? 16 : 32, group = 4 * cols;
+  const int64_t part = 64ll * (4 * (f32 ? rank / 16 : rank / 8) + 2) * 4;
+  Plan p = {};
+  p.wide = static_cast<int64_t>(max_new) * heads > cols;
+  // (as many rows as sequences of max_new tokens have: there is no shorter one)
+  p.narrow = !p.wide || rows != static_cast<int64_t>(n_seqs) * max_new;
+  if (p.narrow && heads > cols) p.narrow = false;
+  const int64_t keys = max_len < 1 ? 1 : max_len < 1 << 29 ? max_len : 1 << 29;
+  const auto divide = [&](int64_t groups, int64_t tile, int64_t slots, int &n, int &range) {
+    const int64_t tiles = (keys + tile - 1) / tile;
+    int64_t want = splits > 0 ? splits : (slots + groups - 1) / groups;
+    if (splits == 0 && want > 64) want = 64;
+    if (want > tiles) want = tiles;
+    if (want < 1) want = 1;
+    const int64_t each = (tiles + want - 1) / want;
+    n = static_cast<int>((tiles + each - 1) / each);
+    range = static_cast<int>(each * tile);
+  };
+  if (p.narrow) {
+    divide(n_seqs, 128, 1024, p.narrow_splits, p.narrow_range);
+    p.narrow_bytes = p.narrow_splits > 1 ? static_cast<size_t>(n_seqs) * p.narrow_splits * part : 0;
+  }
+  if (p.wide) {
+    const int64_t a = rows * heads / group + n_seqs, b = n_seqs * ((static_cast<int64_t>(max_new) * heads + group - 1) / group);
+    p.wide_groups = a < b ? a : b;
+    if (p.wide_groups < 1) p.wide_groups = 1;
+    divide(p.wide_groups, kWideKeys, 512, p.wide_splits, p.wide_range);
+    p.wide_bytes = p.wide_splits > 1 ? static_cast<size_t>(4 * p.wide_groups) * p.wide_splits * part : 0;
+  }
+  return p;
+}
+
+template <int R, bool F32>
+int launch(PagedArgs a, const Plan &p, char *workspace, hipStream_t st) {
+  using W = Form<R, F32, false>;
+  a.both = p.narrow && p.wide;
+  if (p.wide) {
+    PagedArgs w = a;
+    w.splits = p.wide_splits;
+    w.range_keys = p.wide_range;
+    w.part = reinterpret_cast<float *>(workspace + p.narrow_bytes);
+    w.units = 4 * p.wide_groups;
+    hipLaunchKernelGGL((mla_paged_wide_kernel<R, F32>), dim3(static_cast<unsigned>(p.wide_groups * p.wide_splits)), dim3(256),
+                       0, st, w);
+    if (p.wide_splits > 1)
+      hipLaunchKernelGGL((mla_paged_merge_kernel<R, F32, false>),
+                         dim3(static_cast<unsigned>(4 * p.wide_groups), (W::kQuads + 3) / 4), dim3(256), 0, st, w);
+  }
+  if (p.narrow) {
+    a.splits = p.narrow_splits;
+    a.range_keys = p.narrow_range;
+    a.part = reinterpret_cast<float *>(workspace);
+    a.units = a.p.n_seqs;
+    hipLaunchKernelGGL((mla_paged_narrow_kernel<R, F32>), dim3(p.narrow_splits, a.p.n_seqs), dim3(256), 0, st, a);
+    if (p.narrow_splits > 1)
+      hipLaunchKernelGGL((mla_paged_merge_kernel<R, F32, true>), dim3(a.p.n_seqs, (W::kQuads + 3) / 4), dim3(256), 0, st, a);
+  }
+  return check_launch("mla_paged_attn");
+}
+
+// What both entry points ask of the pages.
+int check_pages(const char *what, const void *pages, int64_t page_stride, int64_t n_pages, int page_size,
+                const int32_t *table, int64_t table_stride, int table_rows, int max_pages, const int32_t *cu,
+                const int64_t *kv_len, int n_seqs, int64_t rows, int rank) {
+  SOPHIA_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && rows >= 0 && rows <= 0x1fffffff,
+                 "%s: n_seqs must be 0..65535 and rows 0..2^29 - 1", what);
+  SOPHIA_REQUIRE(page_size >= 1 && page_size <= 65536 && (page_size & (page_size - 1)) == 0,
+                 "%s: page_size must be a power of two, at most 65536", what);
+  SOPHIA_REQUIRE(n_pages >= 0 && n_pages <= 0x7fffffff && page_stride >= static_cast<int64_t>(page_size) * rank &&
+                     page_stride % 8 == 0,
+                 "%s: n_pages must be 0..2^31 - 1, page_stride hold a page and be a multiple of 8", what);
+  SOPHIA_REQUIRE(table_rows >= 0 && max_pages >= 0 && table_stride >= max_pages &&
+                     static_cast<int64_t>(max_pages) * page_size <= 1 << 29,
+                 "%s: the table's rows must hold max_pages entries, of at most 2^29 tokens", what);
+  if (n_seqs == 0 || rows == 0) return SOPHIA_OK;
+  SOPHIA_REQUIRE(cu && kv_len && (table || max_pages == 0 || table_rows == 0) && (pages || n_pages == 0), "%s: NULL pointer", what);
+  SOPHIA_REQUIRE(aligned16(pages), "%s: pages must be 16-byte aligned", what);
+  return SOPHIA_OK;
+}
+
+}  // namespace
+}  // namespace sophia
+
+using namespace sophia;
+
+extern "C" size_t sophia_mla_paged_workspace_size(int n_seqs, int64_t rows, int max_new, int64_t max_len, int heads, int rank,
+                                                  int dtype, int splits) {
+  if (n_seqs < 1 || rows < 1 || max_new < 1 || heads < 1 || rank < 1 || splits < 0) return 0;
+  const Plan p = plan(n_seqs, rows, max_new, max_len, heads, rank, dtype, splits);
+  return p.narrow_bytes + p.wide_bytes;
+}
+
+extern "C" int sophia_mla_paged_attn(const void *qa, int64_t qa_stride, int dtype, const void *pages, int64_t page_stride,
+                                     int64_t n_pages, int page_size, const int32_t *table, int64_t table_stride,
+                                     int table_rows, int max_pages, const int32_t *slots, const int32_t *cu_seqlens,
+                                     const int64_t *kv_len, int n_seqs, int64_t rows, int max_new, int64_t max_len,
+                                     float scale, void *out, int64_t out_stride, int heads, int rank, int splits,
+                                     void *workspace, size_t workspace_bytes, void *stream) {
+  SOPHIA_REQUIRE(dtype == SOPHIA_DTYPE_F32 || dtype == SOPHIA_DTYPE_BF16, "mla_paged_attn: dtype not supported");
+  SOPHIA_REQUIRE(rank == 32 || rank == 64 || rank == 128 || rank == 256,
+                 "mla_paged_attn: rank %d not supported (32, 64, 128 or 256)", rank);
+  SOPHIA_REQUIRE(heads >= 1 && heads <= 128, "mla_paged_attn: heads must be in [1, 128]");
+  SOPHIA_REQUIRE(scale > 0.f, "mla_paged_attn: scale must be > 0");
+  SOPHIA_REQUIRE(max_new >= 1 && splits >= 0 && splits <= 1024, "mla_paged_attn: max_new must be >= 1 and splits 0..1024");
+  if (int rc = check_pages("mla_paged_attn", pages, page_stride, n_pages, page_size, table, table_stride, table_rows, max_pages,
+                           cu_seqlens, kv_len, n_seqs, rows, rank))
+    return rc;
+  SOPHIA_REQUIRE(qa_stride >= static_cast<int64_t>(heads) * rank && out_stride >= static_cast<int64_t>(heads) * rank &&
+                     qa_stride % 8 == 0 && out_stride % 8 == 0,
+                 "mla_paged_attn: row strides must hold a row and be multiples of 8");
+  SOPHIA_REQUIRE(rows * heads <= 1 << 30, "mla_paged_attn: rows * heads must be at most 2^30");
+  if (n_seqs == 0 || rows == 0) return SOPHIA_OK;
+  SOPHIA_REQUIRE(qa && out, "mla_paged_attn: NULL pointer");
+  SOPHIA_REQUIRE(aligned16(qa) && aligned16(out), "mla_paged_attn: qa and out must be 16-byte aligned");
+  const Plan p = plan(n_seqs, rows, max_new, max_len, heads, rank, dtype, splits);
+  SOPHIA_REQUIRE(p.narrow_bytes + p.wide_bytes == 0 ||
+                     (workspace && aligned16(workspace) && workspace_bytes >= p.narrow_bytes + p.wide_bytes),
+                 "mla_paged_attn: workspace too small");
+  SOPHIA_REQUIRE(!p.wide || p.wide_groups * p.wide_splits <= 0x7fffffff / 4, "mla_paged_attn: too much work for one call");
+  const PagedArgs a{{pages, page_stride, n_pages, log2_of(page_size), table, table_stride, table_rows, max_pages, slots,
+                     cu_seqlens, kv_len, n_seqs, rows},
+                    qa, qa_stride, out, out_stride, scale * 1.44269504088896341f, heads, max_new, 1, 1, nullptr, 0, 0};
+  char *ws = static_cast<char *>(workspace);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (rank) {
+#define SOPHIA_MLA_PAGED(r) \
+  case r:                   \
+    return dtype == SOPHIA_DTYPE_F32 ? launch<r, true>(a, p, ws, st) : launch<r, false>(a, p, ws, st);
+    SOPHIA_MLA_PAGED(32) SOPHIA_MLA_PAGED(64) SOPHIA_MLA_PAGED(128) SOPHIA_MLA_PAGED(256)
+#undef SOPHIA_MLA_PAGED
+  }
+  return SOPHIA_OK;
+}
+
+extern "C" int sophia_mla_latent_norms_paged(void *q_lat, int64_t q_stride, void *kv_lat, int64_t kv_stride, int64_t rows,
+                                             int q_rank, int kv_rank, int dtype, const float *q_norm_weight, float q_eps,
+                                             const float *kv_norm_weight, float kv_eps, void *pages, int64_t page_stride,
+                                             int64_t n_pages, int page_size, const int32_t *table, int64_t table_stride,
+                                             int table_rows, int max_pages, const int32_t *slots, const int32_t *cu_seqlens,
+                                             const int64_t *kv_len, int n_seqs, void *stream) {
+  SOPHIA_REQUIRE(dtype == SOPHIA_DTYPE_F32 || dtype == SOPHIA_DTYPE_BF16, "mla_latent_norms_paged: dtype not supported");
+  SOPHIA_REQUIRE(q_rank > 0 && kv_rank > 0 && q_rank % 8 == 0 && kv_rank % 8 == 0 && q_rank + kv_rank <= 512,
+                 "mla_latent_norms_paged: ranks must be positive multiples of 8 with q_rank + kv_rank <= 512");
+  SOPHIA_REQUIRE(q_stride % 8 == 0 && kv_stride % 8 == 0 && q_stride >= q_rank && kv_stride >= kv_rank,
+                 "mla_latent_norms_paged: strides must be multiples of 8 elements and cover a row");
+  if (int rc = check_pages("mla_latent_norms_paged", pages, page_stride, n_pages, page_size, table, table_stride, table_rows,
+                           max_pages, cu_seqlens, kv_len, n_seqs, rows, kv_rank))
+    return rc;
+  if (rows == 0) return SOPHIA_OK;
+  SOPHIA_REQUIRE(q_lat && kv_lat && q_norm_weight && kv_norm_weight, "mla_latent_norms_paged: NULL pointer");
+  SOPHIA_REQUIRE(aligned16(q_lat) && aligned16(kv_lat) && aligned16(q_norm_weight) && aligned16(kv_norm_weight),
+                 "mla_latent_norms_paged: pointers must be 16-byte aligned");
+  const PagedNormArgs a{{pages, page_stride, n_pages, log2_of(page_size), table, table_stride, table_rows, max_pages, slots,
+                         cu_seqlens, kv_len, n_seqs, rows},
+                        q_lat, q_stride, kv_lat, kv_stride, q_rank, kv_rank, q_norm_weight, kv_norm_weight, q_eps, kv_eps};
+  const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == SOPHIA_DTYPE_BF16)
+    hipLaunchKernelGGL(mla_paged_norm_kernel<SOPHIA_DTYPE_BF16>, grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(mla_paged_norm_kernel<SOPHIA_DTYPE_F32>, grid, dim3(256), 0, st, a);
+  return check_launch("mla_latent_norms_paged");
+}

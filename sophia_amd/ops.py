@@ -3,7 +3,7 @@
 Each function checks devices, dtypes and shapes (raising ``RuntimeError`` the
 way the reference's custom ops do, ml/training/pretrain/engine/
 sm120_concurrent_ffn.py:49-59), allocates outputs and scratch from torch's
-caching allocator, and launches the C ABI of ``include/sophia_kda.h`` on the
+caching allocator, and launches the C ABI of ``include/`` on the
 current stream.  Nothing here synchronises the device or reads device data on
 the host, so every call can be captured in a HIP graph.
 
@@ -2082,6 +2082,306 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tens
                  chosen.data_ptr(), ws.data_ptr(), nbytes)
     nat.check(rc, "sophia_tree_accept")
     return path, n_path, next_token, chosen
+
+
+# ------------------------------------------------------------------ paged latents, beams, moves of caches
+BEAMS, MOVES = nat.BEAMS, nat.MOVES   # beams of a group and candidates kept, and moves of one call, at most
+
+
+def _page_pool(pages: torch.Tensor, name: str) -> tuple[int, int, int, int]:
+    """(pages, page size, rank, page stride) of a pool [n_pages, page_size, rank] with dense pages."""
+    if not isinstance(pages, torch.Tensor) or pages.dim() != 3:
+        raise RuntimeError(f"{name} must be [n_pages, page_size, rank]")
+    n, size, rank = pages.shape
+    if (rank > 1 and pages.stride(2) != 1) or (size > 1 and pages.stride(1) != rank):
+        raise RuntimeError(f"{name} must be [n_pages, page_size, rank] with dense pages")
+    return n, size, rank, pages.stride(0) if n > 1 else size * rank
+
+
+def _page_table(table: torch.Tensor, device) -> tuple[int, int, int]:
+    """(rows, pages of a row, row stride) of a page table."""
+    if table.dim() != 2 or table.dtype != torch.int32 or table.device != device or (table.size(1) > 1 and table.stride(1) != 1):
+        raise RuntimeError(f"table must be int32 [slots, max_pages] with dense rows on {device}")
+    return table.size(0), table.size(1), table.stride(0) if table.size(0) > 1 else table.size(1)
+
+
+def _new_tokens(cu_seqlens: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor | None, table_rows: int, device) -> int:
+    """Checks the offsets, lengths and slots of sequences; returns their number."""
+    cu = _int32(cu_seqlens, "cu_seqlens", device)
+    if cu is None or cu.dim() != 1 or cu.numel() < 1:
+        raise RuntimeError("cu_seqlens must hold one offset per sequence and the end of the last")
+    n = cu.numel() - 1
+    _int64(kv_len, "kv_len", n, device)
+    if _int32(slots, "slots", device) is None:
+        if table_rows < n:
+            raise RuntimeError("the table has fewer rows than there are sequences")
+    elif slots.numel() != n:
+        raise RuntimeError(f"slots must hold {n} entries, got {slots.numel()}")
+    return n
+
+
+def mla_paged_attn(qa: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tensor, kv_len: torch.Tensor,
+                   scale: float, *, max_new: int, max_len: int | None = None, slots: torch.Tensor | None = None,
+                   splits: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``mla_decode_attn`` over latents in pages, for any number of new tokens of
+    each sequence: one (a decode step), a chunk of a prompt, or both kinds in one
+    call (sophia_mla_paged_attn).  A row at position p attends to the latents 0 .. p
+    of its sequence, its own among them: write them first
+    (``mla_latent_norms_paged``).
+
+    qa: [rows, heads, rank] (bf16 or fp32, heads <= 128, rank in 32/64/128/256), the
+    last tokens of the sequences that ``cu_seqlens`` int32 [N + 1] delimits;
+    kv_len int64 [N]: all tokens of each, the new ones included.  pages: [n_pages,
+    page_size, rank] of qa's dtype, page_size a power of two, dense pages; table
+    int32 [slots, max_pages]: the pages of each slot's tokens, in order; slots int32
+    [N] (None: s), of which several may have the same pages.  A page id outside the
+    pool is no page: its tokens are not attended to (give -1 for tokens that a
+    sliding window has left behind).  A row without any key gets zeros.
+    ``max_new`` (host int) bounds a sequence's rows: rows past it, and rows of no
+    sequence, are left as they are.  ``max_len`` (host int) bounds kv_len and sizes
+    the key ranges; ``splits`` overrides their number.  qa and out: 16-byte aligned,
+    row strides multiples of 8; out does not overlap qa.  Returns [rows, heads, rank]
+    in qa's dtype."""
+    _gpu(qa, "qa")
+    if qa.dim() != 3:
+        raise RuntimeError(f"qa must be [rows, heads, rank], got {tuple(qa.shape)}")
+    device = qa.device
+    rows, heads, rank = qa.shape
+    _on_device(qa.get_device(), device, (pages, "pages"), (out, "out"))
+    qs = _heads_rows(qa, "qa", heads, rank)
+    n_pages, size, width, page_stride = _page_pool(pages, "pages")
+    if width != rank or pages.dtype != qa.dtype:
+        raise RuntimeError(f"pages must hold latents of rank {rank} in qa's dtype")
+    table_rows, max_pages, table_stride = _page_table(table, device)
+    n = _new_tokens(cu_seqlens, kv_len, slots, table_rows, device)
+    y, os_ = _heads_out(out, rows, heads, rank, qa.dtype, device)
+    bound = max_pages * size if max_len is None else max(0, min(int(max_len), max_pages * size))
+    code = nat.dtype_code(qa.dtype)
+    lib = nat.lib()
+    ws_bytes = lib.sophia_mla_paged_workspace_size(n, rows, int(max_new), bound, heads, rank, code, int(splits))
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
+    rc = _launch(device, lib.sophia_mla_paged_attn, qa.data_ptr(), qs, code, pages.data_ptr(), page_stride, n_pages, size,
+                 table.data_ptr(), table_stride, table_rows, max_pages, nat.ptr(slots), cu_seqlens.data_ptr(),
+                 kv_len.data_ptr(), n, rows, int(max_new), bound, float(scale), y.data_ptr(), os_, heads, rank, int(splits),
+                 nat.ptr(ws), ws_bytes)
+    nat.check(rc, "sophia_mla_paged_attn")
+    return y
+
+
+def mla_latent_norms_paged(q_lat: torch.Tensor, kv_lat: torch.Tensor, q_norm_weight: torch.Tensor, q_eps: float,
+                           kv_norm_weight: torch.Tensor, kv_eps: float, pages: torch.Tensor, table: torch.Tensor,
+                           cu_seqlens: torch.Tensor, kv_len: torch.Tensor, *, slots: torch.Tensor | None = None) -> None:
+    """``mla_latent_norms`` with the latents in pages: q_lat [rows, q_rank] and
+    kv_lat [rows, kv_rank] are normalised in place, and row i of sequence s is written
+    to position kv_len[s] - n + i of its n new tokens' places in the pages
+    (sophia_mla_latent_norms_paged).
+
+    q_lat, kv_lat and pages [n_pages, page_size, kv_rank] have one dtype; table,
+    cu_seqlens, kv_len and slots as in ``mla_paged_attn``, but the slots of one call
+    are different ones, and a page that is written to belongs to one of them.
+    Positions without a page, or before 0, are written nowhere; rows of no sequence
+    are normalised all the same.  The fp32 weights are rounded to the rows' dtype."""
+    _gpu(q_lat, "q_lat")
+    _gpu(kv_lat, "kv_lat")
+    device = q_lat.device
+    if q_lat.dim() != 2 or kv_lat.dim() != 2 or kv_lat.size(0) != q_lat.size(0) or q_lat.dtype != kv_lat.dtype:
+        raise RuntimeError("q_lat and kv_lat must be [rows, rank] of one dtype")
+    rows, q_rank = q_lat.shape
+    kv_rank = kv_lat.size(1)
+    _on_device(q_lat.get_device(), device, (kv_lat, "kv_lat"), (pages, "pages"))
+    qs, ks = _rows(q_lat, "q_lat", q_rank), _rows(kv_lat, "kv_lat", kv_rank)
+    n_pages, size, width, page_stride = _page_pool(pages, "pages")
+    if width != kv_rank or pages.dtype != kv_lat.dtype:
+        raise RuntimeError(f"pages must hold latents of rank {kv_rank} in the rows' dtype")
+    table_rows, max_pages, table_stride = _page_table(table, device)
+    n = _new_tokens(cu_seqlens, kv_len, slots, table_rows, device)
+    weights = []
+    for t, width, name in ((q_norm_weight, q_rank, "q_norm_weight"), (kv_norm_weight, kv_rank, "kv_norm_weight")):
+        weights.append(_f32_values(t, device))
+        if weights[-1].numel() != width:
+            raise RuntimeError(f"{name} must hold {width} values")
+    rc = _launch(device, nat.lib().sophia_mla_latent_norms_paged, q_lat.data_ptr(), qs, kv_lat.data_ptr(), ks, rows, q_rank,
+                 kv_rank, nat.dtype_code(q_lat.dtype), weights[0].data_ptr(), float(q_eps), weights[1].data_ptr(),
+                 float(kv_eps), pages.data_ptr(), page_stride, n_pages, size, table.data_ptr(), table_stride, table_rows,
+                 max_pages, nat.ptr(slots), cu_seqlens.data_ptr(), kv_len.data_ptr(), n)
+    nat.check(rc, "sophia_mla_latent_norms_paged")
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, *, keep: int | None = None,
+                ended: torch.Tensor | None = None, pad_token: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The best continuations of each group of ``beams`` rows (sophia_beam_select):
+    of scores[b] + log_softmax(logits[b])[v] over a group's beams b and the
+    vocabulary the ``keep`` greatest (default: beams), sorted.
+
+    logits: [groups * beams, vocab] (bf16 or fp32, any row stride), adjusted already
+    (``adjust_logits``) if they are to be; scores: fp32 [groups * beams], the log
+    probabilities of the beams (-inf: no beam, as for all but the first of a prompt
+    that has just been read); ended: bool [groups * beams], beams whose only
+    candidate is themselves, with ``pad_token``.  beams and keep are at most 64.
+    Returns (scores fp32, parent int32, token int64), each [groups, keep]; a parent is
+    the index of a beam within its group.  Equal candidates are in the order of their
+    beams and tokens; sums are compared in 64 bits.  Logits that are NaN or -inf are no
+    candidates, a row with +inf, or with a score that is not finite, has none: where a group has fewer than
+    ``keep`` there is -inf, -1, -1."""
+    _gpu(logits, "logits")
+    device = logits.device
+    if logits.dim() != 2 or logits.size(1) < 1:
+        raise RuntimeError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    xs = _rows(logits, "logits", vocab)
+    beams = int(beams)
+    keep = beams if keep is None else int(keep)
+    if not 1 <= beams <= BEAMS or not 1 <= keep <= BEAMS or rows % beams:
+        raise RuntimeError(f"beams and keep must be in [1, {BEAMS}] and logits hold whole groups of {beams} rows, got {rows}")
+    _on_device(logits.get_device(), device, (scores, "scores"), (ended, "ended"))
+    if scores.dtype != torch.float32 or not scores.is_contiguous() or scores.numel() != rows:
+        raise RuntimeError(f"scores must be contiguous fp32 of {rows} entries")
+    if ended is not None and (ended.dtype != torch.bool or not ended.is_contiguous() or ended.numel() != rows):
+        raise RuntimeError(f"ended must be contiguous bool of {rows} entries")
+    lib = nat.lib()
+    groups = rows // beams
+    nbytes = lib.sophia_beam_select_workspace_size(rows, vocab, keep)
+    score = torch.empty((groups, keep), dtype=torch.float32, device=device)
+    parent = torch.empty((groups, keep), dtype=torch.int32, device=device)
+    token = torch.empty((groups, keep), dtype=torch.int64, device=device)
+    ws = torch.empty(-(-nbytes // 8), dtype=torch.int64, device=device)
+    rc = _launch(device, lib.sophia_beam_select, logits.data_ptr(), xs, nat.dtype_code(logits.dtype), rows, vocab,
+                 scores.data_ptr(), nat.ptr(ended), int(pad_token), beams, keep, score.data_ptr(), parent.data_ptr(),
+                 token.data_ptr(), ws.data_ptr(), nbytes)
+    nat.check(rc, "sophia_beam_select")
+    return score, parent, token
+
+
+def _moves(src: torch.Tensor, dst: torch.Tensor) -> int:
+    _gpu(src, "src")
+    _int32(src, "src", src.device)
+    _int32(dst, "dst", src.device)
+    if src.numel() != dst.numel() or src.numel() > MOVES:
+        raise RuntimeError(f"src and dst must hold the same number of entries, at most {MOVES}")
+    return src.numel()
+
+
+def _pools(pools, index: int, device) -> tuple[int, int, int, int]:
+    """What the first pool is, all of them are: (pages, page size, rank, page stride)."""
+    first = pools[0]
+    _on_device(index, device, (first, "pools"))
+    what = _page_pool(first, "pools")
+    for i, t in enumerate(pools[1:], 1):
+        if t.get_device() != index or t.shape != first.shape or t.dtype is not first.dtype or t.stride() != first.stride():
+            _on_device(index, device, (t, "pools"))
+            raise RuntimeError(f"pool {i} must be {first.dtype} {list(first.shape)} with strides {list(first.stride())}, as the first")
+    return what
+
+
+def _addresses(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors]) if tensors else None
+
+
+def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=(), table: torch.Tensor | None = None,
+               cached: torch.Tensor | None = None) -> None:
+    """Cache slots that go on from other slots, in all layers and in place: slot
+    dst[i] becomes what slot src[i] was, for all i as if at once (sophia_cache_fork).
+    For beams: src the slot of the beam that each goes on from, dst its own.
+
+    src, dst: int32 [M], M <= 4096.  A move from or to a slot that is none, or to
+    itself, changes nothing; of several moves to one slot the last one counts.
+    kda: (conv_state, state) of each KDA layer, contiguous fp32 [slots, ...]
+    (conv_state None for all layers: there is none).  mla: the latent cache of each
+    MLA layer, fp32 [slots, max_seq, rank] with dense rows, of which the first
+    cached[i] tokens of src[i] are taken along.  table int32 [slots, max_pages] and
+    pools, the pages of each MLA layer: the ids of the pages that cached[i] tokens
+    fill become shared, the tokens of the page that they fill in part are copied into
+    the one that dst[i] has there, which no other slot has; the ids behind stay.
+    cached: int64 [M]."""
+    n = _moves(src, dst)
+    device, index = src.device, src.get_device()
+    kda, mla, pools = list(kda), list(mla), list(pools)
+    f32 = torch.float32
+    n_slots = None
+    states, convs = [t[1] for t in kda], [t[0] for t in kda]
+    state_elems = conv_elems = slot_stride = max_seq = rank = 0
+    if kda and all(t is None for t in convs):
+        convs = []
+    for name, tensors in (("conv_state", convs), ("state", states)):
+        if not tensors:
+            continue
+        shape = tensors[0].shape if isinstance(tensors[0], torch.Tensor) else None
+        for i, t in enumerate(tensors):
+            if t is None or t.get_device() != index or t.dtype is not f32 or t.shape != shape or not t.is_contiguous():
+                _on_device(index, device, (t, name))
+                raise RuntimeError(f"KDA layer {i}: {name} must be contiguous fp32 [slots, ...] of one shape, as in every layer")
+        if n_slots is not None and shape[0] != n_slots:
+            raise RuntimeError("conv_state and state must have the same number of slots")
+        n_slots = shape[0]
+        elems = tensors[0].numel() // max(n_slots, 1)
+        if name == "state":
+            state_elems = elems
+        else:
+            conv_elems = elems
+    if mla:
+        first = mla[0]
+        _on_device(index, device, (first, "latent_cache"))
+        rank = first.size(-1)
+        slot_stride = _latents(first, rank, "latent_cache")
+        max_seq = first.size(1)
+        for i, t in enumerate(mla):
+            if t.get_device() != index or t.shape != first.shape or t.dtype is not f32 or t.stride() != first.stride():
+                _on_device(index, device, (t, "latent_cache"))
+                raise RuntimeError(f"MLA layer {i}: latent_cache must be fp32 {list(first.shape)}, as in every layer")
+        if n_slots is not None and first.size(0) != n_slots:
+            raise RuntimeError(f"latent_cache must have {n_slots} slots")
+        n_slots = first.size(0)
+    n_pages = size = page_stride = max_pages = table_stride = 0
+    code = nat.DTYPE_F32
+    if pools and table is None:
+        raise RuntimeError("pools need their table")
+    if table is not None:
+        table_rows, max_pages, table_stride = _page_table(table, device)
+        if not pools:
+            raise RuntimeError("a table needs its pools")
+        n_pages, size, width, page_stride = _pools(pools, index, device)
+        code = nat.dtype_code(pools[0].dtype)
+        if mla and width != rank:
+            raise RuntimeError("pools and latent caches must have one rank")
+        rank = width
+        if n_slots is not None and table_rows < n_slots:
+            raise RuntimeError(f"the table must have a row for each of {n_slots} slots")
+        n_slots = table_rows if n_slots is None else n_slots
+    if cached is not None:
+        _int64(cached, "cached", n, device)
+    elif mla or table is not None:
+        raise RuntimeError("latents and pages need cached")
+    if n_slots is None:
+        return
+    lib = nat.lib()
+    nbytes = lib.sophia_move_workspace_size(n)
+    ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device) if nbytes else None
+    rc = _launch(device, lib.sophia_cache_fork, src.data_ptr(), dst.data_ptr(), nat.ptr(cached), n, n_slots, _addresses(states),
+                 state_elems, _addresses(convs), conv_elems, len(kda), _addresses(mla), slot_stride, max_seq, len(mla),
+                 _addresses(pools), page_stride, n_pages, size, len(pools), nat.ptr(table), table_stride, max_pages, rank, code,
+                 nat.ptr(ws), nbytes)
+    nat.check(rc, "sophia_cache_fork")
+
+
+def page_copy(src: torch.Tensor, dst: torch.Tensor, pools) -> None:
+    """Page dst[i] of every pool becomes what page src[i] was, for all i as if at
+    once and in place (sophia_page_copy): pages copied before one of their owners
+    writes to them, or moved together.
+
+    src, dst: int32 [M], M <= 4096, under the rules of ``cache_fork``; pools: [n_pages,
+    page_size, rank] each, of one shape and dtype, dense and 16-byte aligned pages."""
+    n = _moves(src, dst)
+    pools = list(pools)
+    if not pools:
+        return
+    device = src.device
+    n_pages, size, rank, page_stride = _pools(pools, src.get_device(), device)
+    lib = nat.lib()
+    nbytes = lib.sophia_move_workspace_size(n)
+    ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device) if nbytes else None
+    rc = _launch(device, lib.sophia_page_copy, src.data_ptr(), dst.data_ptr(), n, _addresses(pools), len(pools), page_stride,
+                 size * rank, n_pages, nat.dtype_code(pools[0].dtype), nat.ptr(ws), nbytes)
+    nat.check(rc, "sophia_page_copy")
 
 
 from . import torch_ops  # noqa: E402  (registers the sophia:: custom ops; imports this module)
