@@ -6,11 +6,11 @@
 // the order of the logits is that of the candidates).  The second, a work-group per group,
 // joins the sums of each row, in double precision, and takes the greatest of what the parts left.
 //
-// The greatest of many values without sorting them: the values are divided into K >= keep sets
-// of equal size; the least of the sets' maxima is not above the keep-th greatest, as
-// K values are not below it, and only about K log K values are: those are collected, and each
-// finds its place by counting the greater ones.  Equal values are ordered by their index.
-// More than fit (many equal values, or few values above -inf) are found one after the other.
+// The greatest of many values without sorting them: of 64 sets of them the keep-th greatest of
+// the sets' maxima is not above the keep-th greatest of all, and few values are not below it: those
+// are collected, and each finds its place by counting the greater ones.  Equal values are ordered by
+// their index.  More than there is room for (many equal values, or few sets with a value above -inf)
+// are found one after the other.
 #include "common.hpp"
 #include "tree.hpp"
 
@@ -30,7 +30,7 @@ struct BeamArgs {
   const float *scores;
   const uint8_t *ended;     // NULL: none
   int64_t pad;
-  int beams, keep, sets, parts;
+  int beams, keep, parts;
   // Of each (row, part): maximum and sum, and its greatest logits with their tokens.
   double *sum;              // [rows][parts]
   float *top;               // [rows][parts]
@@ -41,77 +41,85 @@ struct BeamArgs {
   int64_t *out_token;
 };
 
-// A work-group's maximum and sum, in every thread.  `s` holds a value per wavefront.
-template <typename T, typename F>
-__device__ __forceinline__ T across(T v, T *s, F f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// What the lanes hold l ^ 1, ^ 2, ^ 4 and ^ 8 away, without the LDS crossbar, of values that
+// are equal within 1, 2, 4 and 8 lanes; then the row swaps.
+template <int OFF>
+__device__ __forceinline__ float lane_other(float v) {
+  if constexpr (OFF == 1) return dpp_rotate<0xb1>(v);    // quad_perm 1, 0, 3, 2
+  if constexpr (OFF == 2) return dpp_rotate<0x4e>(v);    // quad_perm 2, 3, 0, 1
+  if constexpr (OFF == 4) return dpp_rotate<0x141>(v);   // row_half_mirror
+  if constexpr (OFF == 8) return dpp_rotate<0x140>(v);   // row_mirror
+  if constexpr (OFF == 16) return lane_xor16(v);
+  return lane_xor32(v);
+}
+
+// Of a wavefront's values, which are equal within sets of 4 lanes, the greatest.
+__device__ __forceinline__ float top_of_quads(float v) {
+  v = fmaxf(v, lane_other<4>(v));
+  v = fmaxf(v, lane_other<8>(v));
+  v = fmaxf(v, lane_other<16>(v));
+  return fmaxf(v, lane_other<32>(v));
+}
+__device__ __forceinline__ float top_of_lanes(float v) {
+  v = fmaxf(v, lane_other<1>(v));
+  return top_of_quads(fmaxf(v, lane_other<2>(v)));
+}
+
+__device__ __forceinline__ double sum_lanes(double v) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = f(v, __shfl_xor(v, off, 64));
-  __syncthreads();
-  if (lane == 0) s[wave] = v;
-  __syncthreads();
-  v = s[0];
-  for (int i = 1; i < waves; ++i) v = f(v, s[i]);
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
   return v;
 }
 
-// The least of the maxima of `sets` sets of threads, a power of two up to the threads of the
-// work-group and at least one per wavefront; `v` is this thread's maximum.
+// Collected values with their indexes, and the places of the wavefronts' own.
 template <typename T>
-__device__ __forceinline__ T least_of_sets(T v, int sets, T *s) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int size = blockDim.x / sets;   // threads of a set
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const T o = __shfl_xor(v, off, 64);
-    v = (off < size) == (o > v) ? o : v;
-  }
-  __syncthreads();
-  if (lane == 0) s[wave] = v;
-  __syncthreads();
-  v = s[0];
-  for (int i = 1; i < waves; ++i) v = s[i] < v ? s[i] : v;
-  return v;
-}
-
-// The greatest `keep` of the work-group's values in order; each(f) calls f(value, index) for those
-// of this thread that are candidates, in ascending order of their indexes.  write(place, value,
-// index) is called once per place, by any thread; returns how many there are.
-template <typename T>
-struct Collected {
+struct Room {
   T value[kRoom];
   int index[kRoom];
-  int n;
-  T wave[16];
-  int wave_index[16];
+  __device__ __forceinline__ void set(int at, T v, int i) { value[at] = v, index[at] = i; }
+  // How many of those from j0 to j1 come before entry i.
+  __device__ __forceinline__ int before(int i, int j0, int j1) const {
+    const T v = value[i];
+    const int at = index[i];
+    int n = 0;
+#pragma unroll 4
+    for (int j = j0; j < j1; ++j) n += (value[j] > v) | ((value[j] == v) & (index[j] < at));
+    return n;
+  }
+  __device__ __forceinline__ T value_at(int i) const { return value[i]; }
+  __device__ __forceinline__ int index_at(int i) const { return index[i]; }
 };
-template <typename T, typename E, typename W>
-__device__ __forceinline__ int greatest(Collected<T> &c, T mine, int sets, int keep, E each, W write) {
-  const T floor = least_of_sets(mine, sets, c.wave);
-  if (threadIdx.x == 0) c.n = 0;
-  __syncthreads();
-  each([&](T v, int i) {
-    if (v >= floor) {
-      const int at = atomicAdd(&c.n, 1);
-      if (at < kRoom) {
-        c.value[at] = v;
-        c.index[at] = i;
-      }
-    }
-  });
-  __syncthreads();
-  const int n = c.n;
+template <typename T, int WAVES>
+struct Collected {
+  Room<T> room;
+  int n;
+  float top[WAVES], floor[WAVES];
+  double sum[WAVES];
+  T best[WAVES];
+  int best_at[WAVES];
+};
+
+template <typename T, int WAVES>
+__device__ __forceinline__ void collect(Collected<T, WAVES> &c, T v, int i) {
+  const int at = atomicAdd(&c.n, 1);
+  if (at < kRoom) c.room.set(at, v, i);
+}
+
+// The greatest `keep` of what was collected (after a barrier), in order:
+// write(place, value, index) once per place, by any thread.  Returns how many there are.  each(f) calls
+// f(value, index) for this thread's candidates: where more were collected than there is room for, they
+// are found one after the other, each the greatest of those behind the last one.
+template <typename T, int WAVES, typename E, typename W>
+__device__ __forceinline__ int greatest(Collected<T, WAVES> &c, int keep, E each, W write) {
+  const int n = c.n, t = threadIdx.x;
+  constexpr int kThreads = 64 * WAVES;
   if (n <= kRoom) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const T v = c.value[i];
-      const int at = c.index[i];
-      int place = 0;
-      for (int j = 0; j < n; ++j) place += c.value[j] > v || (c.value[j] == v && c.index[j] < at);
-      if (place < keep) write(place, v, at);
+    for (int i = t; i < n; i += kThreads) {
+      const int place = c.room.before(i, 0, n);
+      if (place < keep) write(place, c.room.value_at(i), c.room.index_at(i));
     }
     return min(n, keep);
   }
-  // One after the other: the greatest of those behind the last one.
   T last = 0;
   int last_at = -1;
   for (int place = 0; place < keep; ++place) {
@@ -129,14 +137,14 @@ __device__ __forceinline__ int greatest(Collected<T> &c, T mine, int sets, int k
     }
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
-      c.wave[threadIdx.x >> 6] = best;
-      c.wave_index[threadIdx.x >> 6] = best_at;
+      c.best[threadIdx.x >> 6] = best;
+      c.best_at[threadIdx.x >> 6] = best_at;
     }
     __syncthreads();
-    best = c.wave[0];
-    best_at = c.wave_index[0];
-    for (int i = 1; i < static_cast<int>(blockDim.x >> 6); ++i)
-      if (c.wave[i] > best || (c.wave[i] == best && c.wave_index[i] < best_at)) best = c.wave[i], best_at = c.wave_index[i];
+    best = c.best[0];
+    best_at = c.best_at[0];
+    for (int i = 1; i < WAVES; ++i)
+      if (c.best[i] > best || (c.best[i] == best && c.best_at[i] < best_at)) best = c.best[i], best_at = c.best_at[i];
     if (threadIdx.x == 0) write(place, best, best_at);   // (there are more than kRoom >= keep)
     last = best;
     last_at = best_at;
@@ -148,8 +156,8 @@ __device__ __forceinline__ int greatest(Collected<T> &c, T mine, int sets, int k
 // (VEC), or every 256th.
 template <int DT, bool VEC, int EPT>
 __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
-  __shared__ Collected<float> s;
-  __shared__ double s_sum[4];
+  __shared__ Collected<float, 4> s;
+  __shared__ __attribute__((aligned(16))) float s_quad[64];   // the maxima of four threads each
   const int64_t row = blockIdx.y;
   const int part = blockIdx.x, t = threadIdx.x;
   // (a beam that has ended, or cannot be continued, has no use for its logits)
@@ -157,123 +165,234 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
   const int v0 = part * 256 * EPT, width = min(256 * EPT, a.vocab - v0);
   const int64_t at = row * a.x_stride + v0;
   float x[EPT];
+  if (VEC && width == 256 * EPT) {   // (no branch between the loads: all are under way together)
+    constexpr int kRaw = DT == SOPHIA_DTYPE_BF16 ? 1 : 2;
+    u4 raw[EPT / 8][kRaw];
 #pragma unroll
-  for (int e = 0; e < EPT; e += 8) {
-    if constexpr (VEC) {
-      const int i = 256 * e + 8 * t;
-      if (i + 8 <= width) {
-        const f4 lo = load4(a.x, at + i, DT), hi = load4(a.x, at + i + 4, DT);
+    for (int e = 0; e < EPT; e += 8)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[e + k] = lo[k], x[e + 4 + k] = hi[k];
-      } else {
+      for (int k = 0; k < kRaw; ++k)
+        raw[e / 8][k] = reinterpret_cast<const u4 *>(static_cast<const char *>(a.x) + (at + 256 * e + 8 * t) * (2 * kRaw))[k];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[e + k] = i + k < width ? load_elem(a.x, at + i + k, DT) : -INFINITY;
-      }
-    } else {
+    for (int e = 0; e < EPT; ++e) {
+      const u4 &r = raw[e / 8][DT == SOPHIA_DTYPE_BF16 ? 0 : (e & 7) / 4];
+      if constexpr (DT == SOPHIA_DTYPE_BF16)
+        x[e] = __uint_as_float(e & 1 ? r[(e & 7) / 2] & 0xffff0000u : r[(e & 7) / 2] << 16);
+      else
+        x[e] = __uint_as_float(r[e & 3]);
+    }
+  } else {
+    uint32_t raw[EPT];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int i = 256 * (e + k) + t;
-        x[e + k] = i < width ? load_elem(a.x, at + i, DT) : -INFINITY;
-      }
+    for (int e = 0; e < EPT; ++e) {
+      const int i = VEC ? 256 * (e & ~7) + 8 * t + (e & 7) : 256 * e + t;
+      raw[e] = load_raw(a.x, at + min(i, width - 1), DT);
+    }
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) {
+      const int i = VEC ? 256 * (e & ~7) + 8 * t + (e & 7) : 256 * e + t;
+      x[e] = i < width ? raw_to_f32(raw[e], DT) : -INFINITY;
     }
   }
   const auto index = [&](int e) { return VEC ? 256 * (e & ~7) + 8 * t + (e & 7) : 256 * e + t; };
-  float mine = -INFINITY;
+  // (a maximum passes over NaN, and NaN is not above anything)
+  float top4[EPT / 4], quad = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) {
-    if (!(x[e] > -INFINITY)) x[e] = -INFINITY;   // NaN: no candidate
-    mine = fmaxf(mine, x[e]);
+  for (int e = 0; e < EPT; e += 4) {
+    top4[e / 4] = fmaxf(fmaxf(x[e], x[e + 1]), fmaxf(x[e + 2], x[e + 3]));
+    quad = fmaxf(quad, top4[e / 4]);
   }
-  const float top = across(mine, s.wave, [](float p, float q) { return fmaxf(p, q); });
+  const float mine = quad;
+  quad = fmaxf(quad, lane_other<1>(quad));
+  quad = fmaxf(quad, lane_other<2>(quad));
+  const int lane = t & 63, wave = t >> 6;
+  if ((lane & 3) == 0) s_quad[t >> 2] = quad;
+  float top = top_of_quads(quad);
+  if (lane == 0) s.top[wave] = top;
+  if (t == 0) s.n = 0;
+  __syncthreads();
+  top = fmaxf(fmaxf(s.top[0], s.top[1]), fmaxf(s.top[2], s.top[3]));
   const int64_t slot = row * a.parts + part;
-  double sum = 0.0;
-  if (top > -INFINITY && top < INFINITY) {
-    float p = 0.f;
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) p += __expf(x[e] - top);
-    sum = across(static_cast<double>(p), s_sum, [](double q, double r) { return q + r; });
-  }
-  if (t == 0) {
-    a.top[slot] = top;
-    a.sum[slot] = sum;
-  }
   float *value = a.value + slot * a.keep;
   int32_t *token = a.token + slot * a.keep;
-  const int n = top > -INFINITY
-                    ? greatest<float>(
-                          s, mine, a.sets, a.keep,
-                          [&](auto f) {
+  if (!(top > -INFINITY)) {
+    if (t == 0) a.top[slot] = -INFINITY;
+    for (int i = t; i < a.keep; i += 256) token[i] = -1;
+    return;
+  }
+  {
+    // How many of the 64 maxima are above this one, a quarter of them compared by each lane of the four.
+    int above = 0;
 #pragma unroll
-                            for (int e = 0; e < EPT; ++e)
-                              if (x[e] > -INFINITY) f(x[e], index(e));
-                          },
-                          [&](int place, float v, int i) {
-                            value[place] = v;
-                            token[place] = v0 + i;
-                          })
-                    : 0;
+    for (int i = 0; i < 4; ++i) {
+      const f4 o = *reinterpret_cast<const f4 *>(s_quad + 16 * (lane & 3) + 4 * i);
+      above += (o.x > quad) + (o.y > quad) + (o.z > quad) + (o.w > quad);
+    }
+    above += __builtin_amdgcn_update_dpp(0, above, 0xb1, 0xf, 0xf, true);
+    above += __builtin_amdgcn_update_dpp(0, above, 0x4e, 0xf, 0xf, true);
+    const float kth = -top_of_quads(above < a.keep ? -quad : -INFINITY);
+    if (lane == 0) s.floor[wave] = kth;
+  }
+  if (top < INFINITY) {
+    const float shift = top * 1.44269504088896341f;
+    const auto add = [&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, 1.44269504088896341f, -shift)); };
+    float p[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) p[e & 3] += add(x[e]);
+    float sum = (p[0] + p[1]) + (p[2] + p[3]);
+    if (__any(sum != sum)) {   // NaN among them
+      sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) sum += x[e] == x[e] ? add(x[e]) : 0.f;
+    }
+    sum = wave_sum_dpp(sum);
+    if ((t & 63) == 0) s.sum[t >> 6] = static_cast<double>(sum);
+  }
+  __syncthreads();
+  const float least = fmaxf(fminf(fminf(s.floor[0], s.floor[1]), fminf(s.floor[2], s.floor[3])), -3.402823466e38f);
+  if (mine >= least) {
+#pragma unroll
+    for (int e = 0; e < EPT; e += 4)
+      if (top4[e / 4] >= least) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (x[e + k] >= least) collect(s, x[e + k], index(e + k));
+      }
+  }
+  __syncthreads();
+  if (t == 0) {
+    a.top[slot] = top;
+    a.sum[slot] = (s.sum[0] + s.sum[1]) + (s.sum[2] + s.sum[3]);
+  }
+  const int n = greatest(
+      s, a.keep,
+      [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < EPT; ++e)
+          if (x[e] > -INFINITY) f(x[e], index(e));
+      },
+      [&](int place, float v, int i) {
+        value[place] = v;
+        token[place] = v0 + i;
+      });
   for (int i = n + t; i < a.keep; i += 256) token[i] = -1;
 }
 
 // A group's candidates: of beam b, part p and place j the index ((b parts) + p) keep + j; equal
-// values of one beam are in the order of their tokens, as parts and places are.
-__global__ __launch_bounds__(256) void beam_join_kernel(BeamArgs a) {
-  __shared__ Collected<double> s;
+// values of one beam are in the order of their tokens, as parts and places are.  A wavefront
+// joins the sums of a beam, a part per lane; meanwhile the candidates are under way, the first of
+// all lists first.  The parts' lists are sorted: the keep-th of any of them is not above the
+// keep-th greatest of all, and neither is the keep-th of their first ones.
+constexpr int kJoin = 1024, kHeld = 2;   // threads, and candidates of each that stay in registers
+__global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
+  constexpr int kWaves = kJoin / 64;
+  __shared__ Collected<double, kWaves> s;
   __shared__ double s_lse[kMost];
+  __shared__ int s_kind[kMost];     // of a beam: 0 no candidates, 1 its logits', 2 itself
+  __shared__ float s_first[kWaves][64], s_floor;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.beams;
-  const int t = threadIdx.x;
-  for (int b = t; b < a.beams; b += 256) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int lists = a.beams * a.parts, all = lists * a.keep;
+  const int64_t base = row0 * a.parts * a.keep;
+  // Candidate c is place c / lists of list c % lists.
+  const auto index = [&](int c) {
+    const int place = c / lists;
+    return (c - place * lists) * a.keep + place;
+  };
+  float held[kHeld];
+  int held_token[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int64_t at = base + index(min(t + k * kJoin, all - 1));
+    held[k] = a.value[at];
+    held_token[k] = a.token[at];
+  }
+  for (int b = wave; b < a.beams; b += kWaves) {
     const int64_t row = row0 + b;
-    double lse = INFINITY;   // (no candidates)
-    if (fabsf(a.scores[row]) < INFINITY && !(a.ended && a.ended[row])) {
+    const float score = a.scores[row];
+    const bool done = a.ended && a.ended[row];
+    double lse = 0.0;
+    int kind = fabsf(score) < INFINITY ? 2 : 0;
+    if (kind && !done) {
       float top = -INFINITY;
-      for (int p = 0; p < a.parts; ++p) top = fmaxf(top, a.top[row * a.parts + p]);
-      if (top > -INFINITY && top < INFINITY) {
+      for (int p = lane; p < a.parts; p += 64) top = fmaxf(top, a.top[row * a.parts + p]);
+      top = top_of_lanes(top);
+      kind = top > -INFINITY && top < INFINITY;
+      if (kind) {
         double sum = 0.0;
-        for (int p = 0; p < a.parts; ++p) {
+        for (int p = lane; p < a.parts; p += 64) {
           const float m = a.top[row * a.parts + p];
           if (m > -INFINITY) sum += a.sum[row * a.parts + p] * exp(static_cast<double>(m) - static_cast<double>(top));
         }
-        lse = static_cast<double>(top) + log(sum);
+        lse = static_cast<double>(top) + log(sum_lanes(sum));
       }
     }
-    s_lse[b] = lse;
+    if (lane == 0) {
+      s_lse[b] = lse;
+      s_kind[b] = kind;
+    }
+  }
+  if (t == 0) s.n = 0;
+  __syncthreads();
+  const int each_beam = a.parts * a.keep;
+  const auto candidate = [&](int i, float x, int token) {
+    const int b = i / each_beam;
+    const double score = a.scores[row0 + b];
+    if (s_kind[b] == 1 && token >= 0) return score + (static_cast<double>(x) - s_lse[b]);
+    return s_kind[b] == 2 && i == b * each_beam ? score : -static_cast<double>(INFINITY);
+  };
+  double v[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    v[k] = t + k * kJoin < all ? candidate(index(t + k * kJoin), held[k], held_token[k]) : -INFINITY;
+  const auto each = [&](auto f) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (v[k] > -INFINITY) f(v[k], index(t + k * kJoin));
+    for (int c = t + kHeld * kJoin; c < all; c += kJoin) {
+      const int i = index(c);
+      const double w = candidate(i, a.value[base + i], a.token[base + i]);
+      if (w > -INFINITY) f(w, i);
+    }
+  };
+  // (rounding to fp32 keeps the order, but for equal ones)
+  float last = -INFINITY;   // the keep-th of a list
+  each([&](double w, int i) {
+    if (i % a.keep == a.keep - 1) last = fmaxf(last, static_cast<float>(w));
+  });
+  s_first[wave][lane] = t < lists ? static_cast<float>(v[0]) : -INFINITY;
+  last = top_of_lanes(last);
+  if (lane == 0) s.top[wave] = last;
+  __syncthreads();
+  if (wave == 0) {
+    float first = s_first[0][lane], floor = s.top[lane & (kWaves - 1)];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) first = fmaxf(first, s_first[i][lane]);
+    int above = 0;
+#pragma unroll 16
+    for (int i = 0; i < 64; ++i)
+      above += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(first), i)) > first;
+    floor = top_of_lanes(floor);
+    // the least of those that fewer than keep are above: the keep-th (-inf: there are not so many)
+    const float kth = -top_of_lanes(above < a.keep ? -first : -INFINITY);
+    if (lane == 0) s_floor = fmaxf(floor, kth);
   }
   __syncthreads();
-  const int each_beam = a.parts * a.keep, all = a.beams * each_beam;
-  const auto candidate = [&](int i) {
-    const int b = i / each_beam;
-    const int64_t row = row0 + b;
-    const float score = a.scores[row];
-    if (!(fabsf(score) < INFINITY)) return -static_cast<double>(INFINITY);
-    if (a.ended && a.ended[row]) return i == b * each_beam ? static_cast<double>(score) : -static_cast<double>(INFINITY);
-    const int64_t at = row0 * each_beam + i;
-    if (!(s_lse[b] < INFINITY) || a.token[at] < 0) return -static_cast<double>(INFINITY);
-    return static_cast<double>(score) + (static_cast<double>(a.value[at]) - s_lse[b]);
-  };
-  double mine = -INFINITY;
-  for (int i = t; i < all; i += 256) {
-    const double v = candidate(i);
-    mine = v > mine ? v : mine;
-  }
+  const float floor = s_floor;
+  each([&](double w, int i) {
+    if (static_cast<float>(w) >= floor) collect(s, w, i);
+  });
+  __syncthreads();
   float *out_score = a.out_score + static_cast<int64_t>(blockIdx.x) * a.keep;
   int32_t *out_parent = a.out_parent + static_cast<int64_t>(blockIdx.x) * a.keep;
   int64_t *out_token = a.out_token + static_cast<int64_t>(blockIdx.x) * a.keep;
-  const int n = greatest<double>(
-      s, mine, a.sets, a.keep,
-      [&](auto f) {
-        for (int i = t; i < all; i += 256) {
-          const double v = candidate(i);
-          if (v > -INFINITY) f(v, i);
-        }
-      },
-      [&](int place, double v, int i) {
-        const int b = i / each_beam;
-        out_score[place] = static_cast<float>(v);
-        out_parent[place] = b;
-        out_token[place] = a.ended && a.ended[row0 + b] ? a.pad : a.token[row0 * each_beam + i];
-      });
-  for (int i = n + t; i < a.keep; i += 256) {
+  const int n = greatest(s, a.keep, each, [&](int place, double w, int i) {
+    const int b = i / each_beam;
+    out_score[place] = static_cast<float>(w);
+    out_parent[place] = b;
+    out_token[place] = s_kind[b] == 2 ? a.pad : a.token[base + i];
+  });
+  for (int i = n + t; i < a.keep; i += kJoin) {
     out_score[i] = -INFINITY;
     out_parent[i] = -1;
     out_token[i] = -1;
@@ -313,9 +432,7 @@ extern "C" int sophia_beam_select(const void *logits, int64_t logits_stride, int
   SOPHIA_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
                      workspace_bytes >= sophia_beam_select_workspace_size(rows, vocab, keep),
                  "beam_select: workspace too small");
-  int sets = 4;
-  while (sets < keep) sets *= 2;
-  BeamArgs a{logits, logits_stride, rows, vocab, scores, ended, pad_token, beams, keep, sets, parts,
+  BeamArgs a{logits, logits_stride, rows, vocab, scores, ended, pad_token, beams, keep, parts,
              nullptr, nullptr, nullptr, nullptr, out_scores, out_parent, out_token};
   const int64_t n = rows * parts;
   a.sum = static_cast<double *>(workspace);
@@ -339,6 +456,6 @@ extern "C" int sophia_beam_select(const void *logits, int64_t logits_stride, int
   else SOPHIA_BEAM_DT(SOPHIA_DTYPE_BF16);
 #undef SOPHIA_BEAM_DT
 #undef SOPHIA_BEAM
-  hipLaunchKernelGGL(beam_join_kernel, dim3(static_cast<unsigned>(rows / beams)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(beam_join_kernel, dim3(static_cast<unsigned>(rows / beams)), dim3(kJoin), 0, st, a);
   return check_launch("beam_select");
 }

@@ -15,8 +15,7 @@ namespace sophia {
 namespace {
 
 constexpr int kMoves = SOPHIA_MOVES;
-constexpr int kPlanThreads = 1024;
-constexpr int kHash = 2 * kMoves;
+constexpr int kFew = 64;      // so many moves each work-group plans by itself
 
 // A planned move.
 struct Move {
@@ -44,38 +43,127 @@ struct PlanArgs {
   Move *moves;
 };
 
-__global__ __launch_bounds__(kPlanThreads) void move_plan_kernel(PlanArgs a) {
-  __shared__ int s_src[kMoves], s_dst[kMoves];
-  // By slot: the last move that writes it.  Later the places of the trees' roots.
+// Move i, whose source and destination are given; of a cycle's first move also its last one.
+__device__ __forceinline__ Move planned(const PlanArgs &a, int i, int src, int dst, int flags, int end, int end_src) {
+  const auto tokens = [&](int move) { return a.cached ? static_cast<int>(iclamp64(a.cached[move], 0, 1 << 30)) : 0; };
+  const auto page = [&](int slot, int count) {
+    const int full = count >> a.shift;
+    const int id = a.table && full < a.max_pages ? a.table[slot * a.table_stride + full] : -1;
+    return id >= 0 && id < a.n_pages ? id : -1;
+  };
+  Move m = {};
+  m.src = src;
+  m.dst = dst;
+  m.flags = flags;
+  m.tokens = tokens(i);
+  m.src_page = page(src, m.tokens);
+  m.dst_page = page(dst, m.tokens);
+  m.held_page = -1;
+  if (flags & kSave) {
+    m.held_tokens = tokens(end);
+    m.held_page = page(end_src, m.held_tokens);
+  }
+  return m;
+}
+
+// At most 64 moves, planned by a wavefront: a move per lane, sets of moves as bits.  put(place, move)
+// in any order; returns their number.
+template <typename P>
+__device__ __forceinline__ int plan_few(const PlanArgs &a, P put) {
+  const int i = threadIdx.x & 63, n = a.n;
+  const int src = i < n ? a.src[i] : -1, dst = i < n ? a.dst[i] : -1;
+  const bool ok = src >= 0 && src < a.limit && dst >= 0 && dst < a.limit;
+  const uint64_t all = __ballot(ok);
+  const auto of = [](int v, int lane) { return __builtin_amdgcn_readlane(v, lane); };
+  // The last move to this one's slot, and the last one to the slot that it reads.
+  int last = i, writer = -1;
+  for (uint64_t m = all; m; m &= m - 1) {
+    const int j = __ffsll(static_cast<unsigned long long>(m)) - 1, d = of(dst, j);
+    last = d == dst ? j : last;
+    writer = d == src ? j : writer;
+  }
+  const bool active = ok && last == i && src != dst;
+  const uint64_t live = __ballot(active);
+  const int next = active && writer >= 0 && ((live >> writer) & 1) ? writer : -1;
+  uint64_t readers = 0;       // the moves that have to come before
+  for (uint64_t m = __ballot(next >= 0); m; m &= m - 1) {
+    const int j = __ffsll(static_cast<unsigned long long>(m)) - 1;
+    readers |= of(next, j) == i ? 1ull << j : 0;
+  }
+  // Levels; what is left are cycles, which take levels of their own one after the other.
+  uint64_t left = live;
+  int level = 0, flags = 0, end = 0, root = i, now = 0;
+  for (uint64_t ready; (ready = __ballot(((left >> i) & 1) && !(readers & left))) != 0; left &= ~ready)
+    if ((ready >> i) & 1) level = now++;
+    else ++now;
+  int up = next;
+  for (uint64_t m = left; m;) {
+    const int first = __ffsll(static_cast<unsigned long long>(m)) - 1;
+    for (int j = first;;) {
+      m &= ~(1ull << j);
+      if (i == j) level = now;
+      ++now;
+      const int to = of(next, j);
+      if (to == first) {
+        if (i == j) flags |= kFromSaved, up = -1;
+        if (i == first) flags |= kSave, end = j;
+        break;
+      }
+      j = to;
+    }
+  }
+  // Trees: each move's last one, by doubling.
+  root = up >= 0 ? up : i;
+#pragma unroll
+  for (int r = 0; r < 6; ++r) root = __shfl(root, root, 64);
+  const int key = root << 16 | level << 8 | i;   // (moves that read one slot have one level)
+  int place = 0, same = 0;
+  for (uint64_t m = live; m; m &= m - 1) {
+    const int k = of(key, __ffsll(static_cast<unsigned long long>(m)) - 1);
+    place += k < key;
+    same += k < key && (k >> 16) == root;
+  }
+  const int end_src = __shfl(src, end, 64);
+  if (active) put(place, planned(a, i, src, dst, flags | (same == 0 ? kFirst : 0), end, end_src));
+  return __popcll(live);
+}
+
+// The same for more, by THREADS threads.
+template <int N, int THREADS>
+__global__ __launch_bounds__(THREADS) void move_plan_kernel(PlanArgs a) {
+  constexpr int kEach = N / THREADS, kHash = 2 * N, kBits = __builtin_ctz(2 * N);
+  static_assert(N == kEach * THREADS, "each thread has as many moves");
+  __shared__ int s_src[N], s_dst[N], s_readers[N];   // s_readers: moves that have to come before; then places
+  __shared__ short s_next[N];
+  // By slot, the last move that writes it; later what is found of the trees.
   __shared__ int s_key[kHash], s_by[kHash];
-  __shared__ short s_next[kMoves], s_level[kMoves];   // the move that has to wait for this one; steps from the leaves
-  __shared__ int s_readers[kMoves];                   // moves that have to come before
-  __shared__ short s_end[kMoves];                     // of a cycle's first move: its last one
-  __shared__ int s_left, s_total;
+  __shared__ int s_wave[THREADS / 64];
+  int *const s_count = s_key;                        // of a root: moves of its tree, then the next one's place
+  int *const s_first = s_key + N;                    // the first one's
+  short *const s_jump = reinterpret_cast<short *>(s_by), *const s_low = s_jump + N, *const s_end = s_low + N;
   const int t = threadIdx.x, n = a.n;
-  for (int i = t; i < kHash; i += kPlanThreads) {
+  for (int i = t; i < kHash; i += THREADS) {
     s_key[i] = -1;
     s_by[i] = -1;
   }
-  for (int i = t; i < n; i += kPlanThreads) {
-    const int s = a.src[i], d = a.dst[i];
-    const bool ok = s >= 0 && s < a.limit && d >= 0 && d < a.limit;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = t + k * THREADS;
+    const int s = i < n ? a.src[i] : -1, d = i < n ? a.dst[i] : -1;
     s_src[i] = s;
-    s_dst[i] = ok ? d : -1;
-    s_next[i] = -1;
-    s_level[i] = -1;
+    s_dst[i] = s >= 0 && s < a.limit && d >= 0 && d < a.limit ? d : -1;
     s_readers[i] = 0;
   }
-  if (t == 0) s_total = 0;
   __syncthreads();
-  const auto hash = [](int slot) { return (static_cast<unsigned>(slot) * 2654435761u) >> (32 - 13); };
-  static_assert(kHash == 1 << 13, "the hash's bits");
-  for (int i = t; i < n; i += kPlanThreads) {
-    if (s_dst[i] < 0) continue;
-    unsigned h = hash(s_dst[i]);      // (half of the places stay free)
+  const auto hash = [](int slot) { return (static_cast<unsigned>(slot) * 2654435761u) >> (32 - kBits); };
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = t + k * THREADS, d = s_dst[i];
+    if (d < 0) continue;
+    unsigned h = hash(d);      // (half of the places stay free)
     for (;; h = (h + 1) & (kHash - 1)) {
-      const int was = atomicCAS(&s_key[h], -1, s_dst[i]);
-      if (was == -1 || was == s_dst[i]) break;
+      const int was = atomicCAS(&s_key[h], -1, d);
+      if (was == -1 || was == d) break;
     }
     atomicMax(&s_by[h], i);
   }
@@ -86,146 +174,152 @@ __global__ __launch_bounds__(kPlanThreads) void move_plan_kernel(PlanArgs a) {
       if (s_key[h] == -1) return -1;
     }
   };
-  // What counts: the last move to a slot, if it changes it.
-  for (int i = t; i < n; i += kPlanThreads) {
-    const int d = s_dst[i];
-    s_level[i] = d >= 0 && writer(d) == i && s_src[i] != d ? 0 : -1;
-  }
-  __syncthreads();
-  for (int i = t; i < n; i += kPlanThreads) {
-    if (s_level[i] < 0) continue;
-    atomicAdd(&s_total, 1);
-    const int next = writer(s_src[i]);
-    if (next >= 0 && s_level[next] >= 0) {
-      s_next[i] = static_cast<short>(next);
-      atomicAdd(&s_readers[next], 1);
-    }
-  }
-  __syncthreads();
-  // Levels: a move comes after all that read its slot.  s_readers < 0: done.
-  int level = 1;
-  for (;; ++level) {
-    if (t == 0) s_left = 0;
-    __syncthreads();
-    bool ready[kMoves / kPlanThreads];
+  // What counts is the last move to a slot, if it changes it: so of a slot's writer too.
+  bool active[kEach];
+  int next[kEach];
 #pragma unroll
-    for (int k = 0; k < kMoves / kPlanThreads; ++k) {
-      const int i = t + k * kPlanThreads;
-      ready[k] = i < n && s_level[i] == 0 && s_readers[i] == 0;
-    }
-    __syncthreads();
+  for (int k = 0; k < kEach; ++k) {
+    const int i = t + k * THREADS, d = s_dst[i];
+    active[k] = d >= 0 && s_src[i] != d && writer(d) == i;
+    const int w = active[k] ? writer(s_src[i]) : -1;
+    next[k] = w >= 0 && s_src[w] != s_dst[w] ? w : -1;
+    s_next[i] = static_cast<short>(next[k]);
+    if (next[k] >= 0) atomicAdd(&s_readers[next[k]], 1);
+  }
+  __syncthreads();
+  // By doubling: the move after 1, 2, 4 .. steps, and the lowest on the way.
 #pragma unroll
-    for (int k = 0; k < kMoves / kPlanThreads; ++k) {
-      const int i = t + k * kPlanThreads;
-      if (!ready[k]) continue;
-      s_level[i] = static_cast<short>(level);
-      s_left = 1;
-      if (s_next[i] >= 0) atomicSub(&s_readers[s_next[i]], 1);
-    }
-    __syncthreads();
-    if (s_left == 0) break;
-    __syncthreads();
+  for (int k = 0; k < kEach; ++k) {
+    const int i = t + k * THREADS;
+    s_jump[i] = static_cast<short>(next[k] >= 0 ? next[k] : i);
+    s_low[i] = static_cast<short>(i);
   }
-  // What is left are cycles.  Each begins at its lowest move, whose slot's content is held, and
-  // ends with the move that reads that slot, which waits for nobody any more.
-  for (int i = t; i < n; i += kPlanThreads) s_readers[i] = 0;   // (now: the flags)
-  __syncthreads();
-  for (int i = t; i < n; i += kPlanThreads) {
-    if (s_level[i] != 0) continue;
-    bool lowest = true;
-    for (int j = s_next[i]; j != i && lowest; j = s_next[j]) lowest = j > i;
-    if (lowest) s_readers[i] = kSave;
-  }
-  __syncthreads();
-  for (int i = t; i < n; i += kPlanThreads) {
-    if (!(s_readers[i] & kSave)) continue;
-    int at = level, j = i;
-    for (;;) {
-      const int next = s_next[j];
-      s_level[j] = static_cast<short>(at++);
-      if (next == i) break;
-      j = next;
-    }
-    s_readers[j] |= kFromSaved;
-    s_next[j] = -1;
-    s_end[i] = static_cast<short>(j);
-  }
-  __syncthreads();
-  // Each move's root, the last of its tree, by doubling; then the order: by root, then by level.
-  short *s_root = reinterpret_cast<short *>(s_by);
-  for (int i = t; i < n; i += kPlanThreads) s_root[i] = s_next[i] >= 0 ? s_next[i] : static_cast<short>(i);
   __syncthreads();
   for (int reach = 1; reach < n; reach *= 2) {
-    short up[kMoves / kPlanThreads];
+    short jump[kEach], low[kEach];
 #pragma unroll
-    for (int k = 0; k < kMoves / kPlanThreads; ++k) {
-      const int i = t + k * kPlanThreads;
-      if (i < n) up[k] = s_root[s_root[i]];
+    for (int k = 0; k < kEach; ++k) {
+      const int i = t + k * THREADS, j = s_jump[i];
+      jump[k] = s_jump[j];
+      low[k] = min(s_low[i], s_low[j]);
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kMoves / kPlanThreads; ++k) {
-      const int i = t + k * kPlanThreads;
-      if (i < n) s_root[i] = up[k];
+    for (int k = 0; k < kEach; ++k) {
+      s_jump[t + k * THREADS] = jump[k];
+      s_low[t + k * THREADS] = low[k];
     }
     __syncthreads();
   }
-  const int total = s_total;
-  // A key per move (root, level, move: 13 bits each; what does not count behind), sorted in place by
-  // exchanges.  They lie where the hash was.
-  int size = 1;
-  while (size < n) size *= 2;
-  uint64_t key[kMoves / kPlanThreads];
+  // A tree's root is its last move, or the lowest move of the cycle that it ends in, which has that
+  // cycle's first move.
+  int root[kEach];
 #pragma unroll
-  for (int k = 0; k < kMoves / kPlanThreads; ++k) {
-    const int i = t + k * kPlanThreads;
-    key[k] = i < n && s_level[i] > 0
-                 ? static_cast<uint64_t>(s_root[i]) << 32 | static_cast<uint64_t>(s_level[i]) << 16 | static_cast<uint64_t>(i)
-                 : ~0ull;
+  for (int k = 0; k < kEach; ++k) {
+    const int at = s_jump[t + k * THREADS];
+    root[k] = s_next[at] < 0 ? at : s_low[at];
+    s_count[t + k * THREADS] = 0;
   }
   __syncthreads();
-  uint64_t *s_sort = reinterpret_cast<uint64_t *>(s_key);
-  static_assert(sizeof(s_key) >= sizeof(uint64_t) * kMoves, "the keys fit");
 #pragma unroll
-  for (int k = 0; k < kMoves / kPlanThreads; ++k)
-    if (t + k * kPlanThreads < size) s_sort[t + k * kPlanThreads] = key[k];
+  for (int k = 0; k < kEach; ++k) {
+    s_low[t + k * THREADS] = 0;                      // (now: 1 + the root, of moves on a cycle)
+    if (active[k]) atomicAdd(&s_count[root[k]], 1);
+  }
   __syncthreads();
-  for (int run = 2; run <= size; run *= 2)
-    for (int gap = run / 2; gap > 0; gap /= 2) {
-      for (int p = t; p < size / 2; p += kPlanThreads) {
-        const int lo = (p / gap) * 2 * gap + p % gap, hi = lo + gap;
-        const bool up = (lo & run) == 0;
-        const uint64_t x = s_sort[lo], y = s_sort[hi];
-        if ((x > y) == up) {
-          s_sort[lo] = y;
-          s_sort[hi] = x;
-        }
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = t + k * THREADS;
+    if (!active[k] || next[k] < 0 || root[k] != i) continue;
+    int j = i;
+    for (;;) {
+      s_low[j] = static_cast<short>(i + 1);
+      const int to = s_next[j];
+      if (to == i) break;
+      j = to;
+    }
+    s_end[i] = static_cast<short>(j);
+  }
+  // Where the trees begin: a sum over the roots before, kEach neighbours per thread.
+  int mine[kEach], sum = 0;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    mine[k] = sum;
+    sum += s_count[kEach * t + k];
+  }
+  int scan = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(scan, off, 64);
+    if ((t & 63) >= off) scan += o;
+  }
+  if ((t & 63) == 63) s_wave[t >> 6] = scan;
+  __syncthreads();
+  int before = scan - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w < (t >> 6)) before += s_wave[w];
+    total += s_wave[w];
+  }
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    s_count[kEach * t + k] = before + mine[k];
+    s_first[kEach * t + k] = before + mine[k];
+  }
+  __syncthreads();
+  // A move takes its place when all that read its slot have theirs.  Nobody waits for a cycle here, and of
+  // what is on none there is always one that nothing is before: every thread comes to its end.
+  bool waits[kEach], any = false;
+  int place[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    waits[k] = active[k] && s_low[t + k * THREADS] == 0;
+    any |= waits[k];
+  }
+  while (any) {
+    any = false;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (!waits[k]) continue;
+      if (__hip_atomic_load(&s_readers[t + k * THREADS], __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP) == 0) {
+        place[k] = __hip_atomic_fetch_add(&s_count[root[k]], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (next[k] >= 0) __hip_atomic_fetch_add(&s_readers[next[k]], -1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_WORKGROUP);
+        waits[k] = false;
+      } else {
+        any = true;
       }
-      __syncthreads();
     }
-  for (int p = t; p < total; p += kPlanThreads) {
-    const uint64_t k = s_sort[p];
-    const int i = static_cast<int>(k & 0xffff), root = static_cast<int>(k >> 32);
-    Move m = {};
-    m.src = s_src[i];
-    m.dst = s_dst[i];
-    m.flags = s_readers[i] | (p == 0 || static_cast<int>(s_sort[p - 1] >> 32) != root ? kFirst : 0);
-    m.src_page = m.dst_page = m.held_page = -1;
-    const auto tokens = [&](int move) { return a.cached ? static_cast<int>(iclamp64(a.cached[move], 0, 1 << 30)) : 0; };
-    const auto page = [&](int slot, int count) {
-      const int full = count >> a.shift;
-      const int id = a.table && full < a.max_pages ? a.table[slot * a.table_stride + full] : -1;
-      return id >= 0 && id < a.n_pages ? id : -1;
-    };
-    m.tokens = tokens(i);
-    m.src_page = page(m.src, m.tokens);
-    m.dst_page = page(m.dst, m.tokens);
-    if (m.flags & kSave) {
-      const int end = s_end[i];
-      m.held_tokens = tokens(end);
-      m.held_page = page(s_src[end], m.held_tokens);
+  }
+  __syncthreads();
+  // Then the cycles.
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = t + k * THREADS;
+    if (!active[k] || next[k] < 0 || root[k] != i) continue;
+    int at = s_count[i];
+    for (int j = i;;) {
+      s_readers[j] = at++;
+      const int to = s_next[j];
+      if (to == i) break;
+      j = to;
     }
-    a.moves[p] = m;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = t + k * THREADS;
+    if (!active[k]) continue;
+    int flags = 0, end = 0;
+    if (s_low[i] != 0) {
+      place[k] = s_readers[i];
+      if (root[k] == i) {
+        flags |= kSave;
+        end = s_end[i];
+      }
+      if (next[k] == root[k]) flags |= kFromSaved;
+    }
+    if (place[k] == s_first[root[k]]) flags |= kFirst;
+    a.moves[place[k]] = planned(a, i, s_src[i], s_dst[i], flags, end, s_src[end]);
   }
   if (t == 0) *a.count = total;
 }
@@ -243,9 +337,7 @@ struct Part {
 };
 
 struct MoveArgs {
-  const int32_t *count;
-  const Move *moves;
-  int shift;                 // of the pages
+  PlanArgs plan;
   int n_parts;
   int workers;               // that share the trees
   Part part[kParts];
@@ -255,7 +347,12 @@ static_assert(sizeof(MoveArgs) <= 4000, "kernel arguments");
 
 constexpr int kMoveThreads = 256, kChunk = 16 * kMoveThreads, kBatch = 8;
 
+// FEW: at most kFew moves, planned here by the first wavefront (a launch less, for what takes it
+// about 2 us beside other work-groups' copies); else a list of them, taken kFew at a time.
+template <bool FEW>
 __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
+  __shared__ Move s_moves[kFew + kBatch];
+  __shared__ int s_total;
   int block = blockIdx.x, q = 0;
   while (q + 1 < a.n_parts && block >= a.part[q].tensors * a.part[q].chunks) {
     block -= a.part[q].tensors * a.part[q].chunks;
@@ -264,11 +361,19 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
   const Part p = a.part[q];
   char *base = a.base[p.first + block / p.chunks];
   const int64_t off = static_cast<int64_t>(block % p.chunks) * kChunk + 16 * threadIdx.x;
-  const int total = *a.count;
+  if constexpr (FEW) {
+    if (threadIdx.x < 64) {
+      const int total = plan_few(a.plan, [&](int place, const Move &m) { s_moves[place] = m; });
+      if (threadIdx.x == 0) s_total = total;
+    }
+    __syncthreads();
+  }
   // This worker's trees: those that begin in its share of the list.
+  const int total = FEW ? s_total : *a.plan.count;
+  const Move *list = FEW ? s_moves : a.plan.moves;
   const auto begin = [&](int w) {
     int at = static_cast<int>(static_cast<int64_t>(total) * w / a.workers);
-    while (at < total && !(a.moves[at].flags & kFirst)) ++at;
+    while (at < total && !(list[at].flags & kFirst)) ++at;
     return at;
   };
   const int from = begin(blockIdx.y), to = begin(blockIdx.y + 1);
@@ -280,9 +385,9 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
       case kLatents:
         return off < imin64(p.bytes, static_cast<int64_t>(tokens) * p.token_bytes) ? 16 : 0;
       case kPageTail:
-        return off < static_cast<int64_t>(tokens & ((1 << a.shift) - 1)) * p.token_bytes ? 16 : 0;
+        return off < static_cast<int64_t>(tokens & ((1 << a.plan.shift) - 1)) * p.token_bytes ? 16 : 0;
       default:
-        return static_cast<int>(iclamp64(imin64(p.bytes, 4ll * (tokens >> a.shift)) - off, 0, 16));
+        return static_cast<int>(iclamp64(imin64(p.bytes, 4ll * (tokens >> a.plan.shift)) - off, 0, 16));
     }
   };
   const auto load = [&](int64_t slot, int n) {
@@ -299,32 +404,52 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
     return v;
   };
   const bool tail = p.kind == kPageTail;
+  const bool in = off < p.bytes;
   u4 held = {0u, 0u, 0u, 0u};
-  for (int i0 = from; i0 < to; i0 += kBatch) {
+  // Moves [m, m + n) of s_moves: all loads before the stores, as what a batch reads is not written before it.
+  const auto batch = [&](const Move *m, int n) {
     u4 v[kBatch];
-    // All loads of a batch before its stores: what a batch reads is not written before it.
+    int flags = 0;
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (i0 + k >= to) break;
-      const Move m = a.moves[i0 + k];
-      if (m.flags & kSave) held = load(tail ? m.held_page : m.dst, bytes(m.held_tokens));
-      v[k] = m.flags & kFromSaved ? held : load(tail ? m.src_page : m.src, bytes(m.tokens));
+    for (int k = 0; k < kBatch; ++k) flags |= k < n ? m[k].flags : 0;
+    if (p.kind == kWhole && n == kBatch && !(flags & (kSave | kFromSaved))) {   // (no branch between the loads)
+      if (!in) return;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) v[k] = *reinterpret_cast<const u4 *>(base + m[k].src * p.stride + off);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) *reinterpret_cast<u4 *>(base + m[k].dst * p.stride + off) = v[k];
+      return;
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (i0 + k >= to) break;
-      const Move m = a.moves[i0 + k];
-      const int n = bytes(m.tokens);
-      if (tail && (m.src_page < 0 || m.dst_page < 0)) continue;
-      char *at = base + (tail ? m.dst_page : m.dst) * p.stride + off;
+      if (k >= n) break;
+      if (m[k].flags & kSave) held = load(tail ? m[k].held_page : m[k].dst, bytes(m[k].held_tokens));
+      v[k] = m[k].flags & kFromSaved ? held : load(tail ? m[k].src_page : m[k].src, bytes(m[k].tokens));
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (k >= n) break;
+      const int count = bytes(m[k].tokens);
+      if (tail && (m[k].src_page < 0 || m[k].dst_page < 0)) continue;
+      char *at = base + (tail ? m[k].dst_page : m[k].dst) * p.stride + off;
       if (p.kind != kTable) {
-        if (n) *reinterpret_cast<u4 *>(at) = v[k];
+        if (count) *reinterpret_cast<u4 *>(at) = v[k];
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (4 * i < n) reinterpret_cast<uint32_t *>(at)[i] = v[k][i];
+          if (4 * i < count) reinterpret_cast<uint32_t *>(at)[i] = v[k][i];
       }
     }
+  };
+  for (int i0 = from; i0 < to; i0 += kFew) {
+    const int n = min(kFew, to - i0);
+    if constexpr (!FEW) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * n; i += kMoveThreads)
+        reinterpret_cast<u4 *>(s_moves)[i] = reinterpret_cast<const u4 *>(a.plan.moves + i0)[i];
+      __syncthreads();
+    }
+    for (int i = 0; i < n; i += kBatch) batch(s_moves + (FEW ? i0 : 0) + i, min(kBatch, n - i));
   }
 }
 
@@ -341,16 +466,23 @@ constexpr size_t kHeader = 64;   // of the workspace: the count
 int run_moves(const char *what, PlanArgs plan, MoveArgs a, char *workspace, hipStream_t st) {
   plan.count = reinterpret_cast<int32_t *>(workspace);
   plan.moves = reinterpret_cast<Move *>(workspace + kHeader);
-  a.count = plan.count;
-  a.moves = plan.moves;
+  a.plan = plan;
   int64_t blocks = 0;
   for (int i = 0; i < a.n_parts; ++i) blocks += static_cast<int64_t>(a.part[i].tensors) * a.part[i].chunks;
   if (blocks == 0) return SOPHIA_OK;
   SOPHIA_REQUIRE(blocks <= 0x7fffffff, "%s: too much work for one call", what);
-  // Slots are large, and a thread each 16 bytes of them fills the chip; pages are small, and many.
+  const dim3 threads(kMoveThreads);
+  // Slots are large, and a thread for each 16 bytes of them fills the chip; pages are small, and many.
   a.workers = static_cast<int>(iclamp64((2048 + blocks - 1) / blocks, 1, plan.n));
-  hipLaunchKernelGGL(move_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, plan);
-  hipLaunchKernelGGL(move_kernel, dim3(static_cast<unsigned>(blocks), a.workers), dim3(kMoveThreads), 0, st, a);
+  if (plan.n <= kFew) {
+    hipLaunchKernelGGL(move_kernel<true>, dim3(static_cast<unsigned>(blocks), a.workers), threads, 0, st, a);
+    return check_launch(what);
+  }
+  if (plan.n <= 512)
+    hipLaunchKernelGGL((move_plan_kernel<512, 256>), dim3(1), dim3(256), 0, st, plan);
+  else
+    hipLaunchKernelGGL((move_plan_kernel<kMoves, 1024>), dim3(1), dim3(1024), 0, st, plan);
+  hipLaunchKernelGGL(move_kernel<false>, dim3(static_cast<unsigned>(blocks), a.workers), threads, 0, st, a);
   return check_launch(what);
 }
 
@@ -422,8 +554,7 @@ extern "C" int sophia_cache_fork(const int32_t *src, const int32_t *dst, const i
     a.part[a.n_parts++] = Part{kTable, at, 1, chunks(4ll * max_pages), table_stride * 4, 4ll * max_pages, 0};
     a.base[at++] = reinterpret_cast<char *>(table);
   }
-  a.shift = paged ? log2_of(page_size) : 0;
-  const PlanArgs plan{src, dst, n, n_slots, cached, table, table_stride, max_pages, a.shift, n_pages, nullptr, nullptr};
+  const PlanArgs plan{src, dst, n, n_slots, cached, table, table_stride, max_pages, paged ? log2_of(page_size) : 0, n_pages, nullptr, nullptr};
   return run_moves("cache_fork", plan, a, static_cast<char *>(workspace), static_cast<hipStream_t>(stream));
 }
 
