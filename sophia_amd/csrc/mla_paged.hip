@@ -31,11 +31,20 @@ struct PagedArgs {
   int64_t out_stride;
   float scale_log2;
   int heads, max_new;
-  int splits, range_keys;   // key ranges of a sequence at most, and keys of one
-  float *part;              // partials (splits > 1)
-  int64_t units;            // 32 (16) columns each: how many there is room for in a range's partials
-  int both;                 // narrow sequences are left to the narrow kernel
+  // Narrow: key ranges of a sequence at most, keys of one, and the partials [sequence][range] if there are several.
+  int narrow_blocks, narrow_splits, narrow_keys;
+  float *narrow_part;
+  // Wide: ranges of a sequence at most (a division of it into `wide_splits` > 0), and the partials, of four wavefronts each.
+  int wide_blocks, wide_used, wide_splits, part_cap;
+  float *wide_part;
 };
+constexpr int kLeast = 2;     // tiles of a wide range at least
+// Tiles of a range in shares of the whole work: with fewer more partials, with more the chip waits for the last
+// ones (8 sequences of 300 to 777 new tokens after up to 2,221: 1.0 110 us, 1.3 109, 1.6 101, 2.0 110, with the merge).
+constexpr float kStretch = 1.6f;
+// Work-groups that run at a time.
+template <int R>
+constexpr int kSlots = R <= 128 ? 512 : 256;
 
 template <int R, bool F32, bool NARROW>
 struct Form {
@@ -60,7 +69,7 @@ __device__ __forceinline__ f16v mfma32x32(const bf8 &a, const bf8 &b, const f16v
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-__device__ const u4 zero_chunk = {0u, 0u, 0u, 0u};   // what a key that is not there is read from
+__device__ const u4 zero_rows[64] = {};   // what keys that are not there are read from
 
 // Chunk c (16 bytes) of an LDS row lies at place c ^ turn(row): in bf16 eight rows of one chunk
 // (K) and four rows of two chunks (V, transposing reads), in fp32 sixteen rows of one chunk and
@@ -80,80 +89,151 @@ struct Work {
   Sequence q;
   int col0, cols;           // its first column, and the sequence's
   int first, last;          // tokens of its first and its last column
-  int keys;                 // that its last token sees
-  int k0, k1;               // its range
-  int split, used;
-  int64_t unit;             // of its first wavefront
+  int k0, k1;               // its keys
+  int used;                 // ranges of these columns
+  int64_t part;             // its partial; that of the next range is `step` on
+  int step;
 };
 
-__device__ __forceinline__ bool narrow_cols(const PagedArgs &a, int n, int cols) {
-  return n <= cols / a.heads;
+__device__ __forceinline__ bool narrow_cols(const PagedArgs &a, int n, int cols) { return a.narrow_blocks && n <= cols / a.heads; }
+
+// The columns from w.col0 on of sequence w.q (which is that of all of its rows; those past max_new
+// have no columns); returns the keys that their last token sees.
+__device__ __forceinline__ int columns(const PagedArgs &a, Work &w, int group) {
+  w.q.n = min(w.q.n, a.max_new);
+  w.cols = w.q.n * a.heads;
+  w.first = w.col0 / a.heads;
+  w.last = (min(w.col0 + group, w.cols) - 1) / a.heads;
+  return max(0, min(w.q.pos0 + w.last + 1, w.q.keys));
 }
 
-// The part of find() that both forms share: false if the range is behind the last.
-__device__ __forceinline__ bool range(const PagedArgs &a, Work &w, int group, int split) {
-  const int heads = a.heads;
-  w.cols = w.q.n * heads;
-  w.first = w.col0 / heads;
-  w.last = (min(w.col0 + group, w.cols) - 1) / heads;
-  w.keys = max(0, min(w.q.pos0 + w.last + 1, w.q.keys));
+// Narrow: work-group b has range b % splits of sequence b / splits.
+template <int R, bool F32>
+__device__ __forceinline__ bool find_narrow(const PagedArgs &a, Work &w, int s, int split) {
+  using F = Form<R, F32, true>;
+  w.q = sequence(a.p, s);
+  if (w.q.n == 0 || !narrow_cols(a, w.q.n, F::kCols)) return false;
+  w.col0 = 0;
+  const int keys = columns(a, w, F::kGroup);
   // (the last range has what max_len did not tell of)
-  w.used = max(1, min((w.keys + a.range_keys - 1) / a.range_keys, a.splits));
-  w.split = split;
-  w.k0 = split * a.range_keys;
-  w.k1 = split == a.splits - 1 ? w.keys : min(w.keys, w.k0 + a.range_keys);
+  w.used = max(1, min((keys + a.narrow_keys - 1) / a.narrow_keys, a.narrow_splits));
+  w.k0 = split * a.narrow_keys;
+  w.k1 = split == a.narrow_splits - 1 ? keys : min(keys, w.k0 + a.narrow_keys);
+  w.part = static_cast<int64_t>(s) * a.narrow_splits + split;
+  w.step = 1;
   return split < w.used;
 }
 
-// Narrow: work-group (split, sequence).  Wide: work-group b has split b % splits of group
-// (all - 1 - b / splits) of the list of all groups of all sequences, so that a sequence's last
-// tokens, which see most keys, come first.
-template <int R, bool F32, bool NARROW>
-__device__ __forceinline__ bool find(const PagedArgs &a, Work &w, int block, int split) {
-  using F = Form<R, F32, NARROW>;
-  if constexpr (NARROW) {
-    w.q = sequence(a.p, block);
-    if (w.q.n == 0 || !narrow_cols(a, w.q.n, F::kCols)) return false;
-    w.q.n = min(w.q.n, a.max_new);
-    w.col0 = 0;
-    w.unit = block;
-  } else {
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int s0 = 0;; s0 += 64) {
-      if (s0 >= a.p.n_seqs) return false;
-      const int s = min(s0 + lane, a.p.n_seqs - 1);
-      const int64_t base = iclamp64(a.p.cu[s], 0, a.p.rows);
-      const int n = static_cast<int>(iclamp64(imin64(a.p.cu[s + 1], a.p.rows) - base, 0, 1 << 29));
-      const bool mine = s == s0 + lane && !(a.both && narrow_cols(a, n, F::kCols));
-      const int groups = mine ? (min(n, a.max_new) * a.heads + F::kGroup - 1) / F::kGroup : 0;
-      const int sum = wave_scan(groups), all = __builtin_amdgcn_readlane(sum, 63);
-      if (block < before + all) {
-        const int at = __ffsll(static_cast<unsigned long long>(__ballot(block < before + sum))) - 1;
-        const int g = __builtin_amdgcn_readlane(groups, at);
-        // (late groups first)
-        const int in = block - before - (__builtin_amdgcn_readlane(sum, at) - g);
-        w.q = sequence(a.p, s0 + at);
-        w.q.n = min(w.q.n, a.max_new);
-        w.col0 = (g - 1 - in) * F::kGroup;
-        w.unit = 4 * static_cast<int64_t>(block);
-        break;
-      }
-      before += all;
-    }
+// Wide: a sequence per lane, 64 at a time.  The host does not know the lengths, so every work-group
+// finds its share in the list of all (sequence, range, group), which it counts itself.  Ranges are about
+// equally long, which follows from the whole work.
+template <int R, bool F32>
+struct Lanes {
+  using F = Form<R, F32, false>;
+  const PagedArgs &a;
+  int groups = 0, tiles = 0, fewest = 0;         // of this lane's sequence; tiles of its last group and of its first
+  int used = 0, items = 0, parts = 0;            // ranges, (range, group) items, those of them that are partials
+  __device__ __forceinline__ explicit Lanes(const PagedArgs &args) : a(args) {}
+  __device__ __forceinline__ void look(int s) {
+    const int in = min(s, a.p.n_seqs - 1);
+    const Sequence q = sequence(a.p, in);
+    const int n = s == in && !narrow_cols(a, q.n, F::kCols) ? min(q.n, a.max_new) : 0;
+    groups = (n * a.heads + F::kGroup - 1) / F::kGroup;
+    const auto tiles_to = [&](int token) { return (max(0, min(q.pos0 + token + 1, q.keys)) + kWideKeys - 1) / kWideKeys; };
+    tiles = tiles_to(n - 1);
+    fewest = tiles_to(0);
   }
-  // (positions are of all of a sequence's rows, also of those past max_new)
-  return range(a, w, F::kGroup, split);
+  __device__ __forceinline__ void divide(int length) {
+    const int least = a.wide_splits ? (tiles + a.wide_splits - 1) / a.wide_splits : max(length, (tiles + a.wide_used - 1) / a.wide_used);
+    used = tiles ? (tiles + least - 1) / least : 1;
+    items = used * groups;
+    parts = used > 1 ? items : 0;
+  }
+  // Tiles of a range at most.  With W = sum of groups x tiles, kSlots work-groups at a time have W / kSlots
+  // tiles each.  A sequence's last group has at most twice the tiles of its groups on average, so there are at most
+  // 2 W / length items and one more per group; those of sequences of two ranges or more, the partials, are
+  // at most 4 W / length.
+  __device__ __forceinline__ int range_tiles(int lane) {
+    float work = 0.f;
+    int all = 0;
+    for (int s0 = (a.p.n_seqs - 1) & ~63; s0 >= 0; s0 -= 64) {
+      look(s0 + lane);
+      work += 0.5f * static_cast<float>(groups) * static_cast<float>(tiles + fewest);
+      all += groups;
+    }
+    all = __builtin_amdgcn_readlane(wave_scan(all), 63);
+    work = row_sum16(work);
+    work += lane_xor16(work);
+    work = (work + lane_xor32(work)) * 1.0001f + 1.f;   // (not less than it is, by rounding)
+    return max(kLeast, static_cast<int>(fminf(ceilf(work * kStretch / static_cast<float>(kSlots<R>)), 1 << 29)));
+  }
+};
+
+// Up to 64 sequences' shares of the list, the longest ranges first, so that the last items are short ones: of place i
+// in this order the sequence, its groups, ranges and tiles, and items and partials up to and including it.
+struct Shares {
+  int seq[64], groups[64], used[64], tiles[64], items[64], parts[64];
+  int n, length;
+};
+
+// By one wavefront; the lanes have looked at the sequences from s0 on.
+template <int R, bool F32>
+__device__ __forceinline__ void share(Lanes<R, F32> &l, Shares &t, int s0, int length) {
+  const int lane = threadIdx.x & 63;
+  l.divide(length);
+  const bool real = l.groups > 0;
+  const int key = real ? (l.tiles + l.used - 1) / l.used << 6 | (63 - lane) : -1;
+  int place = 0;
+  for (uint64_t m = __ballot(real); m; m &= m - 1)
+    place += __builtin_amdgcn_readlane(key, __ffsll(static_cast<unsigned long long>(m)) - 1) > key;
+  t.groups[lane] = t.items[lane] = t.parts[lane] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  if (real) {
+    t.seq[place] = s0 + lane;
+    t.groups[place] = l.groups;
+    t.used[place] = l.used;
+    t.tiles[place] = l.tiles;
+    t.items[place] = l.items;
+    t.parts[place] = l.parts;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  const int items = wave_scan(t.items[lane]), parts = wave_scan(t.parts[lane]);
+  t.items[lane] = items;
+  t.parts[lane] = parts;
+  if (lane == 0) t.n = __popcll(__ballot(real));
 }
 
-// The lane's column `col` of a range: the result, or a partial.
+// Group g of place i, its range `split`; `parts` partials come before those of these 64 sequences.
+template <int R, bool F32>
+__device__ __forceinline__ bool take(const PagedArgs &a, const Shares &t, Work &w, int i, int g, int split, int parts) {
+  using F = Form<R, F32, false>;
+  const int groups = t.groups[i], used = t.used[i];
+  w.q = sequence(a.p, t.seq[i]);
+  w.col0 = (groups - 1 - g) * F::kGroup;     // (late groups, which see most keys, first)
+  const int keys = columns(a, w, F::kGroup), tiles = (keys + kWideKeys - 1) / kWideKeys;
+  const int least = max(1, (t.tiles[i] + used - 1) / used);
+  w.used = max(1, (tiles + least - 1) / least);
+  const int mine = tiles / w.used, more = tiles - mine * w.used;   // the first `more` ranges have one more
+  w.k0 = kWideKeys * (mine * split + min(split, more));
+  w.k1 = min(keys, w.k0 + kWideKeys * (mine + (split < more ? 1 : 0)));
+  w.part = parts + (i ? t.parts[i - 1] : 0) + split * groups + g;
+  w.step = groups;
+  return split < w.used && (w.used == 1 || w.part + static_cast<int64_t>(w.used - 1 - split) * groups < a.part_cap);   // (always, see range_tiles)
+}
+
+// The place of the first 64 whose sum is above `item`, by a wavefront.
+__device__ __forceinline__ int place_of(const int *sums, int item) {
+  return __ffsll(static_cast<unsigned long long>(__ballot(item < sums[threadIdx.x & 63]))) - 1;
+}
+
+// The lane's column `col` of a range: the result, or a partial at p.
 template <int R, bool F32, typename V, typename K>
-__device__ __forceinline__ void put(const PagedArgs &a, const Work &w, int64_t unit, int col, float m, float l, V value, K rank) {
+__device__ __forceinline__ void put(const PagedArgs &a, const Work &w, float *p, int col, float m, float l, V value, K rank) {
   constexpr int kQuads = F32 ? R / 16 : R / 8;
   const int lane = threadIdx.x & 63;
   if (w.used > 1) {
-    if (unit >= a.units) return;   // (there is always room, see plan())
-    float *p = a.part + (unit * a.splits + w.split) * kPart<R, F32>;
 #pragma unroll
     for (int j = 0; j < kQuads; ++j) reinterpret_cast<f4 *>(p)[64 * j + lane] = value(j);
     reinterpret_cast<f2 *>(p + 256 * kQuads)[lane] = f2{m, l};
@@ -175,22 +255,40 @@ struct Stage {
   const Work &w;
   int lane, row0;      // this wavefront's first row
   __device__ __forceinline__ Stage(const PagedArgs &args, const Work &work)
-      : a(args), w(work), lane(threadIdx.x & 63), row0(NARROW ? 0 : F::kOwn * static_cast<int>(threadIdx.x >> 6)) {}
-  // The page of key k0 + lane (of the tile's keys, lanes past them repeat), -1 if it is not there.
-  __device__ __forceinline__ int ids(int k0) const {
-    const int j = k0 + (lane & (F::kKeys - 1));
-    return j < w.k1 ? page_of(a.p, w.q.slot, j) : -1;
+      : a(args), w(work), lane(threadIdx.x & 63), row0(NARROW ? 0 : F::kOwn * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {}
+  // The page of key k0 + lane, as the table has it (k0 < k1; of the tile's keys, lanes past them repeat;
+  // past the last key its page), and whether it is one and the key is there: apart, so that nothing waits for the load.
+  __device__ __forceinline__ int load_id(int k0) const {
+    const int j = min(k0 + (lane & (F::kKeys - 1)), w.k1 - 1);
+    return a.p.table[w.q.slot * a.p.table_stride + (j >> a.p.shift)];
   }
+  __device__ __forceinline__ int id_of(int k0, int id) const {
+    return k0 + (lane & (F::kKeys - 1)) < w.k1 && id >= 0 && id < a.p.n_pages ? id : -1;
+  }
+  // Where the rows of a copy lie in one page, its address is a scalar and an offset per lane that does not
+  // change; else (small pages, the last keys) each lane has its own.
   __device__ __forceinline__ void copy(char *tile, int k0, int id) const {
+    constexpr int kRows = 64 / F::kChunks;    // of a copy
+    const bool whole = (1 << a.p.shift) >= kRows && k0 + F::kKeys <= w.k1;
 #pragma unroll
     for (int t = 0; t < F::kLoads; ++t) {
-      const int i = 64 * t + lane, row = row0 + i / F::kChunks, c = (i % F::kChunks) ^ (turn<F32>(row) & (F::kChunks - 1));
-      const int page = __shfl(id, row, 64);
-      const char *from = static_cast<const char *>(a.p.pages) +
-                         (page * a.p.page_stride * (F32 ? 4 : 2) +
-                          static_cast<int64_t>((k0 + row) & ((1 << a.p.shift) - 1)) * F::kBytes + 16 * c);
-      __builtin_amdgcn_global_load_lds(page >= 0 ? from : reinterpret_cast<const char *>(&zero_chunk),
-                                       tile + 16 * (row0 * F::kChunks + 64 * t), 16, 0, 0);
+      const int row = row0 + kRows * t, of = lane / F::kChunks;
+      const int c = (lane % F::kChunks) ^ (turn<F32>(row + of) & (F::kChunks - 1));
+      char *to = tile + 16 * (row0 * F::kChunks + 64 * t);
+      if (whole) {
+        const int page = __builtin_amdgcn_readlane(id, row);
+        const int at = (k0 + row) & ((1 << a.p.shift) - 1);
+        const char *from = static_cast<const char *>(a.p.pages) +
+                           (page * a.p.page_stride * (F32 ? 4 : 2) + static_cast<int64_t>(at) * F::kBytes);
+        from = page >= 0 ? from : reinterpret_cast<const char *>(zero_rows);
+        __builtin_amdgcn_global_load_lds(from + static_cast<uint32_t>(of * F::kBytes + 16 * c), to, 16, 0, 0);
+      } else {
+        const int page = __shfl(id, row + of, 64);
+        const int at = (k0 + row + of) & ((1 << a.p.shift) - 1);
+        const char *from = static_cast<const char *>(a.p.pages) +
+                           (page * a.p.page_stride * (F32 ? 4 : 2) + static_cast<int64_t>(at) * F::kBytes + 16 * c);
+        __builtin_amdgcn_global_load_lds(page >= 0 ? from : reinterpret_cast<const char *>(zero_rows), to, 16, 0, 0);
+      }
     }
   }
   // Chunks that hold a value that is not finite become zeros; returns the rows that had one, of
@@ -270,6 +368,13 @@ struct Bf16Columns {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
         st[kt] = mfma32x32(bits_to_bf8(*reinterpret_cast<const u4 *>(lds + ko[ks] + 32 * kt * F::kBytes)), qf[ks], st[kt]);
+    // (K rows ahead of their products)
+    __builtin_amdgcn_sched_group_barrier(0x100, 3 * KT, 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      __builtin_amdgcn_sched_group_barrier(0x8, KT, 0);
+      if (ks + 3 < KS) __builtin_amdgcn_sched_group_barrier(0x100, KT, 0);
+    }
     if (!all) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
@@ -327,14 +432,17 @@ struct Bf16Columns {
         pw[i] = pack_bf16x2(p0, p1);
         pr[i] = pack_bf16x2(p0 - __uint_as_float(pw[i] << 16), p1 - __uint_as_float(pw[i] & 0xffff0000u));
       }
+      bf8 vf[DT];
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const u2 lo = lds_read_tr(reinterpret_cast<const uint16_t *>(lds + vo[dt] + 16 * kp * F::kBytes));
         const u2 hi = lds_read_tr(reinterpret_cast<const uint16_t *>(lds + (vo[dt] ^ 16) + (16 * kp + 8) * F::kBytes));
-        const bf8 vf = bits_to_bf8(u4{lo.x, lo.y, hi.x, hi.y});
-        ot[dt] = mfma32x32(vf, bits_to_bf8(pw), ot[dt]);
-        ot[dt] = mfma32x32(vf, bits_to_bf8(pr), ot[dt]);
+        vf[dt] = bits_to_bf8(u4{lo.x, lo.y, hi.x, hi.y});
       }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) ot[dt] = mfma32x32(vf[dt], bits_to_bf8(pw), ot[dt]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) ot[dt] = mfma32x32(vf[dt], bits_to_bf8(pr), ot[dt]);
     }
   }
   __device__ __forceinline__ void finish(bool poison) {
@@ -464,14 +572,15 @@ __device__ __forceinline__ uint64_t seen_keys(uint64_t there, int pos, int k0) {
   return n >= 64 ? there : n <= 0 ? 0 : there & ((1ull << n) - 1);
 }
 
+// The tiles of the kernel: two of each kind, in objects of their own, so that the compiler knows that reads of the
+// one do not wait for copies into the other.
 template <int R, bool F32>
-__global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_wide_kernel(PagedArgs a) {
+constexpr int kTileBytes = 4 * Form<R, F32, true>::kTile > Form<R, F32, false>::kTile ? 4 * Form<R, F32, true>::kTile
+                                                                                       : Form<R, F32, false>::kTile;
+
+template <int R, bool F32>
+__device__ __forceinline__ void wide(const PagedArgs &a, const Work &w, char *tile0, char *tile1, uint64_t *s_bad) {
   using F = Form<R, F32, false>;
-  __shared__ __attribute__((aligned(1024))) char s_tile[2][F::kTile];
-  __shared__ uint64_t s_bad[4];
-  Work w;
-  const int splits = a.splits;
-  if (!find<R, F32, false>(a, w, blockIdx.x / splits, blockIdx.x % splits)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Stage<R, F32, false> stage(a, w);
   typename ColumnsOf<R, F32, false>::type c(a);
@@ -480,30 +589,34 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_wide_kernel(P
   const int wave_col = w.col0 + F::kCols * wave;
   const bool idle = wave_col >= w.cols;   // (of the whole wavefront)
   const int wave_last = w.q.pos0 + (min(wave_col + F::kCols, w.cols) - 1) / a.heads, wave_first = w.q.pos0 + wave_col / a.heads;
-  int id = stage.ids(w.k0);
-  uint64_t there = __ballot(id >= 0);
-  if (w.k0 < w.k1) stage.copy(s_tile[0], w.k0, id);
+  uint64_t there = 0;
+  int id = 0;
+  if (w.k0 < w.k1) {
+    id = stage.id_of(w.k0, stage.load_id(w.k0));
+    there = __ballot(id >= 0);
+    stage.copy(tile0, w.k0, id);
+    id = stage.load_id(w.k0 + F::kKeys);
+  }
   c.queries(w.q.base + token, in - token * a.heads);
-  if (w.k0 + F::kKeys < w.k1) id = stage.ids(w.k0 + F::kKeys);
   uint64_t poison = 0;
-  int buf = 0;
-  for (int k0 = w.k0; k0 < w.k1; k0 += F::kKeys, buf ^= 1) {
+  const auto step = [&](int k0, char *tile, char *next) {
     // This wavefront's copies, then the others'.  The next tile's go out only after that, into
     // the buffer that all have left.
-    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : "+v"(id)::"memory");
     __syncthreads();
     const uint64_t now = there;
     if (k0 + F::kKeys < w.k1) {
+      id = stage.id_of(k0 + F::kKeys, id);
       there = __ballot(id >= 0);
-      stage.copy(s_tile[buf ^ 1], k0 + F::kKeys, id);
-      if (k0 + 2 * F::kKeys < w.k1) id = stage.ids(k0 + 2 * F::kKeys);
+      stage.copy(next, k0 + F::kKeys, id);
     }
+    id = stage.load_id(k0 + 2 * F::kKeys);   // (of the last key's page past the end: no branch, which would wait for it)
     // A key that not every column sees would reach all of them through the products (0 times
     // infinity): it enters them as zeros where it is not finite, and the columns that do see it
     // end as NaN.
     uint64_t bad = 0;
     if (k0 + F::kKeys - 1 > w.q.pos0 + w.first && w.first != w.last) {
-      const uint64_t mine = stage.clean(s_tile[buf]);
+      const uint64_t mine = stage.clean(tile);
       if (lane == 0) s_bad[wave] = mine;
       lds_barrier();
       bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
@@ -511,24 +624,23 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_wide_kernel(P
     if (!idle && wave_last >= k0) {
       const uint64_t seen = seen_keys(now, pos, k0);
       poison |= bad & seen;
-      c.tile(s_tile[buf], now == ~0ull && wave_first >= k0 + F::kKeys - 1, seen);
+      c.tile(tile, now == ~0ull && wave_first >= k0 + F::kKeys - 1, seen);
     }
+  };
+  for (int k0 = w.k0; k0 < w.k1; k0 += 2 * F::kKeys) {
+    step(k0, tile0, tile1);
+    if (k0 + F::kKeys < w.k1) step(k0 + F::kKeys, tile1, tile0);
   }
   if (idle) return;
   c.finish(poison != 0);
-  put<R, F32>(a, w, w.unit + wave, col, c.m, c.l, [&](int j) { return c.quad(j); }, [&](int j) { return c.rank(j); });
+  put<R, F32>(a, w, a.wide_part + (4 * w.part + wave) * kPart<R, F32>, col, c.m, c.l, [&](int j) { return c.quad(j); },
+              [&](int j) { return c.rank(j); });
 }
 
 template <int R, bool F32>
-__global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_narrow_kernel(PagedArgs a) {
+__device__ __forceinline__ void narrow(const PagedArgs &a, const Work &w, char *tiles0, char *tiles1, f2 (*s_ml)[64]) {
   using F = Form<R, F32, true>;
   constexpr int kQuads = F::kQuads;
-  // Two tiles of each wavefront; then the wavefronts' sums.
-  __shared__ __attribute__((aligned(1024))) char s_tile[4][2][F::kTile];
-  __shared__ f2 s_ml[4][64];
-  static_assert(sizeof(s_tile) >= 4 * kQuads * 64 * sizeof(f4), "the sums fit the tiles");
-  Work w;
-  if (!find<R, F32, true>(a, w, blockIdx.y, blockIdx.x)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Stage<R, F32, true> stage(a, w);
   typename ColumnsOf<R, F32, true>::type c(a);
@@ -536,23 +648,27 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_narrow_kernel
   const int token = in / a.heads, pos = w.q.pos0 + token;
   constexpr uint64_t kAll = ~0ull >> (64 - F::kKeys);
   constexpr int kStep = 4 * F::kKeys;
+  char *const tile0 = tiles0 + wave * F::kTile, *const tile1 = tiles1 + wave * F::kTile;   // this wavefront's
   const int first = w.k0 + F::kKeys * wave;
-  int id = stage.ids(first);
-  uint64_t there = __ballot(id >= 0) & kAll;
-  if (first < w.k1) stage.copy(s_tile[wave][0], first, id);
+  uint64_t there = 0;
+  int id = 0;
+  if (first < w.k1) {
+    id = stage.id_of(first, stage.load_id(first));
+    there = __ballot(id >= 0) & kAll;
+    stage.copy(tile0, first, id);
+    id = stage.load_id(first + kStep);
+  }
   c.queries(w.q.base + token, in - token * a.heads);
-  if (first + kStep < w.k1) id = stage.ids(first + kStep);
   uint64_t poison = 0;
-  int buf = 0;
-  for (int k0 = first; k0 < w.k1; k0 += kStep, buf ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // (its own copies; nobody else reads them)
+  const auto step = [&](int k0, char *tile, char *next) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : "+v"(id)::"memory");   // (its own copies; nobody else reads them)
     const uint64_t now = there;
-    char *tile = s_tile[wave][buf];
     if (k0 + kStep < w.k1) {
+      id = stage.id_of(k0 + kStep, id);
       there = __ballot(id >= 0) & kAll;
-      stage.copy(s_tile[wave][buf ^ 1], k0 + kStep, id);
-      if (k0 + 2 * kStep < w.k1) id = stage.ids(k0 + 2 * kStep);
+      stage.copy(next, k0 + kStep, id);
     }
+    id = stage.load_id(k0 + 2 * kStep);
     const uint64_t seen = seen_keys(now, pos, k0);
     if (k0 + F::kKeys - 1 > w.q.pos0 && w.last != 0) {   // (as in the wide form)
       poison |= stage.clean(tile) & seen;
@@ -560,10 +676,13 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_narrow_kernel
       __builtin_amdgcn_wave_barrier();
     }
     c.tile(tile, now == kAll && w.q.pos0 >= k0 + F::kKeys - 1, seen);
+  };
+  for (int k0 = first; k0 < w.k1; k0 += 2 * kStep) {
+    step(k0, tile0, tile1);
+    if (k0 + kStep < w.k1) step(k0 + kStep, tile1, tile0);
   }
   c.finish(poison != 0);
   // The wavefronts' columns joined: each scaled to the common maximum, then summed four ranks a thread.
-  __syncthreads();
   s_ml[wave][lane] = f2{c.m, c.l};
   __syncthreads();
   float m = s_ml[0][lane].x;
@@ -576,10 +695,14 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_narrow_kernel
   float l = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) l = fmaf(s_ml[i][lane].y, weight(i), l);
-  f4 *sums = reinterpret_cast<f4 *>(&s_tile[0][0][0]);   // [wave][kQuads][64]
+  // Quad j of wavefront i: the even ones where tile 0 was, the odd ones where tile 1 was.
+  static_assert(4 * (kQuads / 2) * 64 * sizeof(f4) <= 4 * F::kTile, "the sums fit the tiles");
+  const auto sums = [&](int i, int j) {
+    return reinterpret_cast<f4 *>(j & 1 ? tiles1 : tiles0) + (i * (kQuads / 2) + (j >> 1)) * 64 + lane;
+  };
   const float own = weight(wave);
 #pragma unroll
-  for (int j = 0; j < kQuads; ++j) sums[(wave * kQuads + j) * 64 + lane] = c.quad(j) * own;
+  for (int j = 0; j < kQuads; ++j) *sums(wave, j) = c.quad(j) * own;
   __syncthreads();
   constexpr int kMine = (kQuads + 3) / 4;
   f4 v[kMine];
@@ -589,11 +712,10 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_narrow_kernel
     v[t] = f4{0.f, 0.f, 0.f, 0.f};
     if (j < kQuads)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[t] += sums[(i * kQuads + j) * 64 + lane];
+      for (int i = 0; i < 4; ++i) v[t] += *sums(i, j);
   }
   if (w.used > 1) {
-    if (w.unit >= a.units) return;
-    float *p = a.part + (w.unit * a.splits + w.split) * kPart<R, F32>;
+    float *p = a.narrow_part + w.part * kPart<R, F32>;
 #pragma unroll
     for (int t = 0; t < kMine; ++t)
       if (wave + 4 * t < kQuads) reinterpret_cast<f4 *>(p)[64 * (wave + 4 * t) + lane] = v[t];
@@ -608,29 +730,66 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_narrow_kernel
   }
 }
 
-// Joins the ranges of 32 (16) columns: a wavefront four ranks of each, the partials one after
-// the other, several loaded before the first is used.
-template <int R, bool F32, bool NARROW>
-__global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a) {
-  using F = Form<R, F32, NARROW>;
-  const int lane = threadIdx.x & 63, j = 4 * blockIdx.y + (threadIdx.x >> 6);
-  const int sub = NARROW ? 0 : blockIdx.x & 3;
+// The narrow work-groups first, as one of them may have a long chain of tiles.  The wide ones, as many as run at a
+// time, take their items in turn, so that each looks for them once.  WIDE, NARROW: which there are.
+template <int R, bool F32, bool WIDE, bool NARROW>
+__global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_kernel(PagedArgs a) {
+  constexpr int kBytes = NARROW ? kTileBytes<R, F32> : Form<R, F32, false>::kTile;
+  __shared__ __attribute__((aligned(1024))) char s_tile0[kBytes], s_tile1[kBytes];
   Work w;
-  if (!find<R, F32, NARROW>(a, w, NARROW ? blockIdx.x : blockIdx.x >> 2, 0)) return;
-  const int col = w.col0 + F::kCols * sub + (lane & (F::kCols - 1));
-  if (w.used == 1 || j >= F::kQuads || w.col0 + F::kCols * sub >= w.cols || w.unit + sub >= a.units) return;
-  const float *p = a.part + (w.unit + sub) * a.splits * kPart<R, F32>;
+  if (NARROW && static_cast<int>(blockIdx.x) < a.narrow_blocks) {
+    __shared__ f2 s_ml[4][64];
+    if (find_narrow<R, F32>(a, w, blockIdx.x / a.narrow_splits, blockIdx.x % a.narrow_splits))
+      narrow<R, F32>(a, w, s_tile0, s_tile1, s_ml);
+  } else if constexpr (WIDE) {
+    __shared__ uint64_t s_bad[4];
+    __shared__ Shares s_shares;
+    const int grid = gridDim.x - a.narrow_blocks;
+    int block = blockIdx.x - a.narrow_blocks, parts = 0;
+    for (int s0 = 0; s0 < a.p.n_seqs; s0 += 64) {
+      if (threadIdx.x < 64) {
+        Lanes<R, F32> l(a);
+        const int length = s0 == 0 ? l.range_tiles(threadIdx.x) : s_shares.length;
+        if (s0 > 0) l.look(s0 + threadIdx.x);
+        share(l, s_shares, s0, length);
+        if (threadIdx.x == 0) s_shares.length = length;
+      }
+      __syncthreads();
+      const int all = s_shares.items[63];
+      for (; block < all; block += grid) {
+        const int i = __builtin_amdgcn_readfirstlane(place_of(s_shares.items, block));
+        const int item = block - (i ? s_shares.items[i - 1] : 0), groups = s_shares.groups[i];
+        const int split = __builtin_amdgcn_readfirstlane(item / groups), g = __builtin_amdgcn_readfirstlane(item - split * groups);
+        if (take<R, F32>(a, s_shares, w, i, g, split, parts)) wide<R, F32>(a, w, s_tile0, s_tile1, s_bad);
+        __syncthreads();   // (the tiles are free)
+      }
+      block -= all;
+      parts += s_shares.parts[63];
+      __syncthreads();
+    }
+  }
+}
+
+// Joins the ranges of 32 (16) columns, the partials one after the other, several loaded before the first is
+// used.  Work-groups of narrow sequences first (if they have partials): a wavefront four ranks of each column;
+// then those of wide groups: a wavefront EACH times four ranks of its own columns.
+template <int R, bool F32, int QUADS>
+__device__ __forceinline__ void join(const PagedArgs &a, const Work &w, const float *p, int64_t step, int col, int j0) {
+  constexpr int kQuads = Form<R, F32, false>::kQuads, kAhead = 8 / QUADS;
+  const int lane = threadIdx.x & 63;
   float m = -INFINITY, l = 0.f;
-  f4 acc = {0.f, 0.f, 0.f, 0.f};
-  constexpr int kAhead = 8;
+  f4 acc[QUADS];
+#pragma unroll
+  for (int q = 0; q < QUADS; ++q) acc[q] = f4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < w.used; s0 += kAhead) {
     f2 ml[kAhead];
-    f4 v[kAhead];
+    f4 v[kAhead][QUADS];
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
-      const float *ps = p + static_cast<int64_t>(min(s0 + s, w.used - 1)) * kPart<R, F32>;   // the last one again, unused
-      ml[s] = reinterpret_cast<const f2 *>(ps + 256 * F::kQuads)[lane];
-      v[s] = reinterpret_cast<const f4 *>(ps)[64 * j + lane];
+      const float *ps = p + min(s0 + s, w.used - 1) * step;   // the last one again, unused
+      ml[s] = reinterpret_cast<const f2 *>(ps + 256 * kQuads)[lane];
+#pragma unroll
+      for (int q = 0; q < QUADS; ++q) v[s][q] = reinterpret_cast<const f4 *>(ps)[64 * (j0 + q) + lane];
     }
     float top = m;
 #pragma unroll
@@ -638,22 +797,61 @@ __global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a) {
     const float ref = top == -INFINITY ? 0.f : top;
     const float e0 = __builtin_amdgcn_exp2f(m - ref);
     l *= e0;
-    acc *= e0;
+#pragma unroll
+    for (int q = 0; q < QUADS; ++q) acc[q] *= e0;
 #pragma unroll
     for (int s = 0; s < kAhead; ++s)
       if (s0 + s < w.used) {
         const float e = __builtin_amdgcn_exp2f(ml[s].x - ref);
         l = fmaf(ml[s].y, e, l);
-        acc += v[s] * e;
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q) acc[q] += v[s][q] * e;
       }
     m = top;
   }
   if (col >= w.cols) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   const int token = col / a.heads, head = col - token * a.heads;
-  const int rank = F32 ? 16 * j + 4 * (lane >> 4) : 8 * j + 4 * (lane >> 5);
-  store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(head) * R + rank,
-         F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, acc * inv);
+#pragma unroll
+  for (int q = 0; q < QUADS; ++q)
+    store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(head) * R +
+                      (F32 ? 16 * (j0 + q) + 4 * (lane >> 4) : 8 * (j0 + q) + 4 * (lane >> 5)),
+           F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, acc[q] * inv);
+}
+
+template <int R, bool F32, int EACH>
+__global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a, int narrow_units) {
+  using F = Form<R, F32, false>;
+  constexpr int kEach = F::kQuads < EACH ? F::kQuads : EACH;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Work w;
+  int col = lane & (F::kCols - 1);
+  if (static_cast<int>(blockIdx.x) < narrow_units) {
+    const int j = 4 * blockIdx.y + wave;
+    if (j >= F::kQuads || !find_narrow<R, F32>(a, w, blockIdx.x, 0) || w.used == 1) return;
+    join<R, F32, 1>(a, w, a.narrow_part + w.part * kPart<R, F32>, kPart<R, F32>, col, j);
+  } else {
+    if (kEach * static_cast<int>(blockIdx.y) >= F::kQuads) return;
+    __shared__ Shares s_all[4];
+    Shares &t = s_all[wave];     // (each wavefront its own: no barrier)
+    Lanes<R, F32> l(a);
+    const int length = l.range_tiles(lane);
+    int group = blockIdx.x - narrow_units, parts = 0;
+    for (int s0 = 0; s0 < a.p.n_seqs; s0 += 64) {
+      if (s0 > 0) l.look(s0 + lane);
+      share(l, t, s0, length);
+      const int sum = wave_scan(t.groups[lane]), all = __builtin_amdgcn_readlane(sum, 63);
+      if (group < all) {
+        const int i = __ffsll(static_cast<unsigned long long>(__ballot(group < sum))) - 1;
+        const int g = group - (__builtin_amdgcn_readlane(sum, i) - t.groups[i]);
+        if (!take<R, F32>(a, t, w, i, g, 0, parts) || w.used == 1 || w.col0 + F::kCols * wave >= w.cols) return;
+        return join<R, F32, kEach>(a, w, a.wide_part + (4 * w.part + wave) * kPart<R, F32>, 4ll * w.step * kPart<R, F32>,
+                                   col + w.col0 + F::kCols * wave, kEach * blockIdx.y);
+      }
+      group -= all;
+      parts += t.parts[63];
+    }
+  }
 }
 
 // ---- norms ---------------------------------------------------------------------
@@ -745,74 +943,79 @@ int log2_of(int v) {
   return s;
 }
 
-// How the work is divided: which of the two kernels run, their groups and key ranges.
+// How the work is divided: which of the two forms there are, their groups and key ranges.
 struct Plan {
   bool narrow, wide;
-  int64_t wide_groups;      // at most
-  int narrow_splits, wide_splits, narrow_range, wide_range;
-  size_t narrow_bytes, wide_bytes;   // of their partials
+  int64_t wide_groups, wide_items, wide_parts;      // at most
+  int narrow_splits, narrow_keys, wide_used;
+  size_t narrow_bytes, wide_bytes;                  // of their partials
 };
 
 Plan plan(int n_seqs, int64_t rows, int max_new, int64_t max_len, int heads, int rank, int dtype, int splits) {
   const bool f32 = dtype == SOPHIA_DTYPE_F32;
   if (max_new > rows) max_new = static_cast<int>(rows);
   const int cols = f32 ? 16 : 32, group = 4 * cols;
-  const int64_t part = 64ll * (4 * (f32 ? rank / 16 : rank / 8) + 2) * 4;
+  const int64_t part = 64ll * (4 * (f32 ? rank / 16 : rank / 8) + 2) * 4, slots = rank <= 128 ? kSlots<128> : kSlots<256>;
   Plan p = {};
   p.wide = static_cast<int64_t>(max_new) * heads > cols;
   // (as many rows as sequences of max_new tokens have: there is no shorter one)
-  p.narrow = !p.wide || rows != static_cast<int64_t>(n_seqs) * max_new;
-  if (p.narrow && heads > cols) p.narrow = false;
+  p.narrow = !p.wide || (heads <= cols && rows != static_cast<int64_t>(n_seqs) * max_new);
   const int64_t keys = max_len < 1 ? 1 : max_len < 1 << 29 ? max_len : 1 << 29;
-  const auto divide = [&](int64_t groups, int64_t tile, int64_t slots, int &n, int &range) {
-    const int64_t tiles = (keys + tile - 1) / tile;
-    int64_t want = splits > 0 ? splits : (slots + groups - 1) / groups;
-    if (splits == 0 && want > 64) want = 64;
-    if (want > tiles) want = tiles;
-    if (want < 1) want = 1;
-    const int64_t each = (tiles + want - 1) / want;
-    n = static_cast<int>((tiles + each - 1) / each);
-    range = static_cast<int>(each * tile);
-  };
-  if (p.narrow) {
-    divide(n_seqs, 128, 1024, p.narrow_splits, p.narrow_range);
-    p.narrow_bytes = p.narrow_splits > 1 ? static_cast<size_t>(n_seqs) * p.narrow_splits * part : 0;
-  }
   if (p.wide) {
     const int64_t a = rows * heads / group + n_seqs, b = n_seqs * ((static_cast<int64_t>(max_new) * heads + group - 1) / group);
     p.wide_groups = a < b ? a : b;
     if (p.wide_groups < 1) p.wide_groups = 1;
-    divide(p.wide_groups, kWideKeys, 512, p.wide_splits, p.wide_range);
-    p.wide_bytes = p.wide_splits > 1 ? static_cast<size_t>(4 * p.wide_groups) * p.wide_splits * part : 0;
+    const int64_t tiles = (keys + kWideKeys - 1) / kWideKeys;
+    p.wide_used = static_cast<int>(splits > 0 ? imin64(splits, tiles) : imin64(1024, (tiles + kLeast - 1) / kLeast));
+    const int64_t most = p.wide_groups * p.wide_used;
+    p.wide_items = splits > 0 ? p.wide_groups * splits : imin64(most, p.wide_groups + 2 * slots);
+    p.wide_parts = splits > 0 ? p.wide_groups * splits : imin64(most, 4 * slots);
+    p.wide_bytes = (splits > 0 ? splits : p.wide_used) > 1 ? static_cast<size_t>(4 * p.wide_parts) * part : 0;
+    if (p.wide_bytes == 0) p.wide_parts = 0;
+  }
+  if (p.narrow) {
+    const int64_t tiles = (keys + 127) / 128;
+    // Beside wide groups that fill the chip a chain of tiles has time.
+    int64_t want = splits > 0 ? splits : p.wide && p.wide_groups >= slots ? 1 : (1024 + n_seqs - 1) / n_seqs;
+    if (splits == 0 && want > 64) want = 64;
+    want = iclamp64(want, 1, tiles);
+    const int64_t each = (tiles + want - 1) / want;
+    p.narrow_splits = static_cast<int>((tiles + each - 1) / each);
+    p.narrow_keys = static_cast<int>(128 * each);
+    p.narrow_bytes = p.narrow_splits > 1 ? static_cast<size_t>(n_seqs) * p.narrow_splits * part : 0;
   }
   return p;
 }
 
 template <int R, bool F32>
-int launch(PagedArgs a, const Plan &p, char *workspace, hipStream_t st) {
-  using W = Form<R, F32, false>;
-  a.both = p.narrow && p.wide;
-  if (p.wide) {
-    PagedArgs w = a;
-    w.splits = p.wide_splits;
-    w.range_keys = p.wide_range;
-    w.part = reinterpret_cast<float *>(workspace + p.narrow_bytes);
-    w.units = 4 * p.wide_groups;
-    hipLaunchKernelGGL((mla_paged_wide_kernel<R, F32>), dim3(static_cast<unsigned>(p.wide_groups * p.wide_splits)), dim3(256),
-                       0, st, w);
-    if (p.wide_splits > 1)
-      hipLaunchKernelGGL((mla_paged_merge_kernel<R, F32, false>),
-                         dim3(static_cast<unsigned>(4 * p.wide_groups), (W::kQuads + 3) / 4), dim3(256), 0, st, w);
-  }
+int launch(PagedArgs a, const Plan &p, int splits, char *workspace, hipStream_t st) {
   if (p.narrow) {
-    a.splits = p.narrow_splits;
-    a.range_keys = p.narrow_range;
-    a.part = reinterpret_cast<float *>(workspace);
-    a.units = a.p.n_seqs;
-    hipLaunchKernelGGL((mla_paged_narrow_kernel<R, F32>), dim3(p.narrow_splits, a.p.n_seqs), dim3(256), 0, st, a);
-    if (p.narrow_splits > 1)
-      hipLaunchKernelGGL((mla_paged_merge_kernel<R, F32, true>), dim3(a.p.n_seqs, (W::kQuads + 3) / 4), dim3(256), 0, st, a);
+    a.narrow_blocks = a.p.n_seqs * p.narrow_splits;
+    a.narrow_splits = p.narrow_splits;
+    a.narrow_keys = p.narrow_keys;
+    a.narrow_part = reinterpret_cast<float *>(workspace);
   }
+  if (p.wide) {
+    a.wide_blocks = static_cast<int>(p.wide_items);
+    a.wide_used = p.wide_bytes ? p.wide_used : 1;
+    a.wide_splits = splits;
+    a.part_cap = static_cast<int>(p.wide_parts);
+    a.wide_part = reinterpret_cast<float *>(workspace + p.narrow_bytes);
+  }
+  const dim3 grid(static_cast<unsigned>(a.narrow_blocks + a.wide_blocks));
+  if (p.narrow && p.wide) hipLaunchKernelGGL((mla_paged_kernel<R, F32, true, true>), grid, dim3(256), 0, st, a);
+  else if (p.wide) hipLaunchKernelGGL((mla_paged_kernel<R, F32, true, false>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((mla_paged_kernel<R, F32, false, true>), grid, dim3(256), 0, st, a);
+  const int narrow_units = p.narrow_bytes ? a.p.n_seqs : 0;
+  const int64_t units = narrow_units + (p.wide_bytes ? p.wide_groups : 0);
+  // Few groups: a work-group per quad, whose chain of ranges is short; many: four quads, as finding a group costs as
+  // much as joining it (520 groups: 19 us with one, 10 with four; 16 groups in fp32: 7 and 12).
+  constexpr int kQuads = Form<R, F32, false>::kQuads;
+  const unsigned x = static_cast<unsigned>(units);
+  if (p.wide_bytes && p.wide_groups < 256)
+    hipLaunchKernelGGL((mla_paged_merge_kernel<R, F32, 1>), dim3(x, kQuads), dim3(256), 0, st, a, narrow_units);
+  else if (units > 0)
+    hipLaunchKernelGGL((mla_paged_merge_kernel<R, F32, 4>), dim3(x, (kQuads + 3) / 4), dim3(256), 0, st, a, narrow_units);
   return check_launch("mla_paged_attn");
 }
 
@@ -874,16 +1077,16 @@ extern "C" int sophia_mla_paged_attn(const void *qa, int64_t qa_stride, int dtyp
   SOPHIA_REQUIRE(p.narrow_bytes + p.wide_bytes == 0 ||
                      (workspace && aligned16(workspace) && workspace_bytes >= p.narrow_bytes + p.wide_bytes),
                  "mla_paged_attn: workspace too small");
-  SOPHIA_REQUIRE(!p.wide || p.wide_groups * p.wide_splits <= 0x7fffffff / 4, "mla_paged_attn: too much work for one call");
+  SOPHIA_REQUIRE(p.wide_items <= 1 << 28 && 4 * p.wide_groups <= 1 << 28, "mla_paged_attn: too much work for one call");
   const PagedArgs a{{pages, page_stride, n_pages, log2_of(page_size), table, table_stride, table_rows, max_pages, slots,
                      cu_seqlens, kv_len, n_seqs, rows},
-                    qa, qa_stride, out, out_stride, scale * 1.44269504088896341f, heads, max_new, 1, 1, nullptr, 0, 0};
+                    qa, qa_stride, out, out_stride, scale * 1.44269504088896341f, heads, max_new, 0, 1, 1, nullptr, 0, 1, 0, 0, nullptr};
   char *ws = static_cast<char *>(workspace);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   switch (rank) {
 #define SOPHIA_MLA_PAGED(r) \
   case r:                   \
-    return dtype == SOPHIA_DTYPE_F32 ? launch<r, true>(a, p, ws, st) : launch<r, false>(a, p, ws, st);
+    return dtype == SOPHIA_DTYPE_F32 ? launch<r, true>(a, p, splits, ws, st) : launch<r, false>(a, p, splits, ws, st);
     SOPHIA_MLA_PAGED(32) SOPHIA_MLA_PAGED(64) SOPHIA_MLA_PAGED(128) SOPHIA_MLA_PAGED(256)
 #undef SOPHIA_MLA_PAGED
   }
