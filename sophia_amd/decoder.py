@@ -330,6 +330,8 @@ class SophiaMLA(nn.Module):
         npre = int(step["n_prefill_rows"])
         nd = n - npre
         h, d, r = self.num_heads, self.head_dim, self.kv_rank
+        if step.get("paged") is not None:
+            return self._forward_paged(x, step["paged"])
         cache = self.latent_cache
         # q_down, kv_down and output_gate in one GEMM; q_norm, kv_norm and the
         # latent-cache writes of every row in one kernel
@@ -380,6 +382,27 @@ class SophiaMLA(nn.Module):
                                       d ** -0.5, max_len=int(step["max_decode_len"]))   # [D, h, r]
             if self._latent_values(ctx, heads_kernel, out[npre:], gate if npre == 0 else None):
                 return self.o_proj(out.view(n, self.inner_dim))
+        return self._gate_out(x, out, gate)
+
+    def _forward_paged(self, x: torch.Tensor, paged: "PagedStep") -> torch.Tensor:
+        """``forward_mixed`` with the latents in pages: prefill and decode rows
+        alike are the last tokens of their sequences, whose latents are written to
+        their pages by the kernel of the norms and attended to from there, in latent
+        space, where scores and values of a key cost what its expanded K and V would
+        (rank and head_dim being alike) without expanding them."""
+        n, h, d = int(x.size(0)), self.num_heads, self.head_dim
+        pool, where = paged.pools[self], (paged.table, paged.cu_seqlens, paged.kv_len)
+        q_lat, latent, gate = self._project(x)
+        ops.mla_latent_norms_paged(q_lat, latent, self.q_norm.weight, self.q_norm.eps, self.kv_norm.weight, self.kv_norm.eps,
+                                   pool, *where, slots=paged.slots)
+        q = self.q_up(q_lat).view(n, h, d)
+        # (the head kernel reads the weights once per 16 rows: for a step's decode rows)
+        heads_kernel = n <= 512 and self._heads_kernel(q)
+        ctx = ops.mla_paged_attn(self._latent_queries(q, heads_kernel), pool, *where, d ** -0.5, max_new=paged.max_new,
+                                 max_len=paged.max_len, slots=paged.slots)
+        out = torch.empty((n, h, d), dtype=x.dtype, device=x.device)
+        if self._latent_values(ctx, heads_kernel, out, gate):
+            return self.o_proj(out.view(n, self.inner_dim))
         return self._gate_out(x, out, gate)
 
     def forward_tree(self, x: torch.Tensor, trees: "DraftTrees"):
@@ -576,6 +599,20 @@ class SophiaBlock(nn.Module):
             kept.append(keep)
             return out
         return self._mix(partial_block, completed_blocks, attn, pending, defer)
+
+
+@dataclass
+class PagedStep:
+    """Where a step's rows are in the pages (``runtime.PagedLatents``): the
+    arguments of ``ops.mla_paged_attn``, and each MLA layer's pool."""
+
+    pools: dict
+    table: torch.Tensor
+    slots: torch.Tensor
+    cu_seqlens: torch.Tensor
+    kv_len: torch.Tensor
+    max_new: int
+    max_len: int
 
 
 @dataclass
@@ -824,7 +861,7 @@ class Transformer(nn.Module):
                      decode_ids: torch.Tensor | None = None,
                      decode_slots: torch.Tensor | None = None,
                      decode_pos: torch.Tensor | None = None,
-                     max_decode_len: int = 0, all_logits: bool = False) -> torch.Tensor:
+                     max_decode_len: int = 0, all_logits: bool = False, pages=None) -> torch.Tensor:
         """One continuous-batching step over packed rows, which the reference
         cannot express (one start_pos per batch there, T > 1 only at
         start_pos 0, transformer.py:146-160).
@@ -845,6 +882,12 @@ class Transformer(nn.Module):
         [sum(prefill_lens) + D, vocab].  With equal lengths and no continuation
         nothing is copied from the host, so the step is capturable
         (MixedStepGraph); otherwise small index tensors are built on the host.
+
+        With ``pages`` (``runtime.PagedLatents``) the MLA layers keep their latents
+        there, and not in the slots' own caches: slot s's are in the pages of row s of
+        its table, which have to be reserved for the step's tokens before (a token
+        without a page is not attended to).  A step of decode rows is capturable then
+        too.
         """
         dev = self.tok_embeddings.weight.device
         lens = [int(t) for t in prefill_lens]
@@ -879,6 +922,11 @@ class Transformer(nn.Module):
                     prefill_slots=prefill_slots, reads_cache=reads, rectangular=rect,
                     decode_slots=decode_slots, decode_pos=decode_pos,
                     max_decode_len=int(max_decode_len), cu_prefill=None, cu_prefill_host=None)
+        if pages is not None:
+            most = max([p + t for p, t in zip(pos, lens)] + [int(max_decode_len) if D else 0])
+            if most > pages.max_len:
+                raise ValueError(f"sequence exceeds the {pages.max_len} tokens of a row of the page table")
+            step["paged"] = self._paged_step(pages, lens, pos, prefill_slots, decode_slots, decode_pos, D, most)
         if n_p and rect:
             T = lens[0]
             step["cu_prefill"] = torch.arange(0, (n_p + 1) * T, T, dtype=torch.int32, device=dev)
@@ -891,6 +939,10 @@ class Transformer(nn.Module):
             step["row_slot"] = prefill_slots.long()[seq_of_row]
             step["row_pos"] = torch.cat([torch.arange(p, p + t) for p, t in zip(pos, lens)]).to(dev)
             if reads:
+                new = [i for i in range(n_p) if pos[i] == 0]
+                if new:
+                    self.reset_slots(prefill_slots.long()[torch.tensor(new, device=dev)])
+            if reads and pages is None:
                 klens = [p + t for p, t in zip(pos, lens)]
                 cuk_host = torch.tensor([0] + list(itertools.accumulate(klens)), dtype=torch.int32)
                 step["cu_keys_host"] = cuk_host
@@ -898,9 +950,6 @@ class Transformer(nn.Module):
                 seq_of_key = torch.repeat_interleave(torch.arange(n_p), torch.tensor(klens)).to(dev)
                 step["key_slot"] = prefill_slots.long()[seq_of_key]
                 step["key_pos"] = torch.cat([torch.arange(kl) for kl in klens]).to(dev)
-                new = [i for i in range(n_p) if pos[i] == 0]
-                if new:
-                    self.reset_slots(prefill_slots.long()[torch.tensor(new, device=dev)])
             last_pre = (cu_host[1:].long() - 1).to(dev)
         ids = []
         if n_p:
@@ -924,6 +973,40 @@ class Transformer(nn.Module):
         last = torch.cat(parts) if len(parts) > 1 else parts[0]
         return self.output(self._final_mix(hidden[last], completed[last],
                                            None if pending is None else pending[last]))
+
+    def _paged_step(self, pages, lens, pos, prefill_slots, decode_slots, decode_pos, n_decode: int, most: int) -> PagedStep:
+        """Offsets and lengths of a step's sequences, prefills first."""
+        dev = self.tok_embeddings.weight.device
+        pages.ensure_slots(self.runtime_batch_capacity())
+        slots, kv_len, cu = [], [], []
+        rows = sum(lens)
+        if lens:
+            slots.append(prefill_slots.reshape(-1).int())
+            kv_len.append(torch.tensor([p + t for p, t in zip(pos, lens)], dtype=torch.int64).to(dev))
+            cu.append(torch.tensor([0] + list(itertools.accumulate(lens))[:-1], dtype=torch.int32).to(dev))
+        if n_decode:
+            slots.append(decode_slots.reshape(-1).int())
+            kv_len.append(decode_pos.reshape(-1).long() + 1)
+        cu.append(torch.arange(rows, rows + n_decode + 1, dtype=torch.int32, device=dev))
+        join = lambda t: (torch.cat(t) if len(t) > 1 else t[0]).contiguous()  # noqa: E731
+        return PagedStep(pages.pools, pages.table, join(slots), join(cu), join(kv_len), max(lens, default=1), most)
+
+    @torch.no_grad()
+    def fork_slots(self, src: torch.Tensor, dst: torch.Tensor, cached: torch.Tensor, *, pages=None) -> None:
+        """Slots dst[i] go on from slots src[i] (int32 [M], on the device), for all
+        i as if at once: the caches of all layers, in place and in one launch
+        (``ops.cache_fork``).  ``cached`` int64 [M]: tokens in the caches of src[i].
+        With ``pages`` the latents are those: dst[i] shares the pages that src[i] has
+        filled, and has the page that it has filled in part copied into its own,
+        reserved before (``runtime.PagedLatents.reserve``); without, they are the slots'
+        own.  Nothing is read back on the host, so a fork is capturable."""
+        kda = [(layer.attn.conv_history(), layer.attn.recurrent_state) for layer in self.layers if layer.layer_type == "kda"]
+        mla = [layer.attn for layer in self.layers if layer.layer_type == "mla"]
+        if pages is None:
+            ops.cache_fork(src, dst, kda=kda, mla=[m.latent_cache for m in mla], cached=cached)
+            return
+        pages.ensure_slots(self.runtime_batch_capacity())
+        ops.cache_fork(src, dst, kda=kda, pools=[pages.pools[m] for m in mla], table=pages.table if mla else None, cached=cached)
 
     @torch.no_grad()
     def forward_tree(self, trees: DraftTrees) -> DraftStep:

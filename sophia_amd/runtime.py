@@ -16,6 +16,9 @@ only at start_pos 0, runtime_host.py:146-170); here every step is one
 ``pack_trees`` and ``verify_trees`` are greedy decoding with drafted tokens: a
 server proposes a tree of continuations for each running sequence, one step runs
 all of them, and the longest part that the model itself says is kept.
+
+``PagedLatents`` keeps the MLA layers' latents in pages that sequences can share,
+and ``beam_search`` follows the best continuations of prompts in them.
 """
 
 from __future__ import annotations
@@ -25,7 +28,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops
-from .decoder import DraftTrees, Transformer
+from .decoder import DraftTrees, SophiaMLA, Transformer
 from .state import RuntimeCacheSnapshot
 
 
@@ -229,4 +232,231 @@ def verify_trees(model: Transformer, trees: DraftTrees, **controls) -> Verified:
     return Verified(path, n_path, next_token, trees.cached + n_path, logits)
 
 
-__all__ = ["RuntimeCacheState", "SlotAllocator", "Verified", "forward_cached_decode", "pack_trees", "verify_trees"]
+class PagedLatents:
+    """The latents of ``model``'s MLA layers in pages (host bookkeeping, and on the
+    device a pool [n_pages, page_size, kv_rank] per layer and one table).
+
+    A slot holds pages for its tokens, in order; a page may be held by several
+    slots.  ``reserve(slot, length)`` gives a slot pages of its own up to ``length``
+    tokens, ``share(src, dst, length)`` makes a slot go on from the first ``length``
+    tokens of another, ``release(slots)`` gives their pages back (a page is free
+    when its last holder is gone), ``compact()`` moves the held pages to the lowest
+    places of the pools.  ``Transformer.forward_step(pages=)`` writes and reads the
+    pages, ``Transformer.fork_slots(pages=)`` moves them between slots on the device:
+    the slots of such a fork may hold each other's pages afterwards, so they are
+    released together, and not compacted apart.
+
+    ``dtype``: of the pages, that of the model's activations (default: of its
+    embedding).  ``max_len``: tokens of a slot at most (default: max_seq_len)."""
+
+    def __init__(self, model: Transformer, n_pages: int, *, page_size: int = 64, max_len: int | None = None,
+                 dtype: torch.dtype | None = None) -> None:
+        n_pages, page_size = int(n_pages), int(page_size)
+        if n_pages < 1 or not 1 <= page_size <= 65536 or page_size & (page_size - 1):
+            raise ValueError(f"n_pages must be >= 1 and page_size a power of two up to 65536, got {n_pages} and {page_size}")
+        args = model.args
+        rank, q_rank = int(args.mla_kv_rank), int(args.mla_q_rank)
+        if rank not in (32, 64, 128, 256) or q_rank % 8 or q_rank + rank > 512:
+            raise ValueError("paged latents need mla_kv_rank 32, 64, 128 or 256 and mla_q_rank a multiple of 8, together at most 512")
+        weight = model.tok_embeddings.weight
+        self.device, self.page_size, self.n_pages = weight.device, page_size, n_pages
+        longest = int(args.max_seq_len) if max_len is None else int(max_len)
+        if longest < 1:
+            raise ValueError(f"max_len must be >= 1, got {longest}")
+        self._width = -(-longest // page_size)
+        self.max_len = self._width * page_size
+        dt = weight.dtype if dtype is None else dtype
+        self.pools = {m: torch.zeros(n_pages, page_size, rank, dtype=dt, device=self.device)
+                      for m in model.modules() if isinstance(m, SophiaMLA)}
+        self.table = torch.full((int(model.runtime_batch_capacity()), self._width), -1, dtype=torch.int32, device=self.device)
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._holders = [0] * n_pages
+        self._held: dict[int, dict[int, int]] = {}     # of a slot: place in its row -> page
+
+    @property
+    def pages_free(self) -> int:
+        return len(self._free)
+
+    def held(self, slot: int) -> list[int]:
+        """The pages of a slot, in the order of its tokens."""
+        return [p for _, p in sorted(self._held.get(int(slot), {}).items())]
+
+    def ensure_slots(self, n: int) -> None:
+        """Rows of the table for slots 0 .. n - 1 (the old ones stay valid, the table is a new tensor)."""
+        if int(n) > int(self.table.size(0)):
+            grown = self.table.new_full((int(n), self._width), -1)
+            grown[: self.table.size(0)].copy_(self.table)
+            self.table = grown
+
+    def _places(self, length: int) -> int:
+        length = int(length)
+        if not 0 <= length <= self.max_len:
+            raise ValueError(f"a slot holds at most {self.max_len} tokens, got {length}")
+        return -(-length // self.page_size)
+
+    def _set(self, slot: int, places: dict[int, int]) -> None:
+        if places:
+            at = torch.tensor(list(places), dtype=torch.int64).to(self.device)
+            self.table[slot, at] = torch.tensor(list(places.values()), dtype=torch.int32).to(self.device)
+            self._held.setdefault(slot, {}).update(places)
+
+    def reserve(self, slot: int, length: int, *, first: int = 0) -> None:
+        """Pages of its own for the tokens first .. length - 1 of ``slot``, where it
+        has none (all or nothing: RuntimeError where fewer are free).  ``first``: the
+        tokens before are to come from other slots (``fork_slots``)."""
+        slot = int(slot)
+        if slot < 0:
+            raise ValueError(f"slots are >= 0, got {slot}")
+        end, begin = self._places(length), min(int(first), int(length)) // self.page_size
+        if int(first) < 0:
+            raise ValueError(f"first must be >= 0, got {first}")
+        missing = [j for j in range(begin, end) if j not in self._held.get(slot, {})]
+        if len(missing) > len(self._free):
+            raise RuntimeError(f"{len(missing)} pages needed, {len(self._free)} free")
+        self.ensure_slots(slot + 1)
+        places = {}
+        for j in missing:
+            places[j] = self._free.pop()
+            self._holders[places[j]] = 1
+        self._set(slot, places)
+
+    def share(self, src: int, dst: int, length: int) -> None:
+        """Slot ``dst``, which holds no pages, goes on from the first ``length`` tokens of
+        ``src``: it holds the pages that these fill too, and a copy of the one that they fill
+        in part.  (The latents alone: KDA states are moved by ``fork_slots``, or are those of
+        a prompt's ``cache_dump`` at that length.)"""
+        src, dst, places = int(src), int(dst), self._places(length)
+        if self._held.get(dst):
+            raise ValueError(f"slot {dst} holds pages")
+        have = self._held.get(src, {})
+        if any(j not in have for j in range(places)):
+            raise ValueError(f"slot {src} holds fewer than {length} tokens")
+        full = int(length) // self.page_size
+        if places > full and not self._free:
+            raise RuntimeError("1 page needed, 0 free")
+        self.ensure_slots(dst + 1)
+        new = {j: have[j] for j in range(full)}
+        for p in new.values():
+            self._holders[p] += 1
+        if places > full:
+            new[full] = self._free.pop()
+            self._holders[new[full]] = 1
+            self._copy([have[full]], [new[full]])
+        self._set(dst, new)
+
+    def release(self, slots) -> None:
+        """Gives back what ``slots`` hold (each of them once)."""
+        values = [int(s) for s in (slots.tolist() if isinstance(slots, torch.Tensor) else slots)]
+        if len(set(values)) != len(values):
+            raise ValueError(f"slots released twice in one call: {sorted(values)}")
+        values = [s for s in values if s in self._held]
+        for s in values:
+            for p in self._held.pop(s).values():
+                self._holders[p] -= 1
+                if self._holders[p] == 0:
+                    self._free.append(p)
+        self._free.sort(reverse=True)
+        if values:
+            self.table.index_fill_(0, torch.tensor(values, dtype=torch.int64).to(self.device), -1)
+
+    def compact(self) -> int:
+        """Moves pages so that the held ones are the first of the pools, and names them anew
+        in all rows; returns how many are held.  Page ids read before are void."""
+        count = self.n_pages - len(self._free)
+        src = [p for p in range(count, self.n_pages) if self._holders[p]]
+        dst = [p for p in range(count) if not self._holders[p]]
+        if not src:
+            return count
+        self._copy(src, dst)
+        names = torch.arange(self.n_pages, dtype=torch.int32)
+        names[torch.tensor(src)] = torch.tensor(dst, dtype=torch.int32)
+        moved = dict(zip(src, dst))
+        names = names.to(self.device)
+        self.table.copy_(torch.where(self.table >= 0, names[self.table.clamp(min=0).long()], self.table))
+        for places in self._held.values():
+            for j, p in places.items():
+                places[j] = moved.get(p, p)
+        for s, d in moved.items():
+            self._holders[d], self._holders[s] = self._holders[s], 0
+        self._free = list(range(self.n_pages - 1, count - 1, -1))
+        return count
+
+    def _copy(self, src: list[int], dst: list[int]) -> None:
+        for i in range(0, len(src), ops.MOVES):      # (none of the places is a source)
+            pair = [torch.tensor(t[i:i + ops.MOVES], dtype=torch.int32).to(self.device) for t in (src, dst)]
+            ops.page_copy(*pair, list(self.pools.values()))
+
+
+@dataclass
+class Beams:
+    """The outcome of ``beam_search``, on the device, the best beam first: ``tokens``
+    int64 [N, beams, max_new] (``pad_token`` behind an end, -1 in beams that there
+    are not), ``scores`` fp32 [N, beams] (log probabilities; -inf: no such beam),
+    ``ended`` bool [N, beams] (by an end token)."""
+
+    tokens: torch.Tensor
+    scores: torch.Tensor
+    ended: torch.Tensor
+
+
+@torch.no_grad()
+def beam_search(model: Transformer, slots: SlotAllocator, pages: PagedLatents, prompts, *, beams: int, max_new: int,
+                end_token: int | None = None, pad_token: int = 0, adjust=None) -> Beams:
+    """The ``beams`` most probable continuations of each prompt that are found by going on
+    from the ``beams`` best at every token (``max_new`` of them, or up to ``end_token``).
+
+    ``prompts``: token lists (or 1-d tensors) of any lengths.  All beams of a prompt share
+    its pages; each has pages of its own for what it generates.  ``adjust(logits, tokens)``,
+    if given, returns the logits [rows, vocab] to choose by, for the tokens [rows, t] generated
+    so far (``ops.adjust_logits``).  The slots and pages that it takes are given back.  After the
+    prompts nothing is read back on the host."""
+    prompts = [[int(t) for t in (p.tolist() if isinstance(p, torch.Tensor) else p)] for p in prompts]
+    B, N, max_new = int(beams), len(prompts), int(max_new)
+    if N == 0 or any(not p for p in prompts):
+        raise ValueError("prompts must hold a token each at least")
+    if not 1 <= B <= ops.BEAMS or max_new < 1 or N * B > ops.MOVES:
+        raise ValueError(f"beams must be in [1, {ops.BEAMS}], max_new >= 1 and the beams of all prompts at most {ops.MOVES}")
+    lens = [len(p) for p in prompts]
+    longest = max(lens) + max_new - 1           # (the last token is chosen, and goes into no cache)
+    if longest > min(int(model.args.max_seq_len), pages.max_len):
+        raise ValueError("sequence exceeds max_seq_len")
+    dev = pages.device
+    taken = slots.allocate(N * B)
+    mine = [int(s) for s in taken.tolist()]
+    try:
+        for i, s in enumerate(mine):
+            n = lens[i // B]
+            pages.reserve(s, n + max_new - 1, first=0 if i % B == 0 else n)
+        own = taken.view(N, B)
+        at = torch.tensor(lens, dtype=torch.int64).to(dev).repeat_interleave(B)       # tokens in the caches of each beam
+        ids = torch.tensor([t for p in prompts for t in p], dtype=torch.int64).to(dev)
+        logits = model.forward_step(prefill_ids=ids, prefill_lens=lens, prefill_pos=[0] * N, prefill_slots=own[:, 0].contiguous(),
+                                    pages=pages)
+        history = torch.empty((N, 1, 0), dtype=torch.int64, device=dev)
+        scores, ended, width = torch.zeros(N, dtype=torch.float32, device=dev), None, 1
+        for t in range(max_new):
+            if adjust is not None:
+                logits = adjust(logits, history.reshape(N * width, t))
+            scores, parent, token = ops.beam_select(logits, scores.reshape(-1), width, keep=B, ended=ended, pad_token=pad_token)
+            kept = parent.long().clamp(min=0)
+            history = torch.cat([torch.gather(history, 1, kept[:, :, None].expand(N, B, t)), token[:, :, None]], 2)
+            was = torch.zeros((N, B), dtype=torch.bool, device=dev) if ended is None else torch.gather(ended.view(N, width), 1, kept)
+            done = was if end_token is None else was | (token == int(end_token))
+            history[:, :, t] = torch.where(was, int(pad_token), history[:, :, t])
+            ended, width = done.reshape(-1).contiguous(), B
+            if t + 1 == max_new:
+                break
+            src = torch.where(parent >= 0, torch.gather(own, 1, kept), -1).reshape(-1).contiguous()
+            model.fork_slots(src, taken, at, pages=pages)
+            logits = model.forward_step(decode_ids=token.clamp(min=0).reshape(-1), decode_slots=taken, decode_pos=at,
+                                        max_decode_len=longest, pages=pages)
+            at = at + 1
+        tokens = torch.where(torch.isinf(scores)[:, :, None], -1, history)
+        return Beams(tokens, scores, ended.view(N, B) & ~torch.isinf(scores))
+    finally:
+        pages.release(mine)
+        slots.release(mine)
+
+
+__all__ = ["Beams", "PagedLatents", "RuntimeCacheState", "SlotAllocator", "Verified", "beam_search", "forward_cached_decode",
+           "pack_trees", "verify_trees"]
