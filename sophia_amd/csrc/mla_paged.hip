@@ -7,7 +7,7 @@
 // are two tokens.  Two forms of one kernel:
 //   wide   : a work-group takes 4 x 32 columns (fp32: 4 x 16) and a range of their keys; its
 //            wavefronts share tiles of 64 keys and differ in their columns.
-//   narrow : a sequence of at most 32 (16) columns, so one token of it, or two: a work-group
+//   narrow : a sequence of at most 16 columns, so a token of 16 heads: a work-group
 //            takes a range of its keys, and the wavefronts differ in their keys, each with tiles
 //            of its own and no barrier until they join through LDS at the end.
 // A sequence of several ranges leaves partials, which a second kernel joins.
@@ -48,20 +48,23 @@ constexpr int kSlots = R <= 128 ? 512 : 256;
 
 template <int R, bool F32, bool NARROW>
 struct Form {
-  static constexpr int kCols = F32 ? 16 : 32;                     // of a wavefront
+  static constexpr bool k16 = F32 || NARROW;                      // 16 columns to a wavefront, in 16x16 products
+  static constexpr int kCols = k16 ? 16 : 32;
   static constexpr int kGroup = NARROW ? kCols : 4 * kCols;       // of a work-group
   static constexpr int kKeys = !NARROW ? kWideKeys : F32 && R == 256 ? 16 : 32;   // of a tile
   static constexpr int kBytes = R * (F32 ? 4 : 2);                // of a row
   static constexpr int kChunks = kBytes / 16;
   static constexpr int kTile = kKeys * kBytes;
-  static constexpr int kQuads = F32 ? R / 16 : R / 8;             // four ranks each, of a lane's column
+  static constexpr int kQuads = k16 ? R / 16 : R / 8;             // four ranks each, of a lane's column
+  static constexpr int kPart = 64 * (4 * kQuads + 2);             // floats of a wavefront's partial: [kQuads][64 lanes] times four,
+                                                                  // then maximum and sum [64 lanes]
+  static __device__ __forceinline__ int rank(int j) {             // the first of quad j's
+    const int lane = threadIdx.x & 63;
+    return k16 ? 16 * j + 4 * (lane >> 4) : 8 * j + 4 * (lane >> 5);
+  }
   static constexpr int kOwn = NARROW ? kKeys : kKeys / 4;         // rows that a wavefront stages
   static constexpr int kLoads = kOwn * kChunks / 64;
 };
-
-// Floats of a wavefront's partial: [kQuads][64 lanes] times four, then maximum and sum [64 lanes].
-template <int R, bool F32>
-constexpr int kPart = 64 * (4 * (F32 ? R / 16 : R / 8) + 2);
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ bf8 bits_to_bf8(const u4 &v) { return __builtin_bit_cast(bf8, v); }
@@ -107,7 +110,7 @@ __device__ __forceinline__ int columns(const PagedArgs &a, Work &w, int group) {
   return max(0, min(w.q.pos0 + w.last + 1, w.q.keys));
 }
 
-// Narrow: work-group b has range b % splits of sequence b / splits.
+// Narrow: range `split` of sequence s.
 template <int R, bool F32>
 __device__ __forceinline__ bool find_narrow(const PagedArgs &a, Work &w, int s, int split) {
   using F = Form<R, F32, true>;
@@ -137,7 +140,7 @@ struct Lanes {
   __device__ __forceinline__ void look(int s) {
     const int in = min(s, a.p.n_seqs - 1);
     const Sequence q = sequence(a.p, in);
-    const int n = s == in && !narrow_cols(a, q.n, F::kCols) ? min(q.n, a.max_new) : 0;
+    const int n = s == in && !narrow_cols(a, q.n, Form<R, F32, true>::kCols) ? min(q.n, a.max_new) : 0;
     groups = (n * a.heads + F::kGroup - 1) / F::kGroup;
     const auto tiles_to = [&](int token) { return (max(0, min(q.pos0 + token + 1, q.keys)) + kWideKeys - 1) / kWideKeys; };
     tiles = tiles_to(n - 1);
@@ -229,9 +232,10 @@ __device__ __forceinline__ int place_of(const int *sums, int item) {
 }
 
 // The lane's column `col` of a range: the result, or a partial at p.
-template <int R, bool F32, typename V, typename K>
-__device__ __forceinline__ void put(const PagedArgs &a, const Work &w, float *p, int col, float m, float l, V value, K rank) {
-  constexpr int kQuads = F32 ? R / 16 : R / 8;
+template <int R, bool F32, typename V>
+__device__ __forceinline__ void put(const PagedArgs &a, const Work &w, float *p, int col, float m, float l, V value) {
+  using F = Form<R, F32, false>;
+  constexpr int kQuads = F::kQuads;
   const int lane = threadIdx.x & 63;
   if (w.used > 1) {
 #pragma unroll
@@ -242,7 +246,7 @@ __device__ __forceinline__ void put(const PagedArgs &a, const Work &w, float *p,
     const int token = col / a.heads, head = col - token * a.heads;
 #pragma unroll
     for (int j = 0; j < kQuads; ++j)
-      store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(head) * R + rank(j),
+      store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(head) * R + F::rank(j),
              F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, value(j) * inv);
   }
 }
@@ -317,13 +321,13 @@ struct Stage {
   }
 };
 
-// The softmax and value product of a wavefront's columns: bf16 in 32x32x16 MFMAs.  A
+// The softmax and value product of a wavefront's columns: bf16 in 32x32x16 MFMAs (wide).  A
 // probability enters the value product as two bf16 numbers, the second what the first has
 // lost (2^-16 of it remains lost), so that outputs are as close as their own rounding;
 // scores, maxima and sums are fp32.
-template <int R, bool NARROW>
+template <int R>
 struct Bf16Columns {
-  using F = Form<R, false, NARROW>;
+  using F = Form<R, false, false>;
   static constexpr int KS = R / 16, DT = R / 32, KT = F::kKeys / 32;
   const PagedArgs &a;
   bf8 qf[KS];
@@ -455,7 +459,104 @@ struct Bf16Columns {
     const int i = 4 * (j & 3);
     return f4{v[i], v[i + 1], v[i + 2], v[i + 3]};
   }
-  __device__ __forceinline__ int rank(int j) const { return 8 * j + 4 * half; }
+};
+
+// The same for the 16 columns of the narrow form, 16x16x32 MFMAs over 32 keys: one token of 16 heads would leave
+// half of 32 columns empty (4,000 keys by one work-group 52 us with 32 columns, 47 with 16).
+template <int R>
+struct Bf16Narrow {
+  using F = Form<R, false, true>;
+  static constexpr int KS = R / 32, DT = R / 16;
+  static_assert(F::kKeys == 32, "two products of 16 keys");
+  const PagedArgs &a;
+  bf8 qf[KS];
+  f4 ot[DT];
+  float m, l;          // l over this lane's keys alone
+  int lane, grp, l16;
+  int ko[KS], vo[DT];
+  __device__ __forceinline__ explicit Bf16Narrow(const PagedArgs &args) : a(args), m(-INFINITY), l(0.f) {
+    lane = threadIdx.x & 63;
+    grp = lane >> 4;
+    l16 = lane & 15;
+    // K row l16 (16 rows on: a constant), chunk 4 ks + grp; V rows 4 grp + l16 / 4 (16 rows on: a constant).
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ko[ks] = place<R, false>(l16, 4 * ks + grp);
+#pragma unroll
+    for (int b = 0; b < DT; ++b) vo[b] = place<R, false>(4 * grp + (l16 >> 2), 2 * b + ((l16 & 3) >> 1)) + 8 * (l16 & 1);
+#pragma unroll
+    for (int b = 0; b < DT; ++b) ot[b] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ int column() const { return l16; }
+  __device__ __forceinline__ void queries(int64_t row, int head) {
+    const uint16_t *qp = static_cast<const uint16_t *>(a.qa) + row * a.qa_stride + static_cast<int64_t>(head) * R + 8 * grp;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = bits_to_bf8(*reinterpret_cast<const u4 *>(qp + 32 * ks));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+  }
+  __device__ __forceinline__ void tile(const char *lds, bool all, uint64_t seen) {
+    f4 st[2];   // score(key 16 kt + 4 grp + i, this column)
+    st[0] = st[1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+        st[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            bits_to_bf8(*reinterpret_cast<const u4 *>(lds + ko[ks] + 16 * kt * F::kBytes)), qf[ks], st[kt], 0, 0, 0);
+    if (!all) {
+      const uint32_t bits = static_cast<uint32_t>(seen) >> (4 * grp);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st[kt][i] = bits & (1u << (16 * kt + i)) ? st[kt][i] : -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
+                     fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
+    mx = fmaxf(mx, lane_xor16(mx));
+    mx = fmaxf(mx, lane_xor32(mx)) * a.scale_log2;
+    if (__any(mx > m + kSlack)) {   // (as in the wide form)
+      const float m_new = fmaxf(m, mx);
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int b = 0; b < DT; ++b) ot[b] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    u4 pw, pr;   // the probabilities rounded, and the rest
+    float ps = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[kt][2 * i], a.scale_log2, -ref));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[kt][2 * i + 1], a.scale_log2, -ref));
+        ps += p0 + p1;
+        const uint32_t w = pack_bf16x2(p0, p1);
+        pw[2 * kt + i] = w;
+        pr[2 * kt + i] = pack_bf16x2(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
+      }
+    l += ps;
+    // (the k index of lane group grp runs over keys 4 grp .. + 3 and 16 + 4 grp .. + 3, as the scores lie)
+    bf8 vf[DT];
+#pragma unroll
+    for (int b = 0; b < DT; ++b) {
+      const u2 lo = lds_read_tr(reinterpret_cast<const uint16_t *>(lds + vo[b]));
+      const u2 hi = lds_read_tr(reinterpret_cast<const uint16_t *>(lds + vo[b] + 16 * F::kBytes));
+      vf[b] = bits_to_bf8(u4{lo.x, lo.y, hi.x, hi.y});
+    }
+#pragma unroll
+    for (int b = 0; b < DT; ++b) ot[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[b], bits_to_bf8(pw), ot[b], 0, 0, 0);
+#pragma unroll
+    for (int b = 0; b < DT; ++b) ot[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[b], bits_to_bf8(pr), ot[b], 0, 0, 0);
+  }
+  __device__ __forceinline__ void finish(bool poison) {
+    l += lane_xor16(l);
+    l += lane_xor32(l);
+    if (poison) l = NAN;
+  }
+  // ot[b][i] = O[this column][rank 16 b + 4 grp + i] before the 1 / l
+  __device__ __forceinline__ f4 quad(int j) const { return ot[j]; }
 };
 
 // The same in fp32, 16x16x4 MFMAs: a lane's four consecutive ranks of a key are the A
@@ -554,12 +655,15 @@ struct F32Columns {
   }
   // ot[b][i] = O[this column][rank 16 b + 4 grp + i] before the 1 / l
   __device__ __forceinline__ f4 quad(int j) const { return ot[j]; }
-  __device__ __forceinline__ int rank(int j) const { return 16 * j + 4 * grp; }
 };
 
 template <int R, bool F32, bool NARROW>
 struct ColumnsOf {
-  using type = Bf16Columns<R, NARROW>;
+  using type = Bf16Columns<R>;
+};
+template <int R>
+struct ColumnsOf<R, false, true> {
+  using type = Bf16Narrow<R>;
 };
 template <int R, bool NARROW>
 struct ColumnsOf<R, true, NARROW> {
@@ -633,8 +737,7 @@ __device__ __forceinline__ void wide(const PagedArgs &a, const Work &w, char *ti
   }
   if (idle) return;
   c.finish(poison != 0);
-  put<R, F32>(a, w, a.wide_part + (4 * w.part + wave) * kPart<R, F32>, col, c.m, c.l, [&](int j) { return c.quad(j); },
-              [&](int j) { return c.rank(j); });
+  put<R, F32>(a, w, a.wide_part + (4 * w.part + wave) * F::kPart, col, c.m, c.l, [&](int j) { return c.quad(j); });
 }
 
 template <int R, bool F32>
@@ -715,7 +818,7 @@ __device__ __forceinline__ void narrow(const PagedArgs &a, const Work &w, char *
       for (int i = 0; i < 4; ++i) v[t] += *sums(i, j);
   }
   if (w.used > 1) {
-    float *p = a.narrow_part + w.part * kPart<R, F32>;
+    float *p = a.narrow_part + w.part * F::kPart;
 #pragma unroll
     for (int t = 0; t < kMine; ++t)
       if (wave + 4 * t < kQuads) reinterpret_cast<f4 *>(p)[64 * (wave + 4 * t) + lane] = v[t];
@@ -725,7 +828,7 @@ __device__ __forceinline__ void narrow(const PagedArgs &a, const Work &w, char *
 #pragma unroll
     for (int t = 0; t < kMine; ++t)
       if (wave + 4 * t < kQuads)
-        store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(in - token * a.heads) * R + c.rank(wave + 4 * t),
+        store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(in - token * a.heads) * R + F::rank(wave + 4 * t),
                F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, v[t] * inv);
   }
 }
@@ -739,7 +842,10 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_kernel(PagedA
   Work w;
   if (NARROW && static_cast<int>(blockIdx.x) < a.narrow_blocks) {
     __shared__ f2 s_ml[4][64];
-    if (find_narrow<R, F32>(a, w, blockIdx.x / a.narrow_splits, blockIdx.x % a.narrow_splits))
+    // (an odd number of work-groups per sequence: with 8 or 16 the first ranges, which all sequences have, would be on
+    // one XCD: 96 sequences 26 us in place of 18)
+    const int each = a.narrow_splits | 1;
+    if (find_narrow<R, F32>(a, w, blockIdx.x / each, blockIdx.x % each))
       narrow<R, F32>(a, w, s_tile0, s_tile1, s_ml);
   } else if constexpr (WIDE) {
     __shared__ uint64_t s_bad[4];
@@ -770,12 +876,13 @@ __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_kernel(PagedA
   }
 }
 
-// Joins the ranges of 32 (16) columns, the partials one after the other, several loaded before the first is
+// Joins the ranges of a wavefront's columns, the partials one after the other, several loaded before the first is
 // used.  Work-groups of narrow sequences first (if they have partials): a wavefront four ranks of each column;
 // then those of wide groups: a wavefront EACH times four ranks of its own columns.
-template <int R, bool F32, int QUADS>
+template <int R, bool F32, bool NARROW, int QUADS>
 __device__ __forceinline__ void join(const PagedArgs &a, const Work &w, const float *p, int64_t step, int col, int j0) {
-  constexpr int kQuads = Form<R, F32, false>::kQuads, kAhead = 8 / QUADS;
+  using F = Form<R, F32, NARROW>;
+  constexpr int kQuads = F::kQuads, kAhead = 8 / QUADS;
   const int lane = threadIdx.x & 63;
   float m = -INFINITY, l = 0.f;
   f4 acc[QUADS];
@@ -814,8 +921,7 @@ __device__ __forceinline__ void join(const PagedArgs &a, const Work &w, const fl
   const int token = col / a.heads, head = col - token * a.heads;
 #pragma unroll
   for (int q = 0; q < QUADS; ++q)
-    store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(head) * R +
-                      (F32 ? 16 * (j0 + q) + 4 * (lane >> 4) : 8 * (j0 + q) + 4 * (lane >> 5)),
+    store4(a.out, (w.q.base + token) * a.out_stride + static_cast<int64_t>(head) * R + F::rank(j0 + q),
            F32 ? SOPHIA_DTYPE_F32 : SOPHIA_DTYPE_BF16, acc[q] * inv);
 }
 
@@ -825,11 +931,11 @@ __global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a, int n
   constexpr int kEach = F::kQuads < EACH ? F::kQuads : EACH;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Work w;
-  int col = lane & (F::kCols - 1);
   if (static_cast<int>(blockIdx.x) < narrow_units) {
+    using N = Form<R, F32, true>;
     const int j = 4 * blockIdx.y + wave;
-    if (j >= F::kQuads || !find_narrow<R, F32>(a, w, blockIdx.x, 0) || w.used == 1) return;
-    join<R, F32, 1>(a, w, a.narrow_part + w.part * kPart<R, F32>, kPart<R, F32>, col, j);
+    if (j >= N::kQuads || !find_narrow<R, F32>(a, w, blockIdx.x, 0) || w.used == 1) return;
+    join<R, F32, true, 1>(a, w, a.narrow_part + w.part * N::kPart, N::kPart, lane & (N::kCols - 1), j);
   } else {
     if (kEach * static_cast<int>(blockIdx.y) >= F::kQuads) return;
     __shared__ Shares s_all[4];
@@ -845,8 +951,8 @@ __global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a, int n
         const int i = __ffsll(static_cast<unsigned long long>(__ballot(group < sum))) - 1;
         const int g = group - (__builtin_amdgcn_readlane(sum, i) - t.groups[i]);
         if (!take<R, F32>(a, t, w, i, g, 0, parts) || w.used == 1 || w.col0 + F::kCols * wave >= w.cols) return;
-        return join<R, F32, kEach>(a, w, a.wide_part + (4 * w.part + wave) * kPart<R, F32>, 4ll * w.step * kPart<R, F32>,
-                                   col + w.col0 + F::kCols * wave, kEach * blockIdx.y);
+        return join<R, F32, false, kEach>(a, w, a.wide_part + (4 * w.part + wave) * F::kPart, 4ll * w.step * F::kPart,
+                                          (lane & (F::kCols - 1)) + w.col0 + F::kCols * wave, kEach * blockIdx.y);
       }
       group -= all;
       parts += t.parts[63];
@@ -954,8 +1060,9 @@ struct Plan {
 Plan plan(int n_seqs, int64_t rows, int max_new, int64_t max_len, int heads, int rank, int dtype, int splits) {
   const bool f32 = dtype == SOPHIA_DTYPE_F32;
   if (max_new > rows) max_new = static_cast<int>(rows);
-  const int cols = f32 ? 16 : 32, group = 4 * cols;
-  const int64_t part = 64ll * (4 * (f32 ? rank / 16 : rank / 8) + 2) * 4, slots = rank <= 128 ? kSlots<128> : kSlots<256>;
+  const int cols = 16, group = f32 ? 64 : 128;
+  const int64_t part = 64ll * (4 * (f32 ? rank / 16 : rank / 8) + 2) * 4, narrow_part = 64ll * (4 * (rank / 16) + 2) * 4;
+  const int64_t slots = rank <= 128 ? kSlots<128> : kSlots<256>;
   Plan p = {};
   p.wide = static_cast<int64_t>(max_new) * heads > cols;
   // (as many rows as sequences of max_new tokens have: there is no shorter one)
@@ -975,14 +1082,16 @@ Plan plan(int n_seqs, int64_t rows, int max_new, int64_t max_len, int heads, int
   }
   if (p.narrow) {
     const int64_t tiles = (keys + 127) / 128;
-    // Beside wide groups that fill the chip a chain of tiles has time.
-    int64_t want = splits > 0 ? splits : p.wide && p.wide_groups >= slots ? 1 : (1024 + n_seqs - 1) / n_seqs;
-    if (splits == 0 && want > 64) want = 64;
+    // Beside wide groups that fill the chip a chain of tiles has time.  Else ranges to about 768 work-groups, were all
+    // sequences as long as the longest, and 16 at most: more cost the merge what they save.  us in 1, 4, 8, 16 and 32
+    // ranges: one sequence of 4,000 keys 47, 18, 13.0, 11.5, 12.3; of 700 12.4, 10.2, 9.0 (six); 32 of 200 to 4,000 46,
+    // 18.8, 14.9, 13.4, 16.4; 96 of them 48, 22.6, 17.7, 21.5, 28.8; 200 of up to 3,400 40, 23.8, 25.2, 28.5, 38.9.
+    int64_t want = splits > 0 ? splits : p.wide && p.wide_groups >= slots ? 1 : imin64(16, (768 + n_seqs - 1) / n_seqs);
     want = iclamp64(want, 1, tiles);
     const int64_t each = (tiles + want - 1) / want;
     p.narrow_splits = static_cast<int>((tiles + each - 1) / each);
     p.narrow_keys = static_cast<int>(128 * each);
-    p.narrow_bytes = p.narrow_splits > 1 ? static_cast<size_t>(n_seqs) * p.narrow_splits * part : 0;
+    p.narrow_bytes = p.narrow_splits > 1 ? static_cast<size_t>(n_seqs) * p.narrow_splits * narrow_part : 0;
   }
   return p;
 }
@@ -990,7 +1099,7 @@ Plan plan(int n_seqs, int64_t rows, int max_new, int64_t max_len, int heads, int
 template <int R, bool F32>
 int launch(PagedArgs a, const Plan &p, int splits, char *workspace, hipStream_t st) {
   if (p.narrow) {
-    a.narrow_blocks = a.p.n_seqs * p.narrow_splits;
+    a.narrow_blocks = a.p.n_seqs * (p.narrow_splits | 1);
     a.narrow_splits = p.narrow_splits;
     a.narrow_keys = p.narrow_keys;
     a.narrow_part = reinterpret_cast<float *>(workspace);

@@ -16,7 +16,10 @@ FlashKDA seam (sm120_concurrent_ffn.py:375-423), so they drop into
 
 from __future__ import annotations
 
+import array
 import ctypes
+import functools
+
 import torch
 
 from . import _native as nat
@@ -1639,8 +1642,8 @@ def _on_device(index: int, device, *named) -> None:
 def _launch(device, fn, *args) -> int:
     """``fn(*args, stream)`` with ``device`` as the current one (a stream handle
     alone does not name it)."""
-    if device.index == torch.cuda.current_device():
-        return fn(*args, nat.stream_handle(device))
+    if device.index == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
     with torch.cuda.device(device):
         return fn(*args, nat.stream_handle(device))
 
@@ -2093,31 +2096,51 @@ def _page_pool(pages: torch.Tensor, name: str) -> tuple[int, int, int, int]:
     if not isinstance(pages, torch.Tensor) or pages.dim() != 3:
         raise RuntimeError(f"{name} must be [n_pages, page_size, rank]")
     n, size, rank = pages.shape
-    if (rank > 1 and pages.stride(2) != 1) or (size > 1 and pages.stride(1) != rank):
+    page, row, col = pages.stride()
+    if (rank > 1 and col != 1) or (size > 1 and row != rank):
         raise RuntimeError(f"{name} must be [n_pages, page_size, rank] with dense pages")
-    return n, size, rank, pages.stride(0) if n > 1 else size * rank
+    return n, size, rank, page if n > 1 else size * rank
 
 
-def _page_table(table: torch.Tensor, device) -> tuple[int, int, int]:
+def _page_table(table: torch.Tensor, index: int, device) -> tuple[int, int, int]:
     """(rows, pages of a row, row stride) of a page table."""
-    if table.dim() != 2 or table.dtype != torch.int32 or table.device != device or (table.size(1) > 1 and table.stride(1) != 1):
+    if table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != index:
         raise RuntimeError(f"table must be int32 [slots, max_pages] with dense rows on {device}")
-    return table.size(0), table.size(1), table.stride(0) if table.size(0) > 1 else table.size(1)
+    rows, width = table.shape
+    stride, col = table.stride()
+    if width > 1 and col != 1:
+        raise RuntimeError(f"table must be int32 [slots, max_pages] with dense rows on {device}")
+    return rows, width, stride if rows > 1 else width
 
 
-def _new_tokens(cu_seqlens: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor | None, table_rows: int, device) -> int:
+def _new_tokens(cu_seqlens: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor | None, table_rows: int, index: int,
+                device) -> int:
     """Checks the offsets, lengths and slots of sequences; returns their number."""
-    cu = _int32(cu_seqlens, "cu_seqlens", device)
-    if cu is None or cu.dim() != 1 or cu.numel() < 1:
+    n = cu_seqlens.numel() - 1
+    if (cu_seqlens.dtype is not torch.int32 or cu_seqlens.get_device() != index or not cu_seqlens.is_contiguous()
+            or cu_seqlens.dim() != 1 or n < 0):
+        _int32(cu_seqlens, "cu_seqlens", device)
         raise RuntimeError("cu_seqlens must hold one offset per sequence and the end of the last")
-    n = cu.numel() - 1
-    _int64(kv_len, "kv_len", n, device)
-    if _int32(slots, "slots", device) is None:
+    if kv_len.dtype is not torch.int64 or kv_len.get_device() != index or not kv_len.is_contiguous() or kv_len.numel() != n:
+        _int64(kv_len, "kv_len", n, device)
+    if slots is None:
         if table_rows < n:
             raise RuntimeError("the table has fewer rows than there are sequences")
-    elif slots.numel() != n:
+    elif slots.dtype is not torch.int32 or slots.get_device() != index or not slots.is_contiguous() or slots.numel() != n:
+        _int32(slots, "slots", device)
         raise RuntimeError(f"slots must hold {n} entries, got {slots.numel()}")
     return n
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_workspace(*sizes: int) -> int:
+    """Bytes that ``mla_paged_attn`` takes for partials, by sizes alone."""
+    return nat.lib().sophia_mla_paged_workspace_size(*sizes)
+
+
+@functools.lru_cache(maxsize=256)
+def _beam_workspace(*sizes: int) -> int:
+    return nat.lib().sophia_beam_select_workspace_size(*sizes)
 
 
 def mla_paged_attn(qa: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tensor, kv_len: torch.Tensor,
@@ -2145,22 +2168,24 @@ def mla_paged_attn(qa: torch.Tensor, pages: torch.Tensor, table: torch.Tensor, c
     _gpu(qa, "qa")
     if qa.dim() != 3:
         raise RuntimeError(f"qa must be [rows, heads, rank], got {tuple(qa.shape)}")
-    device = qa.device
+    device, dtype, index = qa.device, qa.dtype, qa.get_device()
     rows, heads, rank = qa.shape
-    _on_device(qa.get_device(), device, (pages, "pages"), (out, "out"))
-    qs = _heads_rows(qa, "qa", heads, rank)
+    row, head, col = qa.stride()
+    if (heads > 1 and head != rank) or col != 1:
+        raise RuntimeError("qa must have dense [heads, dim] rows")
+    qs = row if rows > 1 else heads * rank
+    _on_device(index, device, (pages, "pages"), (out, "out"))
     n_pages, size, width, page_stride = _page_pool(pages, "pages")
-    if width != rank or pages.dtype != qa.dtype:
+    if width != rank or pages.dtype is not dtype:
         raise RuntimeError(f"pages must hold latents of rank {rank} in qa's dtype")
-    table_rows, max_pages, table_stride = _page_table(table, device)
-    n = _new_tokens(cu_seqlens, kv_len, slots, table_rows, device)
-    y, os_ = _heads_out(out, rows, heads, rank, qa.dtype, device)
+    table_rows, max_pages, table_stride = _page_table(table, index, device)
+    n = _new_tokens(cu_seqlens, kv_len, slots, table_rows, index, device)
+    y, os_ = _heads_out(out, rows, heads, rank, dtype, device)
     bound = max_pages * size if max_len is None else max(0, min(int(max_len), max_pages * size))
-    code = nat.dtype_code(qa.dtype)
-    lib = nat.lib()
-    ws_bytes = lib.sophia_mla_paged_workspace_size(n, rows, int(max_new), bound, heads, rank, code, int(splits))
+    code = nat.dtype_code(dtype)
+    ws_bytes = _paged_workspace(n, rows, int(max_new), bound, heads, rank, code, int(splits))
     ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
-    rc = _launch(device, lib.sophia_mla_paged_attn, qa.data_ptr(), qs, code, pages.data_ptr(), page_stride, n_pages, size,
+    rc = _launch(device, nat.lib().sophia_mla_paged_attn, qa.data_ptr(), qs, code, pages.data_ptr(), page_stride, n_pages, size,
                  table.data_ptr(), table_stride, table_rows, max_pages, nat.ptr(slots), cu_seqlens.data_ptr(),
                  kv_len.data_ptr(), n, rows, int(max_new), bound, float(scale), y.data_ptr(), os_, heads, rank, int(splits),
                  nat.ptr(ws), ws_bytes)
@@ -2182,26 +2207,27 @@ def mla_latent_norms_paged(q_lat: torch.Tensor, kv_lat: torch.Tensor, q_norm_wei
     Positions without a page, or before 0, are written nowhere; rows of no sequence
     are normalised all the same.  The fp32 weights are rounded to the rows' dtype."""
     _gpu(q_lat, "q_lat")
-    _gpu(kv_lat, "kv_lat")
-    device = q_lat.device
-    if q_lat.dim() != 2 or kv_lat.dim() != 2 or kv_lat.size(0) != q_lat.size(0) or q_lat.dtype != kv_lat.dtype:
+    device, dtype, index = q_lat.device, q_lat.dtype, q_lat.get_device()
+    _on_device(index, device, (kv_lat, "kv_lat"), (pages, "pages"))
+    if q_lat.dim() != 2 or kv_lat.dim() != 2 or kv_lat.dtype is not dtype:
         raise RuntimeError("q_lat and kv_lat must be [rows, rank] of one dtype")
     rows, q_rank = q_lat.shape
-    kv_rank = kv_lat.size(1)
-    _on_device(q_lat.get_device(), device, (kv_lat, "kv_lat"), (pages, "pages"))
+    kv_rows, kv_rank = kv_lat.shape
+    if kv_rows != rows:
+        raise RuntimeError("q_lat and kv_lat must be [rows, rank] of one dtype")
     qs, ks = _rows(q_lat, "q_lat", q_rank), _rows(kv_lat, "kv_lat", kv_rank)
     n_pages, size, width, page_stride = _page_pool(pages, "pages")
-    if width != kv_rank or pages.dtype != kv_lat.dtype:
+    if width != kv_rank or pages.dtype is not dtype:
         raise RuntimeError(f"pages must hold latents of rank {kv_rank} in the rows' dtype")
-    table_rows, max_pages, table_stride = _page_table(table, device)
-    n = _new_tokens(cu_seqlens, kv_len, slots, table_rows, device)
+    table_rows, max_pages, table_stride = _page_table(table, index, device)
+    n = _new_tokens(cu_seqlens, kv_len, slots, table_rows, index, device)
     weights = []
     for t, width, name in ((q_norm_weight, q_rank, "q_norm_weight"), (kv_norm_weight, kv_rank, "kv_norm_weight")):
         weights.append(_f32_values(t, device))
         if weights[-1].numel() != width:
             raise RuntimeError(f"{name} must hold {width} values")
     rc = _launch(device, nat.lib().sophia_mla_latent_norms_paged, q_lat.data_ptr(), qs, kv_lat.data_ptr(), ks, rows, q_rank,
-                 kv_rank, nat.dtype_code(q_lat.dtype), weights[0].data_ptr(), float(q_eps), weights[1].data_ptr(),
+                 kv_rank, nat.dtype_code(dtype), weights[0].data_ptr(), float(q_eps), weights[1].data_ptr(),
                  float(kv_eps), pages.data_ptr(), page_stride, n_pages, size, table.data_ptr(), table_stride, table_rows,
                  max_pages, nat.ptr(slots), cu_seqlens.data_ptr(), kv_len.data_ptr(), n)
     nat.check(rc, "sophia_mla_latent_norms_paged")
@@ -2238,14 +2264,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, *, keep:
         raise RuntimeError(f"scores must be contiguous fp32 of {rows} entries")
     if ended is not None and (ended.dtype != torch.bool or not ended.is_contiguous() or ended.numel() != rows):
         raise RuntimeError(f"ended must be contiguous bool of {rows} entries")
-    lib = nat.lib()
     groups = rows // beams
-    nbytes = lib.sophia_beam_select_workspace_size(rows, vocab, keep)
+    nbytes = _beam_workspace(rows, vocab, keep)
     score = torch.empty((groups, keep), dtype=torch.float32, device=device)
     parent = torch.empty((groups, keep), dtype=torch.int32, device=device)
     token = torch.empty((groups, keep), dtype=torch.int64, device=device)
     ws = torch.empty(-(-nbytes // 8), dtype=torch.int64, device=device)
-    rc = _launch(device, lib.sophia_beam_select, logits.data_ptr(), xs, nat.dtype_code(logits.dtype), rows, vocab,
+    rc = _launch(device, nat.lib().sophia_beam_select, logits.data_ptr(), xs, nat.dtype_code(logits.dtype), rows, vocab,
                  scores.data_ptr(), nat.ptr(ended), int(pad_token), beams, keep, score.data_ptr(), parent.data_ptr(),
                  token.data_ptr(), ws.data_ptr(), nbytes)
     nat.check(rc, "sophia_beam_select")
@@ -2273,8 +2298,9 @@ def _pools(pools, index: int, device) -> tuple[int, int, int, int]:
     return what
 
 
-def _addresses(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors]) if tensors else None
+def _addresses(tensors) -> array.array:
+    """The tensors' addresses as the library reads a list of them (which has to live until it has)."""
+    return array.array("q", [t.data_ptr() for t in tensors])
 
 
 def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=(), table: torch.Tensor | None = None,
@@ -2336,7 +2362,7 @@ def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=()
     if pools and table is None:
         raise RuntimeError("pools need their table")
     if table is not None:
-        table_rows, max_pages, table_stride = _page_table(table, device)
+        table_rows, max_pages, table_stride = _page_table(table, index, device)
         if not pools:
             raise RuntimeError("a table needs its pools")
         n_pages, size, width, page_stride = _pools(pools, index, device)
@@ -2356,9 +2382,10 @@ def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=()
     lib = nat.lib()
     nbytes = lib.sophia_move_workspace_size(n)
     ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device) if nbytes else None
-    rc = _launch(device, lib.sophia_cache_fork, src.data_ptr(), dst.data_ptr(), nat.ptr(cached), n, n_slots, _addresses(states),
-                 state_elems, _addresses(convs), conv_elems, len(kda), _addresses(mla), slot_stride, max_seq, len(mla),
-                 _addresses(pools), page_stride, n_pages, size, len(pools), nat.ptr(table), table_stride, max_pages, rank, code,
+    lists = [_addresses(t) for t in (states, convs, mla, pools)]
+    at = [t.buffer_info()[0] if t else None for t in lists]
+    rc = _launch(device, lib.sophia_cache_fork, src.data_ptr(), dst.data_ptr(), nat.ptr(cached), n, n_slots, at[0],
+                 state_elems, at[1], conv_elems, len(kda), at[2], slot_stride, max_seq, len(mla), at[3], page_stride, n_pages, size, len(pools), nat.ptr(table), table_stride, max_pages, rank, code,
                  nat.ptr(ws), nbytes)
     nat.check(rc, "sophia_cache_fork")
 
@@ -2379,7 +2406,8 @@ def page_copy(src: torch.Tensor, dst: torch.Tensor, pools) -> None:
     lib = nat.lib()
     nbytes = lib.sophia_move_workspace_size(n)
     ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device) if nbytes else None
-    rc = _launch(device, lib.sophia_page_copy, src.data_ptr(), dst.data_ptr(), n, _addresses(pools), len(pools), page_stride,
+    at = _addresses(pools)
+    rc = _launch(device, lib.sophia_page_copy, src.data_ptr(), dst.data_ptr(), n, at.buffer_info()[0], len(pools), page_stride,
                  size * rank, n_pages, nat.dtype_code(pools[0].dtype), nat.ptr(ws), nbytes)
     nat.check(rc, "sophia_page_copy")
 

@@ -52,7 +52,7 @@ def test_attention_of_nothing(nat):  # noqa: F811
 
 def test_attention_workspace(nat):  # noqa: F811
     size = nat.lib().sophia_mla_paged_workspace_size
-    part = 64 * (4 * 16 + 2) * 4                                   # bf16, rank 128
+    part = 64 * (4 * 8 + 2) * 4                                    # 16 columns of rank 128
     assert size(3, 3, 1, 500, 16, 128, 1, 1) == 0
     assert size(3, 3, 1, 500, 16, 128, 1, 2) == 3 * 2 * part
     assert size(3, 3, 1, 100, 16, 128, 1, 9) == 0                  # one tile of keys
