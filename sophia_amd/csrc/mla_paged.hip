@@ -72,7 +72,7 @@ __device__ __forceinline__ f16v mfma32x32(const bf8 &a, const bf8 &b, const f16v
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-__device__ const u4 zero_rows[64] = {};   // what keys that are not there are read from
+__device__ const u4 zero_rows[2048] = {};   // what keys that are not there are read from: 32 rows of 1 KiB at most
 
 // Chunk c (16 bytes) of an LDS row lies at place c ^ turn(row): in bf16 eight rows of one chunk
 // (K) and four rows of two chunks (V, transposing reads), in fp32 sixteen rows of one chunk and
@@ -134,12 +134,13 @@ template <int R, bool F32>
 struct Lanes {
   using F = Form<R, F32, false>;
   const PagedArgs &a;
+  Sequence q;
   int groups = 0, tiles = 0, fewest = 0;         // of this lane's sequence; tiles of its last group and of its first
   int used = 0, items = 0, parts = 0;            // ranges, (range, group) items, those of them that are partials
   __device__ __forceinline__ explicit Lanes(const PagedArgs &args) : a(args) {}
   __device__ __forceinline__ void look(int s) {
     const int in = min(s, a.p.n_seqs - 1);
-    const Sequence q = sequence(a.p, in);
+    q = sequence(a.p, in);
     const int n = s == in && !narrow_cols(a, q.n, Form<R, F32, true>::kCols) ? min(q.n, a.max_new) : 0;
     groups = (n * a.heads + F::kGroup - 1) / F::kGroup;
     const auto tiles_to = [&](int token) { return (max(0, min(q.pos0 + token + 1, q.keys)) + kWideKeys - 1) / kWideKeys; };
@@ -175,7 +176,8 @@ struct Lanes {
 // Up to 64 sequences' shares of the list, the longest ranges first, so that the last items are short ones: of place i
 // in this order the sequence, its groups, ranges and tiles, and items and partials up to and including it.
 struct Shares {
-  int seq[64], groups[64], used[64], tiles[64], items[64], parts[64];
+  int groups[64], used[64], tiles[64], items[64], parts[64];
+  Sequence q[64];
   int n, length;
 };
 
@@ -193,7 +195,7 @@ __device__ __forceinline__ void share(Lanes<R, F32> &l, Shares &t, int s0, int l
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
   __builtin_amdgcn_wave_barrier();
   if (real) {
-    t.seq[place] = s0 + lane;
+    t.q[place] = l.q;
     t.groups[place] = l.groups;
     t.used[place] = l.used;
     t.tiles[place] = l.tiles;
@@ -213,7 +215,7 @@ template <int R, bool F32>
 __device__ __forceinline__ bool take(const PagedArgs &a, const Shares &t, Work &w, int i, int g, int split, int parts) {
   using F = Form<R, F32, false>;
   const int groups = t.groups[i], used = t.used[i];
-  w.q = sequence(a.p, t.seq[i]);
+  w.q = t.q[i];
   w.col0 = (groups - 1 - g) * F::kGroup;     // (late groups, which see most keys, first)
   const int keys = columns(a, w, F::kGroup), tiles = (keys + kWideKeys - 1) / kWideKeys;
   const int least = max(1, (t.tiles[i] + used - 1) / used);
@@ -257,9 +259,16 @@ struct Stage {
   using F = Form<R, F32, NARROW>;
   const PagedArgs &a;
   const Work &w;
-  int lane, row0;      // this wavefront's first row
+  int lane, row0;                 // this wavefront's first row
+  uint32_t offset[F::kLoads];     // of this lane's chunks from that row on, in bytes
   __device__ __forceinline__ Stage(const PagedArgs &args, const Work &work)
-      : a(args), w(work), lane(threadIdx.x & 63), row0(NARROW ? 0 : F::kOwn * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {}
+      : a(args), w(work), lane(threadIdx.x & 63), row0(NARROW ? 0 : F::kOwn * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+#pragma unroll
+    for (int t = 0; t < F::kLoads; ++t) {
+      const int row = 64 / F::kChunks * t + lane / F::kChunks;
+      offset[t] = row * F::kBytes + 16 * ((lane % F::kChunks) ^ (turn<F32>(row0 + row) & (F::kChunks - 1)));
+    }
+  }
   // The page of key k0 + lane, as the table has it (k0 < k1; of the tile's keys, lanes past them repeat;
   // past the last key its page), and whether it is one and the key is there: apart, so that nothing waits for the load.
   __device__ __forceinline__ int load_id(int k0) const {
@@ -269,29 +278,27 @@ struct Stage {
   __device__ __forceinline__ int id_of(int k0, int id) const {
     return k0 + (lane & (F::kKeys - 1)) < w.k1 && id >= 0 && id < a.p.n_pages ? id : -1;
   }
-  // Where the rows of a copy lie in one page, its address is a scalar and an offset per lane that does not
-  // change; else (small pages, the last keys) each lane has its own.
+  // Where this wavefront's rows of a tile lie in one page there is one address, a scalar, and offsets per lane
+  // that do not change; else (small pages, the last keys) each lane has its own addresses.
   __device__ __forceinline__ void copy(char *tile, int k0, int id) const {
-    constexpr int kRows = 64 / F::kChunks;    // of a copy
-    const bool whole = (1 << a.p.shift) >= kRows && k0 + F::kKeys <= w.k1;
+    char *to = tile + 16 * row0 * F::kChunks;
+    const int of = lane / F::kChunks;
+    if ((1 << a.p.shift) >= F::kOwn && k0 + F::kKeys <= w.k1) {
+      const int page = __builtin_amdgcn_readlane(id, row0), at = (k0 + row0) & ((1 << a.p.shift) - 1);
+      const int64_t skip = page * (a.p.page_stride * (F32 ? 4 : 2)) + at * F::kBytes;
+      const char *from = page >= 0 ? static_cast<const char *>(a.p.pages) + skip : reinterpret_cast<const char *>(zero_rows);
 #pragma unroll
-    for (int t = 0; t < F::kLoads; ++t) {
-      const int row = row0 + kRows * t, of = lane / F::kChunks;
-      const int c = (lane % F::kChunks) ^ (turn<F32>(row + of) & (F::kChunks - 1));
-      char *to = tile + 16 * (row0 * F::kChunks + 64 * t);
-      if (whole) {
-        const int page = __builtin_amdgcn_readlane(id, row);
+      for (int t = 0; t < F::kLoads; ++t)
+        __builtin_amdgcn_global_load_lds(from + offset[t], to + 1024 * t, 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int t = 0; t < F::kLoads; ++t) {
+        const int row = row0 + 64 / F::kChunks * t + of, c = (lane % F::kChunks) ^ (turn<F32>(row) & (F::kChunks - 1));
+        const int page = __shfl(id, row, 64);
         const int at = (k0 + row) & ((1 << a.p.shift) - 1);
         const char *from = static_cast<const char *>(a.p.pages) +
-                           (page * a.p.page_stride * (F32 ? 4 : 2) + static_cast<int64_t>(at) * F::kBytes);
-        from = page >= 0 ? from : reinterpret_cast<const char *>(zero_rows);
-        __builtin_amdgcn_global_load_lds(from + static_cast<uint32_t>(of * F::kBytes + 16 * c), to, 16, 0, 0);
-      } else {
-        const int page = __shfl(id, row + of, 64);
-        const int at = (k0 + row + of) & ((1 << a.p.shift) - 1);
-        const char *from = static_cast<const char *>(a.p.pages) +
                            (page * a.p.page_stride * (F32 ? 4 : 2) + static_cast<int64_t>(at) * F::kBytes + 16 * c);
-        __builtin_amdgcn_global_load_lds(page >= 0 ? from : reinterpret_cast<const char *>(zero_rows), to, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(page >= 0 ? from : reinterpret_cast<const char *>(zero_rows), to + 1024 * t, 16, 0, 0);
       }
     }
   }
@@ -367,17 +374,22 @@ struct Bf16Columns {
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    // K rows two steps ahead of their products, by hand: left to itself the compiler waits for each read.
+    constexpr int kAhead = 3;
+    bf8 k[kAhead][KT];
+    const auto read_k = [&](int ks) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
-        st[kt] = mfma32x32(bits_to_bf8(*reinterpret_cast<const u4 *>(lds + ko[ks] + 32 * kt * F::kBytes)), qf[ks], st[kt]);
-    // (K rows ahead of their products)
-    __builtin_amdgcn_sched_group_barrier(0x100, 3 * KT, 0);
+        k[ks % kAhead][kt] = bits_to_bf8(*reinterpret_cast<const u4 *>(lds + ko[ks] + 32 * kt * F::kBytes));
+      __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int ks = 0; ks < kAhead - 1 && ks < KS; ++ks) read_k(ks);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      __builtin_amdgcn_sched_group_barrier(0x8, KT, 0);
-      if (ks + 3 < KS) __builtin_amdgcn_sched_group_barrier(0x100, KT, 0);
+      if (ks + kAhead - 1 < KS) read_k(ks + kAhead - 1);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) st[kt] = mfma32x32(k[ks % kAhead][kt], qf[ks], st[kt]);
     }
     if (!all) {
 #pragma unroll
@@ -937,7 +949,9 @@ __global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a, int n
     if (j >= N::kQuads || !find_narrow<R, F32>(a, w, blockIdx.x, 0) || w.used == 1) return;
     join<R, F32, true, 1>(a, w, a.narrow_part + w.part * N::kPart, N::kPart, lane & (N::kCols - 1), j);
   } else {
-    if (kEach * static_cast<int>(blockIdx.y) >= F::kQuads) return;
+    // (many groups: all quads in one work-group)
+    const int j0 = EACH > 1 ? 0 : blockIdx.y, j1 = EACH > 1 ? F::kQuads : j0 + 1;
+    if (EACH > 1 ? blockIdx.y > 0 : j0 >= F::kQuads) return;
     __shared__ Shares s_all[4];
     Shares &t = s_all[wave];     // (each wavefront its own: no barrier)
     Lanes<R, F32> l(a);
@@ -951,8 +965,10 @@ __global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a, int n
         const int i = __ffsll(static_cast<unsigned long long>(__ballot(group < sum))) - 1;
         const int g = group - (__builtin_amdgcn_readlane(sum, i) - t.groups[i]);
         if (!take<R, F32>(a, t, w, i, g, 0, parts) || w.used == 1 || w.col0 + F::kCols * wave >= w.cols) return;
-        return join<R, F32, false, kEach>(a, w, a.wide_part + (4 * w.part + wave) * F::kPart, 4ll * w.step * F::kPart,
-                                          (lane & (F::kCols - 1)) + w.col0 + F::kCols * wave, kEach * blockIdx.y);
+        const float *p = a.wide_part + (4 * w.part + wave) * F::kPart;
+        for (int j = j0; j < j1; j += kEach)
+          join<R, F32, false, kEach>(a, w, p, 4ll * w.step * F::kPart, (lane & (F::kCols - 1)) + w.col0 + F::kCols * wave, j);
+        return;
       }
       group -= all;
       parts += t.parts[63];
@@ -1086,7 +1102,7 @@ Plan plan(int n_seqs, int64_t rows, int max_new, int64_t max_len, int heads, int
     // sequences as long as the longest, and 16 at most: more cost the merge what they save.  us in 1, 4, 8, 16 and 32
     // ranges: one sequence of 4,000 keys 47, 18, 13.0, 11.5, 12.3; of 700 12.4, 10.2, 9.0 (six); 32 of 200 to 4,000 46,
     // 18.8, 14.9, 13.4, 16.4; 96 of them 48, 22.6, 17.7, 21.5, 28.8; 200 of up to 3,400 40, 23.8, 25.2, 28.5, 38.9.
-    int64_t want = splits > 0 ? splits : p.wide && p.wide_groups >= slots ? 1 : imin64(16, (768 + n_seqs - 1) / n_seqs);
+    int64_t want = splits > 0 ? splits : (p.wide && p.wide_groups >= slots) || tiles <= 6 ? 1 : imin64(16, (768 + n_seqs - 1) / n_seqs);
     want = iclamp64(want, 1, tiles);
     const int64_t each = (tiles + want - 1) / want;
     p.narrow_splits = static_cast<int>((tiles + each - 1) / each);
