@@ -467,15 +467,30 @@ int run_moves(const char *what, PlanArgs plan, MoveArgs a, char *workspace, hipS
   plan.count = reinterpret_cast<int32_t *>(workspace);
   plan.moves = reinterpret_cast<Move *>(workspace + kHeader);
   a.plan = plan;
-  int64_t blocks = 0;
-  for (int i = 0; i < a.n_parts; ++i) blocks += static_cast<int64_t>(a.part[i].tensors) * a.part[i].chunks;
+  const auto blocks_of = [](const MoveArgs &m) {
+    int64_t n = 0;
+    for (int i = 0; i < m.n_parts; ++i) n += static_cast<int64_t>(m.part[i].tensors) * m.part[i].chunks;
+    return n;
+  };
+  const int64_t blocks = blocks_of(a);
   if (blocks == 0) return SOPHIA_OK;
   SOPHIA_REQUIRE(blocks <= 0x7fffffff, "%s: too much work for one call", what);
   const dim3 threads(kMoveThreads);
   // Slots are large, and a thread for each 16 bytes of them fills the chip; pages are small, and many.
   a.workers = static_cast<int>(iclamp64((2048 + blocks - 1) / blocks, 1, plan.n));
   if (plan.n <= kFew) {
-    hipLaunchKernelGGL(move_kernel<true>, dim3(static_cast<unsigned>(blocks), a.workers), threads, 0, st, a);
+    // Every work-group reads the table for its plan: its rows move when all have, in a launch of their own.
+    MoveArgs rows = a;
+    const bool table = a.part[a.n_parts - 1].kind == kTable;
+    if (table) {
+      a.n_parts -= 1;
+      rows.n_parts = 1;
+      rows.workers = plan.n;
+      rows.part[0] = rows.part[a.n_parts];
+    }
+    if (const int64_t n = blocks_of(a))
+      hipLaunchKernelGGL(move_kernel<true>, dim3(static_cast<unsigned>(n), a.workers), threads, 0, st, a);
+    if (table) hipLaunchKernelGGL(move_kernel<true>, dim3(static_cast<unsigned>(blocks_of(rows)), rows.workers), threads, 0, st, rows);
     return check_launch(what);
   }
   if (plan.n <= 512)

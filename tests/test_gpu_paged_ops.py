@@ -404,19 +404,20 @@ def test_page_copy_moves_whole_pages_and_nothing_else(dtype, page, rank):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("n,limit", [(1, 2), (4, 5), (9, 12), (24, 30)])
-def test_fork_moves_every_cache(kind, n, limit):
+@pytest.mark.parametrize("n,limit,width", [(1, 2, 6), (4, 5, 6), (9, 12, 6), (24, 30, 6), (64, 66, 40), (70, 90, 14)])
+def test_fork_moves_every_cache(kind, n, limit, width):
+    """Moves with tokens of their own each: a row of the table that moves is read for the pages of other moves."""
     from sophia_amd import ops
     rng = random.Random(n * 17 + len(kind))
     n -= kind == "swaps" and n % 2
     src, dst = _maps(kind, n, limit, rng)
     gen = torch.Generator().manual_seed(n)
-    heads, page, width = 2, 16, 6
+    heads, page = 2, 16
     kda = [(torch.randn(limit, 3 * heads * 128, 3, generator=gen), torch.randn(limit, heads, 128, 128, generator=gen)) for _ in range(2)]
     mla = [torch.randn(limit, 90, 32, generator=gen) for _ in range(2)]
     table = torch.randperm(limit * width, generator=gen).view(limit, width).int()     # every slot's pages its own
     pools = [torch.randn(limit * width, page, 32, generator=gen).to(BF) for _ in range(2)]
-    cached = torch.tensor([rng.choice([0, 1, 15, 16, 17, 40, 89, 96, 200, -3]) for _ in range(n)], dtype=torch.int64)
+    cached = torch.tensor([rng.choice([0, 1, 15, 16, 17, 40, 89, 96, 200, 600, -3]) for _ in range(n)], dtype=torch.int64)
     dk = [(c.cuda(), s.cuda()) for c, s in kda]
     dm, dp, dt = _dev(*mla), _dev(*pools), table.cuda()
     ops.cache_fork(*(torch.tensor(t, dtype=torch.int32).cuda() for t in (src, dst)), kda=dk, mla=dm, pools=dp, table=dt,
