@@ -416,12 +416,14 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
     int flags = 0;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) flags |= k < n ? m[k].flags : 0;
-    if (p.kind == kWhole && n == kBatch && !(flags & (kSave | kFromSaved))) {   // (no branch between the loads)
+    // Full batches without a branch between their loads, and past the caches: 48 slots in 28 layers 160 us in place of
+    // 205 (of few moves, which the next step reads from the caches, 23 in place of 27 the other way round).
+    if (p.kind == kWhole && n == kBatch && !(flags & (kSave | kFromSaved))) {
       if (!in) return;
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) v[k] = *reinterpret_cast<const u4 *>(base + m[k].src * p.stride + off);
+      for (int k = 0; k < kBatch; ++k) v[k] = __builtin_nontemporal_load(reinterpret_cast<const u4 *>(base + m[k].src * p.stride + off));
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) *reinterpret_cast<u4 *>(base + m[k].dst * p.stride + off) = v[k];
+      for (int k = 0; k < kBatch; ++k) __builtin_nontemporal_store(v[k], reinterpret_cast<u4 *>(base + m[k].dst * p.stride + off));
       return;
     }
 #pragma unroll
