@@ -1222,7 +1222,7 @@ extern "C" int sophia_mla_paged_attn(const void *qa, int64_t qa_stride, int dtyp
   SOPHIA_REQUIRE(rank == 32 || rank == 64 || rank == 128 || rank == 256,
                  "mla_paged_attn: rank %d not supported (32, 64, 128 or 256)", rank);
   SOPHIA_REQUIRE(heads >= 1 && heads <= 128, "mla_paged_attn: heads must be in [1, 128]");
-  SOPHIA_REQUIRE(scale > 0.f, "mla_paged_attn: scale must be > 0");
+  SOPHIA_REQUIRE(scale > 0.f && scale < 1e38f, "mla_paged_attn: scale must be > 0 and finite");
   SOPHIA_REQUIRE(max_new >= 1 && splits >= 0 && splits <= 1024, "mla_paged_attn: max_new must be >= 1 and splits 0..1024");
   if (int rc = check_pages("mla_paged_attn", pages, page_stride, n_pages, page_size, table, table_stride, table_rows, max_pages,
                            cu_seqlens, kv_len, n_seqs, rows, rank))

@@ -2298,13 +2298,17 @@ def _pools(pools, index: int, device) -> tuple[int, int, int, int]:
     return what
 
 
-def _addresses(tensors) -> array.array:
-    """The tensors' addresses as the library reads a list of them (which has to live until it has)."""
-    return array.array("q", [t.data_ptr() for t in tensors])
+def _addresses(tensors, name: str) -> array.array:
+    """The tensors' addresses as the library reads a list of them (which has to live until it has).  A cache
+    that is moved twice at once would come out as neither."""
+    at = array.array("q", [t.data_ptr() for t in tensors])
+    if len(set(at)) < len(at) and tensors[0].numel():
+        raise RuntimeError(f"{name} must be a tensor of its own in each layer")
+    return at
 
 
 def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=(), table: torch.Tensor | None = None,
-               cached: torch.Tensor | None = None) -> None:
+               cached: torch.Tensor | None = None, page_size: int | None = None) -> None:
     """Cache slots that go on from other slots, in all layers and in place: slot
     dst[i] becomes what slot src[i] was, for all i as if at once (sophia_cache_fork).
     For beams: src the slot of the beam that each goes on from, dst its own.
@@ -2318,6 +2322,7 @@ def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=()
     pools, the pages of each MLA layer: the ids of the pages that cached[i] tokens
     fill become shared, the tokens of the page that they fill in part are copied into
     the one that dst[i] has there, which no other slot has; the ids behind stay.
+    page_size: of a table without pools, whose layers are elsewhere.
     cached: int64 [M]."""
     n = _moves(src, dst)
     device, index = src.device, src.get_device()
@@ -2359,17 +2364,22 @@ def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=()
         n_slots = first.size(0)
     n_pages = size = page_stride = max_pages = table_stride = 0
     code = nat.DTYPE_F32
-    if pools and table is None:
-        raise RuntimeError("pools need their table")
+    if table is None and (pools or page_size is not None):
+        raise RuntimeError("pools and page_size need their table")
     if table is not None:
         table_rows, max_pages, table_stride = _page_table(table, index, device)
-        if not pools:
-            raise RuntimeError("a table needs its pools")
-        n_pages, size, width, page_stride = _pools(pools, index, device)
-        code = nat.dtype_code(pools[0].dtype)
-        if mla and width != rank:
-            raise RuntimeError("pools and latent caches must have one rank")
-        rank = width
+        if pools:
+            n_pages, size, width, page_stride = _pools(pools, index, device)
+            code = nat.dtype_code(pools[0].dtype)
+            if mla and width != rank:
+                raise RuntimeError("pools and latent caches must have one rank")
+            if page_size is not None and page_size != size:
+                raise RuntimeError(f"page_size must be {size}, the pools' own")
+            rank = width
+        elif page_size is None:
+            raise RuntimeError("a table needs its pools or page_size")
+        else:
+            size = page_size
         if n_slots is not None and table_rows < n_slots:
             raise RuntimeError(f"the table must have a row for each of {n_slots} slots")
         n_slots = table_rows if n_slots is None else n_slots
@@ -2382,11 +2392,11 @@ def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=()
     lib = nat.lib()
     nbytes = lib.sophia_move_workspace_size(n)
     ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device) if nbytes else None
-    lists = [_addresses(t) for t in (states, convs, mla, pools)]
+    lists = [_addresses(*t) for t in ((states, "state"), (convs, "conv_state"), (mla, "latent_cache"), (pools, "pools"))]
     at = [t.buffer_info()[0] if t else None for t in lists]
     rc = _launch(device, lib.sophia_cache_fork, src.data_ptr(), dst.data_ptr(), nat.ptr(cached), n, n_slots, at[0],
-                 state_elems, at[1], conv_elems, len(kda), at[2], slot_stride, max_seq, len(mla), at[3], page_stride, n_pages, size, len(pools), nat.ptr(table), table_stride, max_pages, rank, code,
-                 nat.ptr(ws), nbytes)
+                 state_elems, at[1], conv_elems, len(kda), at[2], slot_stride, max_seq, len(mla), at[3], page_stride,
+                 n_pages, size, len(pools), nat.ptr(table), table_stride, max_pages, rank, code, nat.ptr(ws), nbytes)
     nat.check(rc, "sophia_cache_fork")
 
 
@@ -2406,7 +2416,7 @@ def page_copy(src: torch.Tensor, dst: torch.Tensor, pools) -> None:
     lib = nat.lib()
     nbytes = lib.sophia_move_workspace_size(n)
     ws = torch.empty(nbytes // 8, dtype=torch.int64, device=device) if nbytes else None
-    at = _addresses(pools)
+    at = _addresses(pools, "pools")
     rc = _launch(device, lib.sophia_page_copy, src.data_ptr(), dst.data_ptr(), n, at.buffer_info()[0], len(pools), page_stride,
                  size * rank, n_pages, nat.dtype_code(pools[0].dtype), nat.ptr(ws), nbytes)
     nat.check(rc, "sophia_page_copy")
