@@ -274,7 +274,8 @@ def _own_beam(s):
 
 def _own_fork(s):
     from sophia_amd import ops
-    ops.cache_fork(s["src"], s["dst"], kda=s["kda"], pools=s["pools"], table=s["table"], cached=s["cached"])
+    ops.cache_fork(s["src"], s["dst"], kda=s["kda"], pools=s["pools"], table=s["table"], cached=s["cached"],
+                   page_size=s["page"])
     return s["kda"], s["pools"], s["table"]
 
 
