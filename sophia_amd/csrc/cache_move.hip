@@ -6,7 +6,9 @@
 // which one slot's content is held in registers.  A first kernel (one work-group) finds the
 // trees and orders each; in the second a thread has the same 16 bytes of every slot of some
 // trees and moves them in that order, so nothing is copied twice and no thread waits for another.
-// Moved bytes are read once and written once.
+// Moved bytes are read once and written once, which is what bounds large calls: 48 slots in 28 layers, 943 MB read and
+// written, 204 us with the plan (4.6 TB/s; a copy has 5.1), 3,000 pages in 7 layers 147 (4.7).  Trees are worked on
+// at once, a tree of many moves in turn: 4,096 moves in three chains take eight times as long as 4,096 of their own.
 #include "common.hpp"
 
 #include "../../include/sophia_pages.h"
@@ -15,7 +17,7 @@ namespace sophia {
 namespace {
 
 constexpr int kMoves = SOPHIA_MOVES;
-constexpr int kFew = 64;      // so many moves each work-group plans by itself
+constexpr int kFew = 64;      // so many moves a work-group plans by itself, or takes from the list at a time
 
 // A planned move.
 struct Move {
@@ -66,87 +68,37 @@ __device__ __forceinline__ Move planned(const PlanArgs &a, int i, int src, int d
   return m;
 }
 
-// At most 64 moves, planned by a wavefront: a move per lane, sets of moves as bits.  put(place, move)
-// in any order; returns their number.
-template <typename P>
-__device__ __forceinline__ int plan_few(const PlanArgs &a, P put) {
-  const int i = threadIdx.x & 63, n = a.n;
-  const int src = i < n ? a.src[i] : -1, dst = i < n ? a.dst[i] : -1;
-  const bool ok = src >= 0 && src < a.limit && dst >= 0 && dst < a.limit;
-  const uint64_t all = __ballot(ok);
-  const auto of = [](int v, int lane) { return __builtin_amdgcn_readlane(v, lane); };
-  // The last move to this one's slot, and the last one to the slot that it reads.
-  int last = i, writer = -1;
-  for (uint64_t m = all; m; m &= m - 1) {
-    const int j = __ffsll(static_cast<unsigned long long>(m)) - 1, d = of(dst, j);
-    last = d == dst ? j : last;
-    writer = d == src ? j : writer;
-  }
-  const bool active = ok && last == i && src != dst;
-  const uint64_t live = __ballot(active);
-  const int next = active && writer >= 0 && ((live >> writer) & 1) ? writer : -1;
-  uint64_t readers = 0;       // the moves that have to come before
-  for (uint64_t m = __ballot(next >= 0); m; m &= m - 1) {
-    const int j = __ffsll(static_cast<unsigned long long>(m)) - 1;
-    readers |= of(next, j) == i ? 1ull << j : 0;
-  }
-  // Levels; what is left are cycles, which take levels of their own one after the other.
-  uint64_t left = live;
-  int level = 0, flags = 0, end = 0, root = i, now = 0;
-  for (uint64_t ready; (ready = __ballot(((left >> i) & 1) && !(readers & left))) != 0; left &= ~ready)
-    if ((ready >> i) & 1) level = now++;
-    else ++now;
-  int up = next;
-  for (uint64_t m = left; m;) {
-    const int first = __ffsll(static_cast<unsigned long long>(m)) - 1;
-    for (int j = first;;) {
-      m &= ~(1ull << j);
-      if (i == j) level = now;
-      ++now;
-      const int to = of(next, j);
-      if (to == first) {
-        if (i == j) flags |= kFromSaved, up = -1;
-        if (i == first) flags |= kSave, end = j;
-        break;
-      }
-      j = to;
-    }
-  }
-  // Trees: each move's last one, by doubling.
-  root = up >= 0 ? up : i;
-#pragma unroll
-  for (int r = 0; r < 6; ++r) root = __shfl(root, root, 64);
-  const int key = root << 16 | level << 8 | i;   // (moves that read one slot have one level)
-  int place = 0, same = 0;
-  for (uint64_t m = live; m; m &= m - 1) {
-    const int k = of(key, __ffsll(static_cast<unsigned long long>(m)) - 1);
-    place += k < key;
-    same += k < key && (k >> 16) == root;
-  }
-  const int end_src = __shfl(src, end, 64);
-  if (active) put(place, planned(a, i, src, dst, flags | (same == 0 ? kFirst : 0), end, end_src));
-  return __popcll(live);
-}
-
-__global__ __launch_bounds__(64) void move_plan_few_kernel(PlanArgs a) {
-  const int total = plan_few(a, [&](int place, const Move &m) { a.moves[place] = m; });
-  if (threadIdx.x == 0) *a.count = total;
-}
-
-// The same for more, by THREADS threads.
-template <int N, int THREADS>
-__global__ __launch_bounds__(THREADS) void move_plan_kernel(PlanArgs a) {
+// The plan of at most N moves, by THREADS threads (the first of a work-group): put(place, move) in any order.  Returns their
+// number to all.  Nothing in it waits for a move's turn: of 4,096 moves in three chains the copies (410 us), not the plan, are what lasts.
+// What bounds it is the latency of its steps: 1.5 us by a wavefront for 64 moves, 12 for 4,096 of which few depend on others.
+template <int N, int THREADS, typename P>
+__device__ __forceinline__ int plan(const PlanArgs &a, P put) {
   constexpr int kEach = N / THREADS, kHash = 2 * N, kBits = __builtin_ctz(2 * N);
   static_assert(N == kEach * THREADS, "each thread has as many moves");
-  __shared__ int s_src[N], s_dst[N], s_readers[N];   // s_readers: moves that have to come before; then places
+  __shared__ int s_src[N], s_dst[N];
   __shared__ short s_next[N];
   // By slot, the last move that writes it; later what is found of the trees.
   __shared__ int s_key[kHash], s_by[kHash];
   __shared__ int s_wave[THREADS / 64];
-  int *const s_count = s_key;                        // of a root: moves of its tree, then the next one's place
-  int *const s_first = s_key + N;                    // the first one's
-  short *const s_jump = reinterpret_cast<short *>(s_by), *const s_low = s_jump + N, *const s_end = s_low + N;
+  int *const s_count = s_key, *const s_first = s_key + N;   // of a root: its tree's moves, and their first place
+  short *const s_jump = reinterpret_cast<short *>(s_by), *const s_low = s_jump + N, *const s_steps = s_low + N,
+        *const s_end = s_steps + N;
+  int *const s_level = s_by;                                 // moves of a tree's levels, then places
   const int t = threadIdx.x, n = a.n;
+  // (What one wavefront writes to LDS it reads in its own order.)
+  const auto sync = [] {
+    if constexpr (THREADS > 64) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  const auto any = [&](bool v) {
+    if constexpr (THREADS > 64) return __syncthreads_or(v) != 0;
+    sync();
+    return __any(v) != 0;
+  };
   for (int i = t; i < kHash; i += THREADS) {
     s_key[i] = -1;
     s_by[i] = -1;
@@ -157,9 +109,8 @@ __global__ __launch_bounds__(THREADS) void move_plan_kernel(PlanArgs a) {
     const int s = i < n ? a.src[i] : -1, d = i < n ? a.dst[i] : -1;
     s_src[i] = s;
     s_dst[i] = s >= 0 && s < a.limit && d >= 0 && d < a.limit ? d : -1;
-    s_readers[i] = 0;
   }
-  __syncthreads();
+  sync();
   const auto hash = [](int slot) { return (static_cast<unsigned>(slot) * 2654435761u) >> (32 - kBits); };
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
@@ -172,7 +123,7 @@ __global__ __launch_bounds__(THREADS) void move_plan_kernel(PlanArgs a) {
     }
     atomicMax(&s_by[h], i);
   }
-  __syncthreads();
+  sync();
   const auto writer = [&](int slot) {
     for (unsigned h = hash(slot);; h = (h + 1) & (kHash - 1)) {
       if (s_key[h] == slot) return s_by[h];
@@ -181,7 +132,7 @@ __global__ __launch_bounds__(THREADS) void move_plan_kernel(PlanArgs a) {
   };
   // What counts is the last move to a slot, if it changes it: so of a slot's writer too.
   bool active[kEach];
-  int next[kEach];
+  int next[kEach];             // the move that has to come after
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
     const int i = t + k * THREADS, d = s_dst[i];
@@ -189,144 +140,154 @@ __global__ __launch_bounds__(THREADS) void move_plan_kernel(PlanArgs a) {
     const int w = active[k] ? writer(s_src[i]) : -1;
     next[k] = w >= 0 && s_src[w] != s_dst[w] ? w : -1;
     s_next[i] = static_cast<short>(next[k]);
-    if (next[k] >= 0) atomicAdd(&s_readers[next[k]], 1);
   }
-  __syncthreads();
-  // By doubling: the move after 1, 2, 4 .. steps, and the lowest on the way.
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = t + k * THREADS;
-    s_jump[i] = static_cast<short>(next[k] >= 0 ? next[k] : i);
-    s_low[i] = static_cast<short>(i);
-  }
-  __syncthreads();
-  for (int reach = 1; reach < n; reach *= 2) {
-    short jump[kEach], low[kEach];
+  sync();
+  // By doubling: the move after 1, 2, 4 .. steps (its tree's last one, which stays), the steps to it, and the lowest
+  // move before it.  On a cycle all are once round when nothing changes any more, or after n steps.
+  const auto follow = [&] {
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      const int i = t + k * THREADS, j = s_jump[i];
-      jump[k] = s_jump[j];
-      low[k] = min(s_low[i], s_low[j]);
+      const int i = t + k * THREADS;
+      s_jump[i] = static_cast<short>(next[k] >= 0 ? next[k] : i);
+      s_steps[i] = next[k] >= 0;
+      s_low[i] = static_cast<short>(i);
     }
-    __syncthreads();
+    sync();
+    for (int reach = 1; reach < n; reach *= 2) {
+      short jump[kEach], low[kEach], steps[kEach];
+      bool moved = false;
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      s_jump[t + k * THREADS] = jump[k];
-      s_low[t + k * THREADS] = low[k];
+      for (int k = 0; k < kEach; ++k) {
+        const int i = t + k * THREADS, j = s_jump[i];
+        jump[k] = s_jump[j];
+        low[k] = min(s_low[i], s_low[j]);
+        steps[k] = static_cast<short>(s_steps[i] + s_steps[j]);
+        moved |= jump[k] != j;
+      }
+      if (!any(moved)) break;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const int i = t + k * THREADS;
+        s_jump[i] = jump[k];
+        s_low[i] = low[k];
+        s_steps[i] = steps[k];
+      }
+      sync();
     }
-    __syncthreads();
-  }
-  // A tree's root is its last move, or the lowest move of the cycle that it ends in, which has that
-  // cycle's first move.
-  int root[kEach];
+  };
+  follow();
+  // A cycle is cut behind its lowest move, whose slot's content is held for the move that comes before it on the cycle:
+  // a tree as the others.  On a cycle is what the steps from somewhere end at that is no last move.
+  int flags[kEach], end[kEach];
+  bool round = false;
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int at = s_jump[t + k * THREADS];
-    root[k] = s_next[at] < 0 ? at : s_low[at];
+    flags[k] = end[k] = 0;
+    round |= s_next[s_jump[t + k * THREADS]] >= 0;
+  }
+  if (any(round)) {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) s_end[t + k * THREADS] = -1;
+    sync();
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int at = s_jump[t + k * THREADS];
+      if (s_next[at] >= 0) s_end[at] = 0;                    // (marked)
+    }
+    sync();
+    bool on[kEach];
+    int lowest[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = t + k * THREADS;
+      on[k] = s_end[i] == 0;
+      lowest[k] = s_low[s_jump[i]];
+    }
+    sync();
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (!on[k] || next[k] != lowest[k]) continue;
+      flags[k] |= kFromSaved;
+      s_end[next[k]] = static_cast<short>(t + k * THREADS);
+      next[k] = -1;
+    }
+    sync();
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (!on[k] || lowest[k] != t + k * THREADS) continue;
+      flags[k] |= kSave;
+      end[k] = s_end[lowest[k]];
+    }
+    sync();
+    follow();
+  }
+  // Places: trees by their last moves, in each the moves with the most others after them first.  A tree of c moves has
+  // at most c such levels, so the moves of all trees' levels are counted in n places, and the sums before them are places.
+  int root[kEach], steps[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    root[k] = s_jump[t + k * THREADS];
+    steps[k] = s_steps[t + k * THREADS];
     s_count[t + k * THREADS] = 0;
   }
-  __syncthreads();
+  sync();
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    s_low[t + k * THREADS] = 0;                      // (now: 1 + the root, of moves on a cycle)
+    s_level[t + k * THREADS] = 0;
     if (active[k]) atomicAdd(&s_count[root[k]], 1);
   }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    const int i = t + k * THREADS;
-    if (!active[k] || next[k] < 0 || root[k] != i) continue;
-    int j = i;
-    for (;;) {
-      s_low[j] = static_cast<short>(i + 1);
-      const int to = s_next[j];
-      if (to == i) break;
-      j = to;
-    }
-    s_end[i] = static_cast<short>(j);
-  }
-  // Where the trees begin: a sum over the roots before, kEach neighbours per thread.
-  int mine[kEach], sum = 0;
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    mine[k] = sum;
-    sum += s_count[kEach * t + k];
-  }
-  int scan = sum;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(scan, off, 64);
-    if ((t & 63) >= off) scan += o;
-  }
-  if ((t & 63) == 63) s_wave[t >> 6] = scan;
-  __syncthreads();
-  int before = scan - sum, total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w < (t >> 6)) before += s_wave[w];
-    total += s_wave[w];
-  }
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    s_count[kEach * t + k] = before + mine[k];
-    s_first[kEach * t + k] = before + mine[k];
-  }
-  __syncthreads();
-  // A move takes its place when all that read its slot have theirs.  Nobody waits for a cycle here, and of
-  // what is on none there is always one that nothing is before: every thread comes to its end.
-  bool waits[kEach], any = false;
-  int place[kEach];
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    waits[k] = active[k] && s_low[t + k * THREADS] == 0;
-    any |= waits[k];
-  }
-  while (any) {
-    any = false;
+  sync();
+  // to[i] = the sum of from[0 .. i); kEach neighbours per thread.  Returns the sum of all.
+  const auto sums = [&](const int *from, int *to) {
+    int mine[kEach], sum = 0;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      if (!waits[k]) continue;
-      if (__hip_atomic_load(&s_readers[t + k * THREADS], __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP) == 0) {
-        place[k] = __hip_atomic_fetch_add(&s_count[root[k]], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_WORKGROUP);
-        if (next[k] >= 0) __hip_atomic_fetch_add(&s_readers[next[k]], -1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_WORKGROUP);
-        waits[k] = false;
-      } else {
-        any = true;
-      }
+      mine[k] = sum;
+      sum += from[kEach * t + k];
     }
-  }
-  __syncthreads();
-  // Then the cycles.
+    int scan = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(scan, off, 64);
+      if ((t & 63) >= off) scan += o;
+    }
+    if ((t & 63) == 63) s_wave[t >> 6] = scan;
+    sync();
+    int before = scan - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < (t >> 6)) before += s_wave[w];
+      total += s_wave[w];
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) to[kEach * t + k] = before + mine[k];
+    sync();
+    return total;
+  };
+  const int total = sums(s_count, s_first);
+  int level[kEach];
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int i = t + k * THREADS;
-    if (!active[k] || next[k] < 0 || root[k] != i) continue;
-    int at = s_count[i];
-    for (int j = i;;) {
-      s_readers[j] = at++;
-      const int to = s_next[j];
-      if (to == i) break;
-      j = to;
-    }
+    level[k] = s_first[root[k]] + s_count[root[k]] - 1 - steps[k];
+    if (active[k]) atomicAdd(&s_level[level[k]], 1);
   }
-  __syncthreads();
+  sync();
+  sums(s_level, s_level);
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
     const int i = t + k * THREADS;
     if (!active[k]) continue;
-    int flags = 0, end = 0;
-    if (s_low[i] != 0) {
-      place[k] = s_readers[i];
-      if (root[k] == i) {
-        flags |= kSave;
-        end = s_end[i];
-      }
-      if (next[k] == root[k]) flags |= kFromSaved;
-    }
-    if (place[k] == s_first[root[k]]) flags |= kFirst;
-    a.moves[place[k]] = planned(a, i, s_src[i], s_dst[i], flags, end, s_src[end]);
+    const int place = atomicAdd(&s_level[level[k]], 1);
+    if (place == s_first[root[k]]) flags[k] |= kFirst;
+    put(place, planned(a, i, s_src[i], s_dst[i], flags[k], end[k], s_src[end[k]]));
   }
-  if (t == 0) *a.count = total;
+  return total;
+}
+
+template <int N, int THREADS>
+__global__ __launch_bounds__(THREADS) void move_plan_kernel(PlanArgs a) {
+  const int total = plan<N, THREADS>(a, [&](int place, const Move &m) { a.moves[place] = m; });
+  if (threadIdx.x == 0) *a.count = total;
 }
 
 // ---- the moves --------------------------------------------------------------------
@@ -365,15 +326,18 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
   const Part p = a.part[q];
   char *base = a.base[p.first + block / p.chunks];
   const int64_t off = static_cast<int64_t>(block % p.chunks) * kChunk + 16 * threadIdx.x;
+  int total;
   if constexpr (FEW) {
     if (threadIdx.x < 64) {
-      const int total = plan_few(a.plan, [&](int place, const Move &m) { s_moves[place] = m; });
-      if (threadIdx.x == 0) s_total = total;
+      const int found = plan<kFew, 64>(a.plan, [&](int place, const Move &m) { s_moves[place] = m; });
+      if (threadIdx.x == 0) s_total = found;
     }
     __syncthreads();
+    total = s_total;
+  } else {
+    total = *a.plan.count;
   }
   // This worker's trees: those that begin in its share of the list.
-  const int total = FEW ? s_total : *a.plan.count;
   const Move *list = FEW ? s_moves : a.plan.moves;
   const auto begin = [&](int w) {
     int at = static_cast<int>(static_cast<int64_t>(total) * w / a.workers);
@@ -416,8 +380,9 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
     int flags = 0;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) flags |= k < n ? m[k].flags : 0;
-    // Full batches without a branch between their loads, and past the caches: 48 slots in 28 layers 160 us in place of
-    // 205 (of few moves, which the next step reads from the caches, 23 in place of 27 the other way round).
+    // Full batches without a branch between their loads, and past the caches: 3,000 pages in 7 layers 147 us in place of 159,
+    // 48 slots in 28 layers 160 in place of 205 where they were in the last cache before, the same where not (of
+    // few moves, which the next step reads from the caches, 23 in place of 27 the other way round).
     if (p.kind == kWhole && n == kBatch && !(flags & (kSave | kFromSaved))) {
       if (!in) return;
 #pragma unroll
@@ -484,18 +449,24 @@ int run_moves(const char *what, PlanArgs plan, MoveArgs a, char *workspace, hipS
   const dim3 threads(kMoveThreads);
   // Slots are large, and a thread for each 16 bytes of them fills the chip; pages are small, and many.
   a.workers = static_cast<int>(iclamp64((2048 + blocks - 1) / blocks, 1, plan.n));
-  // Planned by each work-group itself: a launch less, where all run at once (24 pages in 7 layers 7.4 us in place of
-  // 10), not where they come in turns and plan each time (48 slots in 28 layers 209 us in place of 201), and
-  // not with a table, whose rows others may move while it is read for the plan.
+  // Planned by each work-group itself: a launch less, where all run at once (24 pages in 7 layers 6.3 us in place of
+  // 8.8, 64 11.0 and 11.2), not where they come in turns and plan each time (48 slots in 28 layers 209 us in place of
+  // 201), and not with a table, whose rows others may move while it is read for the plan.
   const bool table = a.part[a.n_parts - 1].kind == kTable;
   if (plan.n <= kFew && !table && blocks * a.workers <= 2048) {
     hipLaunchKernelGGL(move_kernel<true>, dim3(static_cast<unsigned>(blocks), a.workers), threads, 0, st, a);
     return check_launch(what);
   }
-  if (plan.n <= kFew)
-    hipLaunchKernelGGL(move_plan_few_kernel, dim3(1), dim3(64), 0, st, plan);
+  // One wavefront, which waits for nobody, to 128 moves (65 pages of one layer 9.9 us in place of 11.4 by 256 threads; 200 16.4 and
+  // 16.3, 400 20.0 and 15.0); 256 threads to 1,024 (700 pages 17.8 in place of 20.2 by 1,024 threads).
+  if (plan.n <= 64)
+    hipLaunchKernelGGL((move_plan_kernel<64, 64>), dim3(1), dim3(64), 0, st, plan);
+  else if (plan.n <= 128)
+    hipLaunchKernelGGL((move_plan_kernel<128, 64>), dim3(1), dim3(64), 0, st, plan);
   else if (plan.n <= 512)
     hipLaunchKernelGGL((move_plan_kernel<512, 256>), dim3(1), dim3(256), 0, st, plan);
+  else if (plan.n <= 1024)
+    hipLaunchKernelGGL((move_plan_kernel<1024, 256>), dim3(1), dim3(256), 0, st, plan);
   else
     hipLaunchKernelGGL((move_plan_kernel<kMoves, 1024>), dim3(1), dim3(1024), 0, st, plan);
   hipLaunchKernelGGL(move_kernel<false>, dim3(static_cast<unsigned>(blocks), a.workers), threads, 0, st, a);
