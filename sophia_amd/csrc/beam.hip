@@ -11,6 +11,10 @@
 // are collected, and each finds its place by counting the greater ones.  Equal values are ordered by
 // their index.  More than there is room for (many equal values, or few sets with a value above -inf)
 // are found one after the other.
+//
+// 512 rows of 65,536 logits in bf16 (67 MB): 19.2 us, 10.6 of them until the maxima are known, 2.4 for the sums and
+// 6 for what is collected, which the loads of other work-groups hide in part; then 9 to join them.  Four rows in
+// fp32: 4.2 and 6.5, latency.
 #include "common.hpp"
 #include "tree.hpp"
 

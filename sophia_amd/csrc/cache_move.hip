@@ -7,7 +7,7 @@
 // trees and orders each; in the second a thread has the same 16 bytes of every slot of some
 // trees and moves them in that order, so nothing is copied twice and no thread waits for another.
 // Moved bytes are read once and written once, which is what bounds large calls: 48 slots in 28 layers, 943 MB read and
-// written, 204 us with the plan (4.6 TB/s; a copy has 5.1), 3,000 pages in 7 layers 147 (4.7).  Trees are worked on
+// written, 200 us with the plan (4.7 TB/s; a copy has 5.1), 3,000 pages in 7 layers 141 (4.9).  Trees are worked on
 // at once, a tree of many moves in turn: 4,096 moves in three chains take eight times as long as 4,096 of their own.
 #include "common.hpp"
 
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
     int flags = 0;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) flags |= k < n ? m[k].flags : 0;
-    // Full batches without a branch between their loads, and past the caches: 3,000 pages in 7 layers 147 us in place of 159,
+    // Full batches without a branch between their loads, and past the caches: 3,000 pages in 7 layers 128 us in place of 142,
     // 48 slots in 28 layers 160 in place of 205 where they were in the last cache before, the same where not (of
     // few moves, which the next step reads from the caches, 23 in place of 27 the other way round).
     if (p.kind == kWhole && n == kBatch && !(flags & (kSave | kFromSaved))) {

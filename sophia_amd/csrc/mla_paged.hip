@@ -11,6 +11,13 @@
 //            takes a range of its keys, and the wavefronts differ in their keys, each with tiles
 //            of its own and no barrier until they join through LDS at the end.
 // A sequence of several ranges leaves partials, which a second kernel joins.
+//
+// What bounds them (rank 128, 16 heads, bf16): the wide form the matrix pipes and the vector unit in turn, as a
+// wavefront's tile is 48 products (1,536 cycles) and 300 vector instructions (1,700) that wait for one another, of
+// 3,700 in all: 8 sequences of 300 to 777 new tokens after up to 2,221 in 81 us and 9 to join them (411 TFLOP/s with both), 16 new
+// ones of 1,024 161 (426).  Eight wavefronts that take turns at products and softmax, with tiles in threes, were slower
+// (100, 180), and so was a work-group that goes on to its next item by itself (95).  The narrow form is latency: one
+// token after 700 9.2 us, 96 tokens after 221 to 3,090 each 12.2 and 4.
 #include "common.hpp"
 #include "pages.hpp"
 #include "tree.hpp"
@@ -40,7 +47,8 @@ struct PagedArgs {
 };
 constexpr int kLeast = 2;     // tiles of a wide range at least
 // Tiles of a range in shares of the whole work: with fewer more partials, with more the chip waits for the last
-// ones (8 sequences of 300 to 777 new tokens after up to 2,221: 1.0 110 us, 1.3 109, 1.6 101, 2.0 110, with the merge).
+// ones (8 sequences of 300 to 777 new tokens after up to 2,221: 1.0 96.1 us, 1.3 96.2, 1.6 92.1, 2.0 96.7, with the merge;
+// four of 700 after 2,000 118.9, 118.5, 111.9, 118.6).
 constexpr float kStretch = 1.6f;
 // Work-groups that run at a time.
 template <int R>
@@ -474,7 +482,7 @@ struct Bf16Columns {
 };
 
 // The same for the 16 columns of the narrow form, 16x16x32 MFMAs over 32 keys: one token of 16 heads would leave
-// half of 32 columns empty (4,000 keys by one work-group 52 us with 32 columns, 47 with 16).
+// half of 32 columns empty (4,000 keys by one work-group 47 us in place of 52, as copies were then; now 31).
 template <int R>
 struct Bf16Narrow {
   using F = Form<R, false, true>;
@@ -980,7 +988,7 @@ __global__ __launch_bounds__(256) void mla_paged_merge_kernel(PagedArgs a, int n
 // The normalisations that follow MLA's down projections, in place, and the latents into
 // their pages: a wavefront has two rows, whose places its halves look up while the rows are under way;
 // lanes [0, q_rank / 8) hold 8 elements of q each, the next kv_rank / 8 lanes 8 of the latent.  16,624 rows of
-// 384 + 128 in bf16: 38 MB, NORMS.
+// 384 + 128 in bf16: 38 MB read and written in 10.4 us (3.7 TB/s; a copy has 5.1); 96 rows 4.2, a launch and two waits.
 struct PagedNormArgs {
   Pages p;
   void *q;
@@ -1135,9 +1143,10 @@ Plan plan(int n_seqs, int64_t rows, int max_new, int64_t max_len, int heads, int
   if (p.narrow) {
     const int64_t tiles = (keys + 127) / 128;
     // Beside wide groups that fill the chip a chain of tiles has time.  Else ranges to about 768 work-groups, were all
-    // sequences as long as the longest, and 16 at most: more cost the merge what they save.  us in 1, 4, 8, 16 and 32
-    // ranges: one sequence of 4,000 keys 47, 18, 13.0, 11.5, 12.3; of 700 12.4, 10.2, 9.0 (six); 32 of 200 to 4,000 46,
-    // 18.8, 14.9, 13.4, 16.4; 96 of them 48, 22.6, 17.7, 21.5, 28.8; 200 of up to 3,400 40, 23.8, 25.2, 28.5, 38.9.
+    // sequences as long as the longest, and 16 at most: more cost the merge what they save.  us in 1, 4, 8 and 16
+    // ranges: one sequence of 4,000 keys 30.9, 14.2, 10.8, 10.2; 32 of 200 to 4,000 30.1, 14.5, 12.8, 12.3; 96 of them
+    // 31.5, 18.4, 15.4, 19.8; 200 of up to 3,400 27.3, 20.4, 22.2, 25.7.  Of six tiles one range, a launch
+    // less for the host: 9.4, and 8.4 in six on the device.
     int64_t want = splits > 0 ? splits : (p.wide && p.wide_groups >= slots) || tiles <= 6 ? 1 : imin64(16, (768 + n_seqs - 1) / n_seqs);
     want = iclamp64(want, 1, tiles);
     const int64_t each = (tiles + want - 1) / want;

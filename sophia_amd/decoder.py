@@ -999,7 +999,12 @@ class Transformer(nn.Module):
         With ``pages`` the latents are those: dst[i] shares the pages that src[i] has
         filled, and has the page that it has filled in part copied into its own,
         reserved before (``runtime.PagedLatents.reserve``); without, they are the slots'
-        own.  Nothing is read back on the host, so a fork is capturable."""
+        own, which is refused while a prompt's padding is masked (``set_pad_mask``): the
+        mask is of the rows it was given for.  Nothing is read back on the host, so a fork
+        is capturable."""
+        if pages is None and any(getattr(layer.attn, "_prompt_mask", None) is not None for layer in self.layers):
+            raise RuntimeError("a padded prompt is in the caches, whose mask would not go along; "
+                               "set_pad_mask(model, None) when none of its slots is used")
         kda = [(layer.attn.conv_history(), layer.attn.recurrent_state) for layer in self.layers if layer.layer_type == "kda"]
         mla = [layer.attn for layer in self.layers if layer.layer_type == "mla"]
         if pages is None:

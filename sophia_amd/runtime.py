@@ -244,7 +244,7 @@ class PagedLatents:
     places of the pools.  ``Transformer.forward_step(pages=)`` writes and reads the
     pages, ``Transformer.fork_slots(pages=)`` moves them between slots on the device:
     the slots of such a fork may hold each other's pages afterwards, so they are
-    released together, and not compacted apart.
+    released together, and other slots do not ``share`` theirs.
 
     ``dtype``: of the pages, that of the model's activations (default: of its
     embedding).  ``max_len``: tokens of a slot at most (default: max_seq_len)."""
@@ -282,7 +282,8 @@ class PagedLatents:
         return [p for _, p in sorted(self._held.get(int(slot), {}).items())]
 
     def ensure_slots(self, n: int) -> None:
-        """Rows of the table for slots 0 .. n - 1 (the old ones stay valid, the table is a new tensor)."""
+        """Rows of the table for slots 0 .. n - 1 (the old ones stay valid, the table is a new
+        tensor: a step captured before has the old one, as after growth of the caches)."""
         if int(n) > int(self.table.size(0)):
             grown = self.table.new_full((int(n), self._width), -1)
             grown[: self.table.size(0)].copy_(self.table)
@@ -324,13 +325,16 @@ class PagedLatents:
         """Slot ``dst``, which holds no pages, goes on from the first ``length`` tokens of
         ``src``: it holds the pages that these fill too, and a copy of the one that they fill
         in part.  (The latents alone: KDA states are moved by ``fork_slots``, or are those of
-        a prompt's ``cache_dump`` at that length.)"""
+        a prompt's ``cache_dump`` at that length.)  ``src`` has the pages that it was given:
+        ValueError where a fork on the device has put others in their places."""
         src, dst, places = int(src), int(dst), self._places(length)
         if self._held.get(dst):
             raise ValueError(f"slot {dst} holds pages")
         have = self._held.get(src, {})
         if any(j not in have for j in range(places)):
             raise ValueError(f"slot {src} holds fewer than {length} tokens")
+        if places and self.table[src, :places].tolist() != [have[j] for j in range(places)]:
+            raise ValueError(f"slot {src} has pages of other slots, from a fork")
         full = int(length) // self.page_size
         if places > full and not self._free:
             raise RuntimeError("1 page needed, 0 free")

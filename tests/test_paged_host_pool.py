@@ -65,6 +65,28 @@ def test_refusals(call, word):
         p.share(0, 1, 20)
 
 
+def test_a_slot_whose_pages_a_fork_has_changed_is_not_shared():
+    p = _pages()
+    p.reserve(0, 40)
+    p.reserve(1, 40)
+    p.table[0, 1] = p.table[1, 1]                     # (as a fork does on the device)
+    p.share(0, 2, 16)
+    with pytest.raises(ValueError, match="fork"):
+        p.share(0, 3, 32)
+    assert p.held(3) == [] and p.pages_free == 6
+
+
+def test_a_fork_under_a_remembered_mask_is_refused():
+    from sophia_amd.config import ModelArgs
+    from sophia_amd.decoder import Transformer
+    model = Transformer(ModelArgs(vocab_size=64, n_layers=4, ffn_hidden=64, mla_q_rank=64, mla_kv_rank=32, dim=128, num_heads=1,
+                                  max_seq_len=64, max_batch_size=2))
+    model.layers[3].attn._prompt_mask = torch.ones(1, 8, dtype=torch.bool)
+    i32 = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="padded"):
+        model.fork_slots(i32, i32, torch.zeros(1, dtype=torch.int64))
+
+
 def test_construction_refuses():
     for bad in (dict(n=0), dict(page_size=0), dict(page_size=24), dict(page_size=1 << 17), dict(max_len=0)):
         with pytest.raises(ValueError):
