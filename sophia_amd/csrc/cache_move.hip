@@ -8,7 +8,7 @@
 // trees and moves them in that order, so nothing is copied twice and no thread waits for another.
 // Moved bytes are read once and written once, which is what bounds large calls: 48 slots in 28 layers, 943 MB read and
 // written, 200 us with the plan (4.7 TB/s; a copy has 5.1), 3,000 pages in 7 layers 141 (4.9).  Trees are worked on
-// at once, a tree of many moves in turn: 4,096 moves in three chains take eight times as long as 4,096 of their own.
+// at once, a tree of many moves in turn: 4,096 pages of one layer in three chains take 226 us, of their own 51 to 68.
 #include "common.hpp"
 
 #include "../../include/sophia_pages.h"
@@ -22,7 +22,7 @@ constexpr int kFew = 64;      // so many moves a work-group plans by itself, or 
 // A planned move.
 struct Move {
   int32_t src, dst;         // slots, or pages
-  int32_t flags;            // of its place in its tree
+  int32_t flags;            // of its place in its tree, and where the next tree begins (<< kNext)
   int32_t tokens;           // taken along (a fork)
   int32_t src_page, dst_page;   // of the page that these fill in part (-1: none)
   int32_t held_tokens, held_page;   // kSave: the tokens and the source's page of the move at the end
@@ -30,6 +30,7 @@ struct Move {
 constexpr int kFirst = 1;      // the first of its tree
 constexpr int kSave = 2;       // what is in dst before is read at the end of the tree: held
 constexpr int kFromSaved = 4;  // its source is what was held
+constexpr int kNext = 3;
 static_assert(sizeof(Move) == 32, "two loads");
 
 struct PlanArgs {
@@ -69,7 +70,7 @@ __device__ __forceinline__ Move planned(const PlanArgs &a, int i, int src, int d
 }
 
 // The plan of at most N moves, by THREADS threads (the first of a work-group): put(place, move) in any order.  Returns their
-// number to all.  Nothing in it waits for a move's turn: of 4,096 moves in three chains the copies (410 us), not the plan, are what lasts.
+// number to all.  Nothing in it waits for a move's turn, however long the chains (4,096 moves in three: 12 us).
 // What bounds it is the latency of its steps: 1.5 us by a wavefront for 64 moves, 12 for 4,096 of which few depend on others.
 template <int N, int THREADS, typename P>
 __device__ __forceinline__ int plan(const PlanArgs &a, P put) {
@@ -279,6 +280,7 @@ __device__ __forceinline__ int plan(const PlanArgs &a, P put) {
     if (!active[k]) continue;
     const int place = atomicAdd(&s_level[level[k]], 1);
     if (place == s_first[root[k]]) flags[k] |= kFirst;
+    flags[k] |= (s_first[root[k]] + s_count[root[k]]) << kNext;
     put(place, planned(a, i, s_src[i], s_dst[i], flags[k], end[k], s_src[end[k]]));
   }
   return total;
@@ -340,9 +342,10 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(MoveArgs a) {
   // This worker's trees: those that begin in its share of the list.
   const Move *list = FEW ? s_moves : a.plan.moves;
   const auto begin = [&](int w) {
-    int at = static_cast<int>(static_cast<int64_t>(total) * w / a.workers);
-    while (at < total && !(list[at].flags & kFirst)) ++at;
-    return at;
+    const int at = static_cast<int>(static_cast<int64_t>(total) * w / a.workers);
+    if (at >= total) return total;
+    const int flags = list[at].flags;
+    return flags & kFirst ? at : flags >> kNext;
   };
   const int from = begin(blockIdx.y), to = begin(blockIdx.y + 1);
   // How many of the 16 bytes move with so many tokens (the ids of a table may end within them).
