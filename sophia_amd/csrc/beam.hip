@@ -6,15 +6,15 @@
 // the order of the logits is that of the candidates).  The second, a work-group per group,
 // joins the sums of each row, in double precision, and takes the greatest of what the parts left.
 //
-// The greatest of many values without sorting them: of 64 sets of them the keep-th greatest of
-// the sets' maxima is not above the keep-th greatest of all, and few values are not below it: those
+// The greatest of many values without sorting them: of 64 sets of them (256 where more than 32 are kept) the keep-th
+// greatest of the sets' maxima is not above the keep-th greatest of all, and few values are not below it: those
 // are collected, and each finds its place by counting the greater ones.  Equal values are ordered by
 // their index.  More than there is room for (many equal values, or few sets with a value above -inf)
 // are found one after the other.
 //
 // 512 rows of 65,536 logits in bf16 (67 MB): 19.2 us, 10.6 of them until the maxima are known, 2.4 for the sums and
 // 6 for what is collected, which the loads of other work-groups hide in part; then 9 to join them.  Four rows in
-// fp32: 4.2 and 6.5, latency.
+// fp32: 5.0 and 5.6, latency; 64 rows of 32 beams, of which 64 are kept, 12 and 40.
 #include "common.hpp"
 #include "tree.hpp"
 
@@ -74,6 +74,19 @@ __device__ __forceinline__ double sum_lanes(double v) {
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
   return v;
 }
+
+// Of 256 sets' maxima, a set per thread of four wavefronts: the least of those of a wavefront that fewer than `keep`
+// are above (inf: none); of all wavefronts the keep-th greatest.
+__device__ __forceinline__ float kth_of_sets(const float *sets, float mine, int keep) {
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < 256; i += 4) {
+    const f4 o = *reinterpret_cast<const f4 *>(sets + i);
+    above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+  }
+  return -top_of_lanes(above < keep ? -mine : -INFINITY);
+}
+constexpr int kFewKept = 32;   // to which 64 sets are enough: of 8,192 values 44 are collected of 32, 300 of 64 (of 256 sets 75)
 
 // Collected values with their indexes, and the places of the wavefronts' own.
 template <typename T>
@@ -156,27 +169,30 @@ __device__ __forceinline__ int greatest(Collected<T, WAVES> &c, int keep, E each
   return keep;
 }
 
-// Values of a thread in the first pass: EPT of them, eight consecutive ones of 2,048 at a time
-// (VEC), or every 256th.
-template <int DT, bool VEC, int EPT>
+// Values of a thread in the first pass, and of a part: eight consecutive ones of 2,048 at a time (VEC), or every
+// 256th.  (With 8 in place of 32 four times as many parts are joined: 64 rows of 65,536 logits in bf16, eight beams of which 16 are
+// kept, 20.3 us in place of 15.1, 8 rows 16.7 and 12.8, one row 8.6 and 8.7.)
+constexpr int kValues = 32, kPartSize = 256 * kValues;
+template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
   __shared__ Collected<float, 4> s;
-  __shared__ __attribute__((aligned(16))) float s_quad[64];   // the maxima of four threads each
+  __shared__ __attribute__((aligned(16))) float s_quad[64], s_set[256];   // the maxima of four threads each, and of each
   const int64_t row = blockIdx.y;
   const int part = blockIdx.x, t = threadIdx.x;
   // (a beam that has ended, or cannot be continued, has no use for its logits)
   if (!(fabsf(a.scores[row]) < INFINITY) || (a.ended && a.ended[row])) return;
-  const int v0 = part * 256 * EPT, width = min(256 * EPT, a.vocab - v0);
+  constexpr int EPT = kValues;
+  const int v0 = part * kPartSize, width = min(kPartSize, a.vocab - v0);
   const int64_t at = row * a.x_stride + v0;
   float x[EPT];
-  if (VEC && width == 256 * EPT) {   // (no branch between the loads: all are under way together)
+  if (VEC && width % 8 == 0) {   // (no branch between the loads: all are under way together)
     constexpr int kRaw = DT == SOPHIA_DTYPE_BF16 ? 1 : 2;
     u4 raw[EPT / 8][kRaw];
 #pragma unroll
     for (int e = 0; e < EPT; e += 8)
 #pragma unroll
       for (int k = 0; k < kRaw; ++k)
-        raw[e / 8][k] = reinterpret_cast<const u4 *>(static_cast<const char *>(a.x) + (at + 256 * e + 8 * t) * (2 * kRaw))[k];
+        raw[e / 8][k] = reinterpret_cast<const u4 *>(static_cast<const char *>(a.x) + (at + min(256 * e + 8 * t, width - 8)) * (2 * kRaw))[k];
 #pragma unroll
     for (int e = 0; e < EPT; ++e) {
       const u4 &r = raw[e / 8][DT == SOPHIA_DTYPE_BF16 ? 0 : (e & 7) / 4];
@@ -184,6 +200,10 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
         x[e] = __uint_as_float(e & 1 ? r[(e & 7) / 2] & 0xffff0000u : r[(e & 7) / 2] << 16);
       else
         x[e] = __uint_as_float(r[e & 3]);
+    }
+    if (width < kPartSize) {
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) x[e] = 256 * (e & ~7) + 8 * t < width ? x[e] : -INFINITY;
     }
   } else {
     uint32_t raw[EPT];
@@ -211,6 +231,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
   quad = fmaxf(quad, lane_other<2>(quad));
   const int lane = t & 63, wave = t >> 6;
   if ((lane & 3) == 0) s_quad[t >> 2] = quad;
+  if (a.keep > kFewKept) s_set[t] = mine;
   float top = top_of_quads(quad);
   if (lane == 0) s.top[wave] = top;
   if (t == 0) s.n = 0;
@@ -224,7 +245,10 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
     for (int i = t; i < a.keep; i += 256) token[i] = -1;
     return;
   }
-  {
+  if (a.keep > kFewKept) {
+    const float kth = kth_of_sets(s_set, mine, a.keep);
+    if (lane == 0) s.floor[wave] = kth;
+  } else {
     // How many of the 64 maxima are above this one, a quarter of them compared by each lane of the four.
     int above = 0;
 #pragma unroll
@@ -286,14 +310,15 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
 // values of one beam are in the order of their tokens, as parts and places are.  A wavefront
 // joins the sums of a beam, a part per lane; meanwhile the candidates are under way, the first of
 // all lists first.  The parts' lists are sorted: the keep-th of any of them is not above the
-// keep-th greatest of all, and neither is the keep-th of their first ones.
+// keep-th greatest of all, and neither is the keep-th of the threads' sets.
 constexpr int kJoin = 1024, kHeld = 2;   // threads, and candidates of each that stay in registers
 __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
   constexpr int kWaves = kJoin / 64;
   __shared__ Collected<double, kWaves> s;
   __shared__ double s_lse[kMost];
   __shared__ int s_kind[kMost];     // of a beam: 0 no candidates, 1 its logits', 2 itself
-  __shared__ float s_first[kWaves][64], s_floor;
+  __shared__ __attribute__((aligned(16))) float s_first[kWaves][64], s_set[256];
+  __shared__ float s_floor;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.beams;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int lists = a.beams * a.parts, all = lists * a.keep;
@@ -364,11 +389,30 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
   each([&](double w, int i) {
     if (i % a.keep == a.keep - 1) last = fmaxf(last, static_cast<float>(w));
   });
-  s_first[wave][lane] = t < lists ? static_cast<float>(v[0]) : -INFINITY;
+  double best = v[0];
+#pragma unroll
+  for (int k = 1; k < kHeld; ++k) best = fmax(best, v[k]);
+  s_first[wave][lane] = static_cast<float>(best);
   last = top_of_lanes(last);
   if (lane == 0) s.top[wave] = last;
   __syncthreads();
-  if (wave == 0) {
+  if (a.keep > kFewKept) {   // (as in the first pass, four threads to a set)
+    float first = -INFINITY;
+    if (wave < 4) {
+      for (int i = wave; i < kWaves; i += 4) first = fmaxf(first, s_first[i][lane]);
+      s_set[t] = first;
+    }
+    __syncthreads();
+    if (wave < 4) {
+      const float kth = kth_of_sets(s_set, first, a.keep);
+      if (lane == 0) s.floor[wave] = kth;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      const float floor = top_of_lanes(s.top[lane & (kWaves - 1)]);
+      if (lane == 0) s_floor = fmaxf(floor, fminf(fminf(s.floor[0], s.floor[1]), fminf(s.floor[2], s.floor[3])));
+    }
+  } else if (wave == 0) {
     float first = s_first[0][lane], floor = s.top[lane & (kWaves - 1)];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) first = fmaxf(first, s_first[i][lane]);
@@ -403,11 +447,6 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
   }
 }
 
-// Values of a thread: many where there are rows enough to fill the chip.
-int part_values(int64_t rows, int vocab) {
-  return rows * ((vocab + 8191) / 8192) >= 1024 ? 32 : 8;
-}
-
 }  // namespace
 }  // namespace sophia
 
@@ -415,7 +454,7 @@ using namespace sophia;
 
 extern "C" size_t sophia_beam_select_workspace_size(int64_t rows, int vocab, int keep) {
   if (rows < 1 || vocab < 1 || keep < 1) return 0;
-  const int64_t each = 256 * part_values(rows, vocab), parts = (vocab + each - 1) / each;
+  const int64_t parts = (vocab + kPartSize - 1) / kPartSize;
   return static_cast<size_t>(rows * parts) * (8 + 4 + 8 * static_cast<size_t>(keep));
 }
 
@@ -431,7 +470,7 @@ extern "C" int sophia_beam_select(const void *logits, int64_t logits_stride, int
   SOPHIA_REQUIRE(logits_stride >= vocab, "beam_select: row stride smaller than a row");
   if (rows == 0) return SOPHIA_OK;
   SOPHIA_REQUIRE(logits && scores && out_scores && out_parent && out_token, "beam_select: NULL pointer");
-  const int values = part_values(rows, vocab), each = 256 * values, parts = (vocab + each - 1) / each;
+  const int parts = (vocab + kPartSize - 1) / kPartSize;
   SOPHIA_REQUIRE(static_cast<int64_t>(beams) * parts * keep <= 1 << 30, "beam_select: too many candidates");
   SOPHIA_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
                      workspace_bytes >= sophia_beam_select_workspace_size(rows, vocab, keep),
@@ -447,18 +486,12 @@ extern "C" int sophia_beam_select(const void *logits, int64_t logits_stride, int
   const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && logits_stride * esz % 16 == 0;
   const dim3 grid(parts, static_cast<unsigned>(rows));
   const hipStream_t st = static_cast<hipStream_t>(stream);
-#define SOPHIA_BEAM(dt, v, n) hipLaunchKernelGGL((beam_part_kernel<dt, v, n>), grid, dim3(256), 0, st, a)
-#define SOPHIA_BEAM_DT(dt)                                                           \
-  do {                                                                               \
-    if (values == 32) {                                                              \
-      if (vec) SOPHIA_BEAM(dt, true, 32); else SOPHIA_BEAM(dt, false, 32);           \
-    } else {                                                                         \
-      if (vec) SOPHIA_BEAM(dt, true, 8); else SOPHIA_BEAM(dt, false, 8);             \
-    }                                                                                \
-  } while (0)
-  if (dtype == SOPHIA_DTYPE_F32) SOPHIA_BEAM_DT(SOPHIA_DTYPE_F32);
-  else SOPHIA_BEAM_DT(SOPHIA_DTYPE_BF16);
-#undef SOPHIA_BEAM_DT
+#define SOPHIA_BEAM(dt, v) hipLaunchKernelGGL((beam_part_kernel<dt, v>), grid, dim3(256), 0, st, a)
+  if (dtype == SOPHIA_DTYPE_F32) {
+    if (vec) SOPHIA_BEAM(SOPHIA_DTYPE_F32, true); else SOPHIA_BEAM(SOPHIA_DTYPE_F32, false);
+  } else {
+    if (vec) SOPHIA_BEAM(SOPHIA_DTYPE_BF16, true); else SOPHIA_BEAM(SOPHIA_DTYPE_BF16, false);
+  }
 #undef SOPHIA_BEAM
   hipLaunchKernelGGL(beam_join_kernel, dim3(static_cast<unsigned>(rows / beams)), dim3(kJoin), 0, st, a);
   return check_launch("beam_select");

@@ -305,6 +305,16 @@ def test_beams_match_float64(groups, beams, keep, vocab, dtype):
     _beam(logits, scores, beams, keep, torch.rand(rows, generator=gen) < 0.4)
 
 
+@pytest.mark.parametrize("groups,beams,keep,vocab", [(1, 1, 64, 65536), (2, 16, 64, 32008), (1, 16, 33, 40000), (2, 3, 48, 8200), (3, 12, 32, 32768)])
+def test_beams_that_keep_many(groups, beams, keep, vocab):
+    """Lists in one work-group's registers or more, parts that end within 8 values and not."""
+    gen = torch.Generator().manual_seed(keep + vocab)
+    logits = (torch.randn(groups * beams, vocab, generator=gen) * 3).to(BF)
+    logits[:, ::7] = float("-inf")
+    logits[0, 3::11] = float("nan")
+    _beam(logits, -torch.rand(groups * beams, generator=gen), beams, keep)
+
+
 @pytest.mark.parametrize("vocab", [1000, 9000, 40000])
 def test_beams_equal_values_go_to_the_lowest(vocab):
     """Whole rows of one value, few different values, and equal beams: more equal candidates than any set holds."""
