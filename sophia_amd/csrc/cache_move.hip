@@ -7,7 +7,7 @@
 // trees and orders each; in the second a thread has the same 16 bytes of every slot of some
 // trees and moves them in that order, so nothing is copied twice and no thread waits for another.
 // Moved bytes are read once and written once, which is what bounds large calls: 48 slots in 28 layers, 943 MB read and
-// written, 200 us with the plan (4.7 TB/s; a copy has 5.1), 3,000 pages in 7 layers 141 (4.9).  Trees are worked on
+// written, 203 us with the plan (4.7 TB/s; a copy has 5.1), 3,000 pages in 7 layers 141 (4.9).  Trees are worked on
 // at once, a tree of many moves in turn: 4,096 pages of one layer in three chains take 226 us, of their own 51 to 68.
 #include "common.hpp"
 
