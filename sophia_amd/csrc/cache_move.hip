@@ -70,8 +70,9 @@ __device__ __forceinline__ Move planned(const PlanArgs &a, int i, int src, int d
 }
 
 // The plan of at most N moves, by THREADS threads (the first of a work-group): put(place, move) in any order.  Returns their
-// number to all.  Nothing in it waits for a move's turn, however long the chains (4,096 moves in three: 12 us).
-// What bounds it is the latency of its steps: 1.5 us by a wavefront for 64 moves, 12 for 4,096 of which few depend on others.
+// number to all.  Nothing in it waits for a move's turn, however long the chains (4,096 moves in three: 24 us).
+// What bounds it is the latency of its steps: 3.1 us by a wavefront for 64 moves, its launch among them, 11 for 3,000 of which few
+// depend on others.
 template <int N, int THREADS, typename P>
 __device__ __forceinline__ int plan(const PlanArgs &a, P put) {
   constexpr int kEach = N / THREADS, kHash = 2 * N, kBits = __builtin_ctz(2 * N);
