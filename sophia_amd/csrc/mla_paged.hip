@@ -106,7 +106,10 @@ struct Work {
   int step;
 };
 
-__device__ __forceinline__ bool narrow_cols(const PagedArgs &a, int n, int cols) { return a.narrow_blocks && n <= cols / a.heads; }
+// Whether a sequence is the narrow form's: by the rows that are computed, max_new of them at most.
+__device__ __forceinline__ bool narrow_cols(const PagedArgs &a, int n, int cols) {
+  return a.narrow_blocks && min(n, a.max_new) <= cols / a.heads;
+}
 
 // The columns from w.col0 on of sequence w.q (which is that of all of its rows; those past max_new
 // have no columns); returns the keys that their last token sees.
