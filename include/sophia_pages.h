@@ -74,7 +74,9 @@ int sophia_mla_latent_norms_paged(void *q_lat, int64_t q_stride, void *kv_lat, i
  * sorted, equal ones by (beam, token).  ended[b] != 0: the beam's only candidate is its own score
  * with pad_token.  Logits and sums that are NaN or infinite are no candidates (and a row with a
  * logit of +inf or a score that is not finite has none): places without one hold score -inf,
- * parent -1, token -1.  Sums and comparisons are in double precision.
+ * parent -1, token -1.  Exponentials are of logits less the greatest one of their part of a row (8,192
+ * logits), in fp32, and summed in fp32 2,048 at a time; these sums are joined, and candidates formed and
+ * compared, in double precision.  A score below fp32's range is returned as -inf.
  *   out_scores fp32, out_parent int32 (a beam of the group), out_token int64: [groups, keep].
  *   beams, keep 1 .. SOPHIA_BEAMS.
  */

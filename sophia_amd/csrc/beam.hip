@@ -262,8 +262,9 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
     if (lane == 0) s.floor[wave] = kth;
   }
   if (top < INFINITY) {
-    const float shift = top * 1.44269504088896341f;
-    const auto add = [&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, 1.44269504088896341f, -shift)); };
+    // The maximum subtracted first: exact near it whatever its size, and at most -inf for the lowest values.  (A rounded product
+    // top log2 e as reference would be off by a factor of its own in each part, 3e-4 of a sum at 10,000, and infinite from 2.4e38 on.)
+    const auto add = [&](float v) { return __builtin_amdgcn_exp2f((v - top) * 1.44269504088896341f); };
     float p[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < EPT; ++e) p[e & 3] += add(x[e]);
