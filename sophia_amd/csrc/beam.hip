@@ -316,7 +316,8 @@ constexpr int kJoin = 1024, kHeld = 2;   // threads, and candidates of each that
 __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
   constexpr int kWaves = kJoin / 64;
   __shared__ Collected<double, kWaves> s;
-  __shared__ double s_lse[kMost];
+  // Of a beam its greatest logit and the logarithm of its sum relative to it; apart, as next to a large one the other would be lost.
+  __shared__ double s_top[kMost], s_log[kMost];
   __shared__ int s_kind[kMost];     // of a beam: 0 no candidates, 1 its logits', 2 itself
   __shared__ __attribute__((aligned(16))) float s_first[kWaves][64], s_set[256];
   __shared__ float s_floor;
@@ -341,10 +342,10 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
     const int64_t row = row0 + b;
     const float score = a.scores[row];
     const bool done = a.ended && a.ended[row];
-    double lse = 0.0;
+    float top = -INFINITY;
+    double log_sum = 0.0;
     int kind = fabsf(score) < INFINITY ? 2 : 0;
     if (kind && !done) {
-      float top = -INFINITY;
       for (int p = lane; p < a.parts; p += 64) top = fmaxf(top, a.top[row * a.parts + p]);
       top = top_of_lanes(top);
       kind = top > -INFINITY && top < INFINITY;
@@ -354,11 +355,12 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
           const float m = a.top[row * a.parts + p];
           if (m > -INFINITY) sum += a.sum[row * a.parts + p] * exp(static_cast<double>(m) - static_cast<double>(top));
         }
-        lse = static_cast<double>(top) + log(sum_lanes(sum));
+        log_sum = log(sum_lanes(sum));
       }
     }
     if (lane == 0) {
-      s_lse[b] = lse;
+      s_top[b] = top;
+      s_log[b] = log_sum;
       s_kind[b] = kind;
     }
   }
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
   const auto candidate = [&](int i, float x, int token) {
     const int b = i / each_beam;
     const double score = a.scores[row0 + b];
-    if (s_kind[b] == 1 && token >= 0) return score + (static_cast<double>(x) - s_lse[b]);
+    if (s_kind[b] == 1 && token >= 0) return score + ((static_cast<double>(x) - s_top[b]) - s_log[b]);
     return s_kind[b] == 2 && i == b * each_beam ? score : -static_cast<double>(INFINITY);
   };
   double v[kHeld];

@@ -73,6 +73,9 @@ ROWS = {
     "a part, and one of -inf": ([slice(8192, 16384), slice(0, 8192)], [None, -torch.inf]),
     "parts above the lowest": ([slice(8192, None)], [-2.5e38]),
     "the last ones, above the lowest": ([slice(20000, None)], [-2.4e38]),
+    "every one": ([slice(None)], [None]),
+    "every one great": ([slice(None)], [2.5e38]),
+    "all but one, which is low too": ([slice(None), 5], [-2.5e38, -2.4e38]),
 }
 
 
@@ -81,3 +84,18 @@ ROWS = {
 def test_tokens_masked_with_the_types_lowest_value(name, dtype):
     """Finite, so candidates: but behind all others, and without a share of the sums."""
     _check(_row(name, dtype, torch.finfo(dtype).min), torch.tensor([-0.5]), 1, 8)
+
+
+def test_beams_that_differ_by_a_constant_are_ordered_by_their_scores():
+    """The same logits, to which a row adds what leaves them exact: equal continuations, so the beams' own scores decide, and where
+    these are equal the order of the beams."""
+    gen = torch.Generator().manual_seed(3)
+    row = torch.round(torch.randn(1, 40000, generator=gen) * 3 * 256) / 256          # (multiples of 2^-8 below 16)
+    logits = row + torch.tensor([0.0, 8192.0, -1024.0, 100.0])[:, None]
+    got = _check(logits, torch.tensor([-5.0, -5.0, -5.0, -5.0]), 4, 8)
+    assert got[1].tolist() == [[0, 1, 2, 3, 0, 1, 2, 3]]
+    got = _check(logits, torch.tensor([-5.00001, -5.0, -5.000005, -5.00002]), 4, 8)
+    assert got[1].tolist()[0][:4] == [1, 2, 0, 3]
+    for r in range(4):
+        alone = _check(logits[r:r + 1].contiguous(), torch.tensor([-5.0]), 1, 16)
+        assert torch.equal(alone[0], _check(row, torch.tensor([-5.0]), 1, 16)[0])
