@@ -71,7 +71,7 @@ int sophia_mla_latent_norms_paged(void *q_lat, int64_t q_stride, void *kv_lat, i
 /*
  * The best continuations of each group of `beams` rows of logits [groups * beams, vocab]:
  * of the candidates scores[b] + log_softmax(logits[b])[v] of its beams the `keep` greatest,
- * sorted, equal ones by (beam, token).  ended[b] != 0: the beam's only candidate is its own score
+ * sorted, equal ones by beam, then by their logits, then by token.  ended[b] != 0: the beam's only candidate is its own score
  * with pad_token.  Logits and sums that are NaN or infinite are no candidates (and a row with a
  * logit of +inf or a score that is not finite has none): places without one hold score -inf,
  * parent -1, token -1.  Exponentials are of logits less the greatest one of their part of a row (8,192

@@ -9,12 +9,15 @@
 // The greatest of many values without sorting them: of 64 sets of them (256 where more than 32 are kept) the keep-th
 // greatest of the sets' maxima is not above the keep-th greatest of all, and few values are not below it: those
 // are collected, and each finds its place by counting the greater ones.  Equal values are ordered by
-// their index.  More than there is room for (many equal values, or few sets with a value above -inf)
+// their keys: the token's index, and in the join the beam, then the logit, then the token, so that the order of a
+// beam's candidates is that of its logits also where their sums are equal in 64 bits.  More than there is room for (many equal values, or few sets with a value above -inf)
 // are found one after the other.
 //
 // 512 rows of 65,536 logits in bf16 (67 MB): 19.2 us, 10.6 of them until the maxima are known, 2.4 for the sums and
 // 6 for what is collected, which the loads of other work-groups hide in part; then 9 to join them.  Four rows in
 // fp32: 5.0 and 5.6, latency; 64 rows of 32 beams, of which 64 are kept, 12 and 40.
+#include <limits>
+
 #include "common.hpp"
 #include "tree.hpp"
 
@@ -88,83 +91,81 @@ __device__ __forceinline__ float kth_of_sets(const float *sets, float mine, int 
 }
 constexpr int kFewKept = 32;   // to which 64 sets are enough: of 8,192 values 44 are collected of 32, 300 of 64 (of 256 sets 75)
 
-// Collected values with their indexes, and the places of the wavefronts' own.
-template <typename T>
+// Collected values with their keys, the lower before the higher where values are equal.
+template <typename T, typename K>
 struct Room {
   T value[kRoom];
-  int index[kRoom];
-  __device__ __forceinline__ void set(int at, T v, int i) { value[at] = v, index[at] = i; }
+  K key[kRoom];
+  __device__ __forceinline__ void set(int at, T v, K k) { value[at] = v, key[at] = k; }
   // How many of those from j0 to j1 come before entry i.
   __device__ __forceinline__ int before(int i, int j0, int j1) const {
     const T v = value[i];
-    const int at = index[i];
+    const K at = key[i];
     int n = 0;
 #pragma unroll 4
-    for (int j = j0; j < j1; ++j) n += (value[j] > v) | ((value[j] == v) & (index[j] < at));
+    for (int j = j0; j < j1; ++j) n += (value[j] > v) | ((value[j] == v) & (key[j] < at));
     return n;
   }
-  __device__ __forceinline__ T value_at(int i) const { return value[i]; }
-  __device__ __forceinline__ int index_at(int i) const { return index[i]; }
 };
-template <typename T, int WAVES>
+template <typename T, typename K, int WAVES>
 struct Collected {
-  Room<T> room;
+  Room<T, K> room;
   int n;
   float top[WAVES], floor[WAVES];
   double sum[WAVES];
   T best[WAVES];
-  int best_at[WAVES];
+  K best_key[WAVES];
 };
 
-template <typename T, int WAVES>
-__device__ __forceinline__ void collect(Collected<T, WAVES> &c, T v, int i) {
+template <typename T, typename K, int WAVES>
+__device__ __forceinline__ void collect(Collected<T, K, WAVES> &c, T v, K k) {
   const int at = atomicAdd(&c.n, 1);
-  if (at < kRoom) c.room.set(at, v, i);
+  if (at < kRoom) c.room.set(at, v, k);
 }
 
 // The greatest `keep` of what was collected (after a barrier), in order:
-// write(place, value, index) once per place, by any thread.  Returns how many there are.  each(f) calls
-// f(value, index) for this thread's candidates: where more were collected than there is room for, they
+// write(place, value, key) once per place, by any thread.  Returns how many there are.  each(f) calls
+// f(value, key) for this thread's candidates: where more were collected than there is room for, they
 // are found one after the other, each the greatest of those behind the last one.
-template <typename T, int WAVES, typename E, typename W>
-__device__ __forceinline__ int greatest(Collected<T, WAVES> &c, int keep, E each, W write) {
+template <typename T, typename K, int WAVES, typename E, typename W>
+__device__ __forceinline__ int greatest(Collected<T, K, WAVES> &c, int keep, E each, W write) {
   const int n = c.n, t = threadIdx.x;
   constexpr int kThreads = 64 * WAVES;
   if (n <= kRoom) {
     for (int i = t; i < n; i += kThreads) {
       const int place = c.room.before(i, 0, n);
-      if (place < keep) write(place, c.room.value_at(i), c.room.index_at(i));
+      if (place < keep) write(place, c.room.value[i], c.room.key[i]);
     }
     return min(n, keep);
   }
   T last = 0;
-  int last_at = -1;
+  K last_key = 0;
   for (int place = 0; place < keep; ++place) {
     T best = -INFINITY;
-    int best_at = 0x7fffffff;
-    each([&](T v, int i) {
-      if (place > 0 && !(v < last || (v == last && i > last_at))) return;
-      if (v > best || (v == best && i < best_at)) best = v, best_at = i;
+    K best_key = std::numeric_limits<K>::max();
+    each([&](T v, K k) {
+      if (place > 0 && !(v < last || (v == last && k > last_key))) return;
+      if (v > best || (v == best && k < best_key)) best = v, best_key = k;
     });
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
       const T v = __shfl_xor(best, off, 64);
-      const int at = __shfl_xor(best_at, off, 64);
-      if (v > best || (v == best && at < best_at)) best = v, best_at = at;
+      const K k = __shfl_xor(best_key, off, 64);
+      if (v > best || (v == best && k < best_key)) best = v, best_key = k;
     }
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
       c.best[threadIdx.x >> 6] = best;
-      c.best_at[threadIdx.x >> 6] = best_at;
+      c.best_key[threadIdx.x >> 6] = best_key;
     }
     __syncthreads();
     best = c.best[0];
-    best_at = c.best_at[0];
+    best_key = c.best_key[0];
     for (int i = 1; i < WAVES; ++i)
-      if (c.best[i] > best || (c.best[i] == best && c.best_at[i] < best_at)) best = c.best[i], best_at = c.best_at[i];
-    if (threadIdx.x == 0) write(place, best, best_at);   // (there are more than kRoom >= keep)
+      if (c.best[i] > best || (c.best[i] == best && c.best_key[i] < best_key)) best = c.best[i], best_key = c.best_key[i];
+    if (threadIdx.x == 0) write(place, best, best_key);   // (there are more than kRoom >= keep)
     last = best;
-    last_at = best_at;
+    last_key = best_key;
   }
   return keep;
 }
@@ -175,7 +176,7 @@ __device__ __forceinline__ int greatest(Collected<T, WAVES> &c, int keep, E each
 constexpr int kValues = 32, kPartSize = 256 * kValues;
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
-  __shared__ Collected<float, 4> s;
+  __shared__ Collected<float, int, 4> s;
   __shared__ __attribute__((aligned(16))) float s_quad[64], s_set[256];   // the maxima of four threads each, and of each
   const int64_t row = blockIdx.y;
   const int part = blockIdx.x, t = threadIdx.x;
@@ -307,15 +308,23 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
   for (int i = n + t; i < a.keep; i += 256) token[i] = -1;
 }
 
-// A group's candidates: of beam b, part p and place j the index ((b parts) + p) keep + j; equal
-// values of one beam are in the order of their tokens, as parts and places are.  A wavefront
+// A group's candidates: of beam b, part p and place j the index ((b parts) + p) keep + j, which among equal logits
+// of a beam is in the order of their tokens, as parts and places are.  A wavefront
 // joins the sums of a beam, a part per lane; meanwhile the candidates are under way, the first of
 // all lists first.  The parts' lists are sorted: the keep-th of any of them is not above the
 // keep-th greatest of all, and neither is the keep-th of the threads' sets.
 constexpr int kJoin = 1024, kHeld = 2;   // threads, and candidates of each that stay in registers
+// A candidate's key: its beam, its logit, the greater first, and its index within the beam: of 2^15 parts of 2^28 logits, 64 of each.
+constexpr int kIndexBits = 21;
+static_assert((1 << 28) / kPartSize * kMost <= 1 << kIndexBits && kMost <= 1 << (63 - 32 - kIndexBits), "a key has 63 bits");
+__device__ __forceinline__ int64_t candidate_key(int beam, float x, int in) {
+  const uint32_t bits = __float_as_uint(x + 0.f);   // (+0, not -0)
+  const uint32_t descending = bits & 0x80000000u ? bits : ~bits & 0x7fffffffu;
+  return static_cast<int64_t>(beam) << (32 + kIndexBits) | static_cast<int64_t>(descending) << kIndexBits | in;
+}
 __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
   constexpr int kWaves = kJoin / 64;
-  __shared__ Collected<double, kWaves> s;
+  __shared__ Collected<double, int64_t, kWaves> s;
   // Of a beam its greatest logit and the logarithm of its sum relative to it; apart, as next to a large one the other would be lost.
   __shared__ double s_top[kMost], s_log[kMost];
   __shared__ int s_kind[kMost];     // of a beam: 0 no candidates, 1 its logits', 2 itself
@@ -380,16 +389,21 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
   const auto each = [&](auto f) {
 #pragma unroll
     for (int k = 0; k < kHeld; ++k)
-      if (v[k] > -INFINITY) f(v[k], index(t + k * kJoin));
+      if (v[k] > -INFINITY) f(v[k], index(t + k * kJoin), held[k]);
     for (int c = t + kHeld * kJoin; c < all; c += kJoin) {
       const int i = index(c);
-      const double w = candidate(i, a.value[base + i], a.token[base + i]);
-      if (w > -INFINITY) f(w, i);
+      const float x = a.value[base + i];
+      const double w = candidate(i, x, a.token[base + i]);
+      if (w > -INFINITY) f(w, i, x);
     }
+  };
+  const auto key = [&](int i, float x) {
+    const int b = i / each_beam;
+    return candidate_key(b, x, i - b * each_beam);
   };
   // (rounding to fp32 keeps the order, but for equal ones)
   float last = -INFINITY;   // the keep-th of a list
-  each([&](double w, int i) {
+  each([&](double w, int i, float) {
     if (i % a.keep == a.keep - 1) last = fmaxf(last, static_cast<float>(w));
   });
   double best = v[0];
@@ -430,18 +444,19 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(BeamArgs a) {
   }
   __syncthreads();
   const float floor = s_floor;
-  each([&](double w, int i) {
-    if (static_cast<float>(w) >= floor) collect(s, w, i);
+  each([&](double w, int i, float x) {
+    if (static_cast<float>(w) >= floor) collect(s, w, key(i, x));
   });
   __syncthreads();
   float *out_score = a.out_score + static_cast<int64_t>(blockIdx.x) * a.keep;
   int32_t *out_parent = a.out_parent + static_cast<int64_t>(blockIdx.x) * a.keep;
   int64_t *out_token = a.out_token + static_cast<int64_t>(blockIdx.x) * a.keep;
-  const int n = greatest(s, a.keep, each, [&](int place, double w, int i) {
-    const int b = i / each_beam;
+  const auto each_key = [&](auto f) { each([&](double w, int i, float x) { f(w, key(i, x)); }); };
+  const int n = greatest(s, a.keep, each_key, [&](int place, double w, int64_t k) {
+    const int b = static_cast<int>(k >> (32 + kIndexBits)), in = static_cast<int>(k & ((1 << kIndexBits) - 1));
     out_score[place] = static_cast<float>(w);
     out_parent[place] = b;
-    out_token[place] = s_kind[b] == 2 ? a.pad : a.token[base + i];
+    out_token[place] = s_kind[b] == 2 ? a.pad : a.token[base + b * each_beam + in];
   });
   for (int i = n + t; i < a.keep; i += kJoin) {
     out_score[i] = -INFINITY;

@@ -2245,8 +2245,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, *, keep:
     that has just been read); ended: bool [groups * beams], beams whose only
     candidate is themselves, with ``pad_token``.  beams and keep are at most 64.
     Returns (scores fp32, parent int32, token int64), each [groups, keep]; a parent is
-    the index of a beam within its group.  Equal candidates are in the order of their
-    beams and tokens; sums are compared in 64 bits.  Logits that are NaN or -inf are no
+    the index of a beam within its group.  Sums are compared in 64 bits; equal ones
+    are in the order of their beams, within one beam of their logits, and then of their tokens.  Logits that are NaN or -inf are no
     candidates, a row with +inf, or with a score that is not finite, has none: where a group has fewer than
     ``keep`` there is -inf, -1, -1."""
     _gpu(logits, "logits")

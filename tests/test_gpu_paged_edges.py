@@ -22,15 +22,15 @@ def test_the_first_max_new_rows_are_computed_whatever_a_sequence_has(heads, max_
 
 
 # ------------------------------------------------------------------ beams whose logits are large
-def _beams(logits, scores, beams, keep, ended=None):
-    """(score, parent, token) in float64, the greatest logit subtracted before anything is rounded."""
-    x = logits.double()
-    x = torch.where(torch.isnan(x), -torch.inf, x)
-    top = x.max(-1, keepdim=True).values
+def _beams(logits, scores, beams, keep):
+    """(score, parent, token) in float64, the greatest logit subtracted before anything is rounded.  A beam's candidates are in the
+    order of its logits, as score + x - lse is without roundings: in 64 bits sums of different logits may come out equal."""
+    x, token = torch.sort(torch.where(torch.isnan(logits), -torch.inf, logits).double(), dim=-1, descending=True, stable=True)
+    top, V = x[:, :1], x.size(1)
     value = (x - top) - torch.log(torch.exp(x - top).sum(-1, keepdim=True))
-    value = (scores.double()[:, None] + value).view(-1, beams * x.size(1))
-    value, at = torch.sort(value, dim=-1, descending=True, stable=True)
-    return value[:, :keep], at[:, :keep] // x.size(1), at[:, :keep] % x.size(1)
+    value, at = torch.sort((scores.double()[:, None] + value).view(-1, beams * V), dim=-1, descending=True, stable=True)
+    token = torch.gather(token.view(-1, beams * V), 1, at)
+    return value[:, :keep], at[:, :keep] // V, token[:, :keep]
 
 
 def _check(logits, scores, beams, keep):
@@ -76,6 +76,9 @@ ROWS = {
     "every one": ([slice(None)], [None]),
     "every one great": ([slice(None)], [2.5e38]),
     "all but one, which is low too": ([slice(None), 5], [-2.5e38, -2.4e38]),
+    "one great": ([77], [3.0e38]),
+    "one great behind the first part": ([9000], [2.5e38]),
+    "tiny ones": ([slice(None), slice(0, None, 3), slice(1, None, 300), slice(2, None, 1000)], [0.0, -0.0, 1.0e-30, 2.0e-30]),
 }
 
 
@@ -99,3 +102,13 @@ def test_beams_that_differ_by_a_constant_are_ordered_by_their_scores():
     for r in range(4):
         alone = _check(logits[r:r + 1].contiguous(), torch.tensor([-5.0]), 1, 16)
         assert torch.equal(alone[0], _check(row, torch.tensor([-5.0]), 1, 16)[0])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("beams,keep", [(1, 8), (4, 12), (20, 64)])
+def test_groups_of_rows_of_every_kind(beams, keep, dtype):
+    """Sums that are equal in 64 bits though their logits are not, in several beams and in more of them than a set holds."""
+    lowest, gen = torch.finfo(dtype).min, torch.Generator().manual_seed(8)
+    logits = torch.cat([_row(name, dtype, lowest) for name in ROWS] * beams)[:4 * beams]
+    _check(logits, -torch.rand(logits.size(0), generator=gen), beams, keep)
+    _check(logits, torch.full((logits.size(0),), -1.0), beams, keep)
