@@ -410,9 +410,10 @@ def beam_search(model: Transformer, slots: SlotAllocator, pages: PagedLatents, p
     from the ``beams`` best at every token (``max_new`` of them, or up to ``end_token``).
 
     ``prompts``: token lists (or 1-d tensors) of any lengths.  All beams of a prompt share
-    its pages; each has pages of its own for what it generates.  ``adjust(logits, tokens)``,
-    if given, returns the logits [rows, vocab] to choose by, for the tokens [rows, t] generated
-    so far (``ops.adjust_logits``).  The slots and pages that it takes are given back.  After the
+    its pages; each has pages of its own for what it generates.  ``pad_token``, any number, fills
+    the output behind an end.  ``adjust(logits, tokens)``, if given, returns the logits [rows, vocab]
+    to choose by, for the tokens [rows, t] generated so far, pads behind ends among them
+    (``ops.adjust_logits``).  The slots and pages that it takes are given back.  After the
     prompts nothing is read back on the host."""
     prompts = [[int(t) for t in (p.tolist() if isinstance(p, torch.Tensor) else p)] for p in prompts]
     B, N, max_new = int(beams), len(prompts), int(max_new)
@@ -452,8 +453,9 @@ def beam_search(model: Transformer, slots: SlotAllocator, pages: PagedLatents, p
                 break
             src = torch.where(parent >= 0, torch.gather(own, 1, kept), -1).reshape(-1).contiguous()
             model.fork_slots(src, taken, at, pages=pages)
-            logits = model.forward_step(decode_ids=token.clamp(min=0).reshape(-1), decode_slots=taken, decode_pos=at,
-                                        max_decode_len=longest, pages=pages)
+            # (ended beams and places without a beam have a token of the vocabulary run, whose logits nobody reads)
+            ids = torch.where(done, 0, token.clamp(min=0)).reshape(-1)
+            logits = model.forward_step(decode_ids=ids, decode_slots=taken, decode_pos=at, max_decode_len=longest, pages=pages)
             at = at + 1
         tokens = torch.where(torch.isinf(scores)[:, :, None], -1, history)
         return Beams(tokens, scores, ended.view(N, B) & ~torch.isinf(scores))
