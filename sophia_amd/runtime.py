@@ -419,6 +419,8 @@ def beam_search(model: Transformer, slots: SlotAllocator, pages: PagedLatents, p
     B, N, max_new = int(beams), len(prompts), int(max_new)
     if N == 0 or any(not p for p in prompts):
         raise ValueError("prompts must hold a token each at least")
+    if any(not 0 <= t < int(model.args.vocab_size) for p in prompts for t in p):
+        raise ValueError("a token is outside the vocabulary")
     if not 1 <= B <= ops.BEAMS or max_new < 1 or N * B > ops.MOVES:
         raise ValueError(f"beams must be in [1, {ops.BEAMS}], max_new >= 1 and the beams of all prompts at most {ops.MOVES}")
     lens = [len(p) for p in prompts]
@@ -441,7 +443,10 @@ def beam_search(model: Transformer, slots: SlotAllocator, pages: PagedLatents, p
         scores, ended, width = torch.zeros(N, dtype=torch.float32, device=dev), None, 1
         for t in range(max_new):
             if adjust is not None:
+                shape = logits.shape
                 logits = adjust(logits, history.reshape(N * width, t))
+                if logits.shape != shape:
+                    raise ValueError(f"adjust must return logits {list(shape)}, got {list(logits.shape)}")
             scores, parent, token = ops.beam_select(logits, scores.reshape(-1), width, keep=B, ended=ended, pad_token=pad_token)
             kept = parent.long().clamp(min=0)
             history = torch.cat([torch.gather(history, 1, kept[:, :, None].expand(N, B, t)), token[:, :, None]], 2)

@@ -65,3 +65,20 @@ def test_places_without_a_beam_are_fed_a_token_of_the_vocabulary(monkeypatch):
     got = search([[1]], beams=2, max_new=3)
     assert got.tokens.tolist() == [[[4, 4, 4], [-1, -1, -1]]]
     assert all(int(ids.min()) >= 0 for ids in search.fed)
+
+
+@pytest.mark.parametrize("prompt", [[VOCAB], [1, -1, 2], [3, 1 << 40]])
+def test_prompts_outside_the_vocabulary_are_refused(prompt, monkeypatch):
+    search = Search(monkeypatch)
+    with pytest.raises(ValueError, match="vocabulary"):
+        search([[1, 2], prompt], beams=2, max_new=2)
+    assert not search.fed and search.slots.in_use == 0 and search.pages.pages_free == 40
+
+
+@pytest.mark.parametrize("change", [lambda x: torch.cat([x, x], -1), lambda x: x[:, :8], lambda x: x[:1], lambda x: x[None]])
+def test_adjusted_logits_of_another_shape_are_refused(change, monkeypatch):
+    """Wider ones would be tokens that the model does not have."""
+    search = Search(monkeypatch)
+    with pytest.raises(ValueError, match="adjust"):
+        search([[1, 2], [3]], beams=2, max_new=3, adjust=lambda logits, tokens: change(logits))
+    assert search.choices == 0 and search.slots.in_use == 0 and search.pages.pages_free == 40
