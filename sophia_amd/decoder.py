@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import itertools
 import math
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -677,6 +678,13 @@ def init_weights(model: nn.Module, args: ModelArgs) -> None:
     nn.init.zeros_(model.output_attn_residual.query.weight)
 
 
+class _PagePools(weakref.WeakSet):
+    """The ``runtime.PagedLatents`` of a model; a copy of the model has none."""
+
+    def __reduce__(self):
+        return _PagePools, ()
+
+
 class Transformer(nn.Module):
     """The [KDA, KDA, KDA, MLA] x (n_layers / 4) hybrid decoder
     (transformer.py:17-207, transformer_setup.py:67-79), tied embedding."""
@@ -690,6 +698,7 @@ class Transformer(nn.Module):
         self.output_attn_residual = AttentionResidualMixer(args)
         self.output = RuntimeLinear(args.dim, args.vocab_size)
         self.output.weight = self.tok_embeddings.weight  # tie_word_embeddings
+        self._page_pools = _PagePools()
         init_weights(self, args)
 
     def reset_runtime_cache(self) -> None:
@@ -804,6 +813,14 @@ class Transformer(nn.Module):
         for layer in self.layers:
             layer.attn.ensure_batch_capacity(required)
 
+    def _refuse_paged(self, slots, what: str) -> None:
+        """Raises where the latents of one of ``slots`` (a function that lists them, called if there are
+        any pages) are in pages: the slot's own cache, which the caller is about to use, does not have them."""
+        held = {s for pages in self._page_pools for s in pages.slots}
+        both = sorted(held.intersection(slots())) if held else []
+        if both:
+            raise RuntimeError(f"{what}: the latents of slots {both} are in pages (runtime.PagedLatents), not in the slots' caches")
+
     def reset_slots(self, slots: torch.Tensor) -> None:
         """Zero the KDA recurrent state and conv history of cache slots
         ``slots`` in every layer (new sequences; MLA latents need no reset:
@@ -814,10 +831,12 @@ class Transformer(nn.Module):
 
     def cache_dump(self, *, device: str = "cpu", cache_pos: int | None = None,
                    batch_size: int | None = None,
-                   slots: torch.Tensor | None = None) -> RuntimeCacheSnapshot:
+                   slots: torch.Tensor | None = None, latents: bool = True) -> RuntimeCacheSnapshot:
         """Copies of every layer's caches (runtime_host.py:179-194): rows
         [:batch_size] (default: every slot), or the cache slots ``slots`` in
-        that order; MLA latents up to ``cache_pos``."""
+        that order; MLA latents up to ``cache_pos``.  With ``latents`` False the
+        MLA layers' snapshots are None: of slots whose latents are in pages
+        (``runtime.PagedLatents``) there is no other."""
         if slots is None:
             active = self.runtime_batch_capacity() if batch_size is None else int(batch_size)
             if active <= 0:
@@ -825,16 +844,19 @@ class Transformer(nn.Module):
             self.ensure_batch_capacity(active)
         else:
             active = int(slots.numel())
+        if latents:
+            self._refuse_paged(lambda: range(active) if slots is None else slots.tolist(), "cache_dump (latents=False takes the rest)")
         return RuntimeCacheSnapshot(layers=tuple(
             layer.attn.cache_snapshot(device=device, batch_size=active, cache_pos=cache_pos, slots=slots)
-            for layer in self.layers))
+            if latents or layer.layer_type == "kda" else None for layer in self.layers))
 
     def cache_load(self, cache_snapshot: RuntimeCacheSnapshot, *,
                    slots: torch.Tensor | None = None) -> None:
         """Load a snapshot (runtime_host.py:196-212): every layer's snapshot is
         validated first, then all caches are reset and loaded into rows
         [:batch].  With ``slots``, snapshot row i goes to cache slot slots[i]
-        and every other slot keeps its contents (no reset)."""
+        and every other slot keeps its contents (no reset).  Slots whose latents
+        are in pages (``runtime.PagedLatents``) take snapshots without latents."""
         if not isinstance(cache_snapshot, RuntimeCacheSnapshot):
             raise TypeError("cache snapshot must be a RuntimeCacheSnapshot")
         if len(cache_snapshot.layers) > len(self.layers):
@@ -842,6 +864,8 @@ class Transformer(nn.Module):
         if slots is not None and int(slots.numel()) != cache_snapshot.batch_size():
             raise ValueError(f"{int(slots.numel())} slots for a snapshot of "
                              f"{cache_snapshot.batch_size()} rows")
+        if any(layer is not None and layer.latent is not None for layer in cache_snapshot.layers):
+            self._refuse_paged(lambda: range(cache_snapshot.batch_size()) if slots is None else slots.tolist(), "cache_load of a snapshot with latents")
         required = cache_snapshot.batch_size() if slots is None else \
             (int(slots.max()) + 1 if slots.numel() else 0)
         if required:
@@ -886,8 +910,9 @@ class Transformer(nn.Module):
         With ``pages`` (``runtime.PagedLatents``) the MLA layers keep their latents
         there, and not in the slots' own caches: slot s's are in the pages of row s of
         its table, which have to be reserved for the step's tokens before (a token
-        without a page is not attended to).  A step of decode rows is capturable then
-        too.
+        without a page is not attended to).  Every step of a sequence takes them, or
+        none: this one cannot tell where the latents before it are.  A step of decode
+        rows is capturable then too.
         """
         dev = self.tok_embeddings.weight.device
         lens = [int(t) for t in prefill_lens]
@@ -1026,8 +1051,10 @@ class Transformer(nn.Module):
         its decode step has in bf16.  ``commit_tree`` then advances the caches
         along one path of each tree.  Like the decode step it attends to every
         cached latent of its slot, so a prompt whose padding is masked
-        (``set_pad_mask``) is refused until the mask is cleared.
-        Nothing is read back on the host, so the step is capturable.  Values only
+        (``set_pad_mask``) is refused until the mask is cleared, and so is a slot whose
+        latents are in pages (``runtime.PagedLatents``): of an eager step, which
+        reads its slots on the host while any slot has pages.  Otherwise
+        nothing is read back there, so the step is capturable.  Values only
         (no gradient)."""
         _require_gpu(trees.token_ids)
         rows, n = int(trees.token_ids.numel()), int(trees.slots.numel())
@@ -1040,6 +1067,13 @@ class Transformer(nn.Module):
         if any(getattr(layer.attn, "_prompt_mask", None) is not None for layer in self.layers):
             raise RuntimeError("a padded prompt is in the caches, whose pad keys this step would attend to; "
                                "set_pad_mask(model, None) when none of its slots is used")
+
+        def with_nodes():
+            if torch.cuda.is_current_stream_capturing():
+                return []
+            cu = trees.cu_nodes.tolist()
+            return [s for s, a, b in zip(trees.slots.tolist(), cu, cu[1:]) if b > a]
+        self._refuse_paged(with_nodes, "forward_tree")
         ids = trees.token_ids.reshape(-1).clamp(0, int(self.args.vocab_size) - 1)
         hidden = self.tok_embeddings(ids)
         completed = depth_store(hidden, self.args.n_layers, self.args.attn_res_block_size)

@@ -119,6 +119,7 @@ def forward_cached_decode(*, model: Transformer, input_ids: torch.Tensor,
     cache_pos = 0 if cache_state is None else int(cache_state.cache_pos)
     if cache_pos + seqlen > int(model.args.max_seq_len):
         raise ValueError("sequence exceeds max_seq_len")
+    model._refuse_paged(lambda: range(bsz), "forward_cached_decode")
     if cache_state is None:
         if start_pos is not None and int(start_pos) != 0:
             raise ValueError("cache_state is required when start_pos > 0 for cached decode")
@@ -160,8 +161,8 @@ def pack_trees(model: Transformer, trees, slots, cached) -> DraftTrees:
     """``DraftTrees`` on the model's device from host lists: ``trees[s]`` =
     (tokens, parents) of sequence s, node 0 its last known token (parent -1),
     each other node after its parent (an index into the tree); ``slots[s]`` its
-    cache slot and ``cached[s]`` the tokens in it, to which the deepest path is
-    added within max_seq_len."""
+    cache slot, which has no latents in pages (RuntimeError), and ``cached[s]`` the
+    tokens in it, to which the deepest path is added within max_seq_len."""
     dev = model.tok_embeddings.weight.device
     slots, cached = ([int(v) for v in (t.tolist() if isinstance(t, torch.Tensor) else t)] for t in (slots, cached))
     if not len(trees) == len(slots) == len(cached):
@@ -171,6 +172,7 @@ def pack_trees(model: Transformer, trees, slots, cached) -> DraftTrees:
     capacity = model.runtime_batch_capacity()
     if any(not 0 <= s < capacity for s in slots):
         raise ValueError(f"cache slots must be in [0, {capacity})")
+    model._refuse_paged(lambda: slots, "pack_trees")
     tokens, parents, offsets = [], [], [0]
     for (toks, pars), length in zip(trees, cached):
         if len(toks) != len(pars) or not 1 <= len(toks) <= ops.TREE_NODES:
@@ -244,7 +246,9 @@ class PagedLatents:
     places of the pools.  ``Transformer.forward_step(pages=)`` writes and reads the
     pages, ``Transformer.fork_slots(pages=)`` moves them between slots on the device:
     the slots of such a fork may hold each other's pages afterwards, so they are
-    released together, and other slots do not ``share`` theirs.
+    released together, and other slots do not ``share`` theirs.  What works on the slots'
+    own caches refuses a slot that holds pages: drafted steps, cached decoding,
+    ``cache_dump`` and ``cache_load`` with latents.
 
     ``dtype``: of the pages, that of the model's activations (default: of its
     embedding).  ``max_len``: tokens of a slot at most (default: max_seq_len)."""
@@ -272,6 +276,12 @@ class PagedLatents:
         self._free = list(range(n_pages - 1, -1, -1))
         self._holders = [0] * n_pages
         self._held: dict[int, dict[int, int]] = {}     # of a slot: place in its row -> page
+        model._page_pools.add(self)
+
+    @property
+    def slots(self) -> list[int]:
+        """The slots that hold pages: whose latents are here."""
+        return sorted(self._held)
 
     @property
     def pages_free(self) -> int:
@@ -325,7 +335,7 @@ class PagedLatents:
         """Slot ``dst``, which holds no pages, goes on from the first ``length`` tokens of
         ``src``: it holds the pages that these fill too, and a copy of the one that they fill
         in part.  (The latents alone: KDA states are moved by ``fork_slots``, or are those of
-        a prompt's ``cache_dump`` at that length.)  ``src`` has the pages that it was given:
+        a prompt's ``cache_dump(latents=False)`` at that length.)  ``src`` has the pages that it was given:
         ValueError where a fork on the device has put others in their places."""
         src, dst, places = int(src), int(dst), self._places(length)
         if self._held.get(dst):

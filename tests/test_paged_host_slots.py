@@ -1,0 +1,100 @@
+"""Slots whose latents are in pages, and what works on the slots' own caches (CPU, no kernel)."""
+
+from __future__ import annotations
+
+import copy
+import gc
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def served():
+    from sophia_amd.config import ModelArgs
+    from sophia_amd.decoder import Transformer
+    from sophia_amd.runtime import PagedLatents
+    torch.manual_seed(0)
+    model = Transformer(ModelArgs(vocab_size=64, n_layers=4, ffn_hidden=64, mla_q_rank=64, mla_kv_rank=32, dim=128, num_heads=1,
+                                  max_seq_len=64, max_batch_size=4))
+    pages = PagedLatents(model, 12, page_size=16)
+    pages.reserve(1, 20)
+    pages.share(1, 2, 16)
+    return model, pages
+
+
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def test_a_snapshot_of_paged_slots_has_no_latents(served):
+    model, pages = served
+    assert pages.slots == [1, 2]
+    for call in (dict(slots=_i32(0, 2)), dict(slots=_i32(1)), dict(batch_size=2), dict()):
+        with pytest.raises(RuntimeError, match=r"slots \[.*\] are in pages"):
+            model.cache_dump(**call)
+    model.cache_dump(slots=_i32(3, 0))
+    model.cache_dump(batch_size=1)
+    for layer in model.layers[:3]:
+        layer.attn.recurrent_state.normal_()
+    snap = model.cache_dump(slots=_i32(2, 1), latents=False)
+    assert [s is None for s in snap.layers] == [False, False, False, True]
+    assert torch.equal(snap.layers[0].recurrent, model.layers[0].attn.recurrent_state[[2, 1]])
+    model.cache_load(snap, slots=_i32(1, 3))
+    assert torch.equal(model.layers[1].attn.recurrent_state[[1, 3]], snap.layers[1].recurrent)
+
+
+def test_a_snapshot_with_latents_is_not_loaded_into_paged_slots(served):
+    model, pages = served
+    snap = model.cache_dump(slots=_i32(0, 3))
+    before = [t.clone() for t in (model.layers[0].attn.recurrent_state, model.layers[3].attn.latent_cache)]
+    for slots in (_i32(0, 1), _i32(2, 3), None):
+        with pytest.raises(RuntimeError, match="in pages"):
+            model.cache_load(snap, slots=slots)
+    assert torch.equal(before[0], model.layers[0].attn.recurrent_state) and torch.equal(before[1], model.layers[3].attn.latent_cache)
+    model.cache_load(snap, slots=_i32(3, 0))
+    pages.release([1])
+    model.cache_load(snap, slots=_i32(0, 1))
+
+
+def test_drafts_and_cached_decoding_are_not_for_paged_slots(served, monkeypatch):
+    from sophia_amd import decoder
+    from sophia_amd.runtime import forward_cached_decode, pack_trees
+    model, pages = served
+    tree = ([3, 4], [-1, 0])
+    with pytest.raises(RuntimeError, match=r"slots \[2\] are in pages"):
+        pack_trees(model, [tree, tree], [0, 2], [5, 5])
+    trees = pack_trees(model, [tree, tree], [0, 3], [5, 5])
+    monkeypatch.setattr(decoder, "_require_gpu", lambda t: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    trees.slots[1] = 1
+    with pytest.raises(RuntimeError, match=r"slots \[1\] are in pages"):
+        model.forward_tree(trees)
+    # a tree without nodes has a slot of no meaning: the next thing that a CPU model lacks is its kernels
+    trees.cu_nodes[2] = 2
+    with pytest.raises(RuntimeError, match="GPU"):
+        model.forward_tree(trees)
+    with pytest.raises(RuntimeError, match="in pages"):
+        forward_cached_decode(model=model, input_ids=torch.zeros(2, 3, dtype=torch.long), cache_state=None, start_pos=0, logits_to_keep=None)
+
+
+def test_slots_are_the_callers_again_when_their_pages_are_given_back(served):
+    from sophia_amd.runtime import PagedLatents, pack_trees
+    model, pages = served
+    other = PagedLatents(model, 4, page_size=16)
+    other.reserve(3, 1)
+    pages.release([1, 2])
+    with pytest.raises(RuntimeError, match=r"slots \[3\]"):
+        model.cache_dump()
+    del other
+    gc.collect()
+    model.cache_dump()
+    pack_trees(model, [([3], [-1])], [1], [5])
+
+
+def test_a_copy_of_a_model_has_no_pages(served):
+    model, _ = served
+    twin = copy.deepcopy(model)
+    twin.cache_dump()
+    with pytest.raises(RuntimeError, match="in pages"):
+        model.cache_dump()
