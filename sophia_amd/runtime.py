@@ -338,6 +338,8 @@ class PagedLatents:
         a prompt's ``cache_dump(latents=False)`` at that length.)  ``src`` has the pages that it was given:
         ValueError where a fork on the device has put others in their places."""
         src, dst, places = int(src), int(dst), self._places(length)
+        if src < 0 or dst < 0:
+            raise ValueError(f"slots are >= 0, got {src} and {dst}")
         if self._held.get(dst):
             raise ValueError(f"slot {dst} holds pages")
         have = self._held.get(src, {})

@@ -98,3 +98,14 @@ def test_a_copy_of_a_model_has_no_pages(served):
     twin.cache_dump()
     with pytest.raises(RuntimeError, match="in pages"):
         model.cache_dump()
+
+
+@pytest.mark.parametrize("src,dst", [(1, -1), (-1, 3), (1, -4), (-2, -1)])
+def test_pages_are_not_shared_with_a_slot_that_is_none(served, src, dst):
+    """A negative number would name a row of the table from its end, which is another slot's."""
+    _, pages = served
+    before = pages.table.clone()
+    for length in (0, 16):
+        with pytest.raises(ValueError, match="slots are >= 0"):
+            pages.share(src, dst, length)
+    assert torch.equal(pages.table, before) and pages.slots == [1, 2]
