@@ -1023,7 +1023,10 @@ class Transformer(nn.Module):
         (``ops.cache_fork``).  ``cached`` int64 [M]: tokens in the caches of src[i].
         With ``pages`` the latents are those: dst[i] shares the pages that src[i] has
         filled, and has the page that it has filled in part copied into its own,
-        reserved before (``runtime.PagedLatents.reserve``); without, they are the slots'
+        reserved before (``runtime.PagedLatents.reserve``).  cached[i] is not below what
+        dst[i] has from an earlier fork or ``share``: its pages there are other slots', whose
+        tokens would be overwritten, and this call does not know (a sequence that goes
+        back goes on in a slot reserved for it).  Without pages, the latents are the slots'
         own, which is refused while a prompt's padding is masked (``set_pad_mask``): the
         mask is of the rows it was given for.  Nothing is read back on the host, so a fork
         is capturable."""

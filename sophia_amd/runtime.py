@@ -246,7 +246,9 @@ class PagedLatents:
     places of the pools.  ``Transformer.forward_step(pages=)`` writes and reads the
     pages, ``Transformer.fork_slots(pages=)`` moves them between slots on the device:
     the slots of such a fork may hold each other's pages afterwards, so they are
-    released together, and other slots do not ``share`` theirs.  What works on the slots'
+    released together, and other slots do not ``share`` theirs.  Pages that several
+    slots have are read alone: no slot that has them writes below the tokens that are
+    shared, neither in a step nor by a fork into it.  What works on the slots'
     own caches refuses a slot that holds pages: drafted steps, cached decoding,
     ``cache_dump`` and ``cache_load`` with latents.
 
