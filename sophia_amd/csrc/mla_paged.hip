@@ -170,13 +170,10 @@ struct Lanes {
   // at most 4 W / length.
   __device__ __forceinline__ int range_tiles(int lane) {
     float work = 0.f;
-    int all = 0;
     for (int s0 = (a.p.n_seqs - 1) & ~63; s0 >= 0; s0 -= 64) {
       look(s0 + lane);
       work += 0.5f * static_cast<float>(groups) * static_cast<float>(tiles + fewest);
-      all += groups;
     }
-    all = __builtin_amdgcn_readlane(wave_scan(all), 63);
     work = row_sum16(work);
     work += lane_xor16(work);
     work = (work + lane_xor32(work)) * 1.0001f + 1.f;   // (not less than it is, by rounding)
@@ -856,8 +853,9 @@ __device__ __forceinline__ void narrow(const PagedArgs &a, const Work &w, char *
   }
 }
 
-// The narrow work-groups first, as one of them may have a long chain of tiles.  The wide ones, as many as run at a
-// time, take their items in turn, so that each looks for them once.  WIDE, NARROW: which there are.
+// The narrow work-groups first, as one of them may have a long chain of tiles.  Of the wide ones there are as many as the
+// host's bound on the items, so each has one at most; it would take more in turn if offsets that descend made more
+// of them.  WIDE, NARROW: which there are.
 template <int R, bool F32, bool WIDE, bool NARROW>
 __global__ __launch_bounds__(256, R <= 128 ? 2 : 1) void mla_paged_kernel(PagedArgs a) {
   constexpr int kBytes = NARROW ? kTileBytes<R, F32> : Form<R, F32, false>::kTile;
