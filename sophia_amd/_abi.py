@@ -27,8 +27,9 @@ BWD_RECURRENT = 16
 BWD_GRAD_BF16 = 32
 
 TREE_NODES = 64          # SOPHIA_TREE_NODES of include/sophia_draft.h
-BEAMS = 64               # SOPHIA_BEAMS, SOPHIA_MOVES of include/sophia_pages.h
+BEAMS = 64               # SOPHIA_BEAMS, SOPHIA_MOVES, SOPHIA_FORK_MLA of include/sophia_pages.h
 MOVES = 4096
+POOLS = 24
 
 
 class CommitKda(ctypes.Structure):

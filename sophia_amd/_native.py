@@ -34,6 +34,7 @@ from ._abi import (  # noqa: F401
     TREE_NODES,
     BEAMS,
     MOVES,
+    POOLS,
     CommitKda,
     CommitMla,
     packed,

@@ -2088,7 +2088,7 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tens
 
 
 # ------------------------------------------------------------------ paged latents, beams, moves of caches
-BEAMS, MOVES = nat.BEAMS, nat.MOVES   # beams of a group and candidates kept, and moves of one call, at most
+BEAMS, MOVES, POOLS = nat.BEAMS, nat.MOVES, nat.POOLS   # beams of a group and candidates kept, moves and pools of one call, at most
 
 
 def _page_pool(pages: torch.Tensor, name: str) -> tuple[int, int, int, int]:
@@ -2323,7 +2323,7 @@ def cache_fork(src: torch.Tensor, dst: torch.Tensor, *, kda=(), mla=(), pools=()
     fill become shared, the tokens of the page that they fill in part are copied into
     the one that dst[i] has there, which no other slot has; the ids behind stay.
     page_size: of a table without pools, whose layers are elsewhere.
-    cached: int64 [M]."""
+    cached: int64 [M].  At most 48 KDA and 24 MLA layers."""
     n = _moves(src, dst)
     device, index = src.device, src.get_device()
     kda, mla, pools = list(kda), list(mla), list(pools)
@@ -2406,7 +2406,7 @@ def page_copy(src: torch.Tensor, dst: torch.Tensor, pools) -> None:
     writes to them, or moved together.
 
     src, dst: int32 [M], M <= 4096, under the rules of ``cache_fork``; pools: [n_pages,
-    page_size, rank] each, of one shape and dtype, dense and 16-byte aligned pages."""
+    page_size, rank] each, at most 24, of one shape and dtype, dense and 16-byte aligned pages."""
     n = _moves(src, dst)
     pools = list(pools)
     if not pools:

@@ -402,7 +402,9 @@ class PagedLatents:
     def _copy(self, src: list[int], dst: list[int]) -> None:
         for i in range(0, len(src), ops.MOVES):      # (none of the places is a source)
             pair = [torch.tensor(t[i:i + ops.MOVES], dtype=torch.int32).to(self.device) for t in (src, dst)]
-            ops.page_copy(*pair, list(self.pools.values()))
+            pools = list(self.pools.values())
+            for j in range(0, len(pools), ops.POOLS):
+                ops.page_copy(*pair, pools[j:j + ops.POOLS])
 
 
 @dataclass

@@ -109,3 +109,31 @@ def test_pages_are_not_shared_with_a_slot_that_is_none(served, src, dst):
         with pytest.raises(ValueError, match="slots are >= 0"):
             pages.share(src, dst, length)
     assert torch.equal(pages.table, before) and pages.slots == [1, 2]
+
+
+def test_pages_are_copied_in_every_layer_of_a_deep_model(monkeypatch):
+    """More MLA layers than one call of the operator takes, and more pages."""
+    from sophia_amd import ops
+    from sophia_amd.config import ModelArgs
+    from sophia_amd.decoder import Transformer
+    from sophia_amd.runtime import PagedLatents
+    layers = 4 * 30
+    model = Transformer(ModelArgs(vocab_size=8, n_layers=layers, ffn_hidden=16, mla_q_rank=8, mla_kv_rank=32, dim=32, num_heads=1,
+                                  max_seq_len=32, max_batch_size=1))
+    pages = PagedLatents(model, 8, page_size=16)
+    for i, pool in enumerate(pages.pools.values()):
+        pool.copy_((torch.arange(8) + 100 * i).view(8, 1, 1).expand_as(pool))
+    header = open(__file__.rsplit("/", 2)[0] + "/include/sophia_pages.h").read()
+    most = int(header.split("#define SOPHIA_FORK_MLA ")[1].split()[0])
+    assert most == ops.POOLS
+
+    def copy_pages(src, dst, pools):
+        assert len(pools) <= most
+        for pool in pools:
+            pool[dst.long()] = pool[src.long()]
+    monkeypatch.setattr(ops, "page_copy", copy_pages)
+    pages.reserve(0, 20)
+    pages.share(0, 3, 20)
+    assert pages.held(3) == [0, 2]
+    for i, pool in enumerate(pages.pools.values()):
+        assert pool[:, 0, 0].tolist() == [100 * i, 100 * i + 1, 100 * i + 1] + [100 * i + j for j in range(3, 8)]
