@@ -14,8 +14,8 @@
 // are found one after the other.
 //
 // 512 rows of 65,536 logits in bf16 (67 MB): 19.2 us, 10.6 of them until the maxima are known, 2.4 for the sums and
-// 6 for what is collected, which the loads of other work-groups hide in part; then 9 to join them.  Four rows in
-// fp32: 5.0 and 5.6, latency; 64 rows of 32 beams, of which 64 are kept, 12 and 40.
+// 6 for what is collected, which the loads of other work-groups hide in part; then 9.8 to join them.  Four rows in
+// fp32: 5.1 and 5.4, latency; 64 rows of 32 beams, of which 64 are kept, 12 and 40.
 #include <limits>
 
 #include "common.hpp"

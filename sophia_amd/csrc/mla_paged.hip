@@ -17,7 +17,8 @@
 // 3,700 in all: 8 sequences of 300 to 777 new tokens after up to 2,221 in 81 us and 9 to join them (411 TFLOP/s with both), 16 new
 // ones of 1,024 161 (426).  Eight wavefronts that take turns at products and softmax, with tiles in threes, were slower
 // (100, 180), and so was a work-group that goes on to its next item by itself (95).  The narrow form is latency: one
-// token after 700 9.2 us, 96 tokens after 221 to 3,090 each 12.2 and 4.
+// token after 700 9.2 us, 96 tokens after 221 to 3,090 each 12.8 and 4.  Between the forms, two tokens of each of 96 sequences
+// after 208 to 3,982 are the wide form's, three of whose four wavefronts have no columns: 47 us, four tokens 51, one 16.5.
 #include "common.hpp"
 #include "pages.hpp"
 #include "tree.hpp"
