@@ -678,11 +678,11 @@ def init_weights(model: nn.Module, args: ModelArgs) -> None:
     nn.init.zeros_(model.output_attn_residual.query.weight)
 
 
-class _PagePools(weakref.WeakSet):
+class PagePools(weakref.WeakSet):
     """The ``runtime.PagedLatents`` of a model; a copy of the model has none."""
 
     def __reduce__(self):
-        return _PagePools, ()
+        return PagePools, ()
 
 
 class Transformer(nn.Module):
@@ -698,7 +698,7 @@ class Transformer(nn.Module):
         self.output_attn_residual = AttentionResidualMixer(args)
         self.output = RuntimeLinear(args.dim, args.vocab_size)
         self.output.weight = self.tok_embeddings.weight  # tie_word_embeddings
-        self._page_pools = _PagePools()
+        self._page_pools = PagePools()
         init_weights(self, args)
 
     def reset_runtime_cache(self) -> None:
@@ -816,7 +816,7 @@ class Transformer(nn.Module):
     def _refuse_paged(self, slots, what: str) -> None:
         """Raises where the latents of one of ``slots`` (a function that lists them, called if there are
         any pages) are in pages: the slot's own cache, which the caller is about to use, does not have them."""
-        held = {s for pages in self._page_pools for s in pages.slots}
+        held = {s for pages in getattr(self, "_page_pools", ()) for s in pages.slots}
         both = sorted(held.intersection(slots())) if held else []
         if both:
             raise RuntimeError(f"{what}: the latents of slots {both} are in pages (runtime.PagedLatents), not in the slots' caches")
@@ -845,7 +845,7 @@ class Transformer(nn.Module):
         else:
             active = int(slots.numel())
         if latents:
-            self._refuse_paged(lambda: range(active) if slots is None else slots.tolist(), "cache_dump (latents=False takes the rest)")
+            self._refuse_paged(lambda: range(active) if slots is None else slots.reshape(-1).tolist(), "cache_dump (latents=False takes the rest)")
         return RuntimeCacheSnapshot(layers=tuple(
             layer.attn.cache_snapshot(device=device, batch_size=active, cache_pos=cache_pos, slots=slots)
             if latents or layer.layer_type == "kda" else None for layer in self.layers))
@@ -865,7 +865,8 @@ class Transformer(nn.Module):
             raise ValueError(f"{int(slots.numel())} slots for a snapshot of "
                              f"{cache_snapshot.batch_size()} rows")
         if any(layer is not None and layer.latent is not None for layer in cache_snapshot.layers):
-            self._refuse_paged(lambda: range(cache_snapshot.batch_size()) if slots is None else slots.tolist(), "cache_load of a snapshot with latents")
+            self._refuse_paged(lambda: range(cache_snapshot.batch_size()) if slots is None else slots.reshape(-1).tolist(),
+                               "cache_load of a snapshot with latents")
         required = cache_snapshot.batch_size() if slots is None else \
             (int(slots.max()) + 1 if slots.numel() else 0)
         if required:
@@ -1074,8 +1075,8 @@ class Transformer(nn.Module):
         def with_nodes():
             if torch.cuda.is_current_stream_capturing():
                 return []
-            cu = trees.cu_nodes.tolist()
-            return [s for s, a, b in zip(trees.slots.tolist(), cu, cu[1:]) if b > a]
+            cu = trees.cu_nodes.reshape(-1).tolist()
+            return [s for s, a, b in zip(trees.slots.reshape(-1).tolist(), cu, cu[1:]) if b > a]
         self._refuse_paged(with_nodes, "forward_tree")
         ids = trees.token_ids.reshape(-1).clamp(0, int(self.args.vocab_size) - 1)
         hidden = self.tok_embeddings(ids)

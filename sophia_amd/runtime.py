@@ -28,7 +28,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ops
-from .decoder import DraftTrees, SophiaMLA, Transformer
+from .decoder import DraftTrees, PagePools, SophiaMLA, Transformer
 from .state import RuntimeCacheSnapshot
 
 
@@ -278,6 +278,8 @@ class PagedLatents:
         self._free = list(range(n_pages - 1, -1, -1))
         self._holders = [0] * n_pages
         self._held: dict[int, dict[int, int]] = {}     # of a slot: place in its row -> page
+        if getattr(model, "_page_pools", None) is None:      # (a model pickled as a whole before there were any)
+            model._page_pools = PagePools()
         model._page_pools.add(self)
 
     @property

@@ -137,3 +137,21 @@ def test_pages_are_copied_in_every_layer_of_a_deep_model(monkeypatch):
     assert pages.held(3) == [0, 2]
     for i, pool in enumerate(pages.pools.values()):
         assert pool[:, 0, 0].tolist() == [100 * i, 100 * i + 1, 100 * i + 1] + [100 * i + j for j in range(3, 8)]
+
+
+def test_slots_of_any_shape_and_models_from_before(served):
+    """What was taken before there were pages is taken still: slots that are not a row, and a model pickled as a whole without its pools."""
+    from sophia_amd.runtime import PagedLatents
+    model, _ = served
+    snap = model.cache_dump(slots=torch.tensor(3, dtype=torch.int32))
+    assert snap.batch_size() == 1
+    with pytest.raises(RuntimeError, match="in pages"):
+        model.cache_dump(slots=torch.tensor(1, dtype=torch.int32))
+    old = copy.deepcopy(model)
+    del old.__dict__["_page_pools"]
+    old.cache_dump()
+    PagedLatents(old, 4, page_size=16).reserve(0, 1)
+    pages = PagedLatents(old, 4, page_size=16)
+    pages.reserve(0, 1)
+    with pytest.raises(RuntimeError, match=r"slots \[0\]"):
+        old.cache_dump()
